@@ -432,6 +432,67 @@ int tlm_kv_append_fp8(const void* x, int64_t x_batch_stride, int64_t x_row_strid
                       int64_t kv_rows, int64_t B, int64_t T, int64_t D, const float* scale,
                       void* stream);
 
+/* The 4-bit K/V cache: grouped-query attention's keys and values, paged, in OCP MX format: e2m1 elements
+ * (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives) with one e8m0 scale per 32 dims of a token and K/V head,
+ * 1.0625 D bytes per token and K/V head for K and V together. No reference program keeps such a cache; page
+ * addressing is that of tlm_mla_decode and tlm_kv_append_fp8: position p of sequence b lies in page
+ * block_table[b, p / page] (int32 [B, max_pages], dense), place p % page.
+ *   codes   uint8 [pages, 2, H_kv, page, D / 2]: index 0 is K, 1 is V; the even dim in the low half of its
+ *           byte. 16-byte aligned; codes_page_stride bytes from page to page (a multiple of 16, so the pools
+ *           of several layers may alternate), the rest dense.
+ *   scales  uint8 [pages, 2, H_kv, D / 32, page]: exponent + 127; 255 is NaN. 8-byte aligned,
+ *           scales_page_stride bytes from page to page (a multiple of 8).
+ *   D       a multiple of 32, 32 .. 256; page a multiple of 8; H_kv >= 1.
+ * Pools may be of any size (64-bit offsets). Table entries outside [0, pages) are read as zeros and never
+ * written through. */
+
+/* Quantises the new rows of every sequence into their pages: row j < min(count[b], T) of k and v goes to position
+ * start[b] + j; positions outside the table are skipped.
+ *   k, v  [B, T, H_kv, D] of x_dtype (F16 | BF16), heads and dims dense, rows of the given strides
+ *         (elements, multiples of 8; 16-byte aligned): slices of a fused projection will do.
+ * A block's scale is the least power of two 2^e, -126 <= e <= 125, with max |x| <= 7 2^e; x / 2^e is rounded to
+ * nearest even and saturates at 6, so that no element of a block below 2^127 is off by more than 2^e (infinities saturate).
+ * A block with a NaN gets scale 255 and codes 0, and reads as NaN. Of rows that go to the same place
+ * (a page of two sequences) an unspecified mixture stays. */
+int tlm_kv4_append(const void* k, const void* v, int64_t k_batch_stride, int64_t k_row_stride,
+                   int64_t v_batch_stride, int64_t v_row_stride, int x_dtype, const int32_t* start,
+                   const int32_t* count, const int32_t* block_table, int64_t max_pages, int64_t page,
+                   void* codes, int64_t codes_page_stride, void* scales, int64_t scales_page_stride,
+                   int64_t pages, int64_t B, int64_t T, int64_t H_kv, int64_t D, void* stream);
+
+/* Reads cached rows back: rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 of k_out and v_out receive the values of
+ * positions start[b], start[b] + 1, ... of sequence b (start NULL: from 0), the K and V that
+ * tlm_flash_attn_varlen_fwd takes with the same cu_seqlens (int32 [B + 1], ascending).
+ *   k_out, v_out  [total, H_kv, D], dense, 16-byte aligned, out_dtype F16 | BF16 | F32 (exact where the type holds the
+ *                 value, else rounded to nearest even, beyond its range infinite). Positions outside the
+ *                 table give zeros; rows of no sequence are left as they were. */
+int tlm_kv4_read(const void* codes, int64_t codes_page_stride, const void* scales,
+                 int64_t scales_page_stride, int64_t pages, const int32_t* block_table,
+                 int64_t max_pages, int64_t page, const int32_t* start, const int32_t* cu_seqlens,
+                 void* k_out, void* v_out, int64_t B, int64_t total, int64_t H_kv, int64_t D,
+                 int out_dtype, void* stream);
+
+/* Attention of the newest tokens of each sequence over the cache.
+ *   q       [B, T, H, D] of dtype (F16 | BF16), H a multiple of H_kv (query head h reads K/V head
+ *           h / (H / H_kv)); heads and dims dense, strides as tlm_kv4_append's.
+ *   seqlens int32 [B]: cached tokens, the new ones among them (clamped to [0, max_pages * page]).
+ *   count   int32 [B] or NULL: query rows of each sequence (clamped to [0, T]; NULL: T). Query j is position
+ *           seqlens[b] - count[b] + j and, causal, sees keys up to its own; not causal, every key.
+ *   o       [B, T, H, D] of dtype, dense; lse float [B, T, H] or NULL: log2 of the sum of exp of the scaled scores (the
+ *           glse of tlm_flash_attn_splitkv_fwd). A query without a key gets zeros and -inf; rows j >= count[b] are
+ *           left as they were.
+ *   sm_scale in the natural-log domain. Products, softmax and sums are fp32; the weights of V are carried to 16
+ *           bits of precision.
+ *   ws      tlm_kv4_attn_workspace_bytes(...) bytes, 16-byte aligned (device memory, caller-owned; needs no
+ *           initial value). Calls that overlap in time, and graphs whose replays may, need one each. */
+size_t tlm_kv4_attn_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t H_kv, int64_t D);
+int tlm_kv4_attn(const void* q, int64_t q_batch_stride, int64_t q_row_stride, const void* codes,
+                 int64_t codes_page_stride, const void* scales, int64_t scales_page_stride,
+                 int64_t pages, const int32_t* block_table, int64_t max_pages, int64_t page,
+                 const int32_t* seqlens, const int32_t* count, void* o, float* lse, void* ws,
+                 size_t ws_bytes, int64_t B, int64_t T, int64_t H, int64_t H_kv, int64_t D,
+                 int causal, float sm_scale, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -527,3 +527,112 @@ def paged_gather_ref(kv_bytes: np.ndarray, block_table: np.ndarray, seqlens: np.
         rows.append(block_table[b, j // page].astype(np.int64) * page + j % page)
     idx = np.concatenate(rows) if rows else np.zeros(0, np.int64)
     return kv_bytes[idx]
+
+
+# ---------------------------------------------------------------------------------------------
+# The 4-bit K/V cache (tlm_kv4_append / tlm_kv4_read / tlm_kv4_attn): OCP MX e2m1 elements with one e8m0
+# scale per 32 dims. No reference program; the definition is the header's, computed value by value.
+KV4_BLOCK = 32
+KV4_VALUES = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+
+
+def kv4_quantise_ref(x: torch.Tensor):
+    """Rows [..., D] -> codes uint8 [..., D / 2] (even dim in the low half) and scale bytes [..., D / 32]
+    in float64: the block's scale is the least 2^e, -126 <= e <= 125, with max |x| <= 7 2^e; codes are
+    the nearest e2m1 value (a tie takes the even code, beyond 6 is 6), the sign of zero kept. A block
+    with a NaN has scale byte 255 and codes 0."""
+    v = x.double().numpy().reshape(*x.shape[:-1], x.shape[-1] // KV4_BLOCK, KV4_BLOCK)
+    big = np.abs(v).max(-1)
+    bad = np.isnan(big)
+    e = np.full(big.shape, 125, dtype=np.int64)
+    for t in range(124, -127, -1):  # downwards while it still holds
+        e = np.where(big <= 7.0 * 2.0 ** t, t, e)
+    y = np.where(bad[..., None], 0.0, v) / (2.0 ** e)[..., None]
+    grid = np.array(KV4_VALUES)
+    with np.errstate(invalid="ignore"):
+        d = np.abs(np.minimum(np.abs(y), 6.0)[..., None] - grid)
+    tie = d == d.min(-1, keepdims=True)
+    # of two nearest codes the even one
+    code = np.where(tie.sum(-1) == 2, np.where(tie[..., ::2].any(-1), tie[..., ::2].argmax(-1) * 2, 0),
+                    tie.argmax(-1))
+    code = (code | np.where(np.signbit(y), 8, 0)).astype(np.uint8).reshape(x.shape)
+    code = np.where(np.repeat(bad, KV4_BLOCK, -1).reshape(x.shape), 0, code).astype(np.uint8)
+    return code[..., 0::2] | (code[..., 1::2] << 4), np.where(bad, 255, e + 127).astype(np.uint8)
+
+
+def kv4_dequantise_ref(codes: np.ndarray, scales: np.ndarray) -> np.ndarray:
+    """float64 values [..., D] of codes [..., D / 2] and scale bytes [..., D / 32]."""
+    table = np.array(KV4_VALUES + tuple(-v for v in KV4_VALUES))
+    v = np.stack((table[codes & 15], table[codes >> 4]), -1).reshape(*codes.shape[:-1], -1)
+    s = np.where(scales == 255, np.nan, 2.0 ** (scales.astype(np.float64) - 127))
+    return v * np.repeat(s, KV4_BLOCK, -1)
+
+
+def kv4_place(block_table, b: int, p: int, page: int, pages: int):
+    """(page id, place in it) of token position p of sequence b; None outside the table or the pool."""
+    if p < 0 or p >= block_table.shape[1] * page:
+        return None
+    pid = int(block_table[b, p // page])
+    return (pid, p % page) if 0 <= pid < pages else None
+
+
+def kv4_append_ref(k: torch.Tensor, v: torch.Tensor, start, count, block_table, codes: np.ndarray,
+                   scales: np.ndarray):
+    """K, V rows [B, T, H_kv, D] quantised into copies of the pools codes [pages, 2, H_kv, page, D / 2] and
+    scales [pages, 2, H_kv, D / 32, page]; positions without a place are skipped."""
+    codes, scales = codes.copy(), scales.copy()
+    pages, page = codes.shape[0], codes.shape[3]
+    for w, x in enumerate((k, v)):
+        c, e = kv4_quantise_ref(x)
+        for b in range(x.shape[0]):
+            for j in range(min(int(count[b]), x.shape[1])):
+                at = kv4_place(block_table, b, int(start[b]) + j, page, pages)
+                if at is not None:
+                    codes[at[0], w, :, at[1]] = c[b, j]
+                    scales[at[0], w, :, :, at[1]] = e[b, j]
+    return codes, scales
+
+
+def kv4_rows_ref(codes: np.ndarray, scales: np.ndarray, block_table, b: int, start: int, n: int):
+    """Values of positions start .. start + n - 1 of sequence b: float64 K, V [n, H_kv, D]; zeros where
+    there is no place."""
+    pages, _, Hkv, page, half = codes.shape
+    out = np.zeros((2, n, Hkv, 2 * half))
+    at = [kv4_place(block_table, b, start + j, page, pages) for j in range(n)]
+    live = [j for j in range(n) if at[j] is not None]
+    if live:
+        pid, off = (np.array([at[j][i] for j in live]) for i in (0, 1))
+        for w in (0, 1):
+            out[w, live] = kv4_dequantise_ref(codes[pid, w, :, off], scales[pid, w, :, :, off])
+    return out[0], out[1]
+
+
+def kv4_attn_ref(q: torch.Tensor, codes: np.ndarray, scales: np.ndarray, block_table, seqlens, count,
+                 sm_scale: float, causal: bool = True):
+    """float64 output [B, T, H, D] and log2 sum-exp [B, T, H] of grouped-query attention over the cache; NaN
+    in rows j >= count[b], which are not computed. Query j of sequence b is position len - count + j."""
+    B, T, H, D = q.shape
+    Hkv, page = codes.shape[2], codes.shape[3]
+    out = np.full((B, T, H, D), np.nan)
+    lse = np.full((B, T, H), np.nan)
+    for b in range(B):
+        n = max(0, min(int(seqlens[b]), block_table.shape[1] * page))
+        m = max(0, min(int(count[b]) if count is not None else T, T))
+        k, v = kv4_rows_ref(codes, scales, block_table, b, 0, n)
+        k, v = (np.repeat(x, H // Hkv, 1).transpose(1, 0, 2) for x in (k, v))  # [H, n, D]
+        x = q[b, :m].double().numpy().transpose(1, 0, 2)  # [H, m, D]
+        s = np.matmul(x, k.transpose(0, 2, 1)) * sm_scale
+        if causal:
+            s = np.where(np.arange(n) > (n - m + np.arange(m))[:, None], -np.inf, s)
+            seen = np.arange(n) <= n - m + np.arange(m)[:, None]
+        else:
+            seen = np.ones((m, n), dtype=bool)
+        top = s.max(-1, initial=-np.inf)
+        p = np.exp(s - np.where(np.isneginf(top), 0.0, top)[..., None])
+        total = p.sum(-1)
+        for i in range(m):  # masked keys take no part, whatever their values
+            o = np.matmul(p[:, i][:, None, seen[i]], v[:, seen[i]])[:, 0]
+            with np.errstate(invalid="ignore", divide="ignore"):
+                out[b, i] = np.where((total[:, i] > 0)[:, None] | np.isnan(o), o / total[:, i, None], 0.0)
+                lse[b, i] = (np.where(np.isneginf(top[:, i]), 0.0, top[:, i]) + np.log(total[:, i])) / np.log(2.0)
+    return out, lse

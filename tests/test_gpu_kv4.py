@@ -1,0 +1,490 @@
+"""The 4-bit K/V cache on the GPU: tlm_kv4_append and tlm_kv4_read bit for bit and tlm_kv4_attn within
+its roundings of oracle/ref.py's kv4_* (float64), and runs of them together."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import ref
+from tilelang.jit.adapter.mi355x import ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF16, F16 = torch.bfloat16, torch.float16
+
+
+def _i32(v):
+    return torch.as_tensor(np.asarray(v), dtype=torch.int32).to(DEV)
+
+
+def _pools(pages, Hkv, page, D, seed=0, lo=122, hi=127):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randint(0, 256, (pages, 2, Hkv, page, D // 2), generator=g).byte(),
+            torch.randint(lo, hi, (pages, 2, Hkv, D // 32, page), generator=g).byte())
+
+
+def _append(k, v, start, count, bt, codes, scales):
+    c, s = codes.to(DEV), scales.to(DEV)
+    ops.kv4_append(k.to(DEV), v.to(DEV), _i32(start), _i32(count), _i32(bt), c, s)
+    return c.cpu().numpy(), s.cpu().numpy()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("Hkv,D,page", [(1, 32, 8), (8, 128, 64), (3, 96, 24), (2, 256, 16), (5, 64, 40)])
+def test_append_bit_exact(dtype, Hkv, D, page):
+    g = torch.Generator().manual_seed(11)
+    B, T, per = 5, 70, -(-150 // page)
+    k, v = ((torch.randn(B, T, Hkv, D, generator=g) * torch.exp(3 * torch.randn(B, T, Hkv, 1, generator=g))).to(dtype)
+            for _ in "kv")
+    pages = B * per + 3
+    bt = torch.randperm(pages, generator=g)[:B * per].view(B, per).int().numpy()
+    start = np.array([0, 5, per * page - 33, 63, 64], np.int32)  # sequence 2 runs out of its table
+    count = np.array([70, 0, 70, 1, 200], np.int32)              # 200: more than T
+    codes, scales = _pools(pages, Hkv, page, D)
+    got = _append(k, v, start, count, bt, codes, scales)
+    exp = ref.kv4_append_ref(k, v, start, count, bt, codes.numpy(), scales.numpy())
+    assert np.array_equal(got[0], exp[0]) and np.array_equal(got[1], exp[1])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_append_every_value(dtype):
+    """Every 16-bit pattern as the block's only value, and beside a larger one (rounding at each scale)."""
+    bits = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(dtype)
+    x = torch.zeros(1, 1024, 8, 256, dtype=dtype)
+    x.view(-1, 32)[:, 0] = bits
+    y = x.clone()
+    y.view(-1, 32)[:, 1] = torch.ldexp(bits.abs().nan_to_num(0, 0, 0).float(), torch.arange(65536) % 5).to(dtype)
+    codes, scales = _pools(16, 8, 64, 256)
+    bt = np.arange(16, dtype=np.int32).reshape(1, 16)
+    got = _append(x, y, [0], [1024], bt, codes, scales)
+    exp = ref.kv4_append_ref(x, y, [0], [1024], bt, codes.numpy(), scales.numpy())
+    assert np.array_equal(got[0], exp[0]) and np.array_equal(got[1], exp[1])
+
+
+def test_append_corrupt_tables_and_positions():
+    g = torch.Generator().manual_seed(12)
+    k, v = (torch.randn(3, 20, 2, 64, generator=g).to(BF16) for _ in "kv")
+    bt = np.array([[1, -5, 3], [1 << 30, 0, 4], [2, 5, -2147483648]], np.int32)
+    start, count = np.array([4, 0, -7], np.int32), np.array([20, 20, 20], np.int32)
+    codes, scales = _pools(4, 2, 8, 64)  # pages 4 and 5 do not exist
+    got = _append(k, v, start, count, bt, codes, scales)
+    exp = ref.kv4_append_ref(k, v, start, count, bt, codes.numpy(), scales.numpy())
+    assert np.array_equal(got[0], exp[0]) and np.array_equal(got[1], exp[1])
+
+
+def _layers(pages, layers, Hkv, page, D):
+    """Pools of one layer out of several that alternate page by page."""
+    codes = torch.full((pages, layers, 2, Hkv, page, D // 2), 0x11, dtype=torch.uint8, device=DEV)
+    scales = torch.full((pages, layers, 2, Hkv, D // 32, page), 0x22, dtype=torch.uint8, device=DEV)
+    return codes, scales
+
+
+def test_append_and_read_slices():
+    """K and V as slices of one projection's rows, pools as one layer of several; the rest stays."""
+    g = torch.Generator().manual_seed(13)
+    B, T, H, Hkv, D, page = 3, 9, 4, 2, 64, 16
+    qkv = torch.randn(B, T + 2, (H + 2 * Hkv) * D, generator=g).to(BF16).to(DEV)[:, 1:-1]
+    k = qkv[..., H * D:(H + Hkv) * D].view(B, T, Hkv, D)
+    v = qkv[..., (H + Hkv) * D:].view(B, T, Hkv, D)
+    codes, scales = _layers(4, 3, Hkv, page, D)
+    bt, start, count = _i32([[3], [0], [2]]), _i32([2, 0, 7]), _i32([9, 4, 9])
+    ops.kv4_append(k, v, start, count, bt, codes[:, 1], scales[:, 1])
+    exp = ref.kv4_append_ref(k.cpu(), v.cpu(), [2, 0, 7], [9, 4, 9], bt.cpu().numpy(),
+                             np.full((4, 2, Hkv, page, D // 2), 0x11, np.uint8),
+                             np.full((4, 2, Hkv, D // 32, page), 0x22, np.uint8))
+    assert np.array_equal(codes[:, 1].cpu().numpy(), exp[0])
+    assert np.array_equal(scales[:, 1].cpu().numpy(), exp[1])
+    for i in (0, 2):
+        assert (codes[:, i] == 0x11).all() and (scales[:, i] == 0x22).all()
+    cu = _i32([0, 9, 13, 22])
+    ko, vo = (torch.empty(22, Hkv, D, dtype=BF16, device=DEV) for _ in "kv")
+    ops.kv4_read(codes[:, 1], scales[:, 1], bt, start, cu, ko, vo)
+    for got, x in ((ko, k), (vo, v)):
+        x = torch.cat([x[b, :n] for b, n in enumerate((9, 4, 9))]).cpu()
+        assert np.array_equal(got.double().cpu().numpy(), ref.kv4_dequantise_ref(*ref.kv4_quantise_ref(x)))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, torch.float32])
+@pytest.mark.parametrize("Hkv,D,page", [(1, 32, 8), (8, 128, 64), (3, 96, 24), (2, 256, 16)])
+def test_read_bit_exact(dtype, Hkv, D, page):
+    g = torch.Generator().manual_seed(14)
+    B, per = 5, 6
+    pages = B * per
+    codes, scales = _pools(pages, Hkv, page, D, 15, 0, 256)  # every scale, NaN among them
+    bt = torch.randperm(pages, generator=g).view(B, per).int().numpy()
+    bt[1, 2], bt[3, 0] = -1, pages
+    n = [2 * page + 3, 4 * page, 0, 1, per * page + 5]  # the last reads past its table
+    start = [0, 3, 7, 2 * page, 0]
+    cu = np.concatenate([[0], np.cumsum(n)]).astype(np.int32)
+    for first in (None, start):
+        outs = [torch.full((int(cu[-1]) + 3, Hkv, D), 7.0, dtype=dtype, device=DEV) for _ in "kv"]
+        ops.kv4_read(codes.to(DEV), scales.to(DEV), _i32(bt), None if first is None else _i32(first), _i32(cu),
+                     *outs)
+        for w, out in enumerate(outs):
+            exp = np.concatenate([ref.kv4_rows_ref(codes.numpy(), scales.numpy(), bt, b,
+                                                   0 if first is None else start[b], n[b])[w] for b in range(B)])
+            with np.errstate(all="ignore"):  # one rounding, as torch's cast of the fp64 value
+                exp = torch.from_numpy(exp).to(dtype)
+            assert torch.equal(out[:len(exp)].cpu().nan_to_num(123.0, posinf=456.0, neginf=-456.0),
+                               exp.nan_to_num(123.0, posinf=456.0, neginf=-456.0))
+            assert (out[len(exp):] == 7).all()
+
+
+def _attn_case(dtype, B, T, H, Hkv, D, page, lens, seed=0, pages=None, q_scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    per = max(1, -(-max(lens) // page))
+    pages = pages or B * per + 2
+    x = torch.randn(pages, 2, Hkv, page, D, generator=g)
+    x[..., ::17] *= 6
+    codes, scales = ref.kv4_quantise_ref(x)
+    codes, scales = torch.from_numpy(codes), torch.from_numpy(np.ascontiguousarray(scales.swapaxes(-1, -2)))
+    bt = torch.randperm(pages, generator=g)[:B * per].view(B, per).int().numpy()
+    q = (torch.randn(B, T, H, D, generator=g) * q_scale).to(dtype)
+    return q, codes, scales, bt
+
+
+def _stale(codes, scales, bt, lens, page):
+    """NaN in every place that no sequence uses."""
+    codes, scales = codes.clone(), scales.clone()
+    live = torch.zeros(codes.shape[0], page, dtype=torch.bool)
+    for b, n in enumerate(lens):
+        p = np.arange(n)
+        live[torch.from_numpy(bt[b, p // page].astype(np.int64)), torch.from_numpy(p % page)] = True
+    scales[~live[:, None, None, None, :].expand_as(scales)] = 255
+    codes[~live[:, None, None, :, None].expand_as(codes)] = 0
+    return codes, scales
+
+
+def _run(q, codes, scales, bt, lens, count=None, causal=True, scale=None, lse=True, ws_fill=0xFF):
+    B, T, H, D = q.shape
+    out = torch.full((B, T, H, D), 9.0, dtype=q.dtype, device=DEV)
+    z = torch.full((B, T, H), 9.0, device=DEV) if lse else None
+    need = ops.kv4_attn_workspace_bytes(B, T, H, codes.shape[2], D)
+    ws = torch.full((max(16, need),), ws_fill, dtype=torch.uint8, device=DEV)  # all ones: NaN
+    ops.kv4_attn(q.to(DEV), codes.to(DEV), scales.to(DEV), _i32(bt), _i32(lens), out, ws,
+                 D ** -0.5 if scale is None else scale, None if count is None else _i32(count), causal, z)
+    torch.cuda.synchronize()
+    return out.cpu(), None if z is None else z.cpu()
+
+
+def _check(q, codes, scales, bt, lens, count=None, causal=True, scale=None, got=None):
+    """Within the kernel's roundings of the float64 result. A score is a sum of D exact products in fp32 (q
+    and the cached values are exact in its operands): off by at most (D + 2) 2^-24 of the sum of
+    magnitudes A. A weight is off by that times ln 2 log2 e = 1, by exp2 (1 ulp, and its argument's
+    rounding against a reference within the scores' range: 2 A 2^-24) and by 16 bits where it multiplies V (2^-17).
+    Numerator and denominator are sums of up to n weights, (n + 64) 2^-24 each; the quotient is
+    rounded once: by eps / 2, or half of the smallest subnormal, tiny eps / 2 (an output of 4.5e-7 is
+    0.46 of fp16's 2^-24 steps off its nearest multiple: no fp16 value is nearer)."""
+    B, T, H, D = q.shape
+    sm = D ** -0.5 if scale is None else scale
+    page = codes.shape[3]
+    c, s = codes.numpy(), scales.numpy()
+    exp, lse = ref.kv4_attn_ref(q, c, s, bt, lens, count, sm, causal)
+    # sum p |v| / l, and the largest sum of magnitudes of a score, by the same reference on |v| and |q|, |k|
+    mag = c.copy()
+    mag[:, 1] &= 0x77
+    spread, _ = ref.kv4_attn_ref(q, mag, s, bt, lens, count, sm, causal)
+    out, z = got if got is not None else _run(q, codes, scales, bt, lens, count, causal, scale)
+    eps = torch.finfo(q.dtype).eps / 2
+    least = torch.finfo(q.dtype).tiny * eps
+    for b in range(B):
+        n = max(0, min(int(lens[b]), bt.shape[1] * page))
+        m = T if count is None else max(0, min(int(count[b]), T))
+        k, _ = ref.kv4_rows_ref(c, s, bt, b, 0, n)
+        k = np.abs(k).repeat(H // codes.shape[2], 1).transpose(1, 2, 0)
+        a = np.abs(q[b, :m].double().numpy()).transpose(1, 0, 2) @ k * abs(sm) if n else np.zeros((H, m, 1))
+        a = a.max(-1).T[..., None]  # [m, H, 1]
+        rel = 2 * ((D + 4) * 2.0 ** -24 * a + 2.0 ** -23 + 2.0 ** -17 + (n + 64) * 2.0 ** -24)
+        x, e = out[b, :m].double().numpy(), exp[b, :m]
+        bad = np.abs(x - e) > eps * (1 + 2 ** -10) * np.abs(e) + rel * spread[b, :m] + least
+        assert not bad.any(), (b, np.abs(x - e).max())
+        assert np.array_equal(np.isnan(x), np.isnan(e))
+        assert (out[b, m:] == 9).all()
+        if z is not None:
+            zz, ee = z[b, :m].double().numpy(), lse[b, :m]
+            fin = np.isfinite(ee)
+            assert np.array_equal(zz[~fin & ~np.isnan(ee)], ee[~fin & ~np.isnan(ee)])
+            lim = (rel[..., 0] + 2.0 ** -22 * (np.abs(np.where(fin, ee, 0)) + 4)) * 1.5
+            assert (np.abs(zz[fin] - ee[fin]) <= lim[fin]).all()
+            assert (z[b, m:] == 9).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("D", [32, 64, 96, 128, 160, 192, 224, 256])
+def test_attn_head_dims(dtype, D):
+    lens = [1, 33, 500]
+    q, c, s, bt = _attn_case(dtype, 3, 1, 8, 2, D, 16, lens, D)
+    _check(q, *_stale(c, s, bt, lens, 16), bt, lens)
+
+
+@pytest.mark.parametrize("H,Hkv", [(1, 1), (5, 5), (7, 1), (16, 1), (17, 1), (33, 1), (64, 2), (128, 1), (24, 3)])
+def test_attn_head_groups(H, Hkv):
+    lens = [70, 1, 259]
+    q, c, s, bt = _attn_case(BF16, 3, 1, H, Hkv, 128, 64, lens, H)
+    _check(q, *_stale(c, s, bt, lens, 64), bt, lens)
+
+
+@pytest.mark.parametrize("page", [8, 16, 24, 40, 64, 128, 1000])
+def test_attn_pages(page):
+    lens = [1, 7, 8, 31, 32, 33, 63, 64, 65, 127, 129, 300]
+    q, c, s, bt = _attn_case(F16, 12, 1, 8, 2, 64, page, lens, page)
+    _check(q, *_stale(c, s, bt, lens, page), bt, lens)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("T,H,Hkv,D", [(2, 8, 8, 64), (5, 32, 4, 128), (17, 4, 2, 96), (64, 8, 2, 128), (130, 3, 1, 256)])
+def test_attn_several_new_tokens(T, H, Hkv, D, causal):
+    """Chunks of T with fewer of them in some sequences; sequences shorter than their new tokens, whose
+    first rows see nothing when causal; rows past count untouched."""
+    lens, count = [T, 300, T // 2, 0, 450], [T, max(1, T - 1), T, T, 0]
+    q, c, s, bt = _attn_case(BF16, 5, T, H, Hkv, D, 16, lens, T)
+    _check(q, *_stale(c, s, bt, lens, 16), bt, lens, count, causal)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_attn_long_and_short_together(dtype):
+    lens = [6000, 1, 0, 40, 3333, 2, 900]
+    q, c, s, bt = _attn_case(dtype, 7, 1, 16, 4, 128, 64, lens, 3)
+    _check(q, *_stale(c, s, bt, lens, 64), bt, lens)
+
+
+def test_attn_many_sequences():
+    lens = [(7 * i) % 41 for i in range(700)]
+    q, c, s, bt = _attn_case(F16, 700, 1, 4, 2, 64, 8, lens, 4)
+    _check(q, *_stale(c, s, bt, lens, 8), bt, lens)
+
+
+def test_attn_lengths_past_the_table_and_below_zero():
+    q, c, s, bt = _attn_case(BF16, 3, 2, 8, 2, 64, 16, [64, 64, 64], 5)
+    _check(q, c, s, bt, [1000, -3, 2147483647])
+    _check(q, c, s, bt, [64, 10, 64], count=[-1, 1000, 2])
+
+
+def test_attn_missing_pages_read_as_zeros():
+    q, c, s, bt = _attn_case(F16, 3, 1, 8, 2, 128, 16, [100, 90, 48], 6)
+    bt[0, 2], bt[1, 0], bt[2, 2] = -1, c.shape[0], 2147483647
+    _check(q, c, s, bt, [100, 90, 48])
+    bt[2] = -7  # a sequence of zeros: its output is 0, its sum-exp log2 of its length
+    _check(q, c, s, bt, [100, 90, 48])
+
+
+def test_attn_same_page_twice():
+    """Pages that two sequences share (a common prefix) and one that a sequence holds twice."""
+    lens = [80, 95, 70]
+    q, c, s, bt = _attn_case(BF16, 3, 1, 8, 4, 128, 16, lens, 7)
+    bt[1, :3] = bt[0, :3]
+    bt[2, 3] = bt[2, 0]
+    _check(q, c, s, bt, lens)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_attn_sharp_and_large_scores(dtype):
+    """Scores in the thousands: softmax picks single keys; and a scale of 0: the mean of V."""
+    lens = [700, 33, 5]
+    q, c, s, bt = _attn_case(dtype, 3, 1, 8, 2, 128, 64, lens, 8, q_scale=200.0)
+    _check(q, c, s, bt, lens, scale=1.0)
+    _check(q, c, s, bt, lens, scale=0.0)
+    _check(q, c, s, bt, lens, scale=-0.5)
+
+
+def test_attn_growing_scores():
+    """Every tile's maximum far above the last one's, and far below it."""
+    lens = [1500, 1500]
+    q, c, s, bt = _attn_case(BF16, 2, 1, 4, 1, 64, 16, lens, 9)
+    q = torch.ones_like(q)
+    c[:, 0] = 0x22  # K: ones
+    for p in range(1500):
+        for b, up in ((0, p), (1, 1499 - p)):
+            s[int(bt[b, p // 16]), 0, :, :, p % 16] = 118 + up // 100
+    _check(q, c, s, bt, lens, scale=1.0)
+
+
+def test_attn_nan_and_extreme_blocks():
+    """A NaN block of K or V in sight makes the rows that see it NaN, and only those; K's scales at both ends."""
+    lens = [100, 100, 100, 100]
+    q, c, s, bt = _attn_case(BF16, 4, 3, 4, 2, 64, 16, lens, 10)
+    s[int(bt[0, 98 // 16]), 0, 1, 0, 98 % 16] = 255  # K of sequence 0, position 98, head 1: queries 1 and 2
+    s[int(bt[1, 0]), 1, 0, 1, 3] = 255               # V of sequence 1, head 0, dims 32 ..
+    s[int(bt[2, 1]), 0, :, :, 5] = 1                 # a key of nothing
+    out, lse = _run(q, c, s, bt, lens)
+    nan = torch.zeros(4, 3, 4, 64, dtype=torch.bool)
+    nan[0, 1:, 2:] = True
+    nan[1, :, :2, 32:] = True
+    assert torch.equal(out.isnan(), nan)
+    keep = [2, 3]
+    _check(q[keep], c, s, bt[keep], [100, 100], got=(out[keep], lse[keep]))
+
+
+def test_attn_strided_queries_and_layers():
+    g = torch.Generator().manual_seed(15)
+    B, T, H, Hkv, D, page = 3, 2, 8, 2, 64, 16
+    lens = [30, 77, 5]
+    q, c, s, bt = _attn_case(BF16, B, T, H, Hkv, D, page, lens, 11)
+    codes, scales = _layers(c.shape[0], 3, Hkv, page, D)
+    codes[:, 2], scales[:, 2] = c.to(DEV), s.to(DEV)
+    wide = torch.randn(B, T + 1, (H + 4) * D, generator=g).to(BF16).to(DEV)
+    wide[:, 1:, 2 * D:(2 + H) * D] = q.flatten(2).to(DEV)
+    view = wide[:, 1:, 2 * D:(2 + H) * D].view(B, T, H, D)
+    out = torch.full((B, T, H, D), 9.0, dtype=BF16, device=DEV)
+    ws = torch.empty(max(16, ops.kv4_attn_workspace_bytes(B, T, H, Hkv, D)), dtype=torch.uint8, device=DEV)
+    ops.kv4_attn(view, codes[:, 2], scales[:, 2], _i32(bt), _i32(lens), out, ws, D ** -0.5)
+    _check(q, c, s, bt, lens, got=(out.cpu(), None))
+
+
+def test_pools_past_4_gb():
+    """Pages behind the 4 GB of their pool, written, read and attended."""
+    Hkv, page, D = 8, 128, 128
+    pages = (1 << 32) // (Hkv * page * D) + 3
+    codes = torch.empty(pages, 2, Hkv, page, D // 2, dtype=torch.uint8, device=DEV)
+    scales = torch.empty(pages, 2, Hkv, D // 32, page, dtype=torch.uint8, device=DEV)
+    g = torch.Generator().manual_seed(16)
+    k, v = (torch.randn(1, 200, Hkv, D, generator=g).to(BF16) for _ in "kv")
+    bt = np.array([[pages - 1, pages - 2]], np.int32)
+    ops.kv4_append(k.to(DEV), v.to(DEV), _i32([0]), _i32([200]), _i32(bt), codes, scales)
+    ko, vo = (torch.empty(200, Hkv, D, dtype=BF16, device=DEV) for _ in "kv")
+    ops.kv4_read(codes, scales, _i32(bt), None, _i32([0, 200]), ko, vo)
+    for got, x in ((ko, k), (vo, v)):
+        assert np.array_equal(got.double().cpu().numpy(), ref.kv4_dequantise_ref(*ref.kv4_quantise_ref(x[0])))
+    q = torch.randn(1, 1, 16, D, generator=g).to(BF16)
+    out = torch.empty(1, 1, 16, D, dtype=BF16, device=DEV)
+    ws = torch.empty(max(16, ops.kv4_attn_workspace_bytes(1, 1, 16, Hkv, D)), dtype=torch.uint8, device=DEV)
+    ops.kv4_attn(q.to(DEV), codes, scales, _i32(bt), _i32([200]), out, ws, D ** -0.5)
+    _check(q, codes[-2:].cpu(), scales[-2:].cpu(), np.array([[1, 0]], np.int32), [200], got=(out.cpu(), None))
+
+
+def _prompt_and_steps(dtype, H, Hkv, D, page, prompts, chunk, steps):
+    """Prompts written and attended chunk by chunk, then decode steps: every output against the oracle on the
+    cache as it then is."""
+    g = torch.Generator().manual_seed(17)
+    B = len(prompts)
+    per = -(-(max(prompts) + steps) // page)
+    codes, scales = (x.to(DEV) for x in _pools(B * per, Hkv, page, D, 18, 255, 256))  # NaN: nothing written yet
+    bt = torch.randperm(B * per, generator=g).view(B, per).int().numpy()
+    have = np.zeros(B, np.int64)
+    goal = np.array(prompts)
+    ws = torch.empty(max(16, ops.kv4_attn_workspace_bytes(B, chunk, H, Hkv, D)), dtype=torch.uint8, device=DEV)
+    while steps >= 0:
+        T = chunk if (have < goal).any() else 1
+        new = np.minimum(goal - have, T) if T > 1 else np.ones(B, np.int64)
+        q = torch.randn(B, T, H, D, generator=g).to(dtype)
+        k, v = (torch.randn(B, T, Hkv, D, generator=g).to(dtype) for _ in "kv")
+        ops.kv4_append(k.to(DEV), v.to(DEV), _i32(have), _i32(new), _i32(bt), codes, scales)
+        have += new
+        out = torch.full((B, T, H, D), 9.0, dtype=dtype, device=DEV)
+        ops.kv4_attn(q.to(DEV), codes, scales, _i32(bt), _i32(have), out, ws, D ** -0.5, _i32(new))
+        _check(q, codes.cpu(), scales.cpu(), bt, have, new, got=(out.cpu(), None))
+        steps -= T == 1
+    return codes, scales, bt, have, g
+
+
+def test_prompt_then_decode_steps():
+    dtype, H, Hkv, D, page = BF16, 8, 2, 128, 16
+    codes, scales, bt, have, g = _prompt_and_steps(dtype, H, Hkv, D, page, [100, 37, 64], 40, 3)
+    # the prompt read back for attention over unquantised rows gives the same attention: all but the 16-bit
+    # weights of that kernel (eps / 2 of each) are in the bound of the cache's own
+    cu = np.concatenate([[0], np.cumsum(have)]).astype(np.int32)
+    total = int(cu[-1])
+    ko, vo = (torch.empty(total, Hkv, D, dtype=dtype, device=DEV) for _ in "kv")
+    ops.kv4_read(codes, scales, _i32(bt), None, _i32(cu), ko, vo)
+    T = 8
+    q = torch.randn(3, T, H, D, generator=g).to(dtype)
+    flat, o = q.flatten(0, 1).to(DEV), torch.empty(3 * T, H, D, dtype=dtype, device=DEV)
+    ops.flash_attn_varlen_fwd(flat, ko, vo, _i32([0, T, 2 * T, 3 * T]), _i32(cu), T, o, True, D ** -0.5)
+    out, _ = _run(q, codes.cpu(), scales.cpu(), bt, have)
+    spread = vo.abs().max().item()
+    assert (o.view_as(out).cpu().float() - out.float()).abs().max().item() <= 4 * torch.finfo(dtype).eps * spread
+
+
+def test_prompt_then_decode_steps_f16_odd():
+    _prompt_and_steps(F16, 9, 3, 96, 24, [50, 3, 77], 33, 2)
+
+
+def test_same_bits_again_and_on_two_streams():
+    lens = [3000, 100, 1700, 5]
+    q, c, s, bt = _attn_case(BF16, 4, 1, 32, 8, 128, 64, lens, 19)
+    args = (q.to(DEV), c.to(DEV), s.to(DEV), _i32(bt), _i32(lens))
+    need = max(16, ops.kv4_attn_workspace_bytes(4, 1, 32, 8, 128))
+    first = torch.empty_like(args[0])
+    ops.kv4_attn(*args, first, torch.empty(need, dtype=torch.uint8, device=DEV), 0.1)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = [[torch.empty_like(first) for _ in range(6)] for _ in streams]
+    spaces = [torch.empty(need, dtype=torch.uint8, device=DEV) for _ in streams]
+    for i in range(6):
+        for st, o, w in zip(streams, outs, spaces):
+            with torch.cuda.stream(st):
+                ops.kv4_attn(*args, o[i], w, 0.1)
+    torch.cuda.synchronize()
+    assert all(torch.equal(first, o) for os in outs for o in os)
+
+
+def test_decode_step_in_a_graph():
+    """Append and attention captured once, replayed with other rows, lengths and tables; each replay equals the
+    eager calls."""
+    g = torch.Generator().manual_seed(20)
+    B, H, Hkv, D, page = 4, 16, 4, 128, 32
+    lens = [200, 64, 1000, 1]
+    q, c, s, bt = _attn_case(BF16, B, 1, H, Hkv, D, page, [1040] * 4, 21)
+    c, s, q, bt = c.to(DEV), s.to(DEV), q.to(DEV), _i32(bt)
+    k, v = (torch.randn(B, 1, Hkv, D, generator=g).to(BF16).to(DEV) for _ in "kv")
+    start, sl, one = _i32(lens), _i32(lens) + 1, _i32([1] * B)
+    out = torch.empty_like(q)
+    ws = torch.empty(max(16, ops.kv4_attn_workspace_bytes(B, 1, H, Hkv, D)), dtype=torch.uint8, device=DEV)
+
+    def step(out, c, s, ws):
+        ops.kv4_append(k, v, start, one, bt, c, s)
+        ops.kv4_attn(q, c, s, bt, sl, out, ws, D ** -0.5)
+
+    step(out, c, s, ws)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(out, c, s, ws)
+    c2, s2, ws2, out2 = c.clone(), s.clone(), torch.empty_like(ws), torch.empty_like(out)
+    for i in range(5):
+        q.copy_(torch.randn(q.shape, generator=g))
+        k.copy_(torch.randn(k.shape, generator=g))
+        v.copy_(torch.randn(v.shape, generator=g))
+        n = torch.randint(0, 1039, (B,), generator=g).int()
+        start.copy_(n)
+        sl.copy_(n + 1)
+        out.fill_(3.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        step(out2, c2, s2, ws2)
+        torch.cuda.synchronize()
+        assert torch.equal(out, out2) and torch.equal(c, c2) and torch.equal(s, s2), i
+
+
+def test_ops_refusals():
+    q, c, s, bt = _attn_case(BF16, 2, 1, 8, 2, 64, 16, [20, 20], 22)
+    q, c, s, bt, sl = q.to(DEV), c.to(DEV), s.to(DEV), _i32(bt), _i32([20, 20])
+    out, ws = torch.empty_like(q), torch.empty(1 << 24, dtype=torch.uint8, device=DEV)
+    k = torch.zeros(2, 1, 2, 64, dtype=BF16, device=DEV)
+    one = _i32([1, 1])
+    bad = [
+        lambda: ops.kv4_attn(q.cpu(), c, s, bt, sl, out, ws, 0.1),
+        lambda: ops.kv4_attn(q[..., :32], c, s, bt, sl, out, ws, 0.1),
+        lambda: ops.kv4_attn(q.transpose(2, 3).contiguous().transpose(2, 3), c, s, bt, sl, out, ws, 0.1),
+        lambda: ops.kv4_attn(q[:, :, :7], c, s, bt, sl, out, ws, 0.1),
+        lambda: ops.kv4_attn(q, c[:, :1], s, bt, sl, out, ws, 0.1),
+        lambda: ops.kv4_attn(q, c, s[:, :, :, :1], bt, sl, out, ws, 0.1),
+        lambda: ops.kv4_attn(q, c.int(), s, bt, sl, out, ws, 0.1),
+        lambda: ops.kv4_attn(q, c.transpose(2, 3).contiguous().transpose(2, 3), s, bt, sl, out, ws, 0.1),
+        lambda: ops.kv4_attn(q, c, s, bt.long(), sl, out, ws, 0.1),
+        lambda: ops.kv4_attn(q, c, s, bt[:1], sl, out, ws, 0.1),
+        lambda: ops.kv4_attn(q, c, s, bt, sl[:1], out, ws, 0.1),
+        lambda: ops.kv4_attn(q, c, s, bt, sl, out.float(), ws, 0.1),
+        lambda: ops.kv4_attn(q, c, s, bt, sl, out, ws, 0.1, count=one[:1]),
+        lambda: ops.kv4_attn(q, c, s, bt, sl, out, ws, 0.1, lse=torch.empty(2, 1, 8, device=DEV, dtype=BF16)),
+        lambda: ops.kv4_append(k, k[:1], one, one, bt, c, s),
+        lambda: ops.kv4_append(k, k.half(), one, one, bt, c, s),
+        lambda: ops.kv4_append(k, k, one.long(), one, bt, c, s),
+        lambda: ops.kv4_append(k[:, :, :1], k[:, :, :1], one, one, bt, c, s),
+        lambda: ops.kv4_read(c, s, bt, None, one, k[0], k[0]),
+        lambda: ops.kv4_read(c, s, bt, None, _i32([0, 1, 2]), k[:, 0], k[:1, 0]),
+        lambda: ops.kv4_read(c, s, bt, one.long(), _i32([0, 1, 2]), k[:, 0], k[:, 0].clone()),
+    ]
+    for i, f in enumerate(bad):
+        with pytest.raises(ValueError):
+            f()
+            raise AssertionError(i)

@@ -1,0 +1,220 @@
+// The 4-bit K/V cache: quantising rows as they are written, and reading them back.
+//
+// Format (OCP MX): 32 dims of a token and head share a power-of-two scale 2^e; an element is e2m1. With
+// M = max |x| of the block, e is the least exponent with M <= 7 2^e: e2m1 reaches 6 and its widest step
+// is 2, so values up to 7 are off by no more than any other. e follows from M's bits: M = 1.f 2^E gives
+// e = E - 2, one more where 1.f > 1.75. M is the largest of the absolute bit patterns, which orders
+// infinities behind every number and NaN behind those. v_cvt_scalef32_pk_fp4_* divides by the scale, rounds to
+// nearest even, saturates and keeps the sign of zero (every 16-bit pattern compared with exact arithmetic); the reverse
+// conversions are exact and pass a NaN scale on.
+//
+// Bound: HBM. A token and head moves 4 D bytes of 16-bit rows and 1.0625 D bytes of cache.
+#include "tlm_kv4.h"
+
+#include <algorithm>
+
+namespace {
+
+using kv4::Cache;
+constexpr int K4_T = 256;
+constexpr int K4_GRID = 8192;  // workgroups per launch at most
+
+typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef float f2 __attribute__((ext_vector_type(2)));
+
+template <int SEL>
+TLM_DEV uint32_t to_fp4(uint32_t old, uint32_t w, float s, std::true_type) {
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(old, __builtin_bit_cast(b2, w), s, SEL);
+}
+template <int SEL>
+TLM_DEV uint32_t to_fp4(uint32_t old, uint32_t w, float s, std::false_type) {
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(old, __builtin_bit_cast(h2, w), s, SEL);
+}
+
+// Page and place of position p of sequence b; false outside the table or the pool.
+TLM_DEV bool place(const Cache& c, int b, int64_t p, int64_t& pid, int& off) {
+  if (p < 0 || p >= (int64_t)c.max_pages * c.page) return false;
+  const int i = (int)p / c.page;
+  off = (int)p - i * c.page;
+  pid = c.table[(int64_t)b * c.max_pages + i];
+  return pid >= 0 && pid < c.pages;
+}
+
+// Four lanes per block of 32 dims, 8 dims each.
+template <bool BF16>
+__global__ __launch_bounds__(K4_T) void kv4_append_kernel(Cache c, const uint16_t* k, const uint16_t* v,
+                                                          int64_t kb, int64_t kr, int64_t vb, int64_t vr,
+                                                          const int32_t* start, const int32_t* count, int B,
+                                                          int T) {
+  const int per_row = c.Hkv * (c.D / 8);  // chunks of a row of k or v
+  const int64_t chunks = 2 * (int64_t)per_row;
+  for (int b = blockIdx.y; b < B; b += gridDim.y) {
+    const int n = min(count[b], T);
+    const int64_t first = start[b], all = chunks * n;
+    for (int64_t i = (int64_t)blockIdx.x * K4_T + threadIdx.x; i < all; i += (int64_t)gridDim.x * K4_T) {
+      const int j = (int)(i / chunks);
+      int ch = (int)(i - j * chunks);
+      const int w = ch >= per_row;
+      ch -= w * per_row;
+      const int h = ch / (c.D / 8), d8 = ch - h * (c.D / 8);
+      int64_t pid;
+      int off;
+      if (!place(c, b, first + j, pid, off)) continue;  // the four lanes of a block together
+      const uint16_t* src = (w ? v + b * vb + j * vr : k + b * kb + j * kr) + 8 * ch;
+      const u32x4 x = *(const u32x4*)src;
+      uint32_t m = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        m = max(m, max(x[e] & 0x7fffu, (x[e] >> 16) & 0x7fffu));
+      m = max(m, (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0xB1, 0xf, 0xf, false));  // lane ^ 1
+      m = max(m, (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0x4E, 0xf, 0xf, false));  // lane ^ 2
+      const uint32_t f = __float_as_uint(h16<BF16>::to_f32(m));
+      int byte = (int)(f >> 23) - 2 + ((f & 0x7fffffu) > 0x600000u);
+      byte = max(1, min(252, byte));
+      uint32_t code = 0;
+      if (f > 0x7f800000u) {
+        byte = 255;  // NaN
+      } else {
+        const float s = kv4::scale_of(byte);
+        const std::bool_constant<BF16> tag;
+        code = to_fp4<0>(code, x[0], s, tag);
+        code = to_fp4<1>(code, x[1], s, tag);
+        code = to_fp4<2>(code, x[2], s, tag);
+        code = to_fp4<3>(code, x[3], s, tag);
+      }
+      const int64_t at = (int64_t)w * c.Hkv + h;
+      *(uint32_t*)(c.codes + pid * c.codes_page + (at * c.page + off) * (c.D / 2) + 4 * d8) = code;
+      if ((d8 & 3) == 0)
+        c.scales[pid * c.scales_page + (at * (c.D / kv4::BLOCK) + d8 / 4) * c.page + off] = (uint8_t)byte;
+    }
+  }
+}
+
+// 8 dims per thread. OUT: 0 fp16, 1 bf16, 2 fp32.
+template <int OUT>
+__global__ __launch_bounds__(K4_T) void kv4_read_kernel(Cache c, const int32_t* start, const int32_t* cu,
+                                                        uint8_t* k_out, uint8_t* v_out, int B, int64_t total) {
+  constexpr int ES = OUT == 2 ? 4 : 2;
+  const int per_row = c.Hkv * (c.D / 8);
+  const int64_t chunks = 2 * (int64_t)per_row, all = chunks * total;
+  for (int64_t i = (int64_t)blockIdx.x * K4_T + threadIdx.x; i < all; i += (int64_t)gridDim.x * K4_T) {
+    const int64_t r = i / chunks;
+    int ch = (int)(i - r * chunks);
+    const int w = ch >= per_row;
+    ch -= w * per_row;
+    const int h = ch / (c.D / 8), d8 = ch - h * (c.D / 8);
+    int lo = 0, hi = B + 1;  // the last cu <= r
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (cu[mid] <= r) lo = mid + 1;
+      else hi = mid;
+    }
+    const int b = lo - 1;
+    if (b < 0 || b >= B) continue;  // a row of no sequence
+    int64_t pid;
+    int off;
+    uint32_t code = 0, byte = 127;
+    if (place(c, b, (start ? (int64_t)start[b] : 0) + (r - cu[b]), pid, off)) {
+      const int64_t at = (int64_t)w * c.Hkv + h;
+      code = *(const uint32_t*)(c.codes + pid * c.codes_page + (at * c.page + off) * (c.D / 2) + 4 * d8);
+      byte = c.scales[pid * c.scales_page + (at * (c.D / kv4::BLOCK) + d8 / 4) * c.page + off];
+    }
+    const float s = kv4::scale_of(byte);
+    uint8_t* dst = (w ? v_out : k_out) + (r * per_row + ch) * 8 * ES;
+    if constexpr (OUT == 1) {
+      *(u32x4*)dst = u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, s, 0)),
+                           __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, s, 1)),
+                           __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, s, 2)),
+                           __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, s, 3))};
+    } else {
+      const f2 a[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, s, 0),
+                       __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, s, 1),
+                       __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, s, 2),
+                       __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, s, 3)};
+      if constexpr (OUT == 2) {
+        *(f32x4*)dst = f32x4{a[0][0], a[0][1], a[1][0], a[1][1]};
+        *(f32x4*)(dst + 16) = f32x4{a[2][0], a[2][1], a[3][0], a[3][1]};
+      } else {
+        using H = h16<false>;
+        *(u32x4*)dst = u32x4{H::pack(a[0][0], a[0][1]), H::pack(a[1][0], a[1][1]), H::pack(a[2][0], a[2][1]),
+                             H::pack(a[3][0], a[3][1])};
+      }
+    }
+  }
+}
+
+}  // namespace
+
+extern "C" int tlm_kv4_append(const void* k, const void* v, int64_t k_batch_stride, int64_t k_row_stride,
+                              int64_t v_batch_stride, int64_t v_row_stride, int x_dtype,
+                              const int32_t* start, const int32_t* count, const int32_t* block_table,
+                              int64_t max_pages, int64_t page, void* codes, int64_t codes_page_stride,
+                              void* scales, int64_t scales_page_stride, int64_t pages, int64_t B, int64_t T,
+                              int64_t H_kv, int64_t D, void* stream) {
+  Cache c{(uint8_t*)codes, (uint8_t*)scales, codes_page_stride, scales_page_stride, pages, block_table};
+  if (int rc = kv4::check("tlm_kv4_append", c, max_pages, page, H_kv, D, B)) return rc;
+  if (int rc = kv4::check_rows("tlm_kv4_append", "k", k, k_batch_stride, k_row_stride, x_dtype)) return rc;
+  if (int rc = kv4::check_rows("tlm_kv4_append", "v", v, v_batch_stride, v_row_stride, x_dtype)) return rc;
+  if (!start || !count) {
+    tlm_set_error("tlm_kv4_append: null pointer argument");
+    return TLM_EINVAL;
+  }
+  if (T < 0 || T > INT32_MAX) {
+    tlm_set_error("tlm_kv4_append: bad sizes");
+    return TLM_EINVAL;
+  }
+  if (B == 0 || T == 0) return TLM_OK;
+  c.max_pages = (int)max_pages, c.page = (int)page, c.Hkv = (int)H_kv, c.D = (int)D;
+  const int64_t chunks = 2 * H_kv * (D / 8) * T;
+  const int64_t gy = std::min<int64_t>(B, 4096);
+  const int64_t gx = std::min<int64_t>((chunks + K4_T - 1) / K4_T, std::max<int64_t>(1, K4_GRID / gy));
+  const dim3 grid((unsigned)gx, (unsigned)gy);
+  auto go = [&](auto kern) {
+    kern<<<grid, K4_T, 0, (hipStream_t)stream>>>(c, (const uint16_t*)k, (const uint16_t*)v, k_batch_stride,
+                                                 k_row_stride, v_batch_stride, v_row_stride, start, count,
+                                                 (int)B, (int)T);
+  };
+  if (x_dtype == TLM_BF16) go(kv4_append_kernel<true>);
+  else go(kv4_append_kernel<false>);
+  TLM_LAUNCH_CHECK("tlm_kv4_append");
+  return TLM_OK;
+}
+
+extern "C" int tlm_kv4_read(const void* codes, int64_t codes_page_stride, const void* scales,
+                            int64_t scales_page_stride, int64_t pages, const int32_t* block_table,
+                            int64_t max_pages, int64_t page, const int32_t* start,
+                            const int32_t* cu_seqlens, void* k_out, void* v_out, int64_t B, int64_t total,
+                            int64_t H_kv, int64_t D, int out_dtype, void* stream) {
+  Cache c{(uint8_t*)codes, (uint8_t*)scales, codes_page_stride, scales_page_stride, pages, block_table};
+  if (int rc = kv4::check("tlm_kv4_read", c, max_pages, page, H_kv, D, B)) return rc;
+  if (!cu_seqlens || !k_out || !v_out) {
+    tlm_set_error("tlm_kv4_read: null pointer argument");
+    return TLM_EINVAL;
+  }
+  if (out_dtype != TLM_BF16 && out_dtype != TLM_F16 && out_dtype != TLM_F32) {
+    tlm_set_error("tlm_kv4_read: out dtype %d unsupported (BF16, F16 or F32)", out_dtype);
+    return TLM_EUNSUPPORTED;
+  }
+  if (total < 0 || total > INT32_MAX) {
+    tlm_set_error("tlm_kv4_read: bad sizes (total rows up to 2^31 - 1)");
+    return TLM_EINVAL;
+  }
+  if (!tlm_aligned(k_out, 16) || !tlm_aligned(v_out, 16)) {
+    tlm_set_error("tlm_kv4_read: k_out and v_out must be 16-byte aligned");
+    return TLM_EINVAL;
+  }
+  if (B == 0 || total == 0) return TLM_OK;
+  c.max_pages = (int)max_pages, c.page = (int)page, c.Hkv = (int)H_kv, c.D = (int)D;
+  const int64_t chunks = 2 * H_kv * (D / 8) * total;
+  const unsigned grid = (unsigned)std::min<int64_t>((chunks + K4_T - 1) / K4_T, K4_GRID);
+  auto go = [&](auto kern) {
+    kern<<<grid, K4_T, 0, (hipStream_t)stream>>>(c, start, cu_seqlens, (uint8_t*)k_out, (uint8_t*)v_out,
+                                                 (int)B, total);
+  };
+  if (out_dtype == TLM_BF16) go(kv4_read_kernel<1>);
+  else if (out_dtype == TLM_F16) go(kv4_read_kernel<0>);
+  else go(kv4_read_kernel<2>);
+  TLM_LAUNCH_CHECK("tlm_kv4_read");
+  return TLM_OK;
+}

@@ -79,6 +79,14 @@ _SIGNATURES = {
     "tlm_kv_append_fp8": ([c_void_p, c_int64, c_int64, c_int, c_void_p, c_void_p, c_void_p,
                            c_int64, c_int64, c_void_p] + [c_int64] * 5 + [c_void_p, c_void_p],
                           c_int),
+    "tlm_kv4_append": ([c_void_p] * 2 + [c_int64] * 4 + [c_int] + [c_void_p] * 3 + [c_int64] * 2 +
+                       [c_void_p, c_int64] * 2 + [c_int64] * 5 + [c_void_p], c_int),
+    "tlm_kv4_read": ([c_void_p, c_int64] * 2 + [c_int64, c_void_p] + [c_int64] * 2 +
+                     [c_void_p] * 4 + [c_int64] * 4 + [c_int, c_void_p], c_int),
+    "tlm_kv4_attn_workspace_bytes": ([c_int64] * 5, c_size_t),
+    "tlm_kv4_attn": ([c_void_p] + [c_int64] * 2 + [c_void_p, c_int64] * 2 + [c_int64, c_void_p] +
+                     [c_int64] * 2 + [c_void_p] * 5 + [c_size_t] + [c_int64] * 5 +
+                     [c_int, c_float, c_int, c_void_p], c_int),
 }
 
 EXPORTED = tuple(_SIGNATURES)

@@ -480,6 +480,128 @@ def kv_append_fp8(x: torch.Tensor, start: torch.Tensor, count: torch.Tensor,
     return kv
 
 
+def _kv4_pools(codes: torch.Tensor, scales: torch.Tensor):
+    """H_kv, page, D and the pools' page strides of a 4-bit cache; the pools are checked against each
+    other."""
+    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+        raise ValueError("codes and scales must be uint8")
+    if codes.dim() != 5 or scales.dim() != 5 or codes.shape[1] != 2:
+        raise ValueError("codes must be [pages, 2, H_kv, page, D / 2] and scales "
+                         "[pages, 2, H_kv, D / 32, page]")
+    pages, _, Hkv, page, half = codes.shape
+    if half % 16 or scales.shape != (pages, 2, Hkv, half // 16, page):
+        raise ValueError(f"scales {tuple(scales.shape)} do not match codes {tuple(codes.shape)} "
+                         "(D a multiple of 32)")
+    cs, ss = 2 * Hkv * page * half, 2 * Hkv * (half // 16) * page  # bytes of a page
+    if pages > 1 and not (codes.is_contiguous() and scales.is_contiguous()):
+        if not (codes[0].is_contiguous() and scales[0].is_contiguous()):
+            raise ValueError("codes and scales must be dense within a page")
+        cs, ss = codes.stride(0), scales.stride(0)
+    elif pages == 1 and not (codes.is_contiguous() and scales.is_contiguous()):
+        raise ValueError("codes and scales must be dense within a page")
+    return Hkv, page, 2 * half, cs, ss
+
+
+def _kv4_rows(name: str, x: torch.Tensor, heads: int, D: int):
+    """Batch and row stride of [B, T, heads, D] rows whose heads and dims are dense."""
+    if x.dim() != 4 or x.shape[2] != heads or x.shape[3] != D:
+        raise ValueError(f"{name} must be [B, T, {heads}, {D}], got {tuple(x.shape)}")
+    sb, st, sh, sd = x.stride()
+    if sd != 1 or (heads > 1 and sh != D):
+        raise ValueError(f"{name}: heads and dims must be contiguous")
+    row = heads * D
+    return (sb if x.shape[0] > 1 else row), (st if x.shape[1] > 1 else row)
+
+
+def _i32(name: str, t: torch.Tensor, *shape: int):
+    if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of shape {list(shape)}")
+
+
+def kv4_append(k: torch.Tensor, v: torch.Tensor, start: torch.Tensor, count: torch.Tensor,
+               block_table: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor):
+    """Quantise new rows k, v [B, T, H_kv, D] (bf16/fp16; any batch and row stride) into the paged 4-bit
+    cache codes uint8 [pages, 2, H_kv, page, D / 2], scales uint8 [pages, 2, H_kv, D / 32, page] at
+    positions start[b] .. start[b] + count[b] - 1 of each sequence. Returns codes, scales."""
+    dev = _dev(k, v, start, count, block_table, codes, scales)
+    Hkv, page, D, cs, ss = _kv4_pools(codes, scales)
+    ks, vs = _kv4_rows("k", k, Hkv, D), _kv4_rows("v", v, Hkv, D)
+    B, T = k.shape[:2]
+    if v.shape != k.shape or v.dtype != k.dtype:
+        raise ValueError("k and v must share shape and dtype")
+    _i32("start", start, B)
+    _i32("count", count, B)
+    _i32("block_table", block_table, B, block_table.shape[-1])
+    lib.call("tlm_kv4_append", _ptr(k), _ptr(v), *ks, *vs, dtype_code(k.dtype), _ptr(start),
+             _ptr(count), _ptr(block_table), block_table.shape[1], page, _ptr(codes),
+             cs, _ptr(scales), ss, codes.shape[0], B, T, Hkv, D,
+             _stream(dev))
+    return codes, scales
+
+
+def kv4_read(codes: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor,
+             start: Optional[torch.Tensor], cu_seqlens: torch.Tensor, k_out: torch.Tensor,
+             v_out: torch.Tensor):
+    """Read rows of the 4-bit cache back: rows cu_seqlens[b] .. cu_seqlens[b + 1] of k_out, v_out
+    [total, H_kv, D] (bf16/fp16/fp32) receive positions start[b] .. (None: 0 ..) of sequence b."""
+    dev = _dev(codes, scales, block_table, start, cu_seqlens, k_out, v_out)
+    Hkv, page, D, cs, ss = _kv4_pools(codes, scales)
+    _contig("k_out", k_out)
+    _contig("v_out", v_out)
+    if k_out.dim() != 3 or k_out.shape[1:] != (Hkv, D) or v_out.shape != k_out.shape or \
+            v_out.dtype != k_out.dtype:
+        raise ValueError(f"k_out and v_out must be [total, {Hkv}, {D}] of one dtype")
+    if block_table.dim() != 2:
+        raise ValueError("block_table must be [B, max_pages]")
+    B = block_table.shape[0]
+    _i32("block_table", block_table, B, block_table.shape[1])
+    _i32("cu_seqlens", cu_seqlens, B + 1)
+    if start is not None:
+        _i32("start", start, B)
+    lib.call("tlm_kv4_read", _ptr(codes), cs, _ptr(scales), ss,
+             codes.shape[0], _ptr(block_table), block_table.shape[1], page, _ptr(start),
+             _ptr(cu_seqlens), _ptr(k_out), _ptr(v_out), B, k_out.shape[0], Hkv, D,
+             dtype_code(k_out.dtype), _stream(dev))
+    return k_out, v_out
+
+
+def kv4_attn_workspace_bytes(B, T, H, H_kv, D) -> int:
+    return int(lib.load().tlm_kv4_attn_workspace_bytes(B, T, H, H_kv, D))
+
+
+def kv4_attn(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor,
+             seqlens: torch.Tensor, out: torch.Tensor, workspace: torch.Tensor, sm_scale: float,
+             count: Optional[torch.Tensor] = None, causal: bool = True,
+             lse: Optional[torch.Tensor] = None):
+    """Attention of the newest count[b] (None: T) tokens of each sequence, q [B, T, H, D] (any batch and
+    row stride), over its seqlens[b] tokens of the 4-bit cache, those tokens' own among them.
+    out [B, T, H, D]; lse float32 [B, T, H]: log2 of the sum of exp of the scaled scores. Rows from
+    count[b] on are left as they were. workspace: kv4_attn_workspace_bytes(...) bytes, one per stream."""
+    dev = _dev(q, codes, scales, block_table, seqlens, out, workspace, count, lse)
+    Hkv, page, D, cs, ss = _kv4_pools(codes, scales)
+    if q.dim() != 4 or Hkv == 0 or q.shape[2] % Hkv:
+        raise ValueError(f"q must be [B, T, H, {D}] with H a multiple of {Hkv}")
+    B, T, H = q.shape[:3]
+    qs = _kv4_rows("q", q, H, D)
+    _contig("out", out)
+    if out.shape != q.shape or out.dtype != q.dtype:
+        raise ValueError("out must match q in shape and dtype")
+    _i32("seqlens", seqlens, B)
+    if count is not None:
+        _i32("count", count, B)
+    _i32("block_table", block_table, B, block_table.shape[-1])
+    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (B, T, H) or
+                            not lse.is_contiguous()):
+        raise ValueError("lse must be a contiguous float32 [B, T, H] tensor")
+    _contig("workspace", workspace)
+    lib.call("tlm_kv4_attn", _ptr(q), *qs, _ptr(codes), cs, _ptr(scales),
+             ss, codes.shape[0], _ptr(block_table), block_table.shape[1], page,
+             _ptr(seqlens), _ptr(count), _ptr(out), _ptr(lse), _ptr(workspace),
+             workspace.numel() * workspace.element_size(), B, T, H, Hkv, D, 1 if causal else 0,
+             float(sm_scale), dtype_code(q.dtype), _stream(dev))
+    return out
+
+
 def elementwise(inputs, bcast, outputs, code, consts, rows: int, cols: int):
     """Run an elementwise register program (include/tlmi355x.h: tlm_elementwise) over the
     [rows, cols] output domain. inputs: tensors (F32 / F16 / BF16) with their broadcast kinds
