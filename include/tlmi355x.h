@@ -484,7 +484,7 @@ int tlm_kv4_read(const void* codes, int64_t codes_page_stride, const void* scale
  *   sm_scale in the natural-log domain. Products, softmax and sums are fp32; the weights of V are carried to 16
  *           bits of precision.
  *   ws      tlm_kv4_attn_workspace_bytes(...) bytes, 16-byte aligned (device memory, caller-owned; needs no
- *           initial value). Calls that overlap in time, and graphs whose replays may, need one each. */
+ *           initial value; a size for T is enough for fewer rows and any B). Calls that overlap in time, and graphs whose replays may, need one each. */
 size_t tlm_kv4_attn_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t H_kv, int64_t D);
 int tlm_kv4_attn(const void* q, int64_t q_batch_stride, int64_t q_row_stride, const void* codes,
                  int64_t codes_page_stride, const void* scales, int64_t scales_page_stride,

@@ -35,7 +35,7 @@ inline int check(const char* fn, const Cache& c, int64_t max_pages, int64_t page
     tlm_set_error("%s: D must be a multiple of 32 up to 256 and page a multiple of 8", fn);
     return TLM_EUNSUPPORTED;
   }
-  if (page > (1 << 20) || Hkv > (1 << 16) || max_pages > INT32_MAX / page || B > INT32_MAX / max_pages) {
+  if (page > (1 << 20) || Hkv > (1 << 16) || max_pages > (INT32_MAX - 4096) / page || B > INT32_MAX / max_pages) {
     tlm_set_error("%s: problem too large (2^31 positions per table row and entries per table)", fn);
     return TLM_EINVAL;
   }
