@@ -149,7 +149,7 @@ ODD = ctypes.c_void_p(0x1008)
 SHARED = [
     (dict(codes=None), EINVAL, "null"), (dict(scales=None), EINVAL, "null"), (dict(bt=None), EINVAL, "null"),
     (dict(codes=ODD), EINVAL, "aligned"), (dict(scales=ctypes.c_void_p(0x1004)), EINVAL, "aligned"),
-    (dict(page=0), EINVAL, "sizes"), (dict(mp=0), EINVAL, "sizes"), (dict(pages=-1), EINVAL, "sizes"),
+    (dict(page=0), EINVAL, "sizes"), (dict(mp=0), EINVAL, "sizes"), (dict(pages=0), EINVAL, "sizes"),
     (dict(B=-1), EINVAL, "sizes"), (dict(Hkv=0), EINVAL, "sizes"), (dict(D=0), EINVAL, "sizes"),
     (dict(D=100), EUNSUPPORTED, "multiple of 32"), (dict(D=288), EUNSUPPORTED, "up to 256"),
     (dict(page=20), EUNSUPPORTED, "multiple of 8"), (dict(mp=1 << 40), EINVAL, "too large"),

@@ -27,7 +27,7 @@ inline int check(const char* fn, const Cache& c, int64_t max_pages, int64_t page
     tlm_set_error("%s: null pointer argument", fn);
     return TLM_EINVAL;
   }
-  if (c.pages < 0 || max_pages <= 0 || page <= 0 || Hkv <= 0 || D <= 0 || B < 0) {
+  if (c.pages <= 0 || max_pages <= 0 || page <= 0 || Hkv <= 0 || D <= 0 || B < 0) {
     tlm_set_error("%s: bad sizes", fn);
     return TLM_EINVAL;
   }
@@ -37,6 +37,10 @@ inline int check(const char* fn, const Cache& c, int64_t max_pages, int64_t page
   }
   if (page > (1 << 20) || Hkv > (1 << 16) || max_pages > (INT32_MAX - 4096) / page || B > INT32_MAX / max_pages) {
     tlm_set_error("%s: problem too large (2^31 positions per table row and entries per table)", fn);
+    return TLM_EINVAL;
+  }
+  if (Hkv * page > INT32_MAX / D) {
+    tlm_set_error("%s: problem too large (2^31 bytes of codes per page)", fn);
     return TLM_EINVAL;
   }
   if (c.codes_page % 16 != 0 || c.scales_page % 8 != 0 || c.codes_page < Hkv * page * D ||

@@ -12,7 +12,19 @@ constexpr int KA_W = 4;          // waves per workgroup
 constexpr int KA_BN = 32;        // tokens per tile (one wave)
 constexpr int KA_UNIT = KA_W * KA_BN;
 constexpr int KA_PIECE = 1;      // cost of a piece beside its units, in units
+// Workgroups per CU, and stages of a ring in their share of the LDS.
+constexpr int ka_per_cu(int D, int QT) { return QT == 1 ? (D <= 128 ? 3 : 2) : D <= 128 ? 2 : 1; }
+template <int D, int QT>
+constexpr int ka_stages() {
+  const int n = (160 * 1024 / ka_per_cu(D, QT) - 1024) / (KA_W * (32 * D + 256 * ((D + 127) / 128)));
+  return n < 4 ? n : 4;
+}
 constexpr float KA_SLACK = 8.f;  // a reference is kept until a score passes it by this much (log2)
+
+struct KaCut {
+  int b, rt;   // sequence (-1: nothing to join) and row tile
+  int p0, p1;  // first and last range that hold units of it
+};
 
 struct KaArgs {
   Cache c;
@@ -22,10 +34,13 @@ struct KaArgs {
   const int32_t* count;
   uint16_t* o;
   float* lse;
-  int64_t* meta;  // [G][4]: where range r starts: sequence, row tile, cost before the entry, all cost
-  float* part;    // [2 G][Hkv][16 QT][D + 2]
-  int B, T, H, group, causal, G, page_shift;
-  float scale2;  // sm_scale log2(e)
+  KaCut* cuts;  // [G]: the entry that the cut before range r goes through, if it is the entry's first
+  float* part;  // [2 G][Hkv][16 QT][D + 2]: rows, their references, their sums
+  int B, T, H, group, causal, G;
+  uint32_t page_mul;  // tok / page = tok page_mul >> page_shift, for tok < 2^31
+  int page_shift;
+  float scale2;     // |sm_scale| log2(e)
+  uint32_t q_sign;  // the sign of sm_scale on both halves of a word
 };
 
 // An entry of the cost line: 16 QT query rows of one sequence (rows run over its new tokens and, within one,
@@ -132,8 +147,18 @@ struct Segs {
   }
 };
 
-__device__ const u32x4 ka_zeros[64] = {};  // codes and scales of tokens without a page
+__device__ const u32x4 ka_zeros[1] = {};  // codes and scales of tokens without a page
 
+// A tile in a wave's ring of LDS, 16-byte slots: 32 dims of a token each. First K, in the order that the lanes read it
+// as MFMA operands, then V in token order of its operand (token 8 g + i behind 8 g' + i for g > g'), so that all
+// reads are linear in the lane; then the scales, [K, V][D / 32][32 tokens].
+template <int D>
+struct Stage {
+  static constexpr int CODES = 32 * D, NC = D / 32;           // bytes; LDS-DMA instructions of 64 slots
+  static constexpr int NS = (D + 127) / 128, SCALES = 256 * NS;  // 64 words each
+  static constexpr int BYTES = CODES + SCALES, PER = NC + NS;
+};
+// What a lane has of a tile.
 template <int D>
 struct KaTile {
   uint32_t k[2][D / 32], v[8][Segs<D>::N];
@@ -141,22 +166,54 @@ struct KaTile {
   u32x2 vs[Segs<D>::N];
 };
 
+using ldsop::lds_u32;
 template <int N>
-TLM_DEV void ka_load(uint32_t* dst, const uint8_t* p) {  // N bytes
-  if constexpr (N == 16) {
-    const u32x4 x = *(const u32x4*)p;
-    dst[0] = x[0], dst[1] = x[1], dst[2] = x[2], dst[3] = x[3];
-  } else if constexpr (N == 8) {
-    const u32x2 x = *(const u32x2*)p;
-    dst[0] = x[0], dst[1] = x[1];
-  } else if constexpr (N == 4) {
-    dst[0] = *(const uint32_t*)p;
-  } else if constexpr (N == 2) {
-    dst[0] = *(const uint16_t*)p;
-  } else {
-    dst[0] = *p;
-  }
+TLM_DEV void vm_wait() {  // all but the last N vector loads and LDS-DMA instructions of this wave have landed
+  static_assert(N >= 0 && N < 64, "vmcnt is 6 bits");
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_waitcnt(0x3f70 | (N & 15) | ((N >> 4) << 14));
+  __builtin_amdgcn_sched_barrier(0);
 }
+
+// K, V and scales of one segment: LDS addresses of the lane, waited for within the block.
+template <int KO, int VO, int KSO, int VSO>
+TLM_DEV void ka_read128(u32x4& k0, u32x4& k1, uint32_t& s0, uint32_t& s1, u32x2 (&v)[4], u32x2& vs, uint32_t ka,
+                        uint32_t va, uint32_t ksa, uint32_t vsa) {
+  asm volatile(
+      "ds_read_b128 %0, %9 offset:%13\n\t"
+      "ds_read_b128 %1, %9 offset:%14\n\t"
+      "ds_read_u8 %2, %11 offset:%15\n\t"
+      "ds_read_u8 %3, %11 offset:%16\n\t"
+      "ds_read2st64_b32 %4, %10 offset0:0 offset1:1\n\t"
+      "ds_read2st64_b32 %5, %10 offset0:2 offset1:3\n\t"
+      "ds_read2st64_b32 %6, %10 offset0:4 offset1:5\n\t"
+      "ds_read2st64_b32 %7, %10 offset0:6 offset1:7\n\t"
+      "ds_read_b64 %8, %12 offset:%17\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(k0), "=&v"(k1), "=&v"(s0), "=&v"(s1), "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(vs)
+      : "v"(ka), "v"(va + VO), "v"(ksa), "v"(vsa), "i"(KO), "i"(KO + 1024), "i"(KSO), "i"(KSO + 4), "i"(VSO)
+      : "memory");
+}
+#define KA_READ_NARROW(NAME, KT, KOP, VOP, KSTEP, VSTEP)                                                             \
+  template <int KO, int VO, int KSO, int VSO>                                                                       \
+  TLM_DEV void NAME(KT& k0, KT& k1, uint32_t& s0, uint32_t& s1, uint32_t (&v)[8], u32x2& vs, uint32_t ka, uint32_t va, \
+                    uint32_t ksa, uint32_t vsa) {                                                                   \
+    asm volatile(KOP " %0, %13 offset:%17\n\t" KOP " %1, %13 offset:%18\n\t"                                         \
+                     "ds_read_u8 %2, %15 offset:%19\n\tds_read_u8 %3, %15 offset:%20\n\t" VOP                         \
+                     " %4, %14 offset:%22\n\t" VOP " %5, %14 offset:%23\n\t" VOP " %6, %14 offset:%24\n\t" VOP         \
+                     " %7, %14 offset:%25\n\t" VOP " %8, %14 offset:%26\n\t" VOP " %9, %14 offset:%27\n\t" VOP         \
+                     " %10, %14 offset:%28\n\t" VOP " %11, %14 offset:%29\n\t"                                       \
+                     "ds_read_b64 %12, %16 offset:%21\n\ts_waitcnt lgkmcnt(0)"                                       \
+                 : "=&v"(k0), "=&v"(k1), "=&v"(s0), "=&v"(s1), "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]),  \
+                   "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7]), "=&v"(vs)                                    \
+                 : "v"(ka), "v"(va), "v"(ksa), "v"(vsa), "i"(KO), "i"(KO + KSTEP), "i"(KSO), "i"(KSO + 4),          \
+                   "i"(VSO), "i"(VO), "i"(VO + VSTEP), "i"(VO + 2 * VSTEP), "i"(VO + 3 * VSTEP), "i"(VO + 4 * VSTEP), \
+                   "i"(VO + 5 * VSTEP), "i"(VO + 6 * VSTEP), "i"(VO + 7 * VSTEP)                                    \
+                 : "memory");                                                                                       \
+  }
+KA_READ_NARROW(ka_read64, u32x2, "ds_read_b64", "ds_read_u16", 512, 128)
+KA_READ_NARROW(ka_read32, uint32_t, "ds_read_b32", "ds_read_u8", 256, 64)
+#undef KA_READ_NARROW
 
 template <int SEL>
 TLM_DEV uint32_t ka_cvt(uint32_t w, float s) {
@@ -173,13 +230,17 @@ TLM_DEV void ka_split(float x, float y, uint32_t& hi, uint32_t& lo) {
   lo = h16<true>::pack(x - h16<true>::lo(hi), y - h16<true>::hi(hi));
 }
 
-template <int D, int QT, bool BF16>
-__global__ __launch_bounds__(64 * KA_W, (QT == 1 && D <= 128) ? 3 : QT == 1 ? 2 : 1) void kv4_attn_ranges(const KaArgs a) {
+template <int D, int QT, bool BF16, bool PG>
+__global__ __launch_bounds__(64 * KA_W, ka_per_cu(D, QT)) void kv4_attn_ranges(const KaArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   using S = Segs<D>;
   constexpr int MT = 16 * QT, NK = D / 32, ND = D / 16, QN = BF16 ? 1 : 2;
   constexpr int SO = D + 4;  // floats of a row of the exchange
-  __shared__ float so[KA_W][16][SO];
+  using St = Stage<D>;
+  constexpr int NST = ka_stages<D, QT>();
+  static_assert(KA_W * NST * St::BYTES >= KA_W * 16 * SO * (int)sizeof(float), "the exchange lies in the rings");
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[KA_W * NST * St::BYTES];
+  auto so = (float(*)[16][SO])smem;
   __shared__ float sm[KA_W][16], sl[KA_W][16];
   __shared__ int64_t sh[KA_W + 3];
   const Cache& c = a.c;
@@ -198,23 +259,65 @@ __global__ __launch_bounds__(64 * KA_W, (QT == 1 && D <= 128) ? 3 : QT == 1 ? 2 
     return r < ng ? lo : (int64_t)-1;
   });
   if (h == 0 && tid == 0) {
-    int64_t* m = a.meta + 4 * r;
-    m[0] = lo < hi ? start.b : -1;
-    m[1] = start.rt;
-    m[2] = start.before;
-    m[3] = start.total;
+    KaCut cut{-1, 0, 0, 0};
+    const int ng = (int)min((int64_t)a.G, start.total);
+    if (lo < hi && start.before < lo && ka_cut(start.total, ng, r - 1) <= start.before) {
+      const int units = ka_entry<MT>(a, ka_len(a, start.b), ka_new(a, start.b), start.rt).units;
+      const int64_t end = start.before + units + KA_PIECE;
+      int p1 = r;
+      for (int step = 1 << 10; step; step >>= 1)  // G <= 768
+        if (p1 + step < ng && ka_cut(start.total, ng, p1 + step) < end) p1 += step;
+      const int p0 = ka_unit_at(lo, start.before, units) > 0 ? r - 1 : r;
+      if (p1 > p0) cut = KaCut{start.b, start.rt, p0, p1};
+    }
+    a.cuts[r] = cut;
   }
   if (lo >= hi) return;  // whole workgroup
 
-  const int64_t k_head = (int64_t)h * c.page * (D / 2), v_head = (int64_t)(c.Hkv + h) * c.page * (D / 2);
-  const int64_t ks_head = (int64_t)h * c.page * NK, vs_head = (int64_t)(c.Hkv + h) * c.page * NK;
+  const int64_t k_head = (int64_t)h * c.page * (D / 2), ks_head = (int64_t)h * c.page * NK;
   const int kg = jl >> 2, kr = jl & 3;  // the lane's K rows: tokens 8 kg + kr and + 4; its V rows: 8 g .. + 7
+
+  // LDS-DMA: what the lane fetches with each instruction of a tile, from where the tile (PG: it lies in one page) or the
+  // slot's eight tokens (`grp` of them) begin
+  uint32_t off_c[St::NC], off_s[St::NS];
+  int grp_c[St::NC], grp_s[St::NS];
+#pragma unroll
+  for (int j = 0; j < St::NC; ++j) {
+    const bool is_v = 64 * j + lane >= D;
+    const int p = 64 * j + lane - (is_v ? D : 0);
+    int tok = 0, byte = 0;
+    unroll<0, S::N>([&](auto s) {
+      constexpr int W = S::w(s), B0 = S::base(s);
+      const int x = p - B0;
+      if (x < 0 || x >= 16 * W) return;
+      if (is_v) {
+        tok = 8 * (x / (W / 2) % 4) + x / (2 * W);
+        byte = B0 / 2 + 16 * (x % (W / 2));
+      } else {
+        const int m = x % 16, ax = x / 16;
+        tok = 8 * (m >> 2) + 4 * (ax / (W / 2)) + (m & 3);
+        byte = B0 / 2 + 16 * (ax % (W / 2));
+      }
+    });
+    grp_c[j] = tok >> 3;
+    off_c[j] = (uint32_t)((is_v ? c.Hkv * c.page * (D / 2) : 0) + (PG ? tok : tok & 7) * (D / 2) + byte);
+  }
+#pragma unroll
+  for (int j = 0; j < St::NS; ++j) {
+    const int x = 64 * j + lane < D / 2 ? 64 * j + lane : 0;  // lanes past the scales fetch the first word again
+    const int half = x / (8 * NK), blk = x / 8 % NK, w = x % 8;
+    grp_s[j] = w >> 1;
+    off_s[j] = (uint32_t)((half * c.Hkv * NK + blk) * c.page + (PG ? 4 * w : 4 * (w & 1)));
+  }
+  // LDS reads
+  const uint32_t ring = lds_u32(smem) + wave * (NST * St::BYTES);
+  const uint32_t k64 = 256 * (g >> 1) + 16 * jl + 8 * (g & 1), k32 = 16 * jl + 4 * g;
+  const uint32_t ks_l = 8 * kg + kr, vs_l = 8 * g;
 
   int64_t before = start.before;
   int rt = start.rt;
   for (int b = start.b; b < a.B && before < hi; ++b, rt = 0) {
     const int L = ka_len(a, b), n = ka_new(a, b), rts = ka_tiles<MT>(a, n);
-    const int32_t* table = c.table + (int64_t)b * c.max_pages;
     for (; rt < rts && before < hi; ++rt) {
       const KaEntry e = ka_entry<MT>(a, L, n, rt);
       const int64_t at = before;
@@ -236,7 +339,9 @@ __global__ __launch_bounds__(64 * KA_W, (QT == 1 && D <= 128) ? 3 : QT == 1 ? 2 
           constexpr int W = S::w(s), B0 = S::base(s);
 #pragma unroll
           for (int w = 0; w < W / 2; ++w) {
-            const u32x4 x = live ? *(const u32x4*)(p + B0 + 4 * W * g + 8 * w) : u32x4{0, 0, 0, 0};
+            u32x4 x = live ? *(const u32x4*)(p + B0 + 4 * W * g + 8 * w) : u32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int i2 = 0; i2 < 4; ++i2) x[i2] ^= a.q_sign;
             if constexpr (BF16) {
               q[0][t][B0 / 32 + w] = x;
             } else {
@@ -266,40 +371,93 @@ __global__ __launch_bounds__(64 * KA_W, (QT == 1 && D <= 128) ? 3 : QT == 1 ? 2 
 
       const int tend = min(e.keys, u1 * KA_UNIT);  // tokens from here on are not this piece's
       int t0 = u0 * KA_UNIT + wave * KA_BN;
-      auto page_of = [&](int tok) { return a.page_shift >= 0 ? tok >> a.page_shift : tok / c.page; };
-      auto pid_of = [&](int tok) {  // -1 where the token has no page
-        const int i = page_of(tok);
-        int p = -1;
-        if (tok < tend) p = table[i];
-        return p;
+      // the table is only read here: as constant memory its uniform reads are scalar
+      const auto* table = (const __attribute__((address_space(4))) int32_t*)(c.table + (int64_t)b * c.max_pages);
+      auto page_of = [&](int tok) { return (int)((uint64_t)(uint32_t)tok * a.page_mul >> a.page_shift); };
+      constexpr int NP = PG ? 1 : 4;  // pages of a tile: one, or one for each eight tokens
+      int pid[NP];
+      auto look_up = [&](int tk) {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          pid[i] = -1;
+          if (tk + 8 * i < tend) pid[i] = table[page_of(tk + 8 * i)];
+        }
       };
-      int pk = pid_of(t0 + 8 * kg), pv = pid_of(t0 + 8 * g);
-      auto load = [&](KaTile<D>& x, int tk) {
-        const int tok_k = tk + 8 * kg, tok_v = tk + 8 * g;
-        const int pk1 = pid_of(tok_k + KA_UNIT), pv1 = pid_of(tok_v + KA_UNIT);
-        const bool ok_k = pk >= 0 && pk < c.pages, ok_v = pv >= 0 && pv < c.pages;
-        const int off_k = tok_k - page_of(tok_k) * c.page + kr, off_v = tok_v - page_of(tok_v) * c.page;
-        const uint8_t* z = (const uint8_t*)ka_zeros;
-        const uint8_t* ka = ok_k ? c.codes + pk * c.codes_page + k_head + (int64_t)off_k * (D / 2) : z;
-        const uint8_t* ksa = ok_k ? c.scales + pk * c.scales_page + ks_head + off_k : z;
-        const uint8_t* va = ok_v ? c.codes + pv * c.codes_page + v_head + (int64_t)off_v * (D / 2) : z;
-        const uint8_t* vsa = ok_v ? c.scales + pv * c.scales_page + vs_head + off_v : z;
-        const int64_t kst = ok_k ? c.page : 0, vst = ok_v ? c.page : 0;
+      int at_issue = 0, at_read = 0;  // byte offsets of stages
+      auto issue = [&](int tk) {      // the tile whose pages were looked up last; then looks up the next
+        uint8_t* const dst = smem + wave * (NST * St::BYTES) + at_issue;
+        at_issue = at_issue + St::BYTES == NST * St::BYTES ? 0 : at_issue + St::BYTES;
+        auto lds = [&](int off) { return (__attribute__((address_space(3))) void*)(dst + off); };
+        if constexpr (PG) {
+          const bool ok = pid[0] >= 0 && pid[0] < c.pages;  // otherwise a buffer of no bytes: zeros
+          const int64_t p0 = ok ? pid[0] : 0, off = ok ? tk - page_of(tk) * c.page : 0;
+          const __amdgpu_buffer_rsrc_t rc = __builtin_amdgcn_make_buffer_rsrc(
+              (void*)(c.codes + p0 * c.codes_page + k_head + off * (D / 2)), (short)0, ok ? 0x7fffffff : 0, 0x00020000);
+          const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+              (void*)(c.scales + p0 * c.scales_page + ks_head + off), (short)0, ok ? 0x7fffffff : 0, 0x00020000);
+#pragma unroll
+          for (int j = 0; j < St::NC; ++j)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rc, lds(1024 * j), 16, (int)off_c[j], 0, 0, 0);
+#pragma unroll
+          for (int j = 0; j < St::NS; ++j)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, lds(St::CODES + 256 * j), 4, (int)off_s[j], 0, 0, 0);
+        } else {
+          const uint8_t *bc[4], *bs[4];
+          bool ok[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int p = pid[i % NP], tok = tk + 8 * i;
+            ok[i] = p >= 0 && p < c.pages;
+            const int64_t off = tok - page_of(tok) * c.page;
+            bc[i] = c.codes + p * c.codes_page + k_head + off * (D / 2);
+            bs[i] = c.scales + p * c.scales_page + ks_head + off;
+          }
+          auto from = [&](const uint8_t* const (&base)[4], int i, uint32_t off) {
+            const uint8_t* b = i == 0 ? base[0] : i == 1 ? base[1] : i == 2 ? base[2] : base[3];
+            const bool o = i == 0 ? ok[0] : i == 1 ? ok[1] : i == 2 ? ok[2] : ok[3];
+            return (const __attribute__((address_space(1))) void*)(o ? b + off : (const uint8_t*)ka_zeros);
+          };
+#pragma unroll
+          for (int j = 0; j < St::NC; ++j)
+            __builtin_amdgcn_global_load_lds(from(bc, grp_c[j], off_c[j]), lds(1024 * j), 16, 0, 0);
+#pragma unroll
+          for (int j = 0; j < St::NS; ++j)
+            __builtin_amdgcn_global_load_lds(from(bs, grp_s[j], off_s[j]), lds(St::CODES + 256 * j), 4, 0, 0);
+        }
+        look_up(tk + KA_UNIT);
+      };
+      auto read = [&](KaTile<D>& x) {
+        const uint32_t st = ring + at_read;
+        at_read = at_read + St::BYTES == NST * St::BYTES ? 0 : at_read + St::BYTES;
         unroll<0, S::N>([&](auto s) {
           constexpr int W = S::w(s), B0 = S::base(s);
+          constexpr int KO = 16 * B0, VO = 16 * (D + B0), KSO = St::CODES + B0, VSO = St::CODES + D + B0;
+          if constexpr (W == 8) {
+            u32x4 k0, k1;
+            u32x2 v[4];
+            ka_read128<KO, VO, KSO, VSO>(k0, k1, x.ks[0][s], x.ks[1][s], v, x.vs[s], st + 16 * lane, st + 4 * lane,
+                                         st + ks_l + 32 * g, st + vs_l + 32 * (jl >> 2));
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            ka_load<2 * W>(&x.k[i][B0 / 32], ka + i * 4 * (D / 2) + B0 / 2 + 2 * W * g);
-            x.ks[i][s] = ksa[(B0 / 32 + 4 * W * g / 32) * kst + 4 * i];
+            for (int i = 0; i < 4; ++i) {
+              x.k[0][B0 / 32 + i] = k0[i], x.k[1][B0 / 32 + i] = k1[i];
+              x.v[2 * i][s] = v[i][0], x.v[2 * i + 1][s] = v[i][1];
+            }
+          } else {
+            uint32_t v[8];
+            if constexpr (W == 4) {
+              u32x2 k0, k1;
+              ka_read64<KO, VO, KSO, VSO>(k0, k1, x.ks[0][s], x.ks[1][s], v, x.vs[s], st + k64, st + 2 * lane,
+                                          st + ks_l + 32 * (g >> 1), st + vs_l + 32 * (jl >> 3));
+#pragma unroll
+              for (int i = 0; i < 2; ++i) x.k[0][B0 / 32 + i] = k0[i], x.k[1][B0 / 32 + i] = k1[i];
+            } else {
+              ka_read32<KO, VO, KSO, VSO>(x.k[0][B0 / 32], x.k[1][B0 / 32], x.ks[0][s], x.ks[1][s], v, x.vs[s], st + k32,
+                                          st + lane, st + ks_l, st + vs_l);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x.v[i][s] = v[i];
           }
         });
-        unroll<0, S::N>([&](auto s) {
-          constexpr int W = S::w(s), B0 = S::base(s);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) ka_load<W / 2>(&x.v[i][s], va + i * (D / 2) + B0 / 2 + jl * W / 2);
-          x.vs[s] = *(const u32x2*)(vsa + (B0 / 32 + W * jl / 32) * vst);
-        });
-        pk = pk1, pv = pv1;
       };
 
       auto compute = [&](KaTile<D>& x, int tk, auto edge) {
@@ -329,10 +487,11 @@ __global__ __launch_bounds__(64 * KA_W, (QT == 1 && D <= 128) ? 3 : QT == 1 ? 2 
           float y[8], top = -INFINITY;
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            y[i] = sc[t][i >> 2][i & 3] * a.scale2;
-            if constexpr (EDGE) y[i] = tk + 8 * g + i < lim[t] ? y[i] : -INFINITY;
+            y[i] = sc[t][i >> 2][i & 3];
+            if constexpr (EDGE) y[i] = tk + 8 * g + i < lim[t] ? y[i] * a.scale2 : -INFINITY;
             top = fmaxf(top, y[i]);
           }
+          if constexpr (!EDGE) top *= a.scale2;
           if (__any(top > thr[t])) {
             top = xhalf_max(xrow_max(top));  // over the four lanes of the column
             const bool up = top > thr[t];
@@ -344,7 +503,7 @@ __global__ __launch_bounds__(64 * KA_W, (QT == 1 && D <= 128) ? 3 : QT == 1 ? 2 
             for (int i = 0; i < ND; ++i) o[t][i] *= f;
           }
 #pragma unroll
-          for (int i = 0; i < 8; ++i) y[i] = fast_exp2(y[i] - ref[t]);
+          for (int i = 0; i < 8; ++i) y[i] = fast_exp2(EDGE ? y[i] - ref[t] : fmaf(y[i], a.scale2, -ref[t]));
           l[t] += ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -415,21 +574,28 @@ __global__ __launch_bounds__(64 * KA_W, (QT == 1 && D <= 128) ? 3 : QT == 1 ? 2 
       };
 
       if (t0 < tend) {
-        KaTile<D> x, y;
-        load(x, t0);
-        // both tiles of a step are seen whole by every row
-        for (; t0 + KA_UNIT + KA_BN <= min(tend, e.keys_min); t0 += 2 * KA_UNIT) {
-          load(y, t0 + KA_UNIT);
+        KaTile<D> x;
+        look_up(t0);
+        int ti = t0;
+#pragma unroll
+        for (int i = 0; i < NST - 1; ++i, ti += KA_UNIT) issue(ti);
+        auto next = [&] {
+          issue(ti);
+          ti += KA_UNIT;
+          vm_wait<(NST - 1) * St::PER>();
+          read(x);
+        };
+        for (; t0 + KA_BN <= min(tend, e.keys_min); t0 += KA_UNIT) {  // seen whole by every row
+          next();
           compute(x, t0, std::false_type{});
-          load(x, t0 + 2 * KA_UNIT);
-          compute(y, t0 + KA_UNIT, std::false_type{});
         }
         for (; t0 < tend; t0 += KA_UNIT) {
-          load(y, t0 + KA_UNIT);
+          next();
           compute(x, t0, std::true_type{});
-          x = y;
         }
       }
+      vm_wait<0>();  // nothing may land in the exchange
+      __syncthreads();
 
       // the waves' rows meet: 16 at a time
       const bool whole = u0 == 0 && u1 == e.units;
@@ -488,57 +654,62 @@ __global__ __launch_bounds__(64 * KA_W, (QT == 1 && D <= 128) ? 3 : QT == 1 ? 2 
 #endif
 }
 
-// Entries that a cut between two ranges went through: one workgroup per cut, K/V head and 16 rows; the first cut of
-// an entry does the work.
-template <int D, int QT, bool BF16>
+// Entries that lie in several ranges: one workgroup per entry's first cut, K/V head and 4 / WPR rows, WPR waves for
+// a row. Lanes hold 4 dims each and share the pieces; all of a lane's pieces are requested before they are used.
+template <int D, int QT, bool BF16, int WPR>
 __global__ __launch_bounds__(256) void kv4_attn_join(const KaArgs a) {
-  constexpr int MT = 16 * QT;
-  const int h = blockIdx.y, t = blockIdx.z;
-  const int r = blockIdx.x + 1;
-  const int64_t* m = a.meta + 4 * r;
-  const int b = (int)m[0], rt = (int)m[1];
-  if (b < 0) return;
-  const int64_t at = m[2], total = m[3];
-  const int ng = (int)min((int64_t)a.G, total);
-  if (ka_cut(total, ng, r) <= at || ka_cut(total, ng, r - 1) > at) return;
-  const int L = ka_len(a, b), n = ka_new(a, b);
-  const KaEntry e = ka_entry<MT>(a, L, n, rt);
-  const int64_t end = at + e.units + KA_PIECE;
-  for (int x = threadIdx.x; x < 16 * (D / 4); x += 256) {
-    const int row = x / (D / 4), d = 4 * (x - row * (D / 4));
-    const int i = 16 * t + row;
-    if (i >= e.rows) continue;
-    float top = -INFINITY, sum = 0.f;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    int pieces = 0;
-    for (int p = r - 1; p < ng; ++p) {
-      const int64_t lo = ka_cut(total, ng, p), hi = ka_cut(total, ng, p + 1);
-      if (lo >= end) break;
-      const int u0 = ka_unit_at(lo, at, e.units), u1 = ka_unit_at(hi, at, e.units);
-      if (u0 >= u1) continue;
-      if (u0 == 0 && u1 == e.units) {  // one range had it all
-        pieces = 0;
-        break;
-      }
-      ++pieces;
-      const float* slot = a.part + ((int64_t)(u0 == 0 ? 2 * p + 1 : 2 * p) * a.c.Hkv + h) * (MT * (D + 2));
-      const float pm = slot[MT * D + i], ps = slot[MT * D + MT + i];
-      const f32x4 po = *(const f32x4*)(slot + i * D + d);
-      if (pm == -INFINITY) continue;
-      const float next = fmaxf(top, pm);
-      const float f = top == -INFINITY ? 0.f : fast_exp2(top - next), fp = fast_exp2(pm - next);
-      sum = sum * f + ps * fp;
-      acc = acc * f + po * fp;
-      top = next;
-    }
-    if (pieces == 0) return;
-    const int qrow = e.row0 + i, j = qrow / a.group;
-    const int64_t at_o = ((int64_t)b * a.T + j) * a.H + h * a.group + (qrow - j * a.group);
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    *(u32x2*)(a.o + at_o * D + d) = u32x2{h16<BF16>::pack(acc[0] * inv, acc[1] * inv),
-                                          h16<BF16>::pack(acc[2] * inv, acc[3] * inv)};
-    if (a.lse && d == 0) a.lse[at_o] = sum == 0.f ? -INFINITY : top + __log2f(sum);
+  constexpr int MT = 16 * QT, LPG = D / 4, GPW = 64 / LPG;
+  __shared__ f32x4 acc_s[4][64];
+  const int h = blockIdx.y, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int i = blockIdx.z * (4 / WPR) + wave / WPR;  // row of the entry
+  const KaCut cut = a.cuts[blockIdx.x + 1];
+  if (cut.b < 0) return;
+  const KaEntry e = ka_entry<MT>(a, ka_len(a, cut.b), ka_new(a, cut.b), cut.rt);
+  const bool live = i < e.rows;
+  const int np = live ? cut.p1 - cut.p0 + 1 : 0;
+  auto slot = [&](int p) {  // of piece p: the first lies at its range's end, the others at the start
+    return a.part + ((int64_t)(2 * (cut.p0 + p) + (p == 0)) * a.c.Hkv + h) * (MT * (D + 2));
+  };
+  float top = -INFINITY;
+  for (int p = lane; p < np; p += 64) top = fmaxf(top, slot(p)[MT * D + i]);
+  top = wave_max(top);
+  auto weight = [&](float m) { return m == -INFINITY ? 0.f : fast_exp2(m - top); };
+  float sum = 0.f;
+  for (int p = lane; p < np; p += 64) {
+    const float* s = slot(p) + MT * D + i;
+    sum += weight(s[0]) * s[MT];
   }
+  sum = wave_sum(sum);
+  const int grp = lane / LPG, d = 4 * (lane - grp * LPG);
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  constexpr int STEP = GPW * WPR;
+  for (int p = wave % WPR * GPW + grp; grp < GPW && p < np; p += 4 * STEP) {
+    f32x4 o[4];
+    float m[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float* s = slot(min(p + u * STEP, np - 1));
+      o[u] = *(const f32x4*)(s + i * D + d);
+      m[u] = p + u * STEP < np ? s[MT * D + i] : -INFINITY;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (p + u * STEP < np) acc += weight(m[u]) * o[u];
+  }
+  acc_s[wave][lane] = acc;
+  __syncthreads();
+  if (!live || wave % WPR != 0 || lane >= LPG) return;
+  acc = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int w = 0; w < WPR; ++w)
+#pragma unroll
+    for (int u = 0; u < GPW; ++u) acc += acc_s[wave + w][u * LPG + lane];
+  const int qrow = e.row0 + i, j = qrow / a.group;
+  const int64_t at_o = ((int64_t)cut.b * a.T + j) * a.H + h * a.group + (qrow - j * a.group);
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  *(u32x2*)(a.o + at_o * D + d) = u32x2{h16<BF16>::pack(acc[0] * inv, acc[1] * inv),
+                                        h16<BF16>::pack(acc[2] * inv, acc[3] * inv)};
+  if (a.lse && lane == 0) a.lse[at_o] = sum == 0.f ? -INFINITY : top + __log2f(sum);
 }
 
 constexpr int KA_CUS = 256;
@@ -550,18 +721,28 @@ struct KaPlan {
 KaPlan ka_plan(int64_t rows, int64_t Hkv, int64_t D) {
   KaPlan p;
   p.qt = rows <= 16 ? 1 : 2;
-  const int per_cu = p.qt == 1 ? (D <= 128 ? 3 : 2) : 1;
+  const int per_cu = ka_per_cu((int)D, p.qt);
   p.G = (int)std::max<int64_t>(1, KA_CUS * per_cu / Hkv);
-  p.meta = (size_t)p.G * 4 * sizeof(int64_t);
+  p.meta = (size_t)p.G * sizeof(KaCut);
   p.part = (size_t)2 * p.G * Hkv * 16 * p.qt * (D + 2) * sizeof(float);
   return p;
 }
 
 template <int D, int QT, bool BF16>
 void ka_launch(const KaArgs& a, hipStream_t st) {
-  kv4_attn_ranges<D, QT, BF16><<<(unsigned)(a.G * a.c.Hkv), 64 * KA_W, 0, st>>>(a);
-  if (a.G > 1)
-    kv4_attn_join<D, QT, BF16><<<dim3((unsigned)(a.G - 1), (unsigned)a.c.Hkv, QT), 256, 0, st>>>(a);
+  const dim3 grid((unsigned)(a.G * a.c.Hkv));
+  if (a.c.page % KA_BN == 0)
+    kv4_attn_ranges<D, QT, BF16, true><<<grid, 64 * KA_W, 0, st>>>(a);
+  else
+    kv4_attn_ranges<D, QT, BF16, false><<<grid, 64 * KA_W, 0, st>>>(a);
+  if (a.G == 1) return;
+  // pieces per entry, on average: with many, four waves share a row
+  const int rows = (int)std::min<int64_t>(16 * QT, (int64_t)a.T * a.group);
+  const int64_t entries = (int64_t)a.B * (((int64_t)a.T * a.group + 16 * QT - 1) / (16 * QT));
+  if (a.G >= 8 * entries)
+    kv4_attn_join<D, QT, BF16, 4><<<dim3(a.G - 1, a.c.Hkv, rows), 256, 0, st>>>(a);
+  else
+    kv4_attn_join<D, QT, BF16, 1><<<dim3(a.G - 1, a.c.Hkv, (rows + 3) / 4), 256, 0, st>>>(a);
 }
 template <int D>
 void ka_go(const KaArgs& a, int qt, bool bf, hipStream_t st) {
@@ -621,9 +802,13 @@ extern "C" int tlm_kv4_attn(const void* q, int64_t q_batch_stride, int64_t q_row
   }
   c.max_pages = (int)max_pages, c.page = (int)page, c.Hkv = (int)H_kv, c.D = (int)D;
   KaArgs a{c, (const uint16_t*)q, q_batch_stride, q_row_stride, seqlens, count, (uint16_t*)o, lse,
-           (int64_t*)ws, (float*)((char*)ws + p.meta), (int)B, (int)T, (int)H, (int)(H / H_kv), causal != 0, p.G,
-           (page & (page - 1)) == 0 ? __builtin_ctzll((unsigned long long)page) : -1,
-           sm_scale * 1.4426950408889634f};
+           (KaCut*)ws, (float*)((char*)ws + p.meta), (int)B, (int)T, (int)H, (int)(H / H_kv), causal != 0, p.G, 0, 0,
+           fabsf(sm_scale) * 1.4426950408889634f, sm_scale < 0.f ? 0x80008000u : 0u};
+  // with 2^(k-1) < page <= 2^k and m = floor(2^(31+k) / page) + 1: m page - 2^(31+k) <= 2^k, so that tok m / 2^(31+k) is
+  // less than 1 / page above tok / page for tok < 2^31; and m fits 32 bits
+  while ((1ll << a.page_shift) < page) ++a.page_shift;
+  a.page_shift += 31;
+  a.page_mul = (uint32_t)((1ull << a.page_shift) / (uint64_t)page + 1);
   hipStream_t st = (hipStream_t)stream;
   const bool bf = dtype == TLM_BF16;
   switch (D) {
