@@ -17,7 +17,7 @@ namespace {
 
 using kv4::Cache;
 constexpr int K4_T = 256;
-constexpr int K4_GRID = 8192;  // workgroups per launch at most
+constexpr int K4_GRID = 1 << 16;  // workgroups along the tokens at most; they go on from there
 
 typedef __bf16 b2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
@@ -41,107 +41,155 @@ TLM_DEV bool place(const Cache& c, int b, int64_t p, int64_t& pid, int& off) {
   return pid >= 0 && pid < c.pages;
 }
 
-// Four lanes per block of 32 dims, 8 dims each.
+// A workgroup takes K4_T / (D / 8) tokens, 8 dims of a head per thread, and walks through its share of the 2 H_kv
+// heads of K and V, U of them in flight: tokens next to each other make whole lines of codes, a head's D / 8 threads
+// whole lines of rows.
+constexpr int K4_U = 4;
+struct Lane {
+  int d8, tok;  // 8 dims, token of the workgroup
+  bool live;
+};
+TLM_DEV Lane lane_of(int D) {
+  const int per = D / 8, tok = (int)threadIdx.x / per;
+  return Lane{(int)threadIdx.x - tok * per, tok, tok < K4_T / per};
+}
+
 template <bool BF16>
 __global__ __launch_bounds__(K4_T) void kv4_append_kernel(Cache c, const uint16_t* k, const uint16_t* v,
                                                           int64_t kb, int64_t kr, int64_t vb, int64_t vr,
                                                           const int32_t* start, const int32_t* count, int B,
-                                                          int T) {
-  const int per_row = c.Hkv * (c.D / 8);  // chunks of a row of k or v
-  const int64_t chunks = 2 * (int64_t)per_row;
-  for (int b = blockIdx.y; b < B; b += gridDim.y) {
-    const int n = min(count[b], T);
-    const int64_t first = start[b], all = chunks * n;
-    for (int64_t i = (int64_t)blockIdx.x * K4_T + threadIdx.x; i < all; i += (int64_t)gridDim.x * K4_T) {
-      const int j = (int)(i / chunks);
-      int ch = (int)(i - j * chunks);
-      const int w = ch >= per_row;
-      ch -= w * per_row;
-      const int h = ch / (c.D / 8), d8 = ch - h * (c.D / 8);
+                                                          int T, int heads) {
+  const Lane t = lane_of(c.D);
+  const int h0 = blockIdx.y * heads, h1 = min(2 * c.Hkv, h0 + heads);
+  const int tokens = K4_T / (c.D / 8);
+  for (int b = blockIdx.z; b < B; b += gridDim.z) {
+    const int n = t.live ? min(count[b], T) : 0;
+    for (int64_t j = (int64_t)blockIdx.x * tokens + t.tok; j < n; j += (int64_t)gridDim.x * tokens) {
       int64_t pid;
       int off;
-      if (!place(c, b, first + j, pid, off)) continue;  // the four lanes of a block together
-      const uint16_t* src = (w ? v + b * vb + j * vr : k + b * kb + j * kr) + 8 * ch;
-      const u32x4 x = *(const u32x4*)src;
-      uint32_t m = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        m = max(m, max(x[e] & 0x7fffu, (x[e] >> 16) & 0x7fffu));
-      m = max(m, (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0xB1, 0xf, 0xf, false));  // lane ^ 1
-      m = max(m, (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0x4E, 0xf, 0xf, false));  // lane ^ 2
-      const uint32_t f = __float_as_uint(h16<BF16>::to_f32(m));
-      int byte = (int)(f >> 23) - 2 + ((f & 0x7fffffu) > 0x600000u);
-      byte = max(1, min(252, byte));
-      uint32_t code = 0;
-      if (f > 0x7f800000u) {
-        byte = 255;  // NaN
-      } else {
-        const float s = kv4::scale_of(byte);
-        const std::bool_constant<BF16> tag;
-        code = to_fp4<0>(code, x[0], s, tag);
-        code = to_fp4<1>(code, x[1], s, tag);
-        code = to_fp4<2>(code, x[2], s, tag);
-        code = to_fp4<3>(code, x[3], s, tag);
+      if (!place(c, b, start[b] + j, pid, off)) continue;
+      const uint16_t* const ks = k + b * kb + j * kr + 8 * t.d8;
+      const uint16_t* const vs = v + b * vb + j * vr + 8 * t.d8;
+      uint8_t* const codes = c.codes + pid * c.codes_page + (int64_t)off * (c.D / 2) + 4 * t.d8;
+      uint8_t* const scales = c.scales + pid * c.scales_page + (int64_t)(t.d8 / 4) * c.page + off;
+      for (int h = h0; h < h1; h += K4_U) {
+        u32x4 x[K4_U];
+  #pragma unroll
+        for (int u = 0; u < K4_U; ++u) {
+          const int hu = min(h + u, h1 - 1);
+          x[u] = ld_nt((const u32x4*)(hu < c.Hkv ? ks + (int64_t)hu * c.D : vs + (int64_t)(hu - c.Hkv) * c.D));
+        }
+  #pragma unroll
+        for (int u = 0; u < K4_U; ++u) {
+          if (h + u >= h1) break;
+          uint32_t m = 0;
+  #pragma unroll
+          for (int e = 0; e < 4; ++e) m = max(m, max(x[u][e] & 0x7fffu, (x[u][e] >> 16) & 0x7fffu));
+          m = max(m, (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0xB1, 0xf, 0xf, false));  // lane ^ 1
+          m = max(m, (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0x4E, 0xf, 0xf, false));  // lane ^ 2
+          const uint32_t f = __float_as_uint(h16<BF16>::to_f32(m));
+          int byte = (int)(f >> 23) - 2 + ((f & 0x7fffffu) > 0x600000u);
+          byte = max(1, min(252, byte));
+          uint32_t code = 0;
+          if (f > 0x7f800000u) {
+            byte = 255;  // NaN
+          } else {
+            const float s = kv4::scale_of(byte);
+            const std::bool_constant<BF16> tag;
+            code = to_fp4<0>(code, x[u][0], s, tag);
+            code = to_fp4<1>(code, x[u][1], s, tag);
+            code = to_fp4<2>(code, x[u][2], s, tag);
+            code = to_fp4<3>(code, x[u][3], s, tag);
+          }
+          *(uint32_t*)(codes + (int64_t)(h + u) * c.page * (c.D / 2)) = code;
+          if ((t.d8 & 3) == 0) scales[(int64_t)(h + u) * (c.D / kv4::BLOCK) * c.page] = (uint8_t)byte;
+        }
       }
-      const int64_t at = (int64_t)w * c.Hkv + h;
-      *(uint32_t*)(c.codes + pid * c.codes_page + (at * c.page + off) * (c.D / 2) + 4 * d8) = code;
-      if ((d8 & 3) == 0)
-        c.scales[pid * c.scales_page + (at * (c.D / kv4::BLOCK) + d8 / 4) * c.page + off] = (uint8_t)byte;
     }
   }
 }
 
-// 8 dims per thread. OUT: 0 fp16, 1 bf16, 2 fp32.
+// OUT: 0 fp16, 1 bf16, 2 fp32.
+template <int OUT>
+TLM_DEV void put8(uint8_t* dst, uint32_t code, float s) {
+  if constexpr (OUT == 1) {
+    st_nt((u32x4*)dst, u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, s, 0)),
+                             __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, s, 1)),
+                             __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, s, 2)),
+                             __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, s, 3))});
+  } else {
+    const f2 a[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, s, 0),
+                     __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, s, 1),
+                     __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, s, 2),
+                     __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, s, 3)};
+    if constexpr (OUT == 2) {
+      const f32x4 x = {a[0][0], a[0][1], a[1][0], a[1][1]}, y = {a[2][0], a[2][1], a[3][0], a[3][1]};
+      st_nt((u32x4*)dst, __builtin_bit_cast(u32x4, x));
+      st_nt((u32x4*)dst + 1, __builtin_bit_cast(u32x4, y));
+    } else {
+      using H = h16<false>;
+      st_nt((u32x4*)dst, u32x4{H::pack(a[0][0], a[0][1]), H::pack(a[1][0], a[1][1]), H::pack(a[2][0], a[2][1]),
+                               H::pack(a[3][0], a[3][1])});
+    }
+  }
+}
+
+constexpr int K4_CU = 1024;  // sequence starts that are searched in LDS
+
 template <int OUT>
 __global__ __launch_bounds__(K4_T) void kv4_read_kernel(Cache c, const int32_t* start, const int32_t* cu,
-                                                        uint8_t* k_out, uint8_t* v_out, int B, int64_t total) {
+                                                        uint8_t* k_out, uint8_t* v_out, int B, int64_t total,
+                                                        int heads) {
   constexpr int ES = OUT == 2 ? 4 : 2;
-  const int per_row = c.Hkv * (c.D / 8);
-  const int64_t chunks = 2 * (int64_t)per_row, all = chunks * total;
-  for (int64_t i = (int64_t)blockIdx.x * K4_T + threadIdx.x; i < all; i += (int64_t)gridDim.x * K4_T) {
-    const int64_t r = i / chunks;
-    int ch = (int)(i - r * chunks);
-    const int w = ch >= per_row;
-    ch -= w * per_row;
-    const int h = ch / (c.D / 8), d8 = ch - h * (c.D / 8);
-    int lo = 0, hi = B + 1;  // the last cu <= r
+  __shared__ int32_t cu_s[K4_CU];
+  if (B < K4_CU) {
+    for (int i = threadIdx.x; i <= B; i += K4_T) cu_s[i] = cu[i];
+    __syncthreads();
+  }
+  const Lane t = lane_of(c.D);
+  const int h0 = blockIdx.y * heads, h1 = min(2 * c.Hkv, h0 + heads);
+  const int tokens = K4_T / (c.D / 8);
+  for (int64_t r = (int64_t)blockIdx.x * tokens + t.tok; t.live && r < total; r += (int64_t)gridDim.x * tokens) {
+    int lo = 0, hi = B + 1;  // cu[lo - 1] <= r < cu[hi]
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
-      if (cu[mid] <= r) lo = mid + 1;
+      if ((B < K4_CU ? cu_s[mid] : cu[mid]) <= r) lo = mid + 1;
       else hi = mid;
     }
     const int b = lo - 1;
     if (b < 0 || b >= B) continue;  // a row of no sequence
     int64_t pid;
     int off;
-    uint32_t code = 0, byte = 127;
-    if (place(c, b, (start ? (int64_t)start[b] : 0) + (r - cu[b]), pid, off)) {
-      const int64_t at = (int64_t)w * c.Hkv + h;
-      code = *(const uint32_t*)(c.codes + pid * c.codes_page + (at * c.page + off) * (c.D / 2) + 4 * d8);
-      byte = c.scales[pid * c.scales_page + (at * (c.D / kv4::BLOCK) + d8 / 4) * c.page + off];
-    }
-    const float s = kv4::scale_of(byte);
-    uint8_t* dst = (w ? v_out : k_out) + (r * per_row + ch) * 8 * ES;
-    if constexpr (OUT == 1) {
-      *(u32x4*)dst = u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, s, 0)),
-                           __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, s, 1)),
-                           __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, s, 2)),
-                           __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, s, 3))};
-    } else {
-      const f2 a[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, s, 0),
-                       __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, s, 1),
-                       __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, s, 2),
-                       __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, s, 3)};
-      if constexpr (OUT == 2) {
-        *(f32x4*)dst = f32x4{a[0][0], a[0][1], a[1][0], a[1][1]};
-        *(f32x4*)(dst + 16) = f32x4{a[2][0], a[2][1], a[3][0], a[3][1]};
-      } else {
-        using H = h16<false>;
-        *(u32x4*)dst = u32x4{H::pack(a[0][0], a[0][1]), H::pack(a[1][0], a[1][1]), H::pack(a[2][0], a[2][1]),
-                             H::pack(a[3][0], a[3][1])};
+    const bool ok = place(c, b, (start ? (int64_t)start[b] : 0) + (r - (B < K4_CU ? cu_s[b] : cu[b])), pid, off);
+    if (!ok) pid = off = 0;
+    const uint8_t* const codes = c.codes + pid * c.codes_page + (int64_t)off * (c.D / 2) + 4 * t.d8;
+    const uint8_t* const scales = c.scales + pid * c.scales_page + (int64_t)(t.d8 / 4) * c.page + off;
+    const int64_t row = (r * c.Hkv * c.D + 8 * t.d8) * ES;
+    for (int h = h0; h < h1; h += K4_U) {
+      uint32_t code[K4_U], byte[K4_U];
+  #pragma unroll
+      for (int u = 0; u < K4_U; ++u) {
+        const int hu = min(h + u, h1 - 1);
+        code[u] = *(const uint32_t*)(codes + (int64_t)hu * c.page * (c.D / 2));
+        byte[u] = scales[(int64_t)hu * (c.D / kv4::BLOCK) * c.page];
+        if (!ok) code[u] = 0, byte[u] = 127;
+      }
+  #pragma unroll
+      for (int u = 0; u < K4_U; ++u) {
+        const int hu = h + u;
+        if (hu >= h1) break;
+        put8<OUT>((hu < c.Hkv ? k_out + row + (int64_t)hu * c.D * ES : v_out + row + (int64_t)(hu - c.Hkv) * c.D * ES),
+                  code[u], kv4::scale_of(byte[u]));
       }
     }
   }
+}
+
+// Heads (of 2 H_kv) per workgroup: all of them, or fewer where `wgs` workgroups would not fill the CUs.
+inline int heads_per_wg(int64_t wgs, int64_t Hkv) {
+  int64_t heads = 2 * Hkv;
+  while (heads > K4_U && wgs * ((2 * Hkv + heads - 1) / heads) < 16384) heads = (heads + 1) / 2;
+  return (int)heads;
 }
 
 }  // namespace
@@ -166,14 +214,14 @@ extern "C" int tlm_kv4_append(const void* k, const void* v, int64_t k_batch_stri
   }
   if (B == 0 || T == 0) return TLM_OK;
   c.max_pages = (int)max_pages, c.page = (int)page, c.Hkv = (int)H_kv, c.D = (int)D;
-  const int64_t chunks = 2 * H_kv * (D / 8) * T;
-  const int64_t gy = std::min<int64_t>(B, 4096);
-  const int64_t gx = std::min<int64_t>((chunks + K4_T - 1) / K4_T, std::max<int64_t>(1, K4_GRID / gy));
-  const dim3 grid((unsigned)gx, (unsigned)gy);
+  const int64_t per = K4_T / (D / 8), gx = std::min<int64_t>((T + per - 1) / per, K4_GRID);
+  const int64_t gz = std::min<int64_t>(B, 65535);
+  const int heads = heads_per_wg(gx * gz, H_kv);
+  const dim3 grid((unsigned)gx, (unsigned)((2 * H_kv + heads - 1) / heads), (unsigned)gz);
   auto go = [&](auto kern) {
     kern<<<grid, K4_T, 0, (hipStream_t)stream>>>(c, (const uint16_t*)k, (const uint16_t*)v, k_batch_stride,
                                                  k_row_stride, v_batch_stride, v_row_stride, start, count,
-                                                 (int)B, (int)T);
+                                                 (int)B, (int)T, heads);
   };
   if (x_dtype == TLM_BF16) go(kv4_append_kernel<true>);
   else go(kv4_append_kernel<false>);
@@ -206,11 +254,12 @@ extern "C" int tlm_kv4_read(const void* codes, int64_t codes_page_stride, const 
   }
   if (B == 0 || total == 0) return TLM_OK;
   c.max_pages = (int)max_pages, c.page = (int)page, c.Hkv = (int)H_kv, c.D = (int)D;
-  const int64_t chunks = 2 * H_kv * (D / 8) * total;
-  const unsigned grid = (unsigned)std::min<int64_t>((chunks + K4_T - 1) / K4_T, K4_GRID);
+  const int64_t per = K4_T / (D / 8), gx = std::min<int64_t>((total + per - 1) / per, K4_GRID);
+  const int heads = heads_per_wg(gx, H_kv);
+  const dim3 grid((unsigned)gx, (unsigned)((2 * H_kv + heads - 1) / heads));
   auto go = [&](auto kern) {
     kern<<<grid, K4_T, 0, (hipStream_t)stream>>>(c, start, cu_seqlens, (uint8_t*)k_out, (uint8_t*)v_out,
-                                                 (int)B, total);
+                                                 (int)B, total, heads);
   };
   if (out_dtype == TLM_BF16) go(kv4_read_kernel<1>);
   else if (out_dtype == TLM_F16) go(kv4_read_kernel<0>);

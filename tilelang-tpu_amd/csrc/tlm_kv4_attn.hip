@@ -37,6 +37,7 @@ struct KaArgs {
   KaCut* cuts;  // [G]: the entry that the cut before range r goes through, if it is the entry's first
   float* part;  // [2 G][Hkv][16 QT][D + 2]: rows, their references, their sums
   int B, T, H, group, causal, G;
+  int once;           // codes are read by one row tile only: past the caches
   uint32_t page_mul;  // tok / page = tok page_mul >> page_shift, for tok < 2^31
   int page_shift;
   float scale2;     // |sm_scale| log2(e)
@@ -395,9 +396,15 @@ __global__ __launch_bounds__(64 * KA_W, ka_per_cu(D, QT)) void kv4_attn_ranges(c
               (void*)(c.codes + p0 * c.codes_page + k_head + off * (D / 2)), (short)0, ok ? 0x7fffffff : 0, 0x00020000);
           const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
               (void*)(c.scales + p0 * c.scales_page + ks_head + off), (short)0, ok ? 0x7fffffff : 0, 0x00020000);
+          if (a.once) {
 #pragma unroll
-          for (int j = 0; j < St::NC; ++j)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rc, lds(1024 * j), 16, (int)off_c[j], 0, 0, 0);
+            for (int j = 0; j < St::NC; ++j)
+              __builtin_amdgcn_raw_ptr_buffer_load_lds(rc, lds(1024 * j), 16, (int)off_c[j], 0, 0, CP_NT);
+          } else {
+#pragma unroll
+            for (int j = 0; j < St::NC; ++j)
+              __builtin_amdgcn_raw_ptr_buffer_load_lds(rc, lds(1024 * j), 16, (int)off_c[j], 0, 0, CP_PLAIN);
+          }
 #pragma unroll
           for (int j = 0; j < St::NS; ++j)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, lds(St::CODES + 256 * j), 4, (int)off_s[j], 0, 0, 0);
@@ -802,7 +809,7 @@ extern "C" int tlm_kv4_attn(const void* q, int64_t q_batch_stride, int64_t q_row
   }
   c.max_pages = (int)max_pages, c.page = (int)page, c.Hkv = (int)H_kv, c.D = (int)D;
   KaArgs a{c, (const uint16_t*)q, q_batch_stride, q_row_stride, seqlens, count, (uint16_t*)o, lse,
-           (KaCut*)ws, (float*)((char*)ws + p.meta), (int)B, (int)T, (int)H, (int)(H / H_kv), causal != 0, p.G, 0, 0,
+           (KaCut*)ws, (float*)((char*)ws + p.meta), (int)B, (int)T, (int)H, (int)(H / H_kv), causal != 0, p.G, T * (H / H_kv) <= 16 * p.qt, 0, 0,
            fabsf(sm_scale) * 1.4426950408889634f, sm_scale < 0.f ? 0x80008000u : 0u};
   // with 2^(k-1) < page <= 2^k and m = floor(2^(31+k) / page) + 1: m page - 2^(31+k) <= 2^k, so that tok m / 2^(31+k) is
   // less than 1 / page above tok / page for tok < 2^31; and m fits 32 bits
