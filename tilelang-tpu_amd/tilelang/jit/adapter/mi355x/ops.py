@@ -481,41 +481,73 @@ def kv_append_fp8(x: torch.Tensor, start: torch.Tensor, count: torch.Tensor,
 
 
 def _kv4_pools(codes: torch.Tensor, scales: torch.Tensor):
-    """H_kv, page, D and the pools' page strides of a 4-bit cache; the pools are checked against each
-    other."""
-    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+    """pages, H_kv, page, D and the pools' page strides of a 4-bit cache; the pools are checked against
+    each other."""
+    u8 = torch.uint8
+    if codes.dtype is not u8 or scales.dtype is not u8:
         raise ValueError("codes and scales must be uint8")
-    if codes.dim() != 5 or scales.dim() != 5 or codes.shape[1] != 2:
+    shape = codes.shape
+    if len(shape) != 5 or shape[1] != 2:
         raise ValueError("codes must be [pages, 2, H_kv, page, D / 2] and scales "
                          "[pages, 2, H_kv, D / 32, page]")
-    pages, _, Hkv, page, half = codes.shape
+    pages, _, Hkv, page, half = shape
     if half % 16 or scales.shape != (pages, 2, Hkv, half // 16, page):
-        raise ValueError(f"scales {tuple(scales.shape)} do not match codes {tuple(codes.shape)} "
+        raise ValueError(f"scales {tuple(scales.shape)} do not match codes {tuple(shape)} "
                          "(D a multiple of 32)")
     cs, ss = 2 * Hkv * page * half, 2 * Hkv * (half // 16) * page  # bytes of a page
-    if pages > 1 and not (codes.is_contiguous() and scales.is_contiguous()):
-        if not (codes[0].is_contiguous() and scales[0].is_contiguous()):
+    if not (codes.is_contiguous() and scales.is_contiguous()):
+        if pages < 2 or not (codes[0].is_contiguous() and scales[0].is_contiguous()):
             raise ValueError("codes and scales must be dense within a page")
         cs, ss = codes.stride(0), scales.stride(0)
-    elif pages == 1 and not (codes.is_contiguous() and scales.is_contiguous()):
-        raise ValueError("codes and scales must be dense within a page")
-    return Hkv, page, 2 * half, cs, ss
+    return pages, Hkv, page, 2 * half, cs, ss
 
 
 def _kv4_rows(name: str, x: torch.Tensor, heads: int, D: int):
-    """Batch and row stride of [B, T, heads, D] rows whose heads and dims are dense."""
-    if x.dim() != 4 or x.shape[2] != heads or x.shape[3] != D:
-        raise ValueError(f"{name} must be [B, T, {heads}, {D}], got {tuple(x.shape)}")
+    """B, T and the batch and row stride of [B, T, heads, D] rows whose heads and dims are dense."""
+    shape = x.shape
+    if len(shape) != 4 or shape[2] != heads or shape[3] != D:
+        raise ValueError(f"{name} must be [B, T, {heads}, {D}], got {tuple(shape)}")
     sb, st, sh, sd = x.stride()
-    if sd != 1 or (heads > 1 and sh != D):
+    if sd != 1 or (sh != D and heads > 1):
         raise ValueError(f"{name}: heads and dims must be contiguous")
-    row = heads * D
-    return (sb if x.shape[0] > 1 else row), (st if x.shape[1] > 1 else row)
+    B, T = shape[0], shape[1]
+    row = heads * D  # a dim of one has no stride of its own
+    return B, T, (sb if B > 1 else row), (st if T > 1 else row)
 
 
-def _i32(name: str, t: torch.Tensor, *shape: int):
-    if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous():
+def _i32(name: str, t: torch.Tensor, shape):
+    if t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 tensor of shape {list(shape)}")
+
+
+def _kv4_table(t: torch.Tensor, B: int) -> int:
+    """max_pages of a block table."""
+    shape = t.shape
+    if len(shape) != 2 or shape[0] != B or t.dtype is not torch.int32 or not t.is_contiguous():
+        raise ValueError(f"block_table must be a contiguous int32 tensor [{B}, max_pages]")
+    return shape[1]
+
+
+def _kv4_call(fn: str, tensors, *args):
+    """Calls ``fn`` with the device of ``tensors`` current (None among them: an argument not given) and that
+    device's current stream as the last argument."""
+    try:
+        index = tensors[0].get_device()
+        for t in tensors:
+            if t is not None and t.get_device() != index:
+                index = -1
+    except AttributeError:
+        index = -1
+    if index < 0:
+        _dev(*tensors)  # says what is wrong
+        raise ValueError("the mi355x kernels take HIP device tensors")
+    if torch._C._cuda_getDevice() != index:
+        with torch.cuda.device(index):
+            lib.ensure_device(index)
+            return lib.call(fn, *args, torch._C._cuda_getCurrentRawStream(index))
+    if index not in lib._inited:
+        lib.ensure_device(index)
+    return lib.call(fn, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
 def kv4_append(k: torch.Tensor, v: torch.Tensor, start: torch.Tensor, count: torch.Tensor,
@@ -523,19 +555,18 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, start: torch.Tensor, count: tor
     """Quantise new rows k, v [B, T, H_kv, D] (bf16/fp16; any batch and row stride) into the paged 4-bit
     cache codes uint8 [pages, 2, H_kv, page, D / 2], scales uint8 [pages, 2, H_kv, D / 32, page] at
     positions start[b] .. start[b] + count[b] - 1 of each sequence. Returns codes, scales."""
-    dev = _dev(k, v, start, count, block_table, codes, scales)
-    Hkv, page, D, cs, ss = _kv4_pools(codes, scales)
-    ks, vs = _kv4_rows("k", k, Hkv, D), _kv4_rows("v", v, Hkv, D)
-    B, T = k.shape[:2]
-    if v.shape != k.shape or v.dtype != k.dtype:
+    pages, Hkv, page, D, cs, ss = _kv4_pools(codes, scales)
+    B, T, kb, kr = _kv4_rows("k", k, Hkv, D)
+    vB, vT, vb, vr = _kv4_rows("v", v, Hkv, D)
+    if vB != B or vT != T or v.dtype is not k.dtype:
         raise ValueError("k and v must share shape and dtype")
-    _i32("start", start, B)
-    _i32("count", count, B)
-    _i32("block_table", block_table, B, block_table.shape[-1])
-    lib.call("tlm_kv4_append", _ptr(k), _ptr(v), *ks, *vs, dtype_code(k.dtype), _ptr(start),
-             _ptr(count), _ptr(block_table), block_table.shape[1], page, _ptr(codes),
-             cs, _ptr(scales), ss, codes.shape[0], B, T, Hkv, D,
-             _stream(dev))
+    _i32("start", start, (B,))
+    _i32("count", count, (B,))
+    max_pages = _kv4_table(block_table, B)
+    _kv4_call("tlm_kv4_append", (k, v, start, count, block_table, codes, scales), k.data_ptr(),
+              v.data_ptr(), kb, kr, vb, vr, dtype_code(k.dtype), start.data_ptr(), count.data_ptr(),
+              block_table.data_ptr(), max_pages, page, codes.data_ptr(), cs, scales.data_ptr(), ss,
+              pages, B, T, Hkv, D)
     return codes, scales
 
 
@@ -544,24 +575,24 @@ def kv4_read(codes: torch.Tensor, scales: torch.Tensor, block_table: torch.Tenso
              v_out: torch.Tensor):
     """Read rows of the 4-bit cache back: rows cu_seqlens[b] .. cu_seqlens[b + 1] of k_out, v_out
     [total, H_kv, D] (bf16/fp16/fp32) receive positions start[b] .. (None: 0 ..) of sequence b."""
-    dev = _dev(codes, scales, block_table, start, cu_seqlens, k_out, v_out)
-    Hkv, page, D, cs, ss = _kv4_pools(codes, scales)
-    _contig("k_out", k_out)
-    _contig("v_out", v_out)
-    if k_out.dim() != 3 or k_out.shape[1:] != (Hkv, D) or v_out.shape != k_out.shape or \
-            v_out.dtype != k_out.dtype:
+    pages, Hkv, page, D, cs, ss = _kv4_pools(codes, scales)
+    shape = k_out.shape
+    if len(shape) != 3 or shape[1] != Hkv or shape[2] != D or v_out.shape != shape or \
+            v_out.dtype is not k_out.dtype:
         raise ValueError(f"k_out and v_out must be [total, {Hkv}, {D}] of one dtype")
-    if block_table.dim() != 2:
-        raise ValueError("block_table must be [B, max_pages]")
-    B = block_table.shape[0]
-    _i32("block_table", block_table, B, block_table.shape[1])
-    _i32("cu_seqlens", cu_seqlens, B + 1)
+    if not (k_out.is_contiguous() and v_out.is_contiguous()):
+        raise ValueError("k_out and v_out must be contiguous")
+    if cu_seqlens.dim() != 1 or cu_seqlens.numel() == 0:
+        raise ValueError("cu_seqlens must be int32 [B + 1]")
+    B = cu_seqlens.numel() - 1
+    _i32("cu_seqlens", cu_seqlens, (B + 1,))
+    max_pages = _kv4_table(block_table, B)
     if start is not None:
-        _i32("start", start, B)
-    lib.call("tlm_kv4_read", _ptr(codes), cs, _ptr(scales), ss,
-             codes.shape[0], _ptr(block_table), block_table.shape[1], page, _ptr(start),
-             _ptr(cu_seqlens), _ptr(k_out), _ptr(v_out), B, k_out.shape[0], Hkv, D,
-             dtype_code(k_out.dtype), _stream(dev))
+        _i32("start", start, (B,))
+    _kv4_call("tlm_kv4_read", (codes, scales, block_table, start, cu_seqlens, k_out, v_out),
+              codes.data_ptr(), cs, scales.data_ptr(), ss, pages, block_table.data_ptr(), max_pages,
+              page, _ptr(start), cu_seqlens.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), B,
+              shape[0], Hkv, D, dtype_code(k_out.dtype))
     return k_out, v_out
 
 
@@ -577,28 +608,28 @@ def kv4_attn(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, block_t
     row stride), over its seqlens[b] tokens of the 4-bit cache, those tokens' own among them.
     out [B, T, H, D]; lse float32 [B, T, H]: log2 of the sum of exp of the scaled scores. Rows from
     count[b] on are left as they were. workspace: kv4_attn_workspace_bytes(...) bytes, one per stream."""
-    dev = _dev(q, codes, scales, block_table, seqlens, out, workspace, count, lse)
-    Hkv, page, D, cs, ss = _kv4_pools(codes, scales)
-    if q.dim() != 4 or Hkv == 0 or q.shape[2] % Hkv:
+    pages, Hkv, page, D, cs, ss = _kv4_pools(codes, scales)
+    shape = q.shape
+    if len(shape) != 4 or Hkv == 0 or shape[2] % Hkv:
         raise ValueError(f"q must be [B, T, H, {D}] with H a multiple of {Hkv}")
-    B, T, H = q.shape[:3]
-    qs = _kv4_rows("q", q, H, D)
-    _contig("out", out)
-    if out.shape != q.shape or out.dtype != q.dtype:
-        raise ValueError("out must match q in shape and dtype")
-    _i32("seqlens", seqlens, B)
+    H = shape[2]
+    B, T, qb, qr = _kv4_rows("q", q, H, D)
+    if out.shape != shape or out.dtype is not q.dtype or not out.is_contiguous():
+        raise ValueError("out must be contiguous and match q in shape and dtype")
+    _i32("seqlens", seqlens, (B,))
     if count is not None:
-        _i32("count", count, B)
-    _i32("block_table", block_table, B, block_table.shape[-1])
-    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (B, T, H) or
+        _i32("count", count, (B,))
+    max_pages = _kv4_table(block_table, B)
+    if lse is not None and (lse.dtype is not torch.float32 or lse.shape != (B, T, H) or
                             not lse.is_contiguous()):
         raise ValueError("lse must be a contiguous float32 [B, T, H] tensor")
-    _contig("workspace", workspace)
-    lib.call("tlm_kv4_attn", _ptr(q), *qs, _ptr(codes), cs, _ptr(scales),
-             ss, codes.shape[0], _ptr(block_table), block_table.shape[1], page,
-             _ptr(seqlens), _ptr(count), _ptr(out), _ptr(lse), _ptr(workspace),
-             workspace.numel() * workspace.element_size(), B, T, H, Hkv, D, 1 if causal else 0,
-             float(sm_scale), dtype_code(q.dtype), _stream(dev))
+    if not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous")
+    _kv4_call("tlm_kv4_attn", (q, codes, scales, block_table, seqlens, out, workspace, count, lse),
+              q.data_ptr(), qb, qr, codes.data_ptr(), cs, scales.data_ptr(), ss, pages,
+              block_table.data_ptr(), max_pages, page, seqlens.data_ptr(), _ptr(count),
+              out.data_ptr(), _ptr(lse), workspace.data_ptr(), workspace.nbytes, B, T, H, Hkv, D,
+              1 if causal else 0, sm_scale, dtype_code(q.dtype))
     return out
 
 
