@@ -170,7 +170,9 @@ def _check(q, codes, scales, bt, lens, count=None, causal=True, scale=None, got=
     """Within the kernel's roundings of the float64 result. A score is a sum of D exact products in fp32 (q
     and the cached values are exact in its operands): off by at most (D + 2) 2^-24 of the sum of
     magnitudes A. A weight is off by that times ln 2 log2 e = 1, by exp2 (1 ulp, and its argument's
-    rounding against a reference within the scores' range: 2 A 2^-24) and by 16 bits where it multiplies V (2^-17).
+    rounding against a reference within the scores' range: 2 A 2^-24) and by its rounding where it multiplies V: with fp16
+    queries two bf16 terms (2^-17), with bf16 ones fp16 (half a step is 2^-11; weights under fp16's normal range, which
+    are below 2^-21 of the largest, by 2^-25 / 2^7 of it, less than the 2^-24 that is counted for each key below).
     Numerator and denominator are sums of up to n weights, (n + 64) 2^-24 each; the quotient is
     rounded once: by eps / 2, or half of the smallest subnormal, tiny eps / 2 (an output of 4.5e-7 is
     0.46 of fp16's 2^-24 steps off its nearest multiple: no fp16 value is nearer)."""
@@ -186,6 +188,7 @@ def _check(q, codes, scales, bt, lens, count=None, causal=True, scale=None, got=
     out, z = got if got is not None else _run(q, codes, scales, bt, lens, count, causal, scale)
     eps = torch.finfo(q.dtype).eps / 2
     least = torch.finfo(q.dtype).tiny * eps
+    weight = 2.0 ** -11 if q.dtype == BF16 else 2.0 ** -16
     for b in range(B):
         n = max(0, min(int(lens[b]), bt.shape[1] * page))
         m = T if count is None else max(0, min(int(count[b]), T))
@@ -193,7 +196,7 @@ def _check(q, codes, scales, bt, lens, count=None, causal=True, scale=None, got=
         k = np.abs(k).repeat(H // codes.shape[2], 1).transpose(1, 2, 0)
         a = np.abs(q[b, :m].double().numpy()).transpose(1, 0, 2) @ k * abs(sm) if n else np.zeros((H, m, 1))
         a = a.max(-1).T[..., None]  # [m, H, 1]
-        rel = 2 * ((D + 4) * 2.0 ** -24 * a + 2.0 ** -23 + 2.0 ** -17 + (n + 64) * 2.0 ** -24)
+        rel = 2 * ((D + 4) * 2.0 ** -24 * a + 2.0 ** -23 + (n + 64) * 2.0 ** -24) + weight
         x, e = out[b, :m].double().numpy(), exp[b, :m]
         bad = np.abs(x - e) > eps * (1 + 2 ** -10) * np.abs(e) + rel * spread[b, :m] + least
         assert not bad.any(), (b, np.abs(x - e).max())

@@ -19,7 +19,9 @@ constexpr int ka_stages() {
   const int n = (160 * 1024 / ka_per_cu(D, QT) - 1024) / (KA_W * (32 * D + 256 * ((D + 127) / 128)));
   return n < 4 ? n : 4;
 }
-constexpr float KA_SLACK = 8.f;  // a reference is kept until a score passes it by this much (log2)
+// Weights are 2^(s - reference): 2^BIAS for the score that set the reference, which is kept until another passes
+// that one by SLACK. At most 2^15, an fp16 number, and normal ones down to 2^-25 of the largest.
+constexpr float KA_BIAS = 11.f, KA_SLACK = 4.f;
 
 struct KaCut {
   int b, rt;   // sequence (-1: nothing to join) and row tile
@@ -72,7 +74,22 @@ TLM_DEV int ka_new(const KaArgs& a, int b) { return a.count ? max(0, min(a.count
 template <int MT>
 TLM_DEV int ka_tiles(const KaArgs& a, int n) { return (n * a.group + MT - 1) / MT; }
 
-TLM_DEV int64_t ka_cut(int64_t total, int g, int r) { return total / g * r + total % g * r / g; }
+// Ranges of the cost line: range r of g starts at floor(r total / g) (g <= 768: products of the rest fit 32 bits).
+struct KaCuts {
+  int64_t quot;
+  uint32_t rem, g;
+  TLM_DEV KaCuts(int64_t total, int ranges) : g((uint32_t)ranges) {
+    if (total >> 32) {
+      quot = total / ranges;
+      rem = (uint32_t)(total - quot * ranges);
+    } else {
+      const uint32_t q = (uint32_t)total / g;
+      quot = q;
+      rem = (uint32_t)total - q * g;
+    }
+  }
+  TLM_DEV int64_t at(int r) const { return quot * r + rem * (uint32_t)r / g; }
+};
 
 // Units of an entry at cost `before` that fall into range [lo, hi): none of its first KA_PIECE.
 TLM_DEV int ka_unit_at(int64_t x, int64_t before, int units) {
@@ -150,22 +167,24 @@ struct Segs {
 
 __device__ const u32x4 ka_zeros[1] = {};  // codes and scales of tokens without a page
 
-// A tile in a wave's ring of LDS, 16-byte slots: 32 dims of a token each. First K, in the order that the lanes read it
-// as MFMA operands, then V in token order of its operand (token 8 g + i behind 8 g' + i for g > g'), so that all
-// reads are linear in the lane; then the scales, [K, V][D / 32][32 tokens].
+// A tile in a wave's ring of LDS, in 16-byte slots (32 dims of a token): K in the order that the lanes read it as MFMA
+// operands, then V in token order of its operand, so that all reads are linear in the lane; then the scales,
+// [K, V][D / 32][32 tokens].
 template <int D>
 struct Stage {
   static constexpr int CODES = 32 * D, NC = D / 32;           // bytes; LDS-DMA instructions of 64 slots
   static constexpr int NS = (D + 127) / 128, SCALES = 256 * NS;  // 64 words each
   static constexpr int BYTES = CODES + SCALES, PER = NC + NS;
 };
-// What a lane has of a tile.
+// What a lane has of a tile: K of tokens jl and 16 + jl; V of tokens 4 g + (0 .. 3) and 16 + 4 g + (0 .. 3), so
+// that a lane's scores are those of its V rows.
 template <int D>
 struct KaTile {
   uint32_t k[2][D / 32], v[8][Segs<D>::N];
   uint32_t ks[2][Segs<D>::N];
   u32x2 vs[Segs<D>::N];
 };
+TLM_DEV int ka_token(int g, int i) { return 16 * (i >> 2) + 4 * g + (i & 3); }  // of a lane's V row i
 
 using ldsop::lds_u32;
 template <int N>
@@ -189,10 +208,10 @@ TLM_DEV void ka_read128(u32x4& k0, u32x4& k1, uint32_t& s0, uint32_t& s1, u32x2 
       "ds_read2st64_b32 %5, %10 offset0:2 offset1:3\n\t"
       "ds_read2st64_b32 %6, %10 offset0:4 offset1:5\n\t"
       "ds_read2st64_b32 %7, %10 offset0:6 offset1:7\n\t"
-      "ds_read_b64 %8, %12 offset:%17\n\t"
+      "ds_read2_b32 %8, %12 offset0:0 offset1:4\n\t"
       "s_waitcnt lgkmcnt(0)"
       : "=&v"(k0), "=&v"(k1), "=&v"(s0), "=&v"(s1), "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(vs)
-      : "v"(ka), "v"(va + VO), "v"(ksa), "v"(vsa), "i"(KO), "i"(KO + 1024), "i"(KSO), "i"(KSO + 4), "i"(VSO)
+      : "v"(ka), "v"(va + VO), "v"(ksa), "v"(vsa + VSO), "i"(KO), "i"(KO + 1024), "i"(KSO), "i"(KSO + 16)
       : "memory");
 }
 #define KA_READ_NARROW(NAME, KT, KOP, VOP, KSTEP, VSTEP)                                                             \
@@ -204,11 +223,11 @@ TLM_DEV void ka_read128(u32x4& k0, u32x4& k1, uint32_t& s0, uint32_t& s1, u32x2 
                      " %4, %14 offset:%22\n\t" VOP " %5, %14 offset:%23\n\t" VOP " %6, %14 offset:%24\n\t" VOP         \
                      " %7, %14 offset:%25\n\t" VOP " %8, %14 offset:%26\n\t" VOP " %9, %14 offset:%27\n\t" VOP         \
                      " %10, %14 offset:%28\n\t" VOP " %11, %14 offset:%29\n\t"                                       \
-                     "ds_read_b64 %12, %16 offset:%21\n\ts_waitcnt lgkmcnt(0)"                                       \
+                     "ds_read2_b32 %12, %16 offset0:0 offset1:4\n\ts_waitcnt lgkmcnt(0)"                                       \
                  : "=&v"(k0), "=&v"(k1), "=&v"(s0), "=&v"(s1), "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]),  \
                    "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7]), "=&v"(vs)                                    \
-                 : "v"(ka), "v"(va), "v"(ksa), "v"(vsa), "i"(KO), "i"(KO + KSTEP), "i"(KSO), "i"(KSO + 4),          \
-                   "i"(VSO), "i"(VO), "i"(VO + VSTEP), "i"(VO + 2 * VSTEP), "i"(VO + 3 * VSTEP), "i"(VO + 4 * VSTEP), \
+                 : "v"(ka), "v"(va), "v"(ksa), "v"(vsa + VSO), "i"(KO), "i"(KO + KSTEP), "i"(KSO), "i"(KSO + 16),   \
+                   "i"(0), "i"(VO), "i"(VO + VSTEP), "i"(VO + 2 * VSTEP), "i"(VO + 3 * VSTEP), "i"(VO + 4 * VSTEP), \
                    "i"(VO + 5 * VSTEP), "i"(VO + 6 * VSTEP), "i"(VO + 7 * VSTEP)                                    \
                  : "memory");                                                                                       \
   }
@@ -216,58 +235,550 @@ KA_READ_NARROW(ka_read64, u32x2, "ds_read_b64", "ds_read_u16", 512, 128)
 KA_READ_NARROW(ka_read32, uint32_t, "ds_read_b32", "ds_read_u8", 256, 64)
 #undef KA_READ_NARROW
 
-template <int SEL>
+// Two codes of a word, times their scale, as 16-bit floats: exact in bf16; in fp16 for the scales of fits_f16.
+template <bool F16, int SEL>
 TLM_DEV uint32_t ka_cvt(uint32_t w, float s) {
-  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, SEL));
+  if constexpr (F16)
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, SEL));
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, SEL));
 }
+template <bool F16>
 TLM_DEV f32x4 ka_mma(u32x4 a, u32x4 b, f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
-                                                 0, 0);
+  if constexpr (F16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
+                                                   0);
 }
+// Scale bytes 109 .. 140 (2^-18 .. 2^13): every code times them is an fp16 number, subnormal ones among them, which
+// the matrix cores take. Zero where all bytes of w are such: plus 19 they are 128 .. 159, and a byte's carry comes from
+// one that is out of range itself.
+TLM_DEV uint32_t ka_not_f16(uint32_t w) { return ((w + 0x13131313u) ^ 0x80808080u) & 0xe0e0e0e0u; }
 
-// Two floats -> their bf16 parts and the bf16 parts of what is left: 16 bits of each.
+// Two floats -> their bf16 parts and the bf16 parts of what is left: 16 bits of each. An infinity leaves nothing.
 TLM_DEV void ka_split(float x, float y, uint32_t& hi, uint32_t& lo) {
   hi = h16<true>::pack(x, y);
   lo = h16<true>::pack(x - h16<true>::lo(hi), y - h16<true>::hi(hi));
 }
+TLM_DEV void ka_split_f16(u32x4 x, u32x4& hi, u32x4& lo) {  // fp16 words: exact
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float y0 = h16<false>::lo(x[i]), y1 = h16<false>::hi(x[i]);
+    hi[i] = h16<true>::pack(y0, y1);
+    const float z0 = h16<true>::lo(hi[i]), z1 = h16<true>::hi(hi[i]);
+    lo[i] = h16<true>::pack(fabsf(z0) < INFINITY ? y0 - z0 : 0.f, fabsf(z1) < INFINITY ? y1 - z1 : 0.f);
+  }
+}
 
-template <int D, int QT, bool BF16, bool PG>
-__global__ __launch_bounds__(64 * KA_W, ka_per_cu(D, QT)) void kv4_attn_ranges(const KaArgs a) {
-#if defined(__HIP_DEVICE_COMPILE__)
+// A range's part of an entry, for one K/V head.
+struct KaPiece {
+  int b, h, t0, t1;  // tokens t0 .. t1 - 1
+  KaEntry e;
+  float* slot;  // where its rows go unless it is all of the entry
+};
+struct KaShared {
+  float m[KA_W][16], l[KA_W][16];
+};
+
+// What a lane fetches with each LDS-DMA instruction of a tile, from where its part of the tile (32 / NP tokens) begins.
+template <int D, int NP>
+struct KaFetch {
   using S = Segs<D>;
-  constexpr int MT = 16 * QT, NK = D / 32, ND = D / 16, QN = BF16 ? 1 : 2;
-  constexpr int SO = D + 4;  // floats of a row of the exchange
   using St = Stage<D>;
-  constexpr int NST = ka_stages<D, QT>();
+  uint32_t off_c[St::NC], off_s[St::NS];
+  int part_c[St::NC], part_s[St::NS];
+  TLM_DEV KaFetch(const Cache& c, int lane) {
+    constexpr int PT = KA_BN / NP, NK = D / 32;
+#pragma unroll
+    for (int j = 0; j < St::NC; ++j) {
+      const bool is_v = 64 * j + lane >= D;
+      const int p = 64 * j + lane - (is_v ? D : 0);
+      int tok = 0, byte = 0;
+      unroll<0, S::N>([&](auto s) {
+        constexpr int W = S::w(s), B0 = S::base(s);
+        const int x = p - B0;
+        if (x < 0 || x >= 16 * W) return;
+        if (is_v) {
+          tok = ka_token(x / (W / 2) % 4, x / (2 * W));
+          byte = B0 / 2 + 16 * (x % (W / 2));
+        } else {
+          tok = 16 * (x / (8 * W)) + x % 16;
+          byte = B0 / 2 + 16 * (x / 16 % (W / 2));
+        }
+      });
+      part_c[j] = tok / PT;
+      off_c[j] = (uint32_t)((is_v ? c.Hkv * c.page * (D / 2) : 0) + tok % PT * (D / 2) + byte);
+    }
+  #pragma unroll
+    for (int j = 0; j < St::NS; ++j) {
+      const int x = 64 * j + lane < D / 2 ? 64 * j + lane : 0;  // lanes past the scales fetch the first word again
+      const int half = x / (8 * NK), blk = x / 8 % NK, tok = 4 * (x % 8);
+      part_s[j] = tok / PT;
+      off_s[j] = (uint32_t)((half * c.Hkv * NK + blk) * c.page + tok % PT);
+    }
+  }
+};
+
+// One piece. NP: pages that a tile may touch, 1 (page a multiple of 32), 2 (of 16) or 4.
+template <int D, int QT, bool BF16, int NP>
+TLM_DEV void ka_piece(const KaArgs& a, const KaPiece& pc, const KaFetch<D, NP>& fetch, uint8_t* smem, KaShared& sh) {
+  using S = Segs<D>;
+  using St = Stage<D>;
+  constexpr int MT = 16 * QT, NK = D / 32, ND = D / 16, NST = ka_stages<D, QT>(), PT = KA_BN / NP;
+  constexpr int SO = D + 4;  // floats of a row of the exchange
   static_assert(KA_W * NST * St::BYTES >= KA_W * 16 * SO * (int)sizeof(float), "the exchange lies in the rings");
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[KA_W * NST * St::BYTES];
   auto so = (float(*)[16][SO])smem;
-  __shared__ float sm[KA_W][16], sl[KA_W][16];
-  __shared__ int64_t sh[KA_W + 3];
   const Cache& c = a.c;
+  const KaEntry& e = pc.e;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, jl = lane & 15;
-  const int h = blockIdx.x % c.Hkv, r = blockIdx.x / c.Hkv;
+  const int b = pc.b, h = pc.h, L = e.L, n = e.n;
+  const int64_t k_head = (int64_t)h * c.page * (D / 2), ks_head = (int64_t)h * c.page * NK;
+  const uint32_t ring = lds_u32(smem) + wave * (NST * St::BYTES);
+  const uint32_t k64 = 256 * (g >> 1) + 16 * jl + 8 * (g & 1), k32 = 16 * jl + 4 * g;
+  const uint32_t ks_l = jl, vs_l = 4 * g;
+
+  const int tend = pc.t1;
+  int t0 = pc.t0 + wave * KA_BN;
+  f32x4 o[QT][ND];
+  float ref[QT], thr[QT], l[QT];
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    ref[t] = 0.f, thr[t] = -INFINITY, l[t] = 0.f;
+#pragma unroll
+    for (int i = 0; i < ND; ++i) o[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  // the table is only read here: as constant memory its uniform reads are scalar
+  const auto* table = (const __attribute__((address_space(4))) int32_t*)(c.table + (int64_t)b * c.max_pages);
+  auto page_of = [&](int tok) { return (int)((uint64_t)(uint32_t)tok * a.page_mul >> a.page_shift); };
+  struct Pages {
+    int id[NP];
+  };
+  auto look_up = [&](int tk) {  // -1 where the piece has no such tokens
+    Pages p;
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      p.id[i] = -1;
+      if (tk + PT * i < tend) p.id[i] = table[page_of(tk + PT * i)];
+    }
+    return p;
+  };
+  int at_issue = 0, at_read = 0;  // byte offsets of stages
+  auto issue = [&](int tk, const Pages& pg) {
+    uint8_t* const dst = smem + wave * (NST * St::BYTES) + at_issue;
+    at_issue = at_issue + St::BYTES == NST * St::BYTES ? 0 : at_issue + St::BYTES;
+    auto lds = [&](int off) { return (__attribute__((address_space(3))) void*)(dst + off); };
+    if constexpr (NP == 1) {
+      const bool ok = pg.id[0] >= 0 && pg.id[0] < c.pages;  // otherwise a buffer of no bytes: zeros
+      const int64_t p0 = ok ? pg.id[0] : 0, off = ok ? tk - page_of(tk) * c.page : 0;
+      const __amdgpu_buffer_rsrc_t rc = __builtin_amdgcn_make_buffer_rsrc(
+          (void*)(c.codes + p0 * c.codes_page + k_head + off * (D / 2)), (short)0, ok ? 0x7fffffff : 0, 0x00020000);
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+          (void*)(c.scales + p0 * c.scales_page + ks_head + off), (short)0, ok ? 0x7fffffff : 0, 0x00020000);
+      if (a.once) {
+#pragma unroll
+        for (int j = 0; j < St::NC; ++j)
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(rc, lds(1024 * j), 16, (int)fetch.off_c[j], 0, 0, CP_NT);
+      } else {
+#pragma unroll
+        for (int j = 0; j < St::NC; ++j)
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(rc, lds(1024 * j), 16, (int)fetch.off_c[j], 0, 0, CP_PLAIN);
+      }
+#pragma unroll
+      for (int j = 0; j < St::NS; ++j)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, lds(St::CODES + 256 * j), 4, (int)fetch.off_s[j], 0, 0, 0);
+    } else {
+      const uint8_t *bc[NP], *bs[NP];
+      bool ok[NP], all = true;
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        const int64_t p = pg.id[i];
+        ok[i] = p >= 0 && p < c.pages;
+        all = all && ok[i];
+        const int64_t off = tk + PT * i - page_of(tk + PT * i) * c.page;
+        bc[i] = c.codes + p * c.codes_page + k_head + off * (D / 2);
+        bs[i] = c.scales + p * c.scales_page + ks_head + off;
+      }
+      auto from = [&](const uint8_t* const (&base)[NP], int i, uint32_t off, bool every) {
+        const uint8_t* b = base[0];
+        bool o = ok[0];
+#pragma unroll
+        for (int n = 1; n < NP; ++n) b = i == n ? base[n] : b, o = i == n ? ok[n] : o;
+        b += off;
+        if (!every) b = o ? b : (const uint8_t*)ka_zeros;
+        return (const __attribute__((address_space(1))) void*)b;
+      };
+      auto get = [&](bool every) {
+#pragma unroll
+        for (int j = 0; j < St::NC; ++j)
+          __builtin_amdgcn_global_load_lds(from(bc, fetch.part_c[j], fetch.off_c[j], every), lds(1024 * j), 16, 0, 0);
+#pragma unroll
+        for (int j = 0; j < St::NS; ++j)
+          __builtin_amdgcn_global_load_lds(from(bs, fetch.part_s[j], fetch.off_s[j], every), lds(St::CODES + 256 * j), 4, 0, 0);
+      };
+      if (all) get(true);
+      else get(false);
+    }
+  };
+  auto read = [&](KaTile<D>& x) {
+    const uint32_t st = ring + at_read;
+    at_read = at_read + St::BYTES == NST * St::BYTES ? 0 : at_read + St::BYTES;
+    unroll<0, S::N>([&](auto s) {
+      constexpr int W = S::w(s), B0 = S::base(s);
+      constexpr int KO = 16 * B0, VO = 16 * (D + B0), KSO = St::CODES + B0, VSO = St::CODES + D + B0;
+      if constexpr (W == 8) {
+        u32x4 k0, k1;
+        u32x2 v[4];
+        ka_read128<KO, VO, KSO, VSO>(k0, k1, x.ks[0][s], x.ks[1][s], v, x.vs[s], st + 16 * lane, st + 4 * lane,
+                                     st + ks_l + 32 * g, st + vs_l + 32 * (jl >> 2));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          x.k[0][B0 / 32 + i] = k0[i], x.k[1][B0 / 32 + i] = k1[i];
+          x.v[2 * i][s] = v[i][0], x.v[2 * i + 1][s] = v[i][1];
+        }
+      } else {
+        uint32_t v[8];
+        if constexpr (W == 4) {
+          u32x2 k0, k1;
+          ka_read64<KO, VO, KSO, VSO>(k0, k1, x.ks[0][s], x.ks[1][s], v, x.vs[s], st + k64, st + 2 * lane,
+                                      st + ks_l + 32 * (g >> 1), st + vs_l + 32 * (jl >> 3));
+#pragma unroll
+          for (int i = 0; i < 2; ++i) x.k[0][B0 / 32 + i] = k0[i], x.k[1][B0 / 32 + i] = k1[i];
+        } else {
+          ka_read32<KO, VO, KSO, VSO>(x.k[0][B0 / 32], x.k[1][B0 / 32], x.ks[0][s], x.ks[1][s], v, x.vs[s], st + k32,
+                                      st + lane, st + ks_l, st + vs_l);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x.v[i][s] = v[i];
+      }
+    });
+  };
+
+  u32x4 q[QT][NK];  // columns jl of the 16-row tiles
+  int lim[QT];      // keys that they see
+  // S^T of the tile: rows are keys, columns queries
+  auto scores = [&](const KaTile<D>& x, f32x4 (&sc)[QT][2], auto f16) {
+    constexpr bool F16 = decltype(f16)::value;
+    unroll<0, S::N>([&](auto s) {
+      constexpr int W = S::w(s), B0 = S::base(s);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float f = kv4::scale_of(x.ks[i][s]);
+#pragma unroll
+        for (int w = 0; w < W / 2; ++w) {
+          const uint32_t kw = x.k[i][B0 / 32 + w];
+          const u32x4 kf = {ka_cvt<F16, 0>(kw, f), ka_cvt<F16, 1>(kw, f), ka_cvt<F16, 2>(kw, f), ka_cvt<F16, 3>(kw, f)};
+#pragma unroll
+          for (int t = 0; t < QT; ++t) {
+            if constexpr (BF16 || F16) {
+              sc[t][i] = ka_mma<F16>(kf, q[t][B0 / 32 + w], sc[t][i]);
+            } else {
+              u32x4 qh, ql;
+              ka_split_f16(q[t][B0 / 32 + w], qh, ql);
+              sc[t][i] = ka_mma<false>(kf, ql, ka_mma<false>(kf, qh, sc[t][i]));
+            }
+          }
+        }
+      }
+    });
+  };
+  // the column's reference moves when a score passes it by too much
+  auto weigh = [&](int t, float top) {
+    if (__any(top > thr[t])) {
+      top = xhalf_max(xrow_max(top));  // over the four lanes of the column
+      const bool up = top > thr[t];
+      const float f = !up ? 1.f : thr[t] == -INFINITY ? 0.f : fast_exp2(ref[t] - (top - KA_BIAS));
+      ref[t] = up ? top - KA_BIAS : ref[t];
+      thr[t] = up ? top + KA_SLACK : thr[t];
+      l[t] *= f;
+#pragma unroll
+      for (int i = 0; i < ND; ++i) o[t][i] *= f;
+    }
+  };
+  // V^T operands of each 16 dims: row jl is a dim, the lane's eight tokens lie along
+  auto values = [&](auto f16, auto&& word, auto&& scale, auto&& use) {
+    constexpr bool F16 = decltype(f16)::value;
+    unroll<0, S::N>([&](auto s) {
+      constexpr int W = S::w(s), B0 = S::base(s);
+      unroll<0, W / 2>([&](auto sel) {
+        uint32_t cv[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) cv[i] = ka_cvt<F16, sel>(word(i, s), scale(i, s));
+        u32x4 even, other;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          even[i] = __builtin_amdgcn_perm(cv[2 * i + 1], cv[2 * i], 0x05040100);
+          other[i] = __builtin_amdgcn_perm(cv[2 * i + 1], cv[2 * i], 0x07060302);
+        }
+        use(B0 / 16 + 2 * sel, even);
+        use(B0 / 16 + 2 * sel + 1, other);
+      });
+    });
+  };
+
+  // What a last tile has beyond the keys becomes zeros of scale 1.
+  auto clear = [&](KaTile<D>& x, int tk) {
+    unroll<0, S::N>([&](auto s) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int at = 8 * (i & 3);
+        const bool out = tk + ka_token(g, i) >= e.keys;
+        x.v[i][s] = out ? 0u : x.v[i][s];
+        x.vs[s][i >> 2] = out ? (x.vs[s][i >> 2] & ~(255u << at)) | 127u << at : x.vs[s][i >> 2];
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) x.ks[i][s] = tk + 16 * i + jl >= e.keys ? 127u : x.ks[i][s];
+    });
+  };
+  // Whether fp16 holds all V (bf16 queries) or K (fp16 queries) of the tile.
+  auto suits = [&](const KaTile<D>& x) {
+    uint32_t no = 0;
+    unroll<0, S::N>([&](auto s) {
+      no |= BF16 ? ka_not_f16(x.vs[s][0]) | ka_not_f16(x.vs[s][1])
+                 : (ka_not_f16(x.ks[0][s]) | ka_not_f16(x.ks[1][s])) & 255u;
+    });
+    return !__any(no != 0);
+  };
+  // A tile. ALL: every row sees all of it. FAST (it suits): V (bf16 queries) or K (fp16) in fp16; else all in bf16, weights
+  // and fp16 queries in two terms.
+  auto compute = [&](KaTile<D>& x, int tk, auto all, auto form) {
+    constexpr bool ALL = decltype(all)::value, FAST = decltype(form)::value, PV16 = BF16 && FAST;
+    f32x4 sc[QT][2];
+#pragma unroll
+    for (int t = 0; t < QT; ++t) sc[t][0] = sc[t][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    scores(x, sc, std::bool_constant<!BF16 && FAST>{});
+    if constexpr (!ALL) {
+#pragma unroll
+      for (int t = 0; t < QT; ++t)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          sc[t][i >> 2][i & 3] = tk + ka_token(g, i) < lim[t] ? sc[t][i >> 2][i & 3] : -INFINITY;
+    }
+    u32x4 ph[QT], pl[QT];
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = fmaxf(top, sc[t][i >> 2][i & 3]);
+      weigh(t, top * a.scale2);
+      float y[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = fast_exp2(fmaf(sc[t][i >> 2][i & 3], a.scale2, -ref[t]));
+      l[t] += ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (PV16) {
+          ph[t][i] = h16<false>::pack(y[2 * i], y[2 * i + 1]);
+        } else {
+          uint32_t hw, lw;
+          ka_split(y[2 * i], y[2 * i + 1], hw, lw);
+          ph[t][i] = hw, pl[t][i] = lw;
+        }
+      }
+    }
+    if constexpr (!ALL && !PV16) {
+      // NaN of V that a row does not see must not meet its weight of 0: such blocks become zeros, and the rows that see
+      // one become NaN by their count of it
+      u32x4 seen[QT];
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int t = 0; t < QT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          seen[t][i] = (tk + ka_token(g, 2 * i) < lim[t] ? 0x3f80u : 0u) |
+                       (tk + ka_token(g, 2 * i + 1) < lim[t] ? 0x3f800000u : 0u);
+      unroll<0, S::N>([&](auto s) {
+        constexpr int W = S::w(s), B0 = S::base(s);
+        u32x4 bad = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int at = 8 * (i & 3);
+          const bool nan = ((x.vs[s][i >> 2] >> at) & 255u) > 252u;
+          bad[i >> 1] |= !nan ? 0u : (i & 1) ? 0x3f800000u : 0x3f80u;
+          x.v[i][s] = nan ? 0u : x.v[i][s];
+          x.vs[s][i >> 2] = nan ? (x.vs[s][i >> 2] & ~(255u << at)) | 127u << at : x.vs[s][i >> 2];
+        }
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+          const f32x4 count = ka_mma<false>(bad, seen[t], f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+          for (int d = 0; d < W; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[t][B0 / 16 + d][i] = count[i] > 0.f ? NAN : o[t][B0 / 16 + d][i];
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      });
+    }
+    if constexpr (!FAST) __builtin_amdgcn_sched_barrier(0);
+    values(std::bool_constant<PV16>{}, [&](int i, int s) { return x.v[i][s]; },
+           [&](int i, int s) { return kv4::scale_of((x.vs[s][i >> 2] >> (8 * (i & 3))) & 255u); },
+           [&](int d, u32x4 vf) {
+#pragma unroll
+             for (int t = 0; t < QT; ++t) {
+               o[t][d] = ka_mma<PV16>(vf, ph[t], o[t][d]);
+               if constexpr (!PV16) o[t][d] = ka_mma<false>(vf, pl[t], o[t][d]);
+             }
+             if constexpr (!FAST) __builtin_amdgcn_sched_barrier(0);  // fewer registers
+           });
+  };
+
+  if (t0 < tend) {
+    Pages pg[NST];
+#pragma unroll
+    for (int i = 0; i < NST; ++i) pg[i] = look_up(t0 + i * KA_UNIT);
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      const int i = 16 * t + jl;
+      const int row = e.row0 + i, j = row / a.group;
+      const bool live = i < e.rows;
+      lim[t] = live && a.causal ? max(0, L - n + 1 + j) : e.keys;
+      const uint16_t* p = a.q + b * a.qb + j * a.qr + (int64_t)(h * a.group + row - j * a.group) * D;
+      unroll<0, S::N>([&](auto s) {
+        constexpr int W = S::w(s), B0 = S::base(s);
+#pragma unroll
+        for (int w = 0; w < W / 2; ++w)
+          q[t][B0 / 32 + w] = live ? *(const u32x4*)(p + B0 + 4 * W * g + 8 * w) : u32x4{0, 0, 0, 0};
+      });
+    }
+#pragma unroll
+    for (int i = 0; i < NST - 1; ++i) issue(t0 + i * KA_UNIT, pg[i]);
+    Pages ahead = pg[NST - 1];
+    int ti = t0 + (NST - 1) * KA_UNIT;
+#pragma unroll
+    for (int t = 0; t < QT; ++t)
+#pragma unroll
+      for (int i = 0; i < NK; ++i)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) q[t][i][w] ^= a.q_sign;
+
+    auto next = [&] {  // the tile at t0 is in LDS, and one more on the way
+      issue(ti, ahead);
+      ti += KA_UNIT;
+      ahead = look_up(ti);
+      vm_wait<(NST - 1) * St::PER>();
+    };
+    // Loops of one form each (a choice within a loop costs registers): tiles that every row sees whole, the others, and
+    // from the first tile on that does not suit
+    const int whole_end = min(tend, e.keys_min);
+    bool fast = true;
+    for (; t0 + KA_BN <= whole_end; t0 += KA_UNIT) {
+      next();
+      KaTile<D> x;
+      read(x);
+      fast = suits(x);
+      if (!fast) break;
+      compute(x, t0, std::true_type{}, std::true_type{});
+    }
+    if (fast)
+      for (; t0 < tend; t0 += KA_UNIT) {
+        next();
+        KaTile<D> x;
+        read(x);
+        clear(x, t0);
+        fast = suits(x);
+        if (!fast) break;
+        compute(x, t0, std::false_type{}, std::true_type{});
+      }
+    if (!fast) {
+      at_read = at_read == 0 ? (NST - 1) * St::BYTES : at_read - St::BYTES;  // that tile again
+      for (bool first = true; t0 < tend; t0 += KA_UNIT, first = false) {
+        if (!first) next();
+        KaTile<D> x;
+        read(x);
+        clear(x, t0);
+        compute(x, t0, std::false_type{}, std::false_type{});
+      }
+    }
+  }
+  vm_wait<0>();  // nothing may land in the exchange
+  __syncthreads();
+
+  // the waves' rows meet: 16 at a time
+  #pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    float sum = l[t];
+    sum += __shfl_xor(sum, 16, 64);
+    sum += __shfl_xor(sum, 32, 64);
+    if (g == 0) {
+      sh.m[wave][jl] = thr[t] == -INFINITY && sum == 0.f ? -INFINITY : ref[t];
+      sh.l[wave][jl] = sum;
+    }
+    unroll<0, S::N>([&](auto s) {
+      constexpr int W = S::w(s), B0 = S::base(s);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int d = 0; d < W; ++d) so[wave][jl][B0 + 4 * W * g + W * i + d] = o[t][B0 / 16 + d][i];
+    });
+    __syncthreads();
+    for (int x = tid; x < 16 * (D / 4); x += 64 * KA_W) {
+      const int row = x / (D / 4), d = 4 * (x - row * (D / 4));
+      const int i = 16 * t + row;
+      if (i >= e.rows) continue;
+      float m = -INFINITY, sum2 = 0.f;
+      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < KA_W; ++w) m = fmaxf(m, sh.m[w][row]);
+#pragma unroll
+      for (int w = 0; w < KA_W; ++w) {
+        if (sh.m[w][row] == -INFINITY) continue;
+        const float f = fast_exp2(sh.m[w][row] - m);
+        sum2 += f * sh.l[w][row];
+        acc += f * *(const f32x4*)&so[w][row][d];
+      }
+      if (pc.slot == nullptr) {
+        const int qrow = e.row0 + i, j = qrow / a.group;
+        const int64_t at_o = ((int64_t)b * a.T + j) * a.H + h * a.group + (qrow - j * a.group);
+        const float inv = sum2 == 0.f ? 0.f : 1.f / sum2;
+        *(u32x2*)(a.o + at_o * D + d) = u32x2{h16<BF16>::pack(acc[0] * inv, acc[1] * inv),
+                                              h16<BF16>::pack(acc[2] * inv, acc[3] * inv)};
+        if (a.lse && d == 0) a.lse[at_o] = sum2 == 0.f ? -INFINITY : m + __log2f(sum2);
+      } else {
+        *(f32x4*)(pc.slot + i * D + d) = acc;
+        if (d == 0) {
+          pc.slot[MT * D + i] = m;
+          pc.slot[MT * D + MT + i] = sum2;
+        }
+      }
+    }
+    __syncthreads();
+  }
+}
+
+template <int D, int QT, bool BF16, int NP>
+__global__ __launch_bounds__(64 * KA_W, ka_per_cu(D, QT)) void kv4_attn_ranges(const KaArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  constexpr int MT = 16 * QT;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[KA_W * ka_stages<D, QT>() * Stage<D>::BYTES];
+  __shared__ KaShared sh;
+  __shared__ int64_t find[KA_W + 3];
+  const int tid = threadIdx.x;
+  const int h = blockIdx.x % a.c.Hkv, r = blockIdx.x / a.c.Hkv;
 
   int64_t lo = 0, hi = 0;
-  const KaPoint start = ka_find<MT>(a, sh, [&](int64_t total) {
+  const KaPoint start = ka_find<MT>(a, find, [&](int64_t total) {
     const int ng = (int)min((int64_t)a.G, total);
     if (r < ng) {
-      lo = ka_cut(total, ng, r);
-      hi = ka_cut(total, ng, r + 1);
+      const KaCuts cuts(total, ng);
+      lo = cuts.at(r);
+      hi = cuts.at(r + 1);
     }
     return r < ng ? lo : (int64_t)-1;
   });
   if (h == 0 && tid == 0) {
     KaCut cut{-1, 0, 0, 0};
     const int ng = (int)min((int64_t)a.G, start.total);
-    if (lo < hi && start.before < lo && ka_cut(start.total, ng, r - 1) <= start.before) {
+    const KaCuts cuts(start.total, max(1, ng));
+    if (lo < hi && start.before < lo && cuts.at(r - 1) <= start.before) {
       const int units = ka_entry<MT>(a, ka_len(a, start.b), ka_new(a, start.b), start.rt).units;
       const int64_t end = start.before + units + KA_PIECE;
       int p1 = r;
-      for (int step = 1 << 10; step; step >>= 1)  // G <= 768
-        if (p1 + step < ng && ka_cut(start.total, ng, p1 + step) < end) p1 += step;
+#pragma unroll 1
+      for (int step = 512; step; step >>= 1)
+        if (p1 + step < ng && cuts.at(p1 + step) < end) p1 += step;
       const int p0 = ka_unit_at(lo, start.before, units) > 0 ? r - 1 : r;
       if (p1 > p0) cut = KaCut{start.b, start.rt, p0, p1};
     }
@@ -275,387 +786,24 @@ __global__ __launch_bounds__(64 * KA_W, ka_per_cu(D, QT)) void kv4_attn_ranges(c
   }
   if (lo >= hi) return;  // whole workgroup
 
-  const int64_t k_head = (int64_t)h * c.page * (D / 2), ks_head = (int64_t)h * c.page * NK;
-  const int kg = jl >> 2, kr = jl & 3;  // the lane's K rows: tokens 8 kg + kr and + 4; its V rows: 8 g .. + 7
-
-  // LDS-DMA: what the lane fetches with each instruction of a tile, from where the tile (PG: it lies in one page) or the
-  // slot's eight tokens (`grp` of them) begin
-  uint32_t off_c[St::NC], off_s[St::NS];
-  int grp_c[St::NC], grp_s[St::NS];
-#pragma unroll
-  for (int j = 0; j < St::NC; ++j) {
-    const bool is_v = 64 * j + lane >= D;
-    const int p = 64 * j + lane - (is_v ? D : 0);
-    int tok = 0, byte = 0;
-    unroll<0, S::N>([&](auto s) {
-      constexpr int W = S::w(s), B0 = S::base(s);
-      const int x = p - B0;
-      if (x < 0 || x >= 16 * W) return;
-      if (is_v) {
-        tok = 8 * (x / (W / 2) % 4) + x / (2 * W);
-        byte = B0 / 2 + 16 * (x % (W / 2));
-      } else {
-        const int m = x % 16, ax = x / 16;
-        tok = 8 * (m >> 2) + 4 * (ax / (W / 2)) + (m & 3);
-        byte = B0 / 2 + 16 * (ax % (W / 2));
-      }
-    });
-    grp_c[j] = tok >> 3;
-    off_c[j] = (uint32_t)((is_v ? c.Hkv * c.page * (D / 2) : 0) + (PG ? tok : tok & 7) * (D / 2) + byte);
-  }
-#pragma unroll
-  for (int j = 0; j < St::NS; ++j) {
-    const int x = 64 * j + lane < D / 2 ? 64 * j + lane : 0;  // lanes past the scales fetch the first word again
-    const int half = x / (8 * NK), blk = x / 8 % NK, w = x % 8;
-    grp_s[j] = w >> 1;
-    off_s[j] = (uint32_t)((half * c.Hkv * NK + blk) * c.page + (PG ? 4 * w : 4 * (w & 1)));
-  }
-  // LDS reads
-  const uint32_t ring = lds_u32(smem) + wave * (NST * St::BYTES);
-  const uint32_t k64 = 256 * (g >> 1) + 16 * jl + 8 * (g & 1), k32 = 16 * jl + 4 * g;
-  const uint32_t ks_l = 8 * kg + kr, vs_l = 8 * g;
-
+  const KaFetch<D, NP> fetch(a.c, tid & 63);
   int64_t before = start.before;
   int rt = start.rt;
   for (int b = start.b; b < a.B && before < hi; ++b, rt = 0) {
     const int L = ka_len(a, b), n = ka_new(a, b), rts = ka_tiles<MT>(a, n);
     for (; rt < rts && before < hi; ++rt) {
-      const KaEntry e = ka_entry<MT>(a, L, n, rt);
+      KaPiece pc;
+      pc.e = ka_entry<MT>(a, L, n, rt);
       const int64_t at = before;
-      before += e.units + KA_PIECE;
-      const int u0 = ka_unit_at(lo, at, e.units), u1 = ka_unit_at(hi, at, e.units);
-      if (u0 >= u1 && !(e.units == 0 && lo <= at)) continue;
-
-      // Q: column jl of each 16-row tile, as (one or two terms of) bf16
-      u32x4 q[QN][QT][NK];
-      int lim[QT];
-#pragma unroll
-      for (int t = 0; t < QT; ++t) {
-        const int i = 16 * t + jl;
-        const int row = e.row0 + i, j = row / a.group;
-        const bool live = i < e.rows;
-        lim[t] = live && a.causal ? max(0, L - n + 1 + j) : e.keys;
-        const uint16_t* p = a.q + b * a.qb + j * a.qr + (int64_t)(h * a.group + row - j * a.group) * D;
-        unroll<0, S::N>([&](auto s) {
-          constexpr int W = S::w(s), B0 = S::base(s);
-#pragma unroll
-          for (int w = 0; w < W / 2; ++w) {
-            u32x4 x = live ? *(const u32x4*)(p + B0 + 4 * W * g + 8 * w) : u32x4{0, 0, 0, 0};
-#pragma unroll
-            for (int i2 = 0; i2 < 4; ++i2) x[i2] ^= a.q_sign;
-            if constexpr (BF16) {
-              q[0][t][B0 / 32 + w] = x;
-            } else {
-              u32x4 xh, xl;
-#pragma unroll
-              for (int i2 = 0; i2 < 4; ++i2) {
-                const float y0 = h16<false>::lo(x[i2]), y1 = h16<false>::hi(x[i2]);
-                const uint32_t hw = h16<true>::pack(y0, y1);
-                const float z0 = h16<true>::lo(hw), z1 = h16<true>::hi(hw);
-                xh[i2] = hw;  // an infinity has nothing left
-                xl[i2] = h16<true>::pack(fabsf(z0) < INFINITY ? y0 - z0 : 0.f, fabsf(z1) < INFINITY ? y1 - z1 : 0.f);
-              }
-              q[0][t][B0 / 32 + w] = xh;
-              q[QN - 1][t][B0 / 32 + w] = xl;
-            }
-          }
-        });
-      }
-      f32x4 o[QT][ND];
-      float ref[QT], thr[QT], l[QT];
-#pragma unroll
-      for (int t = 0; t < QT; ++t) {
-        ref[t] = 0.f, thr[t] = -INFINITY, l[t] = 0.f;
-#pragma unroll
-        for (int i = 0; i < ND; ++i) o[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-      }
-
-      const int tend = min(e.keys, u1 * KA_UNIT);  // tokens from here on are not this piece's
-      int t0 = u0 * KA_UNIT + wave * KA_BN;
-      // the table is only read here: as constant memory its uniform reads are scalar
-      const auto* table = (const __attribute__((address_space(4))) int32_t*)(c.table + (int64_t)b * c.max_pages);
-      auto page_of = [&](int tok) { return (int)((uint64_t)(uint32_t)tok * a.page_mul >> a.page_shift); };
-      constexpr int NP = PG ? 1 : 4;  // pages of a tile: one, or one for each eight tokens
-      int pid[NP];
-      auto look_up = [&](int tk) {
-#pragma unroll
-        for (int i = 0; i < NP; ++i) {
-          pid[i] = -1;
-          if (tk + 8 * i < tend) pid[i] = table[page_of(tk + 8 * i)];
-        }
-      };
-      int at_issue = 0, at_read = 0;  // byte offsets of stages
-      auto issue = [&](int tk) {      // the tile whose pages were looked up last; then looks up the next
-        uint8_t* const dst = smem + wave * (NST * St::BYTES) + at_issue;
-        at_issue = at_issue + St::BYTES == NST * St::BYTES ? 0 : at_issue + St::BYTES;
-        auto lds = [&](int off) { return (__attribute__((address_space(3))) void*)(dst + off); };
-        if constexpr (PG) {
-          const bool ok = pid[0] >= 0 && pid[0] < c.pages;  // otherwise a buffer of no bytes: zeros
-          const int64_t p0 = ok ? pid[0] : 0, off = ok ? tk - page_of(tk) * c.page : 0;
-          const __amdgpu_buffer_rsrc_t rc = __builtin_amdgcn_make_buffer_rsrc(
-              (void*)(c.codes + p0 * c.codes_page + k_head + off * (D / 2)), (short)0, ok ? 0x7fffffff : 0, 0x00020000);
-          const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-              (void*)(c.scales + p0 * c.scales_page + ks_head + off), (short)0, ok ? 0x7fffffff : 0, 0x00020000);
-          if (a.once) {
-#pragma unroll
-            for (int j = 0; j < St::NC; ++j)
-              __builtin_amdgcn_raw_ptr_buffer_load_lds(rc, lds(1024 * j), 16, (int)off_c[j], 0, 0, CP_NT);
-          } else {
-#pragma unroll
-            for (int j = 0; j < St::NC; ++j)
-              __builtin_amdgcn_raw_ptr_buffer_load_lds(rc, lds(1024 * j), 16, (int)off_c[j], 0, 0, CP_PLAIN);
-          }
-#pragma unroll
-          for (int j = 0; j < St::NS; ++j)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, lds(St::CODES + 256 * j), 4, (int)off_s[j], 0, 0, 0);
-        } else {
-          const uint8_t *bc[4], *bs[4];
-          bool ok[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int p = pid[i % NP], tok = tk + 8 * i;
-            ok[i] = p >= 0 && p < c.pages;
-            const int64_t off = tok - page_of(tok) * c.page;
-            bc[i] = c.codes + p * c.codes_page + k_head + off * (D / 2);
-            bs[i] = c.scales + p * c.scales_page + ks_head + off;
-          }
-          auto from = [&](const uint8_t* const (&base)[4], int i, uint32_t off) {
-            const uint8_t* b = i == 0 ? base[0] : i == 1 ? base[1] : i == 2 ? base[2] : base[3];
-            const bool o = i == 0 ? ok[0] : i == 1 ? ok[1] : i == 2 ? ok[2] : ok[3];
-            return (const __attribute__((address_space(1))) void*)(o ? b + off : (const uint8_t*)ka_zeros);
-          };
-#pragma unroll
-          for (int j = 0; j < St::NC; ++j)
-            __builtin_amdgcn_global_load_lds(from(bc, grp_c[j], off_c[j]), lds(1024 * j), 16, 0, 0);
-#pragma unroll
-          for (int j = 0; j < St::NS; ++j)
-            __builtin_amdgcn_global_load_lds(from(bs, grp_s[j], off_s[j]), lds(St::CODES + 256 * j), 4, 0, 0);
-        }
-        look_up(tk + KA_UNIT);
-      };
-      auto read = [&](KaTile<D>& x) {
-        const uint32_t st = ring + at_read;
-        at_read = at_read + St::BYTES == NST * St::BYTES ? 0 : at_read + St::BYTES;
-        unroll<0, S::N>([&](auto s) {
-          constexpr int W = S::w(s), B0 = S::base(s);
-          constexpr int KO = 16 * B0, VO = 16 * (D + B0), KSO = St::CODES + B0, VSO = St::CODES + D + B0;
-          if constexpr (W == 8) {
-            u32x4 k0, k1;
-            u32x2 v[4];
-            ka_read128<KO, VO, KSO, VSO>(k0, k1, x.ks[0][s], x.ks[1][s], v, x.vs[s], st + 16 * lane, st + 4 * lane,
-                                         st + ks_l + 32 * g, st + vs_l + 32 * (jl >> 2));
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              x.k[0][B0 / 32 + i] = k0[i], x.k[1][B0 / 32 + i] = k1[i];
-              x.v[2 * i][s] = v[i][0], x.v[2 * i + 1][s] = v[i][1];
-            }
-          } else {
-            uint32_t v[8];
-            if constexpr (W == 4) {
-              u32x2 k0, k1;
-              ka_read64<KO, VO, KSO, VSO>(k0, k1, x.ks[0][s], x.ks[1][s], v, x.vs[s], st + k64, st + 2 * lane,
-                                          st + ks_l + 32 * (g >> 1), st + vs_l + 32 * (jl >> 3));
-#pragma unroll
-              for (int i = 0; i < 2; ++i) x.k[0][B0 / 32 + i] = k0[i], x.k[1][B0 / 32 + i] = k1[i];
-            } else {
-              ka_read32<KO, VO, KSO, VSO>(x.k[0][B0 / 32], x.k[1][B0 / 32], x.ks[0][s], x.ks[1][s], v, x.vs[s], st + k32,
-                                          st + lane, st + ks_l, st + vs_l);
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x.v[i][s] = v[i];
-          }
-        });
-      };
-
-      auto compute = [&](KaTile<D>& x, int tk, auto edge) {
-        constexpr bool EDGE = decltype(edge)::value;
-        f32x4 sc[QT][2];
-#pragma unroll
-        for (int t = 0; t < QT; ++t) sc[t][0] = sc[t][1] = f32x4{0.f, 0.f, 0.f, 0.f};
-        unroll<0, S::N>([&](auto s) {
-          constexpr int W = S::w(s), B0 = S::base(s);
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const float f = kv4::scale_of(x.ks[i][s]);
-#pragma unroll
-            for (int w = 0; w < W / 2; ++w) {
-              const uint32_t kw = x.k[i][B0 / 32 + w];
-              const u32x4 kf = {ka_cvt<0>(kw, f), ka_cvt<1>(kw, f), ka_cvt<2>(kw, f), ka_cvt<3>(kw, f)};
-#pragma unroll
-              for (int t = 0; t < QT; ++t)
-#pragma unroll
-                for (int u = 0; u < QN; ++u) sc[t][i] = ka_mma(kf, q[u][t][B0 / 32 + w], sc[t][i]);
-            }
-          }
-        });
-        u32x4 ph[QT], pl[QT];
-#pragma unroll
-        for (int t = 0; t < QT; ++t) {
-          float y[8], top = -INFINITY;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            y[i] = sc[t][i >> 2][i & 3];
-            if constexpr (EDGE) y[i] = tk + 8 * g + i < lim[t] ? y[i] * a.scale2 : -INFINITY;
-            top = fmaxf(top, y[i]);
-          }
-          if constexpr (!EDGE) top *= a.scale2;
-          if (__any(top > thr[t])) {
-            top = xhalf_max(xrow_max(top));  // over the four lanes of the column
-            const bool up = top > thr[t];
-            const float f = !up ? 1.f : thr[t] == -INFINITY ? 0.f : fast_exp2(ref[t] - top);
-            ref[t] = up ? top : ref[t];
-            thr[t] = up ? top + KA_SLACK : thr[t];
-            l[t] *= f;
-#pragma unroll
-            for (int i = 0; i < ND; ++i) o[t][i] *= f;
-          }
-#pragma unroll
-          for (int i = 0; i < 8; ++i) y[i] = fast_exp2(EDGE ? y[i] - ref[t] : fmaf(y[i], a.scale2, -ref[t]));
-          l[t] += ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t hw, lw;
-            ka_split(y[2 * i], y[2 * i + 1], hw, lw);
-            ph[t][i] = hw, pl[t][i] = lw;
-          }
-        }
-        bool odd = false;  // some V that 0 times is not 0, in a tile that not every row sees all of
-        if constexpr (EDGE) {
-          unroll<0, S::N>([&](auto s) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const uint32_t byte = (x.vs[s][i >> 2] >> (8 * (i & 3))) & 255u;
-              if (tk + 8 * g + i >= e.keys) {
-                x.v[i][s] = 0;
-                x.vs[s][i >> 2] &= ~(255u << (8 * (i & 3)));
-              } else {
-                odd |= byte > 252u;
-              }
-            }
-          });
-          odd = __any(odd);
-        }
-        auto values = [&](auto&& word, auto&& scale, auto&& use) {
-          unroll<0, S::N>([&](auto s) {
-            constexpr int W = S::w(s), B0 = S::base(s);
-            unroll<0, W / 2>([&](auto sel) {
-              uint32_t cv[8];
-#pragma unroll
-              for (int i = 0; i < 8; ++i) cv[i] = ka_cvt<sel>(word(i, s), scale(i, s));
-              u32x4 even, other;
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                even[i] = __builtin_amdgcn_perm(cv[2 * i + 1], cv[2 * i], 0x05040100);
-                other[i] = __builtin_amdgcn_perm(cv[2 * i + 1], cv[2 * i], 0x07060302);
-              }
-              use(B0 / 16 + 2 * sel, even);
-              use(B0 / 16 + 2 * sel + 1, other);
-            });
-          });
-        };
-        auto word = [&](int i, int s) { return x.v[i][s]; };
-        auto scale = [&](int i, int s) { return kv4::scale_of((x.vs[s][i >> 2] >> (8 * (i & 3))) & 255u); };
-        if (!EDGE || !odd) {
-          values(word, scale, [&](int d, u32x4 vf) {
-#pragma unroll
-            for (int t = 0; t < QT; ++t) o[t][d] = ka_mma(vf, pl[t], ka_mma(vf, ph[t], o[t][d]));
-          });
-        } else {
-          // row by row: what the row does not see is 0 before it meets the row's weight of 0
-          for (int t = 0; t < QT; ++t)
-            for (int col = 0; col < 16; ++col) {
-              const int seen = __shfl(lim[t], col, 64);
-              values([&](int i, int s) { return tk + 8 * g + i < seen ? x.v[i][s] : 0u; },
-                     [&](int i, int s) { return tk + 8 * g + i < seen ? scale(i, s) : 1.f; },
-                     [&](int d, u32x4 vf) {
-#pragma unroll
-                       for (int t2 = 0; t2 < QT; ++t2) {
-                         if (t2 != t) continue;
-                         const f32x4 y = ka_mma(vf, pl[t2], ka_mma(vf, ph[t2], o[t2][d]));
-#pragma unroll
-                         for (int i = 0; i < 4; ++i) o[t2][d][i] = jl == col ? y[i] : o[t2][d][i];
-                       }
-                     });
-            }
-        }
-      };
-
-      if (t0 < tend) {
-        KaTile<D> x;
-        look_up(t0);
-        int ti = t0;
-#pragma unroll
-        for (int i = 0; i < NST - 1; ++i, ti += KA_UNIT) issue(ti);
-        auto next = [&] {
-          issue(ti);
-          ti += KA_UNIT;
-          vm_wait<(NST - 1) * St::PER>();
-          read(x);
-        };
-        for (; t0 + KA_BN <= min(tend, e.keys_min); t0 += KA_UNIT) {  // seen whole by every row
-          next();
-          compute(x, t0, std::false_type{});
-        }
-        for (; t0 < tend; t0 += KA_UNIT) {
-          next();
-          compute(x, t0, std::true_type{});
-        }
-      }
-      vm_wait<0>();  // nothing may land in the exchange
-      __syncthreads();
-
-      // the waves' rows meet: 16 at a time
-      const bool whole = u0 == 0 && u1 == e.units;
-      float* slot = a.part + ((int64_t)(u0 == 0 ? 2 * r + 1 : 2 * r) * c.Hkv + h) * (MT * (D + 2));
-#pragma unroll
-      for (int t = 0; t < QT; ++t) {
-        float sum = l[t];
-        sum += __shfl_xor(sum, 16, 64);
-        sum += __shfl_xor(sum, 32, 64);
-        if (g == 0) {
-          sm[wave][jl] = thr[t] == -INFINITY && sum == 0.f ? -INFINITY : ref[t];
-          sl[wave][jl] = sum;
-        }
-        unroll<0, S::N>([&](auto s) {
-          constexpr int W = S::w(s), B0 = S::base(s);
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int d = 0; d < W; ++d) so[wave][jl][B0 + 4 * W * g + W * i + d] = o[t][B0 / 16 + d][i];
-        });
-        __syncthreads();
-        for (int x = tid; x < 16 * (D / 4); x += 64 * KA_W) {
-          const int row = x / (D / 4), d = 4 * (x - row * (D / 4));
-          const int i = 16 * t + row;
-          if (i >= e.rows) continue;
-          float m = -INFINITY, sum2 = 0.f;
-          f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int w = 0; w < KA_W; ++w) m = fmaxf(m, sm[w][row]);
-#pragma unroll
-          for (int w = 0; w < KA_W; ++w) {
-            if (sm[w][row] == -INFINITY) continue;
-            const float f = fast_exp2(sm[w][row] - m);
-            sum2 += f * sl[w][row];
-            acc += f * *(const f32x4*)&so[w][row][d];
-          }
-          if (whole) {
-            const int qrow = e.row0 + i, j = qrow / a.group;
-            const int64_t at_o = ((int64_t)b * a.T + j) * a.H + h * a.group + (qrow - j * a.group);
-            const float inv = sum2 == 0.f ? 0.f : 1.f / sum2;
-            *(u32x2*)(a.o + at_o * D + d) = u32x2{h16<BF16>::pack(acc[0] * inv, acc[1] * inv),
-                                                  h16<BF16>::pack(acc[2] * inv, acc[3] * inv)};
-            if (a.lse && d == 0) a.lse[at_o] = sum2 == 0.f ? -INFINITY : m + __log2f(sum2);
-          } else {
-            *(f32x4*)(slot + i * D + d) = acc;
-            if (d == 0) {
-              slot[MT * D + i] = m;
-              slot[MT * D + MT + i] = sum2;
-            }
-          }
-        }
-        __syncthreads();
-      }
+      before += pc.e.units + KA_PIECE;
+      const int u0 = ka_unit_at(lo, at, pc.e.units), u1 = ka_unit_at(hi, at, pc.e.units);
+      if (u0 >= u1 && !(pc.e.units == 0 && lo <= at)) continue;
+      pc.b = b, pc.h = h;
+      pc.t0 = u0 * KA_UNIT, pc.t1 = min(pc.e.keys, u1 * KA_UNIT);
+      pc.slot = nullptr;
+      if (u0 > 0 || u1 < pc.e.units)
+        pc.slot = a.part + ((int64_t)(u0 == 0 ? 2 * r + 1 : 2 * r) * a.c.Hkv + h) * (MT * (D + 2));
+      ka_piece<D, QT, BF16, NP>(a, pc, fetch, smem, sh);
     }
   }
 #endif
@@ -727,7 +875,7 @@ struct KaPlan {
 };
 KaPlan ka_plan(int64_t rows, int64_t Hkv, int64_t D) {
   KaPlan p;
-  p.qt = rows <= 16 ? 1 : 2;
+  p.qt = rows <= 16 || D > 128 ? 1 : 2;
   const int per_cu = ka_per_cu((int)D, p.qt);
   p.G = (int)std::max<int64_t>(1, KA_CUS * per_cu / Hkv);
   p.meta = (size_t)p.G * sizeof(KaCut);
@@ -738,10 +886,9 @@ KaPlan ka_plan(int64_t rows, int64_t Hkv, int64_t D) {
 template <int D, int QT, bool BF16>
 void ka_launch(const KaArgs& a, hipStream_t st) {
   const dim3 grid((unsigned)(a.G * a.c.Hkv));
-  if (a.c.page % KA_BN == 0)
-    kv4_attn_ranges<D, QT, BF16, true><<<grid, 64 * KA_W, 0, st>>>(a);
-  else
-    kv4_attn_ranges<D, QT, BF16, false><<<grid, 64 * KA_W, 0, st>>>(a);
+  if (a.c.page % 32 == 0) kv4_attn_ranges<D, QT, BF16, 1><<<grid, 64 * KA_W, 0, st>>>(a);
+  else if (a.c.page % 16 == 0) kv4_attn_ranges<D, QT, BF16, 2><<<grid, 64 * KA_W, 0, st>>>(a);
+  else kv4_attn_ranges<D, QT, BF16, 4><<<grid, 64 * KA_W, 0, st>>>(a);
   if (a.G == 1) return;
   // pieces per entry, on average: with many, four waves share a row
   const int rows = (int)std::min<int64_t>(16 * QT, (int64_t)a.T * a.group);
@@ -753,10 +900,10 @@ void ka_launch(const KaArgs& a, hipStream_t st) {
 }
 template <int D>
 void ka_go(const KaArgs& a, int qt, bool bf, hipStream_t st) {
-  if (qt == 1)
-    bf ? ka_launch<D, 1, true>(a, st) : ka_launch<D, 1, false>(a, st);
-  else
-    bf ? ka_launch<D, 2, true>(a, st) : ka_launch<D, 2, false>(a, st);
+  if constexpr (D <= 128) {
+    if (qt == 2) return bf ? ka_launch<D, 2, true>(a, st) : ka_launch<D, 2, false>(a, st);
+  }
+  bf ? ka_launch<D, 1, true>(a, st) : ka_launch<D, 1, false>(a, st);
 }
 
 }  // namespace
@@ -808,9 +955,11 @@ extern "C" int tlm_kv4_attn(const void* q, int64_t q_batch_stride, int64_t q_row
     return TLM_EINVAL;
   }
   c.max_pages = (int)max_pages, c.page = (int)page, c.Hkv = (int)H_kv, c.D = (int)D;
+  // (a scale of 0 becomes the least there is: masked scores are -inf, and -inf times 0 is no weight)
+  const float scale2 = std::max(fabsf(sm_scale) * 1.4426950408889634f, 0x1p-149f);
   KaArgs a{c, (const uint16_t*)q, q_batch_stride, q_row_stride, seqlens, count, (uint16_t*)o, lse,
            (KaCut*)ws, (float*)((char*)ws + p.meta), (int)B, (int)T, (int)H, (int)(H / H_kv), causal != 0, p.G, T * (H / H_kv) <= 16 * p.qt, 0, 0,
-           fabsf(sm_scale) * 1.4426950408889634f, sm_scale < 0.f ? 0x80008000u : 0u};
+           scale2, sm_scale < 0.f ? 0x80008000u : 0u};
   // with 2^(k-1) < page <= 2^k and m = floor(2^(31+k) / page) + 1: m page - 2^(31+k) <= 2^k, so that tok m / 2^(31+k) is
   // less than 1 / page above tok / page for tok < 2^31; and m fits 32 bits
   while ((1ll << a.page_shift) < page) ++a.page_shift;
