@@ -195,45 +195,59 @@ TLM_DEV void vm_wait() {  // all but the last N vector loads and LDS-DMA instruc
   __builtin_amdgcn_sched_barrier(0);
 }
 
-// K, V and scales of one segment: LDS addresses of the lane, waited for within the block.
-template <int KO, int VO, int KSO, int VSO>
-TLM_DEV void ka_read128(u32x4& k0, u32x4& k1, uint32_t& s0, uint32_t& s1, u32x2 (&v)[4], u32x2& vs, uint32_t ka,
-                        uint32_t va, uint32_t ksa, uint32_t vsa) {
-  asm volatile(
-      "ds_read_b128 %0, %9 offset:%13\n\t"
-      "ds_read_b128 %1, %9 offset:%14\n\t"
-      "ds_read_u8 %2, %11 offset:%15\n\t"
-      "ds_read_u8 %3, %11 offset:%16\n\t"
-      "ds_read2st64_b32 %4, %10 offset0:0 offset1:1\n\t"
-      "ds_read2st64_b32 %5, %10 offset0:2 offset1:3\n\t"
-      "ds_read2st64_b32 %6, %10 offset0:4 offset1:5\n\t"
-      "ds_read2st64_b32 %7, %10 offset0:6 offset1:7\n\t"
-      "ds_read2_b32 %8, %12 offset0:0 offset1:4\n\t"
-      "s_waitcnt lgkmcnt(0)"
-      : "=&v"(k0), "=&v"(k1), "=&v"(s0), "=&v"(s1), "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(vs)
-      : "v"(ka), "v"(va + VO), "v"(ksa), "v"(vsa + VSO), "i"(KO), "i"(KO + 1024), "i"(KSO), "i"(KSO + 16)
-      : "memory");
-}
-#define KA_READ_NARROW(NAME, KT, KOP, VOP, KSTEP, VSTEP)                                                             \
-  template <int KO, int VO, int KSO, int VSO>                                                                       \
-  TLM_DEV void NAME(KT& k0, KT& k1, uint32_t& s0, uint32_t& s1, uint32_t (&v)[8], u32x2& vs, uint32_t ka, uint32_t va, \
-                    uint32_t ksa, uint32_t vsa) {                                                                   \
-    asm volatile(KOP " %0, %13 offset:%17\n\t" KOP " %1, %13 offset:%18\n\t"                                         \
-                     "ds_read_u8 %2, %15 offset:%19\n\tds_read_u8 %3, %15 offset:%20\n\t" VOP                         \
-                     " %4, %14 offset:%22\n\t" VOP " %5, %14 offset:%23\n\t" VOP " %6, %14 offset:%24\n\t" VOP         \
-                     " %7, %14 offset:%25\n\t" VOP " %8, %14 offset:%26\n\t" VOP " %9, %14 offset:%27\n\t" VOP         \
-                     " %10, %14 offset:%28\n\t" VOP " %11, %14 offset:%29\n\t"                                       \
-                     "ds_read2_b32 %12, %16 offset0:0 offset1:4\n\ts_waitcnt lgkmcnt(0)"                                       \
-                 : "=&v"(k0), "=&v"(k1), "=&v"(s0), "=&v"(s1), "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]),  \
-                   "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7]), "=&v"(vs)                                    \
-                 : "v"(ka), "v"(va), "v"(ksa), "v"(vsa + VSO), "i"(KO), "i"(KO + KSTEP), "i"(KSO), "i"(KSO + 16),   \
-                   "i"(0), "i"(VO), "i"(VO + VSTEP), "i"(VO + 2 * VSTEP), "i"(VO + 3 * VSTEP), "i"(VO + 4 * VSTEP), \
-                   "i"(VO + 5 * VSTEP), "i"(VO + 6 * VSTEP), "i"(VO + 7 * VSTEP)                                    \
-                 : "memory");                                                                                       \
+// A segment's part of a tile for the lane, from its LDS addresses; waited for within the block. K with all scales first, V
+// only when the scores are done (fewer registers).
+template <int W, int KO, int KSO, int VSO>
+TLM_DEV void ka_read_k(uint32_t (&k0)[W / 2], uint32_t (&k1)[W / 2], uint32_t& s0, uint32_t& s1, u32x2& vs, uint32_t ka,
+                       uint32_t ksa, uint32_t vsa) {
+  std::conditional_t<W == 8, u32x4, std::conditional_t<W == 4, u32x2, uint32_t>> a, b;
+#define KA_READ_K(OP)                                                                                                 \
+  asm volatile(OP " %0, %5 offset:%8\n\t" OP " %1, %5 offset:%9\n\tds_read_u8 %2, %6 offset:%10\n\t"                  \
+                  "ds_read_u8 %3, %6 offset:%11\n\tds_read2_b32 %4, %7 offset0:0 offset1:4\n\ts_waitcnt lgkmcnt(0)"    \
+               : "=&v"(a), "=&v"(b), "=&v"(s0), "=&v"(s1), "=&v"(vs)                                                  \
+               : "v"(ka), "v"(ksa), "v"(vsa + VSO), "i"(KO), "i"(KO + 128 * W), "i"(KSO), "i"(KSO + 16)               \
+               : "memory")
+  if constexpr (W == 8) KA_READ_K("ds_read_b128");
+  else if constexpr (W == 4) KA_READ_K("ds_read_b64");
+  else KA_READ_K("ds_read_b32");
+#undef KA_READ_K
+  if constexpr (W == 2) {
+    k0[0] = a, k1[0] = b;
+  } else {
+#pragma unroll
+    for (int i = 0; i < W / 2; ++i) k0[i] = a[i], k1[i] = b[i];
   }
-KA_READ_NARROW(ka_read64, u32x2, "ds_read_b64", "ds_read_u16", 512, 128)
-KA_READ_NARROW(ka_read32, uint32_t, "ds_read_b32", "ds_read_u8", 256, 64)
-#undef KA_READ_NARROW
+}
+template <int W, int VO>
+TLM_DEV void ka_read_v(uint32_t (&v)[8], uint32_t va) {
+  if constexpr (W == 8) {
+    u32x2 x[4];
+    asm volatile(
+        "ds_read2st64_b32 %0, %4 offset0:0 offset1:1\n\t"
+        "ds_read2st64_b32 %1, %4 offset0:2 offset1:3\n\t"
+        "ds_read2st64_b32 %2, %4 offset0:4 offset1:5\n\t"
+        "ds_read2st64_b32 %3, %4 offset0:6 offset1:7\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3])
+        : "v"(va + VO)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = x[i >> 1][i & 1];
+  } else {
+#define KA_READ_V(OP)                                                                                                 \
+  asm volatile(OP " %0, %8 offset:%9\n\t" OP " %1, %8 offset:%10\n\t" OP " %2, %8 offset:%11\n\t" OP                  \
+                  " %3, %8 offset:%12\n\t" OP " %4, %8 offset:%13\n\t" OP " %5, %8 offset:%14\n\t" OP                 \
+                  " %6, %8 offset:%15\n\t" OP " %7, %8 offset:%16\n\ts_waitcnt lgkmcnt(0)"                           \
+               : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]),           \
+                 "=&v"(v[7])                                                                                          \
+               : "v"(va), "i"(VO), "i"(VO + 32 * W), "i"(VO + 64 * W), "i"(VO + 96 * W), "i"(VO + 128 * W),           \
+                 "i"(VO + 160 * W), "i"(VO + 192 * W), "i"(VO + 224 * W)                                              \
+               : "memory")
+    if constexpr (W == 4) KA_READ_V("ds_read_u16");
+    else KA_READ_V("ds_read_u8");
+#undef KA_READ_V
+  }
+}
 
 // Two codes of a word, times their scale, as 16-bit floats: exact in bf16; in fp16 for the scales of fits_f16.
 template <bool F16, int SEL>
@@ -338,7 +352,6 @@ TLM_DEV void ka_piece(const KaArgs& a, const KaPiece& pc, const KaFetch<D, NP>& 
   const int64_t k_head = (int64_t)h * c.page * (D / 2), ks_head = (int64_t)h * c.page * NK;
   const uint32_t ring = lds_u32(smem) + wave * (NST * St::BYTES);
   const uint32_t k64 = 256 * (g >> 1) + 16 * jl + 8 * (g & 1), k32 = 16 * jl + 4 * g;
-  const uint32_t ks_l = jl, vs_l = 4 * g;
 
   const int tend = pc.t1;
   int t0 = pc.t0 + wave * KA_BN;
@@ -423,37 +436,27 @@ TLM_DEV void ka_piece(const KaArgs& a, const KaPiece& pc, const KaFetch<D, NP>& 
       else get(false);
     }
   };
-  auto read = [&](KaTile<D>& x) {
+  auto read_k = [&](KaTile<D>& x) {  // and the scales
+    const uint32_t st = ring + at_read;
+    unroll<0, S::N>([&](auto s) {
+      constexpr int W = S::w(s), B0 = S::base(s);
+      uint32_t k0[W / 2], k1[W / 2];
+      ka_read_k<W, 16 * B0, St::CODES + B0, St::CODES + D + B0>(
+          k0, k1, x.ks[0][s], x.ks[1][s], x.vs[s], st + (W == 8 ? 16u * lane : W == 4 ? k64 : k32),
+          st + jl + 32 * (4 * W * g / 32), st + 4 * g + 32 * (W * jl / 32));
+#pragma unroll
+      for (int i = 0; i < W / 2; ++i) x.k[0][B0 / 32 + i] = k0[i], x.k[1][B0 / 32 + i] = k1[i];
+    });
+  };
+  auto read_v = [&](KaTile<D>& x) {  // and on to the next stage
     const uint32_t st = ring + at_read;
     at_read = at_read + St::BYTES == NST * St::BYTES ? 0 : at_read + St::BYTES;
     unroll<0, S::N>([&](auto s) {
       constexpr int W = S::w(s), B0 = S::base(s);
-      constexpr int KO = 16 * B0, VO = 16 * (D + B0), KSO = St::CODES + B0, VSO = St::CODES + D + B0;
-      if constexpr (W == 8) {
-        u32x4 k0, k1;
-        u32x2 v[4];
-        ka_read128<KO, VO, KSO, VSO>(k0, k1, x.ks[0][s], x.ks[1][s], v, x.vs[s], st + 16 * lane, st + 4 * lane,
-                                     st + ks_l + 32 * g, st + vs_l + 32 * (jl >> 2));
+      uint32_t v[8];
+      ka_read_v<W, 16 * (D + B0)>(v, st + W / 2 * lane);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          x.k[0][B0 / 32 + i] = k0[i], x.k[1][B0 / 32 + i] = k1[i];
-          x.v[2 * i][s] = v[i][0], x.v[2 * i + 1][s] = v[i][1];
-        }
-      } else {
-        uint32_t v[8];
-        if constexpr (W == 4) {
-          u32x2 k0, k1;
-          ka_read64<KO, VO, KSO, VSO>(k0, k1, x.ks[0][s], x.ks[1][s], v, x.vs[s], st + k64, st + 2 * lane,
-                                      st + ks_l + 32 * (g >> 1), st + vs_l + 32 * (jl >> 3));
-#pragma unroll
-          for (int i = 0; i < 2; ++i) x.k[0][B0 / 32 + i] = k0[i], x.k[1][B0 / 32 + i] = k1[i];
-        } else {
-          ka_read32<KO, VO, KSO, VSO>(x.k[0][B0 / 32], x.k[1][B0 / 32], x.ks[0][s], x.ks[1][s], v, x.vs[s], st + k32,
-                                      st + lane, st + ks_l, st + vs_l);
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x.v[i][s] = v[i];
-      }
+      for (int i = 0; i < 8; ++i) x.v[i][s] = v[i];
     });
   };
 
@@ -520,17 +523,21 @@ TLM_DEV void ka_piece(const KaArgs& a, const KaPiece& pc, const KaFetch<D, NP>& 
   };
 
   // What a last tile has beyond the keys becomes zeros of scale 1.
-  auto clear = [&](KaTile<D>& x, int tk) {
+  auto clear_scales = [&](KaTile<D>& x, int tk) {
     unroll<0, S::N>([&](auto s) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int at = 8 * (i & 3);
-        const bool out = tk + ka_token(g, i) >= e.keys;
-        x.v[i][s] = out ? 0u : x.v[i][s];
-        x.vs[s][i >> 2] = out ? (x.vs[s][i >> 2] & ~(255u << at)) | 127u << at : x.vs[s][i >> 2];
+        x.vs[s][i >> 2] = tk + ka_token(g, i) < e.keys ? x.vs[s][i >> 2] : (x.vs[s][i >> 2] & ~(255u << at)) | 127u << at;
       }
 #pragma unroll
-      for (int i = 0; i < 2; ++i) x.ks[i][s] = tk + 16 * i + jl >= e.keys ? 127u : x.ks[i][s];
+      for (int i = 0; i < 2; ++i) x.ks[i][s] = tk + 16 * i + jl < e.keys ? x.ks[i][s] : 127u;
+    });
+  };
+  auto clear_v = [&](KaTile<D>& x, int tk) {
+    unroll<0, S::N>([&](auto s) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x.v[i][s] = tk + ka_token(g, i) < e.keys ? x.v[i][s] : 0u;
     });
   };
   // Whether fp16 holds all V (bf16 queries) or K (fp16 queries) of the tile.
@@ -579,6 +586,8 @@ TLM_DEV void ka_piece(const KaArgs& a, const KaPiece& pc, const KaFetch<D, NP>& 
         }
       }
     }
+    read_v(x);
+    if constexpr (!ALL) clear_v(x, tk);
     if constexpr (!ALL && !PV16) {
       // NaN of V that a row does not see must not meet its weight of 0: such blocks become zeros, and the rows that see
       // one become NaN by their count of it
@@ -667,7 +676,7 @@ TLM_DEV void ka_piece(const KaArgs& a, const KaPiece& pc, const KaFetch<D, NP>& 
     for (; t0 + KA_BN <= whole_end; t0 += KA_UNIT) {
       next();
       KaTile<D> x;
-      read(x);
+      read_k(x);
       fast = suits(x);
       if (!fast) break;
       compute(x, t0, std::true_type{}, std::true_type{});
@@ -676,21 +685,18 @@ TLM_DEV void ka_piece(const KaArgs& a, const KaPiece& pc, const KaFetch<D, NP>& 
       for (; t0 < tend; t0 += KA_UNIT) {
         next();
         KaTile<D> x;
-        read(x);
-        clear(x, t0);
+        read_k(x);
+        clear_scales(x, t0);
         fast = suits(x);
         if (!fast) break;
         compute(x, t0, std::false_type{}, std::true_type{});
       }
-    if (!fast) {
-      at_read = at_read == 0 ? (NST - 1) * St::BYTES : at_read - St::BYTES;  // that tile again
-      for (bool first = true; t0 < tend; t0 += KA_UNIT, first = false) {
-        if (!first) next();
-        KaTile<D> x;
-        read(x);
-        clear(x, t0);
-        compute(x, t0, std::false_type{}, std::false_type{});
-      }
+    for (bool here = true; !fast && t0 < tend; t0 += KA_UNIT, here = false) {
+      if (!here) next();
+      KaTile<D> x;
+      read_k(x);
+      clear_scales(x, t0);
+      compute(x, t0, std::false_type{}, std::false_type{});
     }
   }
   vm_wait<0>();  // nothing may land in the exchange
