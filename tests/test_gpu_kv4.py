@@ -491,3 +491,22 @@ def test_ops_refusals():
         with pytest.raises(ValueError):
             f()
             raise AssertionError(i)
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_attn_random(seed):
+    """Batches, heads, dims, pages, lengths and new tokens at random: how the work is cut depends on all of them."""
+    r = np.random.RandomState(100 + seed)
+    D = int(r.choice([32, 64, 96, 128, 160, 192, 224, 256]))
+    Hkv = int(r.choice([1, 2, 3, 8]))
+    H = Hkv * int(r.choice([1, 2, 4, 5, 8, 17]))
+    page = int(r.choice([8, 16, 24, 32, 48, 64]))
+    B = int(r.choice([1, 2, 5, 20, 65, 130]))
+    T = int(r.choice([1, 1, 2, 7, 40])) if B <= 20 else int(r.choice([1, 3]))
+    top = int(np.exp(r.uniform(0, np.log(20000 // B))))
+    lens = r.randint(0, top + 1, B)
+    lens[r.randint(B)] = max(1, top)
+    count = r.randint(0, T + 1, B) if r.rand() < 0.5 else None
+    dtype = BF16 if r.rand() < 0.5 else F16
+    q, c, s, bt = _attn_case(dtype, B, T, H, Hkv, D, page, list(lens), seed)
+    _check(q, *_stale(c, s, bt, lens, page), bt, lens, count, bool(r.rand() < 0.7))

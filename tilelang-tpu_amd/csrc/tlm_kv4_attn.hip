@@ -11,7 +11,7 @@ using ldsop::unroll;
 constexpr int KA_W = 4;          // waves per workgroup
 constexpr int KA_BN = 32;        // tokens per tile (one wave)
 constexpr int KA_UNIT = KA_W * KA_BN;
-constexpr int KA_PIECE = 1;      // cost of a piece beside its units, in units
+constexpr int KA_PIECE = 2;      // cost of a piece beside its units, in units
 // Workgroups per CU, and stages of a ring in their share of the LDS.
 constexpr int ka_per_cu(int D, int QT) { return QT == 1 ? (D <= 128 ? 3 : 2) : D <= 128 ? 2 : 1; }
 template <int D, int QT>
@@ -39,6 +39,7 @@ struct KaArgs {
   KaCut* cuts;  // [G]: the entry that the cut before range r goes through, if it is the entry's first
   float* part;  // [2 G][Hkv][16 QT][D + 2]: rows, their references, their sums
   int B, T, H, group, causal, G;
+  int few;            // ka_find64 will do
   int once;           // codes are read by one row tile only: past the caches
   uint32_t page_mul;  // tok / page = tok page_mul >> page_shift, for tok < 2^31
   int page_shift;
@@ -89,6 +90,12 @@ struct KaCuts {
     }
   }
   TLM_DEV int64_t at(int r) const { return quot * r + rem * (uint32_t)r / g; }
+  TLM_DEV int range_of(int64_t x, int64_t total) const {  // the one that holds x: estimated, then exact
+    int r = max(0, min((int)g - 1, (int)((float)x * (float)g / (float)total)));
+    while (at(r) > x) --r;
+    while (r + 1 < (int)g && at(r + 1) <= x) ++r;
+    return r;
+  }
 };
 
 // Units of an entry at cost `before` that fall into range [lo, hi): none of its first KA_PIECE.
@@ -100,7 +107,7 @@ TLM_DEV int ka_unit_at(int64_t x, int64_t before, int units) {
 // The whole cost, and the entry that holds position `at` of it (at < 0: none); by a block of KA_W waves.
 struct KaPoint {
   int64_t total, before;
-  int b, rt;
+  int b, rt, L, n;
 };
 template <int MT, typename F>
 TLM_DEV KaPoint ka_find(const KaArgs& a, int64_t* sh, F&& want) {
@@ -150,6 +157,42 @@ TLM_DEV KaPoint ka_find(const KaArgs& a, int64_t* sh, F&& want) {
   p.before = sh[KA_W];
   p.b = (int)sh[KA_W + 1];
   p.rt = (int)sh[KA_W + 2];
+  p.L = at >= 0 ? ka_len(a, p.b) : 0;
+  p.n = at >= 0 ? ka_new(a, p.b) : 0;
+  return p;
+}
+// The same for up to 64 sequences, a lane each, by every wave for itself: no barrier, one trip to memory.
+template <int MT, typename F>
+TLM_DEV KaPoint ka_find64(const KaArgs& a, F&& want) {
+  const int lane = threadIdx.x & 63;
+  int L = 0, n = 0, mine = 0;  // (the caller has made sure that all costs together fit)
+  if (lane < a.B) {
+    L = ka_len(a, lane), n = ka_new(a, lane);
+    const int rts = ka_tiles<MT>(a, n);
+    for (int rt = 0; rt < rts; ++rt) mine += ka_entry<MT>(a, L, n, rt).units + KA_PIECE;
+  }
+  int x = mine;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(x, o, 64);
+    if (lane >= o) x += y;
+  }
+  KaPoint p{};
+  const int total = __builtin_amdgcn_readlane(x, 63);
+  p.total = total;
+  const int at = (int)want((int64_t)total);
+  const uint64_t m = __ballot(at >= x - mine && at < x);
+  if (m == 0) return p;
+  p.b = __builtin_ctzll(m);
+  p.L = __builtin_amdgcn_readlane(L, p.b);
+  p.n = __builtin_amdgcn_readlane(n, p.b);
+  int s = __builtin_amdgcn_readlane(x - mine, p.b);
+  for (;; ++p.rt) {
+    const int cost = ka_entry<MT>(a, p.L, p.n, p.rt).units + KA_PIECE;
+    if (at < s + cost) break;
+    s += cost;
+  }
+  p.before = s;
   return p;
 }
 
@@ -765,7 +808,7 @@ __global__ __launch_bounds__(64 * KA_W, ka_per_cu(D, QT)) void kv4_attn_ranges(c
   const int h = blockIdx.x % a.c.Hkv, r = blockIdx.x / a.c.Hkv;
 
   int64_t lo = 0, hi = 0;
-  const KaPoint start = ka_find<MT>(a, find, [&](int64_t total) {
+  auto want = [&](int64_t total) {
     const int ng = (int)min((int64_t)a.G, total);
     if (r < ng) {
       const KaCuts cuts(total, ng);
@@ -773,20 +816,19 @@ __global__ __launch_bounds__(64 * KA_W, ka_per_cu(D, QT)) void kv4_attn_ranges(c
       hi = cuts.at(r + 1);
     }
     return r < ng ? lo : (int64_t)-1;
-  });
+  };
+  const KaPoint start = a.few ? ka_find64<MT>(a, want) : ka_find<MT>(a, find, want);
   if (h == 0 && tid == 0) {
     KaCut cut{-1, 0, 0, 0};
-    const int ng = (int)min((int64_t)a.G, start.total);
-    const KaCuts cuts(start.total, max(1, ng));
-    if (lo < hi && start.before < lo && cuts.at(r - 1) <= start.before) {
-      const int units = ka_entry<MT>(a, ka_len(a, start.b), ka_new(a, start.b), start.rt).units;
-      const int64_t end = start.before + units + KA_PIECE;
-      int p1 = r;
-#pragma unroll 1
-      for (int step = 512; step; step >>= 1)
-        if (p1 + step < ng && cuts.at(p1 + step) < end) p1 += step;
-      const int p0 = ka_unit_at(lo, start.before, units) > 0 ? r - 1 : r;
-      if (p1 > p0) cut = KaCut{start.b, start.rt, p0, p1};
+    if (lo < hi && start.before < lo) {
+      const int ng = (int)min((int64_t)a.G, start.total);
+      const KaCuts cuts(start.total, ng);
+      if (cuts.at(r - 1) <= start.before) {
+        const int units = ka_entry<MT>(a, start.L, start.n, start.rt).units;
+        const int p0 = cuts.range_of(start.before + KA_PIECE, start.total);
+        const int p1 = cuts.range_of(start.before + KA_PIECE + units - 1, start.total);
+        if (units > 0 && p1 > p0) cut = KaCut{start.b, start.rt, p0, p1};
+      }
     }
     a.cuts[r] = cut;
   }
@@ -796,7 +838,8 @@ __global__ __launch_bounds__(64 * KA_W, ka_per_cu(D, QT)) void kv4_attn_ranges(c
   int64_t before = start.before;
   int rt = start.rt;
   for (int b = start.b; b < a.B && before < hi; ++b, rt = 0) {
-    const int L = ka_len(a, b), n = ka_new(a, b), rts = ka_tiles<MT>(a, n);
+    const int L = b == start.b ? start.L : ka_len(a, b), n = b == start.b ? start.n : ka_new(a, b);
+    const int rts = ka_tiles<MT>(a, n);
     for (; rt < rts && before < hi; ++rt) {
       KaPiece pc;
       pc.e = ka_entry<MT>(a, L, n, rt);
@@ -961,10 +1004,12 @@ extern "C" int tlm_kv4_attn(const void* q, int64_t q_batch_stride, int64_t q_row
     return TLM_EINVAL;
   }
   c.max_pages = (int)max_pages, c.page = (int)page, c.Hkv = (int)H_kv, c.D = (int)D;
+  const int64_t tiles = (T * (H / H_kv) + 16 * p.qt - 1) / (16 * p.qt);
+  const int few = B <= 64 && tiles <= INT32_MAX / (64 * (max_pages * page / KA_UNIT + 1 + KA_PIECE));
   // (a scale of 0 becomes the least there is: masked scores are -inf, and -inf times 0 is no weight)
   const float scale2 = std::max(fabsf(sm_scale) * 1.4426950408889634f, 0x1p-149f);
   KaArgs a{c, (const uint16_t*)q, q_batch_stride, q_row_stride, seqlens, count, (uint16_t*)o, lse,
-           (KaCut*)ws, (float*)((char*)ws + p.meta), (int)B, (int)T, (int)H, (int)(H / H_kv), causal != 0, p.G, T * (H / H_kv) <= 16 * p.qt, 0, 0,
+           (KaCut*)ws, (float*)((char*)ws + p.meta), (int)B, (int)T, (int)H, (int)(H / H_kv), causal != 0, p.G, few, T * (H / H_kv) <= 16 * p.qt, 0, 0,
            scale2, sm_scale < 0.f ? 0x80008000u : 0u};
   // with 2^(k-1) < page <= 2^k and m = floor(2^(31+k) / page) + 1: m page - 2^(31+k) <= 2^k, so that tok m / 2^(31+k) is
   // less than 1 / page above tok / page for tok < 2^31; and m fits 32 bits
