@@ -440,8 +440,9 @@ int tlm_kv_append_fp8(const void* x, int64_t x_batch_stride, int64_t x_row_strid
  *   codes   uint8 [pages, 2, H_kv, page, D / 2]: index 0 is K, 1 is V; the even dim in the low half of its
  *           byte. 16-byte aligned; codes_page_stride bytes from page to page (a multiple of 16, so the pools
  *           of several layers may alternate), the rest dense.
- *   scales  uint8 [pages, 2, H_kv, D / 32, page]: exponent + 127; 255 is NaN. 8-byte aligned,
- *           scales_page_stride bytes from page to page (a multiple of 8).
+ *   scales  uint8 [pages, 2, H_kv, D / 32, page]: exponent + 127, 1 .. 252; 255 is NaN (253 and 254, whose
+ *           larger values overflow fp32, are never written). 8-byte aligned, scales_page_stride bytes from page to page (a
+ *           multiple of 8).
  *   D       a multiple of 32, 32 .. 256; page a multiple of 8; pages and H_kv >= 1.
  * Pools may be of any size (64-bit offsets). Table entries outside [0, pages) are read as zeros and never
  * written through. */
@@ -482,7 +483,8 @@ int tlm_kv4_read(const void* codes, int64_t codes_page_stride, const void* scale
  *           glse of tlm_flash_attn_splitkv_fwd). A query without a key gets zeros and -inf; rows j >= count[b] are
  *           left as they were.
  *   sm_scale in the natural-log domain. Products, softmax and sums are fp32; the weights of V are rounded
- *           to 16 bits of precision (dtype F16) or to fp16's 11 (BF16).
+ *           to 16 bits of precision (dtype F16) or to fp16's 11 (BF16). Sums of V beyond 2^110 overflow. A call's bits
+ *           depend on its lengths and counts alone.
  *   ws      tlm_kv4_attn_workspace_bytes(...) bytes, 16-byte aligned (device memory, caller-owned; needs no
  *           initial value; a size for T is enough for fewer rows and any B). Calls that overlap in time, and graphs whose replays may, need one each. */
 size_t tlm_kv4_attn_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t H_kv, int64_t D);

@@ -171,8 +171,9 @@ def _check(q, codes, scales, bt, lens, count=None, causal=True, scale=None, got=
     and the cached values are exact in its operands): off by at most (D + 2) 2^-24 of the sum of
     magnitudes A. A weight is off by that times ln 2 log2 e = 1, by exp2 (1 ulp, and its argument's
     rounding against a reference within the scores' range: 2 A 2^-24) and by its rounding where it multiplies V: with fp16
-    queries two bf16 terms (2^-17), with bf16 ones fp16 (half a step is 2^-11; weights under fp16's normal range, which
-    are below 2^-21 of the largest, by 2^-25 / 2^7 of it, less than the 2^-24 that is counted for each key below).
+    queries two bf16 terms (2^-17), with bf16 ones fp16 (half a step is 2^-11, and half of fp16's smallest, 2^-25, where
+    the largest weight is 2^11 at least: n 2^-36 of the largest |v| of the dim in all; where the key that has the
+    weight has a V of 0, as in one of 64 keys at 57 bits above the others, that is more than the rest).
     Numerator and denominator are sums of up to n weights, (n + 64) 2^-24 each; the quotient is
     rounded once: by eps / 2, or half of the smallest subnormal, tiny eps / 2 (an output of 4.5e-7 is
     0.46 of fp16's 2^-24 steps off its nearest multiple: no fp16 value is nearer)."""
@@ -192,13 +193,21 @@ def _check(q, codes, scales, bt, lens, count=None, causal=True, scale=None, got=
     for b in range(B):
         n = max(0, min(int(lens[b]), bt.shape[1] * page))
         m = T if count is None else max(0, min(int(count[b]), T))
-        k, _ = ref.kv4_rows_ref(c, s, bt, b, 0, n)
+        k, v = ref.kv4_rows_ref(c, s, bt, b, 0, n)
         k = np.abs(k).repeat(H // codes.shape[2], 1).transpose(1, 2, 0)
         a = np.abs(q[b, :m].double().numpy()).transpose(1, 0, 2) @ k * abs(sm) if n else np.zeros((H, m, 1))
         a = a.max(-1).T[..., None]  # [m, H, 1]
+        v = np.nan_to_num(np.abs(v)).max(0, initial=0.0).repeat(H // codes.shape[2], 0)  # [H, D]
+        small = n * 2.0 ** -36 * v if q.dtype == BF16 else 0.0
         rel = 2 * ((D + 4) * 2.0 ** -24 * a + 2.0 ** -23 + (n + 64) * 2.0 ** -24) + weight
         x, e = out[b, :m].double().numpy(), exp[b, :m]
-        bad = np.abs(x - e) > eps * (1 + 2 ** -10) * np.abs(e) + rel * spread[b, :m] + least
+        # beyond the type's range values become infinite, surely so by more than they may be off
+        lim, most = eps * (1 + 2 ** -10) * np.abs(e) + rel * spread[b, :m], torch.finfo(q.dtype).max * (1 + eps)
+        inf = np.abs(e) - lim > most
+        assert (x[inf] == np.copysign(np.inf, e[inf])).all()
+        inf |= np.isinf(x) & (np.abs(e) + lim > most)
+        x, e = np.where(inf, 0.0, x), np.where(inf, 0.0, e)
+        bad = np.abs(x - e) > eps * (1 + 2 ** -10) * np.abs(e) + rel * spread[b, :m] + small + least
         assert not bad.any(), (b, np.abs(x - e).max())
         assert np.array_equal(np.isnan(x), np.isnan(e))
         assert (out[b, m:] == 9).all()
@@ -315,6 +324,51 @@ def test_attn_nan_and_extreme_blocks():
     assert torch.equal(out.isnan(), nan)
     keep = [2, 3]
     _check(q[keep], c, s, bt[keep], [100, 100], got=(out[keep], lse[keep]))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("D,T,H,Hkv", [(64, 1, 8, 2), (128, 1, 4, 4), (128, 9, 8, 2), (256, 1, 8, 1), (96, 3, 4, 2)])
+def test_attn_scales_outside_fp16(dtype, D, T, H, Hkv):
+    """Blocks of K and V whose values fp16 does not hold, from some tile on, in single tiles and in the last one; and
+    blocks of zeros."""
+    lens = [900, 333, 64, 31]
+    q, c, s, bt = _attn_case(dtype, 4, T, H, Hkv, D, 16, lens, D + T)
+    page = lambda b, p: (int(bt[b, p // 16]), p % 16)
+    for b, first, n in ((0, 500, 3), (0, 890, 10), (1, 0, 2), (1, 332, 1), (3, 5, 1)):
+        for p in range(first, first + n):
+            i, off = page(b, p)
+            s[i, 1, :, :, off] = torch.tensor([60, 100, 141, 200])[p % 4]  # V
+            s[i, 0, :, 0, off] = torch.tensor([1, 40, 108, 90])[p % 4]     # K: next to nothing
+    i, off = page(2, 40)
+    s[i, 0, :, :, off] = 143  # a key of up to 6 2^16, seen by queries scaled down
+    q[2] = (q[2].float() * 2.0 ** -12).to(dtype)
+    i, off = page(0, 100)
+    c[i, :, :, off], s[i, :, :, :, off] = 0, 1  # zeros
+    _check(q, *_stale(c, s, bt, lens, 16), bt, lens)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("T,H,Hkv,D", [(5, 4, 2, 128), (40, 4, 1, 64), (3, 8, 8, 256), (6, 2, 1, 96)])
+def test_attn_nan_of_later_tokens(dtype, T, H, Hkv, D):
+    """A NaN of V or K at a position makes NaN of the queries at and behind it, and of none before it."""
+    lens = [77, T, 200]
+    q, c, s, bt = _attn_case(dtype, 3, T, H, Hkv, D, 16, lens, T + 31)
+    clean = _run(q, c, s, bt, lens)
+    at = [lens[0] - 2, lens[1] - 1, lens[2] - T]  # seen by the last two, the last, all
+    for b, p in enumerate(at):
+        s[int(bt[b, p // 16]), 1 if b != 1 else 0, Hkv - 1, D // 32 - 1, p % 16] = 255
+    out, lse = _run(q, c, s, bt, lens)
+    nan = torch.zeros(out.shape, dtype=torch.bool)
+    head = H - H // Hkv
+    nan[0, T - 2:, head:, D - 32:] = True
+    nan[1, T - 1:, head:] = True
+    nan[2, :, head:, D - 32:] = True
+    assert torch.equal(out.isnan(), nan)
+    assert torch.equal(lse.isnan(), nan.all(-1))
+    # the others as before, but for the form in which the tile was computed
+    eps = torch.finfo(dtype).eps
+    err = (out.float() - clean[0].float()).abs()[~nan]
+    assert (err <= 2 * eps * clean[0].float().abs()[~nan] + 2.0 ** -9 * clean[0].float().abs().max()).all()
 
 
 def test_attn_strided_queries_and_layers():

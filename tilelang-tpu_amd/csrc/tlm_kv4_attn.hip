@@ -990,7 +990,7 @@ extern "C" int tlm_kv4_attn(const void* q, int64_t q_batch_stride, int64_t q_row
     return TLM_EINVAL;
   }
   if (B == 0 || T == 0) return TLM_OK;
-  if (H > INT32_MAX / B || T > INT32_MAX / (B * H)) {
+  if (H > (INT32_MAX - 64) / B || T > (INT32_MAX - 64) / (B * H)) {
     tlm_set_error("tlm_kv4_attn: problem too large (2^31 query rows)");
     return TLM_EINVAL;
   }
