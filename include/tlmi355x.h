@@ -483,8 +483,8 @@ int tlm_kv4_read(const void* codes, int64_t codes_page_stride, const void* scale
  *           glse of tlm_flash_attn_splitkv_fwd). A query without a key gets zeros and -inf; rows j >= count[b] are
  *           left as they were.
  *   sm_scale in the natural-log domain. Products, softmax and sums are fp32; the weights of V are rounded
- *           to 16 bits of precision (dtype F16) or to fp16's 11 (BF16). Sums of V beyond 2^110 overflow. A call's bits
- *           depend on its lengths and counts alone.
+ *           to 16 bits of precision (dtype F16) or to fp16's 11 (BF16). Sums of V beyond 2^110 overflow. How the
+ *           keys are cut, and so the last bits, depends on all lengths and counts of the call, never on timing.
  *   ws      tlm_kv4_attn_workspace_bytes(...) bytes, 16-byte aligned (device memory, caller-owned; needs no
  *           initial value; a size for T is enough for fewer rows and any B). Calls that overlap in time, and graphs whose replays may, need one each. */
 size_t tlm_kv4_attn_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t H_kv, int64_t D);

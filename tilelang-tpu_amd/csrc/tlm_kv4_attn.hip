@@ -1,4 +1,36 @@
-// Grouped-query attention over the 4-bit K/V cache (tlm_kv4_attn).
+// Grouped-query attention over the 4-bit K/V cache (tlm_kv4_attn): the newest tokens of each sequence attend to what is
+// cached of it. No program of the reference does this.
+//
+// Per query row: s_t = sm_scale q k_t, o = sum_t 2^((s_t - m) log2 e) v_t / sum_t 2^((s_t - m) log2 e) in one pass over the keys,
+// m a reference that follows the running maximum. A K/V head's rows are its new tokens times its query heads; a
+// workgroup holds 16 or 32 of them (QT).
+//
+// What bounds it: one new token, the stream of codes: 64 sequences of 512 .. 8,192 tokens, 32 / 8 heads of 128 (bf16): 304 MB
+// in 55 us, 5.5 TB/s; the same without the arithmetic 52 us. Few tokens, the chain launch, lengths, table, tile, exchange: 6.4 us
+// for one sequence of 1,000, 2.9 for the join. Prompt chunks, instruction issue: two chunks of 1,024 over 8,192 and 16,384
+// tokens 530 us (690 TFLOP/s); a 32-token tile of 32 rows issues 32 MFMAs (512 cycles), 64 conversions and 32 permutations (420) and
+// the softmax (340), which hide under each other little (one wave's MFMA and VALU work do not overlap at all).
+//
+//   * Partition: entry (sequence, row tile) costs its 128-token units plus KA_PIECE; the cost line of the batch is cut into
+//     G equal ranges, one workgroup each per K/V head, found from the lengths by the workgroups themselves. A
+//     range's part of an entry (a piece) is the output or, where the entry was cut, goes to the workspace, from where
+//     kv4_attn_join merges it. Pieces priced at 1 unit: 5 % slower at 24 sequences of 1 .. 2,047 tokens, the same elsewhere.
+//   * Its four waves take 32-token tiles in turn, each with its own reference, sums and O^T: no barrier until the piece
+//     ends. Every wave has an LDS ring of 2 to 4 tiles that it fills by LDS-DMA (one instruction per 64 blocks of 32 dims, one for
+//     all scales at D 128) with a per-lane order that makes every LDS read linear in the lane. Prefetch into registers, 13 loads
+//     per tile: 85 us instead of 79 at that stage, and per-lane addresses where a page id is now scalar.
+//   * S^T = K Q^T: a lane's 16 bytes of K are one block, so one scale; v_cvt_scalef32_pk_*_fp4 makes two operands of a byte,
+//     scale included, exactly. The MFMA leaves a lane the scores of 8 tokens of one query, and just those 8 tokens' rows of V
+//     are what O^T += V^T P^T wants of it: P never moves between lanes. V^T costs one permutation per pair of values.
+//   * Types: bf16 queries meet K in bf16 and their weights, as fp16 numbers, V in fp16 (half a step of a weight is 2^-12 to
+//     2^-11; the output's is 2^-9 to 2^-8). fp16 queries meet K in fp16, their weights V in bf16 in two terms, since one rounding
+//     to fp16 would show in an fp16 output (1.4 times its error). Where a scale does not suit fp16, the rest of the piece runs in
+//     bf16, weights and fp16 queries in two terms. Both forms in one loop would spill: with scratch memory in use the kernel
+//     above takes 68 instead of 55 us.
+//   * The reference of a row moves when a score passes it by 2^KA_SLACK only, so O is rescaled a few times per row.
+//   * Codes that only one row tile reads bypass the caches (74 -> 65 us); those of longer chunks are shared through the L2 of
+//     the XCD that the K/V head's workgroups are on (8 heads).
+//   * 64 rows per wave (one wave per SIMD): 680 instead of 555 us for the chunks.
 #include "tlm_kv4.h"
 
 #include <algorithm>
@@ -43,8 +75,8 @@ struct KaArgs {
   int once;           // codes are read by one row tile only: past the caches
   uint32_t page_mul;  // tok / page = tok page_mul >> page_shift, for tok < 2^31
   int page_shift;
-  float scale2;     // |sm_scale| log2(e)
-  uint32_t q_sign;  // the sign of sm_scale on both halves of a word
+  float scale2;       // |sm_scale| log2(e)
+  uint32_t q_sign;    // the sign of sm_scale on both halves of a word
 };
 
 // An entry of the cost line: 16 QT query rows of one sequence (rows run over its new tokens and, within one,
@@ -98,7 +130,7 @@ struct KaCuts {
   }
 };
 
-// Units of an entry at cost `before` that fall into range [lo, hi): none of its first KA_PIECE.
+// Position x of the cost line in units of an entry that starts at `before`: its KA_PIECE come first.
 TLM_DEV int ka_unit_at(int64_t x, int64_t before, int units) {
   const int64_t u = x - before - KA_PIECE;
   return u < 0 ? 0 : u > units ? units : (int)u;
@@ -292,7 +324,7 @@ TLM_DEV void ka_read_v(uint32_t (&v)[8], uint32_t va) {
   }
 }
 
-// Two codes of a word, times their scale, as 16-bit floats: exact in bf16; in fp16 for the scales of fits_f16.
+// Two codes of a word, times their scale, as 16-bit floats: exact in bf16; in fp16 for the scales that ka_not_f16 passes.
 template <bool F16, int SEL>
 TLM_DEV uint32_t ka_cvt(uint32_t w, float s) {
   if constexpr (F16)
@@ -367,7 +399,7 @@ struct KaFetch {
       part_c[j] = tok / PT;
       off_c[j] = (uint32_t)((is_v ? c.Hkv * c.page * (D / 2) : 0) + tok % PT * (D / 2) + byte);
     }
-  #pragma unroll
+#pragma unroll
     for (int j = 0; j < St::NS; ++j) {
       const int x = 64 * j + lane < D / 2 ? 64 * j + lane : 0;  // lanes past the scales fetch the first word again
       const int half = x / (8 * NK), blk = x / 8 % NK, tok = 4 * (x % 8);
@@ -746,7 +778,7 @@ TLM_DEV void ka_piece(const KaArgs& a, const KaPiece& pc, const KaFetch<D, NP>& 
   __syncthreads();
 
   // the waves' rows meet: 16 at a time
-  #pragma unroll
+#pragma unroll
   for (int t = 0; t < QT; ++t) {
     float sum = l[t];
     sum += __shfl_xor(sum, 16, 64);
