@@ -55,9 +55,9 @@ constexpr int ka_stages() {
 // that one by SLACK. At most 2^15, an fp16 number, and normal ones down to 2^-25 of the largest.
 constexpr float KA_BIAS = 11.f, KA_SLACK = 4.f;
 
-struct KaCut {
-  int b, rt;   // sequence (-1: nothing to join) and row tile
-  int p0, p1;  // first and last range that hold units of it
+struct alignas(32) KaCut {
+  int b, rt, n;  // sequence (-1: nothing to join), row tile, new tokens
+  int p0, p1;    // first and last range that hold units of it
 };
 
 struct KaArgs {
@@ -851,7 +851,7 @@ __global__ __launch_bounds__(64 * KA_W, ka_per_cu(D, QT)) void kv4_attn_ranges(c
   };
   const KaPoint start = a.few ? ka_find64<MT>(a, want) : ka_find<MT>(a, find, want);
   if (h == 0 && tid == 0) {
-    KaCut cut{-1, 0, 0, 0};
+    KaCut cut{-1, 0, 0, 0, 0};
     if (lo < hi && start.before < lo) {
       const int ng = (int)min((int64_t)a.G, start.total);
       const KaCuts cuts(start.total, ng);
@@ -859,7 +859,7 @@ __global__ __launch_bounds__(64 * KA_W, ka_per_cu(D, QT)) void kv4_attn_ranges(c
         const int units = ka_entry<MT>(a, start.L, start.n, start.rt).units;
         const int p0 = cuts.range_of(start.before + KA_PIECE, start.total);
         const int p1 = cuts.range_of(start.before + KA_PIECE + units - 1, start.total);
-        if (units > 0 && p1 > p0) cut = KaCut{start.b, start.rt, p0, p1};
+        if (units > 0 && p1 > p0) cut = KaCut{start.b, start.rt, start.n, p0, p1};
       }
     }
     a.cuts[r] = cut;
@@ -891,57 +891,74 @@ __global__ __launch_bounds__(64 * KA_W, ka_per_cu(D, QT)) void kv4_attn_ranges(c
 }
 
 // Entries that lie in several ranges: one workgroup per entry's first cut, K/V head and 4 / WPR rows, WPR waves for
-// a row. Lanes hold 4 dims each and share the pieces; all of a lane's pieces are requested before they are used.
+// a row. Lanes hold 4 dims each; a row's groups of D / 4 lanes share its pieces, four of them requested at once and merged
+// against a running reference, then the groups' results meet in LDS: two trips to memory, the cut and the pieces.
 template <int D, int QT, bool BF16, int WPR>
 __global__ __launch_bounds__(256) void kv4_attn_join(const KaArgs a) {
-  constexpr int MT = 16 * QT, LPG = D / 4, GPW = 64 / LPG;
+  constexpr int MT = 16 * QT, LPG = D / 4, GPW = 64 / LPG, STEP = GPW * WPR;
   __shared__ f32x4 acc_s[4][64];
+  __shared__ float top_s[4][GPW], sum_s[4][GPW];
   const int h = blockIdx.y, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int i = blockIdx.z * (4 / WPR) + wave / WPR;  // row of the entry
   const KaCut cut = a.cuts[blockIdx.x + 1];
   if (cut.b < 0) return;
-  const KaEntry e = ka_entry<MT>(a, ka_len(a, cut.b), ka_new(a, cut.b), cut.rt);
-  const bool live = i < e.rows;
-  const int np = live ? cut.p1 - cut.p0 + 1 : 0;
-  auto slot = [&](int p) {  // of piece p: the first lies at its range's end, the others at the start
-    return a.part + ((int64_t)(2 * (cut.p0 + p) + (p == 0)) * a.c.Hkv + h) * (MT * (D + 2));
-  };
-  float top = -INFINITY;
-  for (int p = lane; p < np; p += 64) top = fmaxf(top, slot(p)[MT * D + i]);
-  top = wave_max(top);
-  auto weight = [&](float m) { return m == -INFINITY ? 0.f : fast_exp2(m - top); };
-  float sum = 0.f;
-  for (int p = lane; p < np; p += 64) {
-    const float* s = slot(p) + MT * D + i;
-    sum += weight(s[0]) * s[MT];
-  }
-  sum = wave_sum(sum);
+  const int row = cut.rt * MT + i;
+  const int np = i < MT && row < cut.n * a.group ? cut.p1 - cut.p0 + 1 : 0;
   const int grp = lane / LPG, d = 4 * (lane - grp * LPG);
+  float top = -INFINITY, sum = 0.f;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  constexpr int STEP = GPW * WPR;
   for (int p = wave % WPR * GPW + grp; grp < GPW && p < np; p += 4 * STEP) {
     f32x4 o[4];
-    float m[4];
+    float m[4], l[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const float* s = slot(min(p + u * STEP, np - 1));
+      const int pu = min(p + u * STEP, np - 1);
+      // the first piece lies at its range's end, the others at the start
+      const float* s = a.part + ((int64_t)(2 * (cut.p0 + pu) + (pu == 0)) * a.c.Hkv + h) * (MT * (D + 2));
       o[u] = *(const f32x4*)(s + i * D + d);
-      m[u] = p + u * STEP < np ? s[MT * D + i] : -INFINITY;
+      m[u] = s[MT * D + i];
+      l[u] = s[MT * D + MT + i];
     }
+    float next = top;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (p + u * STEP >= np) m[u] = -INFINITY;
+      next = fmaxf(next, m[u]);
+    }
+    if (next == -INFINITY) continue;
+    const float f = top == -INFINITY ? 0.f : fast_exp2(top - next);
+    sum *= f;
+    acc *= f;
 #pragma unroll
     for (int u = 0; u < 4; ++u)
-      if (p + u * STEP < np) acc += weight(m[u]) * o[u];
+      if (m[u] != -INFINITY) {
+        const float w = fast_exp2(m[u] - next);
+        sum += w * l[u];
+        acc += w * o[u];
+      }
+    top = next;
   }
   acc_s[wave][lane] = acc;
+  if (grp < GPW && d == 0) top_s[wave][grp] = top, sum_s[wave][grp] = sum;
   __syncthreads();
-  if (!live || wave % WPR != 0 || lane >= LPG) return;
+  if (np == 0 || wave % WPR != 0 || lane >= LPG) return;
+  top = -INFINITY, sum = 0.f;
   acc = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int w = 0; w < WPR; ++w)
 #pragma unroll
-    for (int u = 0; u < GPW; ++u) acc += acc_s[wave + w][u * LPG + lane];
-  const int qrow = e.row0 + i, j = qrow / a.group;
-  const int64_t at_o = ((int64_t)cut.b * a.T + j) * a.H + h * a.group + (qrow - j * a.group);
+    for (int u = 0; u < GPW; ++u) top = fmaxf(top, top_s[wave + w][u]);
+#pragma unroll
+  for (int w = 0; w < WPR; ++w)
+#pragma unroll
+    for (int u = 0; u < GPW; ++u) {
+      if (top_s[wave + w][u] == -INFINITY) continue;
+      const float f = fast_exp2(top_s[wave + w][u] - top);
+      sum += f * sum_s[wave + w][u];
+      acc += f * acc_s[wave + w][u * LPG + lane];
+    }
+  const int j = row / a.group;
+  const int64_t at_o = ((int64_t)cut.b * a.T + j) * a.H + h * a.group + (row - j * a.group);
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   *(u32x2*)(a.o + at_o * D + d) = u32x2{h16<BF16>::pack(acc[0] * inv, acc[1] * inv),
                                         h16<BF16>::pack(acc[2] * inv, acc[3] * inv)};
