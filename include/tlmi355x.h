@@ -445,7 +445,7 @@ int tlm_kv_append_fp8(const void* x, int64_t x_batch_stride, int64_t x_row_strid
  *           multiple of 8).
  *   D       a multiple of 32, 32 .. 256; page a multiple of 8; pages and H_kv >= 1.
  * Pools may be of any size (64-bit offsets). Table entries outside [0, pages) are read as zeros and never
- * written through. */
+ * written through. Calls without rows (B, T or total 0) do nothing; what would hold rows or sequences may be null then. */
 
 /* Quantises the new rows of every sequence into their pages: row j < min(count[b], T) of k and v goes to position
  * start[b] + j; positions outside the table are skipped.
@@ -480,13 +480,14 @@ int tlm_kv4_read(const void* codes, int64_t codes_page_stride, const void* scale
  *   count   int32 [B] or NULL: query rows of each sequence (clamped to [0, T]; NULL: T). Query j is position
  *           seqlens[b] - count[b] + j and, causal, sees keys up to its own; not causal, every key.
  *   o       [B, T, H, D] of dtype, dense; lse float [B, T, H] or NULL: log2 of the sum of exp of the scaled scores (the
- *           glse of tlm_flash_attn_splitkv_fwd). A query without a key gets zeros and -inf; rows j >= count[b] are
- *           left as they were.
+ *           glse of tlm_flash_attn_splitkv_fwd). A query without a key, or whose scores are all -inf, gets zeros
+ *           and -inf; rows j >= count[b] are left as they were.
  *   sm_scale in the natural-log domain. Products, softmax and sums are fp32; the weights of V are rounded
  *           to 16 bits of precision (dtype F16) or to fp16's 11 (BF16). Sums of V beyond 2^110 overflow. How the
  *           keys are cut, and so the last bits, depends on all lengths and counts of the call, never on timing.
  *   ws      tlm_kv4_attn_workspace_bytes(...) bytes, 16-byte aligned (device memory, caller-owned; needs no
- *           initial value; a size for T is enough for fewer rows and any B). Calls that overlap in time, and graphs whose replays may, need one each. */
+ *           initial value; a size for T is enough for fewer rows and any B). Calls that overlap in time, and graphs
+ *           whose replays may, need one each. */
 size_t tlm_kv4_attn_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t H_kv, int64_t D);
 int tlm_kv4_attn(const void* q, int64_t q_batch_stride, int64_t q_row_stride, const void* codes,
                  int64_t codes_page_stride, const void* scales, int64_t scales_page_stride,

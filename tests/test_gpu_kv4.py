@@ -564,3 +564,70 @@ def test_attn_random(seed):
     dtype = BF16 if r.rand() < 0.5 else F16
     q, c, s, bt = _attn_case(dtype, B, T, H, Hkv, D, page, list(lens), seed)
     _check(q, *_stale(c, s, bt, lens, page), bt, lens, count, bool(r.rand() < 0.7))
+
+
+@pytest.mark.parametrize("H,Hkv,D", [(1000, 1000, 32), (1040, 520, 160)])
+def test_attn_more_kv_heads_than_workgroups_at_once(H, Hkv, D):
+    lens = [100, 0, 37]
+    q, c, s, bt = _attn_case(BF16, 3, 1, H, Hkv, D, 8, lens, 31)
+    _check(q, *_stale(c, s, bt, lens, 8), bt, lens)
+
+
+def test_attn_large_pages():
+    lens = [16500, 8199, 8201]
+    q, c, s, bt = _attn_case(F16, 3, 2, 2, 1, 32, 8200, lens, 32)
+    _check(q, *_stale(c, s, bt, lens, 8200), bt, lens)
+
+
+def test_attn_one_query_for_all_sequences():
+    """An expanded batch: a batch stride of 0."""
+    lens = [300, 5, 64]
+    q, c, s, bt = _attn_case(BF16, 1, 3, 8, 2, 64, 16, [300] * 3, 33, pages=60)
+    bt = np.arange(57, dtype=np.int32).reshape(3, 19)
+    qd = q.to(DEV).expand(3, 3, 8, 64)
+    out, z = torch.empty(3, 3, 8, 64, dtype=BF16, device=DEV), torch.empty(3, 3, 8, device=DEV)
+    ws = torch.empty(ops.kv4_attn_workspace_bytes(3, 3, 8, 2, 64), dtype=torch.uint8, device=DEV)
+    ops.kv4_attn(qd, c.to(DEV), s.to(DEV), _i32(bt), _i32(lens), out, ws, 0.125, lse=z)
+    _check(q.expand(3, 3, 8, 64).contiguous(), c, s, bt, lens, got=(out.cpu(), z.cpu()))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_attn_scores_of_minus_infinity(dtype):
+    """A query that gives all keys -inf is answered like one without keys; a score of +inf or NaN makes its row NaN. Their
+    neighbours in the tile are as without them."""
+    lens = [200, 200]
+    q, c, s, bt = _attn_case(dtype, 2, 1, 8, 2, 64, 16, lens, 34)
+    q[:, :, :, 0] = 0
+    c[:, 0, :, :, 0] = c[:, 0, :, :, 0] & 0xF0 | 2    # dim 0 of K: 1
+    want = _run(q, c, s, bt, lens)
+    bad = q.clone()
+    bad[0, 0, 2, 0] = -torch.inf
+    bad[0, 0, 6, 0], bad[1, 0, 1, 0], bad[1, 0, 7, 0] = -torch.inf, torch.inf, torch.nan
+    out, z = _run(bad, c, s, bt, lens)
+    for b, h in ((0, 2), (0, 6)):
+        assert (out[b, 0, h] == 0).all() and z[b, 0, h] == -torch.inf
+    assert out[1, 0, 1].isnan().all() and out[1, 0, 7].isnan().all() and z[1, 0, 7].isnan()
+    keep = torch.ones(2, 8, dtype=torch.bool)
+    keep[0, 2] = keep[0, 6] = keep[1, 1] = keep[1, 7] = False
+    assert torch.equal(out[:, 0][keep], want[0][:, 0][keep]) and torch.equal(z[:, 0][keep], want[1][:, 0][keep])
+
+    one = c.clone()  # one key's dim 0 is -1: its score is +inf
+    p = int(bt[0, 150 // 16])
+    one[p, 0, :, 150 % 16, 0] = one[p, 0, :, 150 % 16, 0] & 0xF0 | 10
+    out, z = _run(bad, one, s, bt, lens)
+    assert out[0, 0, 2].isnan().all()
+
+
+def test_empty_batches_and_steps():
+    q, c, s, bt = _attn_case(BF16, 2, 1, 8, 2, 64, 16, [20, 20], 35)
+    c, s, bt, n = c.to(DEV), s.to(DEV), _i32(bt), _i32([20, 20])
+    before = c.clone(), s.clone()
+    ws = torch.empty(1 << 22, dtype=torch.uint8, device=DEV)
+    for B, T in ((0, 1), (2, 0), (0, 0)):
+        x, kv = torch.empty(B, T, 8, 64, dtype=BF16, device=DEV), torch.empty(B, T, 2, 64, dtype=BF16, device=DEV)
+        ops.kv4_append(kv, kv, n[:B], n[:B], bt[:B], c, s)
+        ops.kv4_attn(x, c, s, bt[:B], n[:B], x.clone(), ws, 0.1, count=n[:B], lse=torch.empty(B, T, 8, device=DEV))
+        ops.kv4_read(c, s, bt[:B], None, torch.zeros(B + 1, dtype=torch.int32, device=DEV), kv.flatten(0, 1),
+                     kv.flatten(0, 1))
+    torch.cuda.synchronize()
+    assert torch.equal(c, before[0]) and torch.equal(s, before[1])

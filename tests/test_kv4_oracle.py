@@ -191,3 +191,19 @@ def test_empty_calls_do_nothing():
     assert _append(B=0) == 0 and _append(T=0) == 0
     assert _read(B=0) == 0 and _read(total=0) == 0
     assert _attn(B=0) == 0 and _attn(T=0) == 0
+
+
+def test_empty_calls_take_null_rows():
+    none = dict(k=None, v=None, q=None, o=None)
+    for no in (dict(B=0, bt=None, start=None, count=None, sl=None), dict(T=0)):
+        assert _append(**none, **no) == 0 and _attn(**none, **no, ws=None, wb=0) == 0
+    assert _read(total=0, k=None, v=None) == 0 and _read(B=0, total=0, bt=None, k=None, v=None) == 0
+
+
+@pytest.mark.parametrize("H,Hkv,D", [(8, 8, 64), (32, 8, 128), (7, 1, 96), (16, 2, 256), (64, 1, 128), (2000, 1000, 32)])
+def test_workspace_of_a_chunk_is_enough_for_steps(H, Hkv, D):
+    size = lib.load().tlm_kv4_attn_workspace_bytes
+    sizes = [size(3, T, H, Hkv, D) for T in (1, 2, 3, 5, 8, 17, 40, 200, 5000)]
+    assert sizes == sorted(sizes) and sizes[0] > 0
+    assert size(100, 8, H, Hkv, D) == size(1, 8, H, Hkv, D)
+    assert size(0, 1, H, Hkv, D) == 0

@@ -23,7 +23,7 @@ TLM_DEV float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
 // Checks what the entry points share; 0 or a status with the message set.
 inline int check(const char* fn, const Cache& c, int64_t max_pages, int64_t page, int64_t Hkv, int64_t D,
                  int64_t B) {
-  if (!c.codes || !c.scales || !c.table) {
+  if (!c.codes || !c.scales || (!c.table && B != 0)) {
     tlm_set_error("%s: null pointer argument", fn);
     return TLM_EINVAL;
   }
@@ -55,10 +55,10 @@ inline int check(const char* fn, const Cache& c, int64_t max_pages, int64_t page
   return TLM_OK;
 }
 
-// Rows [B, T, heads, D] with heads and dims dense.
-inline int check_rows(const char* fn, const char* name, const void* x, int64_t batch_stride,
+// Rows [B, T, heads, D] with heads and dims dense; without any, x may be null.
+inline int check_rows(const char* fn, const char* name, const void* x, bool any, int64_t batch_stride,
                       int64_t row_stride, int dtype) {
-  if (!x) {
+  if (any && !x) {
     tlm_set_error("%s: null pointer argument", fn);
     return TLM_EINVAL;
   }

@@ -77,16 +77,16 @@ __global__ __launch_bounds__(K4_T) void kv4_append_kernel(Cache c, const uint16_
       uint8_t* const scales = c.scales + pid * c.scales_page + (int64_t)(t.d8 / 4) * c.page + off;
       for (int h = h0; h < h1; h += K4_U) {
         u32x4 x[K4_U];
-  #pragma unroll
+#pragma unroll
         for (int u = 0; u < K4_U; ++u) {
           const int hu = min(h + u, h1 - 1);
           x[u] = ld_nt((const u32x4*)(hu < c.Hkv ? ks + (int64_t)hu * c.D : vs + (int64_t)(hu - c.Hkv) * c.D));
         }
-  #pragma unroll
+#pragma unroll
         for (int u = 0; u < K4_U; ++u) {
           if (h + u >= h1) break;
           uint32_t m = 0;
-  #pragma unroll
+#pragma unroll
           for (int e = 0; e < 4; ++e) m = max(m, max(x[u][e] & 0x7fffu, (x[u][e] >> 16) & 0x7fffu));
           m = max(m, (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0xB1, 0xf, 0xf, false));  // lane ^ 1
           m = max(m, (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0x4E, 0xf, 0xf, false));  // lane ^ 2
@@ -170,14 +170,14 @@ __global__ __launch_bounds__(K4_T) void kv4_read_kernel(Cache c, const int32_t* 
     const int64_t row = (r * c.Hkv * c.D + 8 * t.d8) * ES;
     for (int h = h0; h < h1; h += K4_U) {
       uint32_t code[K4_U], byte[K4_U];
-  #pragma unroll
+#pragma unroll
       for (int u = 0; u < K4_U; ++u) {
         const int hu = min(h + u, h1 - 1);
         code[u] = *(const uint32_t*)(codes + (int64_t)hu * c.page * (c.D / 2));
         byte[u] = scales[(int64_t)hu * (c.D / kv4::BLOCK) * c.page];
         if (!ok) code[u] = 0, byte[u] = 127;
       }
-  #pragma unroll
+#pragma unroll
       for (int u = 0; u < K4_U; ++u) {
         const int hu = h + u;
         if (hu >= h1) break;
@@ -205,9 +205,10 @@ extern "C" int tlm_kv4_append(const void* k, const void* v, int64_t k_batch_stri
                               int64_t H_kv, int64_t D, void* stream) {
   Cache c{(uint8_t*)codes, (uint8_t*)scales, codes_page_stride, scales_page_stride, pages, block_table};
   if (int rc = kv4::check("tlm_kv4_append", c, max_pages, page, H_kv, D, B)) return rc;
-  if (int rc = kv4::check_rows("tlm_kv4_append", "k", k, k_batch_stride, k_row_stride, x_dtype)) return rc;
-  if (int rc = kv4::check_rows("tlm_kv4_append", "v", v, v_batch_stride, v_row_stride, x_dtype)) return rc;
-  if (!start || !count) {
+  const bool any = B != 0 && T != 0;
+  if (int rc = kv4::check_rows("tlm_kv4_append", "k", k, any, k_batch_stride, k_row_stride, x_dtype)) return rc;
+  if (int rc = kv4::check_rows("tlm_kv4_append", "v", v, any, v_batch_stride, v_row_stride, x_dtype)) return rc;
+  if (B != 0 && (!start || !count)) {
     tlm_set_error("tlm_kv4_append: null pointer argument");
     return TLM_EINVAL;
   }
@@ -215,7 +216,7 @@ extern "C" int tlm_kv4_append(const void* k, const void* v, int64_t k_batch_stri
     tlm_set_error("tlm_kv4_append: bad sizes");
     return TLM_EINVAL;
   }
-  if (B == 0 || T == 0) return TLM_OK;
+  if (!any) return TLM_OK;
   c.max_pages = (int)max_pages, c.page = (int)page, c.Hkv = (int)H_kv, c.D = (int)D;
   const int64_t per = K4_T / (D / 8), gx = std::min<int64_t>((T + per - 1) / per, K4_GRID);
   const int64_t gz = std::min<int64_t>(B, 65535);
@@ -239,7 +240,7 @@ extern "C" int tlm_kv4_read(const void* codes, int64_t codes_page_stride, const 
                             int64_t H_kv, int64_t D, int out_dtype, void* stream) {
   Cache c{(uint8_t*)codes, (uint8_t*)scales, codes_page_stride, scales_page_stride, pages, block_table};
   if (int rc = kv4::check("tlm_kv4_read", c, max_pages, page, H_kv, D, B)) return rc;
-  if (!cu_seqlens || !k_out || !v_out) {
+  if (!cu_seqlens || (total != 0 && (!k_out || !v_out))) {
     tlm_set_error("tlm_kv4_read: null pointer argument");
     return TLM_EINVAL;
   }

@@ -55,7 +55,7 @@ constexpr int ka_stages() {
 // that one by SLACK. At most 2^15, an fp16 number, and normal ones down to 2^-25 of the largest.
 constexpr float KA_BIAS = 11.f, KA_SLACK = 4.f;
 
-struct alignas(32) KaCut {
+struct alignas(16) KaCut {
   int b, rt, n;  // sequence (-1: nothing to join), row tile, new tokens
   int p0, p1;    // first and last range that hold units of it
 };
@@ -1025,8 +1025,9 @@ extern "C" int tlm_kv4_attn(const void* q, int64_t q_batch_stride, int64_t q_row
                             int causal, float sm_scale, int dtype, void* stream) {
   Cache c{(uint8_t*)codes, (uint8_t*)scales, codes_page_stride, scales_page_stride, pages, block_table};
   if (int rc = kv4::check("tlm_kv4_attn", c, max_pages, page, H_kv, D, B)) return rc;
-  if (int rc = kv4::check_rows("tlm_kv4_attn", "q", q, q_batch_stride, q_row_stride, dtype)) return rc;
-  if (!seqlens || !o) {
+  const bool any = B != 0 && T != 0;
+  if (int rc = kv4::check_rows("tlm_kv4_attn", "q", q, any, q_batch_stride, q_row_stride, dtype)) return rc;
+  if ((B != 0 && !seqlens) || (any && !o)) {
     tlm_set_error("tlm_kv4_attn: null pointer argument");
     return TLM_EINVAL;
   }
@@ -1038,7 +1039,7 @@ extern "C" int tlm_kv4_attn(const void* q, int64_t q_batch_stride, int64_t q_row
     tlm_set_error("tlm_kv4_attn: o must be 16-byte and lse 4-byte aligned");
     return TLM_EINVAL;
   }
-  if (B == 0 || T == 0) return TLM_OK;
+  if (!any) return TLM_OK;
   if (H > (INT32_MAX - 64) / B || T > (INT32_MAX - 64) / (B * H)) {
     tlm_set_error("tlm_kv4_attn: problem too large (2^31 query rows)");
     return TLM_EINVAL;
@@ -1058,8 +1059,8 @@ extern "C" int tlm_kv4_attn(const void* q, int64_t q_batch_stride, int64_t q_row
   // (a scale of 0 becomes the least there is: masked scores are -inf, and -inf times 0 is no weight)
   const float scale2 = std::max(fabsf(sm_scale) * 1.4426950408889634f, 0x1p-149f);
   KaArgs a{c, (const uint16_t*)q, q_batch_stride, q_row_stride, seqlens, count, (uint16_t*)o, lse,
-           (KaCut*)ws, (float*)((char*)ws + p.meta), (int)B, (int)T, (int)H, (int)(H / H_kv), causal != 0, p.G, few, T * (H / H_kv) <= 16 * p.qt, 0, 0,
-           scale2, sm_scale < 0.f ? 0x80008000u : 0u};
+           (KaCut*)ws, (float*)((char*)ws + p.meta), (int)B, (int)T, (int)H, (int)(H / H_kv), causal != 0, p.G, few,
+           T * (H / H_kv) <= 16 * p.qt, 0, 0, scale2, sm_scale < 0.f ? 0x80008000u : 0u};
   // with 2^(k-1) < page <= 2^k and m = floor(2^(31+k) / page) + 1: m page - 2^(31+k) <= 2^k, so that tok m / 2^(31+k) is
   // less than 1 / page above tok / page for tok < 2^31; and m fits 32 bits
   while ((1ll << a.page_shift) < page) ++a.page_shift;
