@@ -571,6 +571,9 @@ def test_attn_more_kv_heads_than_workgroups_at_once(H, Hkv, D):
     lens = [100, 0, 37]
     q, c, s, bt = _attn_case(BF16, 3, 1, H, Hkv, D, 8, lens, 31)
     _check(q, *_stale(c, s, bt, lens, 8), bt, lens)
+    _check(q, c, s, bt, [0, 0, 0])
+    _check(q[:1], c, s, bt[:1], [0])
+    _check(q[:1], c, s, bt[:1], [1])
 
 
 def test_attn_large_pages():
@@ -631,3 +634,12 @@ def test_empty_batches_and_steps():
                      kv.flatten(0, 1))
     torch.cuda.synchronize()
     assert torch.equal(c, before[0]) and torch.equal(s, before[1])
+
+
+@pytest.mark.parametrize("B,D,Hkv", [(1, 128, 8), (2, 256, 2), (3, 256, 1), (1, 64, 1), (5, 128, 2), (2, 32, 90)])
+def test_attn_few_units_per_workgroup(B, D, Hkv):
+    """Lengths from none to more units than there are workgroups."""
+    q, c, s, bt = _attn_case(BF16, B, 1, 2 * Hkv, Hkv, D, 64, [36000 // B // Hkv + 900] * B, 36)
+    for n in (0, 1, 128, 129, 600, 36000 // B // Hkv + 900):
+        lens = [max(0, n - 70 * b) for b in range(B)]
+        _check(q, c, s, bt, lens)

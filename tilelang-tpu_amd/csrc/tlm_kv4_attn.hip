@@ -12,7 +12,7 @@
 // the softmax (340), which hide under each other little (one wave's MFMA and VALU work do not overlap at all).
 //
 //   * Partition: entry (sequence, row tile) costs its 128-token units plus KA_PIECE; the cost line of the batch is cut into
-//     G equal ranges, one workgroup each per K/V head, found from the lengths by the workgroups themselves. A
+//     up to G equal ranges, one workgroup each per K/V head, found from the lengths by the workgroups themselves. A
 //     range's part of an entry (a piece) is the output or, where the entry was cut, goes to the workspace, from where
 //     kv4_attn_join merges it. Pieces priced at 1 unit: 5 % slower at 24 sequences of 1 .. 2,047 tokens, the same elsewhere.
 //   * Its four waves take 32-token tiles in turn, each with its own reference, sums and O^T: no barrier until the piece
@@ -44,6 +44,7 @@ constexpr int KA_W = 4;          // waves per workgroup
 constexpr int KA_BN = 32;        // tokens per tile (one wave)
 constexpr int KA_UNIT = KA_W * KA_BN;
 constexpr int KA_PIECE = 2;      // cost of a piece beside its units, in units
+constexpr int KA_LEAST = 3;      // of a range, where a CU has more than one
 // Workgroups per CU, and stages of a ring in their share of the LDS.
 constexpr int ka_per_cu(int D, int QT) { return QT == 1 ? (D <= 128 ? 3 : 2) : D <= 128 ? 2 : 1; }
 template <int D, int QT>
@@ -129,6 +130,14 @@ struct KaCuts {
     return r;
   }
 };
+
+// Ranges of a cost line: one workgroup per CU with anything, more where each gets KA_LEAST (two with a unit each on a CU take
+// longer than one with both, and leave the join twice the pieces: 12 sequences of 1,000 .. 6,000, 2 heads of 256, 13.6 + 4.0 us
+// instead of 15.8 + 5.0; 2 and 4 as the least 15.4 and 13.6).
+template <int D, int QT>
+TLM_DEV int ka_ranges(const KaArgs& a, int64_t total) {
+  return (int)min(total, max((int64_t)max(1, a.G / ka_per_cu(D, QT)), min((int64_t)a.G, total / KA_LEAST)));
+}
 
 // Position x of the cost line in units of an entry that starts at `before`: its KA_PIECE come first.
 TLM_DEV int ka_unit_at(int64_t x, int64_t before, int units) {
@@ -841,7 +850,7 @@ __global__ __launch_bounds__(64 * KA_W, ka_per_cu(D, QT)) void kv4_attn_ranges(c
 
   int64_t lo = 0, hi = 0;
   auto want = [&](int64_t total) {
-    const int ng = (int)min((int64_t)a.G, total);
+    const int ng = ka_ranges<D, QT>(a, total);
     if (r < ng) {
       const KaCuts cuts(total, ng);
       lo = cuts.at(r);
@@ -853,7 +862,7 @@ __global__ __launch_bounds__(64 * KA_W, ka_per_cu(D, QT)) void kv4_attn_ranges(c
   if (h == 0 && tid == 0) {
     KaCut cut{-1, 0, 0, 0, 0};
     if (lo < hi && start.before < lo) {
-      const int ng = (int)min((int64_t)a.G, start.total);
+      const int ng = ka_ranges<D, QT>(a, start.total);
       const KaCuts cuts(start.total, ng);
       if (cuts.at(r - 1) <= start.before) {
         const int units = ka_entry<MT>(a, start.L, start.n, start.rt).units;
