@@ -643,3 +643,12 @@ def test_attn_few_units_per_workgroup(B, D, Hkv):
     for n in (0, 1, 128, 129, 600, 36000 // B // Hkv + 900):
         lens = [max(0, n - 70 * b) for b in range(B)]
         _check(q, c, s, bt, lens)
+
+
+@pytest.mark.parametrize("B,T,H,Hkv,causal", [(1, 700, 6, 2, True), (1, 515, 8, 1, False), (2, 300, 7, 1, True), (33, 40, 4, 2, True)])
+def test_attn_many_row_tiles(B, T, H, Hkv, causal):
+    """Chunks of more row tiles than a wave has lanes for the sequence, of unequal numbers of tokens."""
+    lens = [T + 100 - 37 * b % 120 for b in range(B)]
+    count = [T - 13 * b % T for b in range(B)]
+    q, c, s, bt = _attn_case(BF16, B, T, H, Hkv, 64, 16, lens, 37)
+    _check(q, *_stale(c, s, bt, lens, 16), bt, lens, count, causal)

@@ -72,7 +72,7 @@ struct KaArgs {
   KaCut* cuts;  // [G]: the entry that the cut before range r goes through, if it is the entry's first
   float* part;  // [2 G][Hkv][16 QT][D + 2]: rows, their references, their sums
   int B, T, H, group, causal, G;
-  int few;            // ka_find64 will do
+  int few;            // ka_find64 will do, with 2^(few - 1) lanes per sequence
   int once;           // codes are read by one row tile only: past the caches
   uint32_t page_mul;  // tok / page = tok page_mul >> page_shift, for tok < 2^31
   int page_shift;
@@ -202,15 +202,18 @@ TLM_DEV KaPoint ka_find(const KaArgs& a, int64_t* sh, F&& want) {
   p.n = at >= 0 ? ka_new(a, p.b) : 0;
   return p;
 }
-// The same for up to 64 sequences, a lane each, by every wave for itself: no barrier, one trip to memory.
+// The same for up to 64 sequences by every wave for itself: no barrier, one trip to memory. A sequence has 2^(few - 1) lanes,
+// as many as there are, each with a run of its row tiles (one prompt of 8,192 tokens has 1,024 of them).
 template <int MT, typename F>
 TLM_DEV KaPoint ka_find64(const KaArgs& a, F&& want) {
-  const int lane = threadIdx.x & 63;
-  int L = 0, n = 0, mine = 0;  // (the caller has made sure that all costs together fit)
-  if (lane < a.B) {
-    L = ka_len(a, lane), n = ka_new(a, lane);
-    const int rts = ka_tiles<MT>(a, n);
-    for (int rt = 0; rt < rts; ++rt) mine += ka_entry<MT>(a, L, n, rt).units + KA_PIECE;
+  const int lane = threadIdx.x & 63, sh = a.few - 1, seq = lane >> sh;
+  int L = 0, n = 0, rt0 = 0, mine = 0;  // (the caller has made sure that all costs together fit)
+  if (seq < a.B) {
+    L = ka_len(a, seq), n = ka_new(a, seq);
+    const int rts = ka_tiles<MT>(a, n), run = (rts + (1 << sh) - 1) >> sh;
+    rt0 = min(rts, (lane & ((1 << sh) - 1)) * run);
+    const int rt1 = min(rts, rt0 + run);
+    for (int rt = rt0; rt < rt1; ++rt) mine += ka_entry<MT>(a, L, n, rt).units + KA_PIECE;
   }
   int x = mine;
 #pragma unroll
@@ -224,10 +227,12 @@ TLM_DEV KaPoint ka_find64(const KaArgs& a, F&& want) {
   const int at = (int)want((int64_t)total);
   const uint64_t m = __ballot(at >= x - mine && at < x);
   if (m == 0) return p;
-  p.b = __builtin_ctzll(m);
-  p.L = __builtin_amdgcn_readlane(L, p.b);
-  p.n = __builtin_amdgcn_readlane(n, p.b);
-  int s = __builtin_amdgcn_readlane(x - mine, p.b);
+  const int from = __builtin_ctzll(m);
+  p.b = from >> sh;
+  p.L = __builtin_amdgcn_readlane(L, from);
+  p.n = __builtin_amdgcn_readlane(n, from);
+  p.rt = __builtin_amdgcn_readlane(rt0, from);
+  int s = __builtin_amdgcn_readlane(x - mine, from);
   for (;; ++p.rt) {
     const int cost = ka_entry<MT>(a, p.L, p.n, p.rt).units + KA_PIECE;
     if (at < s + cost) break;
@@ -1064,7 +1069,9 @@ extern "C" int tlm_kv4_attn(const void* q, int64_t q_batch_stride, int64_t q_row
   }
   c.max_pages = (int)max_pages, c.page = (int)page, c.Hkv = (int)H_kv, c.D = (int)D;
   const int64_t tiles = (T * (H / H_kv) + 16 * p.qt - 1) / (16 * p.qt);
-  const int few = B <= 64 && tiles <= INT32_MAX / (64 * (max_pages * page / KA_UNIT + 1 + KA_PIECE));
+  int few = 0;
+  if (B <= 64 && tiles <= INT32_MAX / (B * (max_pages * page / KA_UNIT + 1 + KA_PIECE)))
+    for (few = 1; B << few <= 64;) ++few;
   // (a scale of 0 becomes the least there is: masked scores are -inf, and -inf times 0 is no weight)
   const float scale2 = std::max(fabsf(sm_scale) * 1.4426950408889634f, 0x1p-149f);
   KaArgs a{c, (const uint16_t*)q, q_batch_stride, q_row_stride, seqlens, count, (uint16_t*)o, lse,
