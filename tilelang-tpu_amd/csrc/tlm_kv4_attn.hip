@@ -74,8 +74,8 @@ struct KaArgs {
   int B, T, H, group, causal, G;
   int few;            // ka_find64 will do, with 2^(few - 1) lanes per sequence
   int once;           // codes are read by one row tile only: past the caches
-  uint32_t page_mul;  // tok / page = tok page_mul >> page_shift, for tok < 2^31
-  int page_shift;
+  uint32_t page_mul, group_mul;  // x / page = x page_mul >> page_shift, for x < 2^31; the same for group
+  int page_shift, group_shift;
   float scale2;       // |sm_scale| log2(e)
   uint32_t q_sign;    // the sign of sm_scale on both halves of a word
 };
@@ -88,6 +88,9 @@ struct KaEntry {
   int keys, keys_min; // keys that its last row sees, and its first
   int units;
 };
+TLM_DEV int ka_token_of(const KaArgs& a, int row) {  // row / group
+  return (int)((uint64_t)(uint32_t)row * a.group_mul >> a.group_shift);
+}
 template <int MT>
 TLM_DEV KaEntry ka_entry(const KaArgs& a, int L, int n, int rt) {
   KaEntry e;
@@ -95,8 +98,8 @@ TLM_DEV KaEntry ka_entry(const KaArgs& a, int L, int n, int rt) {
   e.row0 = rt * MT;
   e.rows = min(MT, n * a.group - e.row0);
   if (a.causal) {
-    e.keys = max(0, L - n + 1 + (e.row0 + e.rows - 1) / a.group);
-    e.keys_min = max(0, L - n + 1 + e.row0 / a.group);
+    e.keys = max(0, L - n + 1 + ka_token_of(a, e.row0 + e.rows - 1));
+    e.keys_min = max(0, L - n + 1 + ka_token_of(a, e.row0));
   } else {
     e.keys = e.keys_min = L;
   }
@@ -108,11 +111,13 @@ TLM_DEV int ka_new(const KaArgs& a, int b) { return a.count ? max(0, min(a.count
 template <int MT>
 TLM_DEV int ka_tiles(const KaArgs& a, int n) { return (n * a.group + MT - 1) / MT; }
 
-// Ranges of the cost line: range r of g starts at floor(r total / g) (g <= 768: products of the rest fit 32 bits).
+// Ranges of the cost line: range r of g starts at floor(r total / g). With g <= 768 products of the rest are below 2^20, and
+// (x + 1/2) / g is 1 / 1536 away from every integer, more than fp32 is off by (2^-21 of 768 at most).
 struct KaCuts {
   int64_t quot;
   uint32_t rem, g;
-  TLM_DEV KaCuts(int64_t total, int ranges) : g((uint32_t)ranges) {
+  float inv;
+  TLM_DEV KaCuts(int64_t total, int ranges) : g((uint32_t)ranges), inv(__builtin_amdgcn_rcpf((float)ranges)) {
     if (total >> 32) {
       quot = total / ranges;
       rem = (uint32_t)(total - quot * ranges);
@@ -122,7 +127,7 @@ struct KaCuts {
       rem = (uint32_t)total - q * g;
     }
   }
-  TLM_DEV int64_t at(int r) const { return quot * r + rem * (uint32_t)r / g; }
+  TLM_DEV int64_t at(int r) const { return quot * r + (uint32_t)(((float)(rem * (uint32_t)r) + 0.5f) * inv); }
   TLM_DEV int range_of(int64_t x, int64_t total) const {  // the one that holds x: estimated, then exact
     int r = max(0, min((int)g - 1, (int)((float)x * (float)g / (float)total)));
     while (at(r) > x) --r;
@@ -136,7 +141,8 @@ struct KaCuts {
 // instead of 15.8 + 5.0; 2 and 4 as the least 15.4 and 13.6).
 template <int D, int QT>
 TLM_DEV int ka_ranges(const KaArgs& a, int64_t total) {
-  return (int)min(total, max((int64_t)max(1, a.G / ka_per_cu(D, QT)), min((int64_t)a.G, total / KA_LEAST)));
+  if (total >= KA_LEAST * a.G) return a.G;
+  return min((int)total, max(max(1, a.G / ka_per_cu(D, QT)), (int)total / KA_LEAST));
 }
 
 // Position x of the cost line in units of an entry that starts at `before`: its KA_PIECE come first.
@@ -730,7 +736,7 @@ TLM_DEV void ka_piece(const KaArgs& a, const KaPiece& pc, const KaFetch<D, NP>& 
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
       const int i = 16 * t + jl;
-      const int row = e.row0 + i, j = row / a.group;
+      const int row = e.row0 + i, j = ka_token_of(a, row);
       const bool live = i < e.rows;
       lim[t] = live && a.causal ? max(0, L - n + 1 + j) : e.keys;
       const uint16_t* p = a.q + b * a.qb + j * a.qr + (int64_t)(h * a.group + row - j * a.group) * D;
@@ -825,7 +831,7 @@ TLM_DEV void ka_piece(const KaArgs& a, const KaPiece& pc, const KaFetch<D, NP>& 
         acc += f * *(const f32x4*)&so[w][row][d];
       }
       if (pc.slot == nullptr) {
-        const int qrow = e.row0 + i, j = qrow / a.group;
+        const int qrow = e.row0 + i, j = ka_token_of(a, qrow);
         const int64_t at_o = ((int64_t)b * a.T + j) * a.H + h * a.group + (qrow - j * a.group);
         const float inv = sum2 == 0.f ? 0.f : 1.f / sum2;
         *(u32x2*)(a.o + at_o * D + d) = u32x2{h16<BF16>::pack(acc[0] * inv, acc[1] * inv),
@@ -971,7 +977,7 @@ __global__ __launch_bounds__(256) void kv4_attn_join(const KaArgs a) {
       sum += f * sum_s[wave + w][u];
       acc += f * acc_s[wave + w][u * LPG + lane];
     }
-  const int j = row / a.group;
+  const int j = ka_token_of(a, row);
   const int64_t at_o = ((int64_t)cut.b * a.T + j) * a.H + h * a.group + (row - j * a.group);
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   *(u32x2*)(a.o + at_o * D + d) = u32x2{h16<BF16>::pack(acc[0] * inv, acc[1] * inv),
@@ -1076,12 +1082,15 @@ extern "C" int tlm_kv4_attn(const void* q, int64_t q_batch_stride, int64_t q_row
   const float scale2 = std::max(fabsf(sm_scale) * 1.4426950408889634f, 0x1p-149f);
   KaArgs a{c, (const uint16_t*)q, q_batch_stride, q_row_stride, seqlens, count, (uint16_t*)o, lse,
            (KaCut*)ws, (float*)((char*)ws + p.meta), (int)B, (int)T, (int)H, (int)(H / H_kv), causal != 0, p.G, few,
-           T * (H / H_kv) <= 16 * p.qt, 0, 0, scale2, sm_scale < 0.f ? 0x80008000u : 0u};
-  // with 2^(k-1) < page <= 2^k and m = floor(2^(31+k) / page) + 1: m page - 2^(31+k) <= 2^k, so that tok m / 2^(31+k) is
-  // less than 1 / page above tok / page for tok < 2^31; and m fits 32 bits
-  while ((1ll << a.page_shift) < page) ++a.page_shift;
-  a.page_shift += 31;
-  a.page_mul = (uint32_t)((1ull << a.page_shift) / (uint64_t)page + 1);
+           T * (H / H_kv) <= 16 * p.qt, 0, 0, 0, 0, scale2, sm_scale < 0.f ? 0x80008000u : 0u};
+  // with 2^(k-1) < d <= 2^k and m = floor(2^(31+k) / d) + 1: m d - 2^(31+k) <= 2^k, so that x m / 2^(31+k) is
+  // less than 1 / d above x / d for x < 2^31; and m fits 32 bits
+  auto reciprocal = [](int64_t d, uint32_t& mul, int& shift) {
+    for (shift = 31; (1ll << (shift - 31)) < d;) ++shift;
+    mul = (uint32_t)((1ull << shift) / (uint64_t)d + 1);
+  };
+  reciprocal(page, a.page_mul, a.page_shift);
+  reciprocal(a.group, a.group_mul, a.group_shift);
   hipStream_t st = (hipStream_t)stream;
   const bool bf = dtype == TLM_BF16;
   switch (D) {
