@@ -652,3 +652,17 @@ def test_attn_many_row_tiles(B, T, H, Hkv, causal):
     count = [T - 13 * b % T for b in range(B)]
     q, c, s, bt = _attn_case(BF16, B, T, H, Hkv, 64, 16, lens, 37)
     _check(q, *_stale(c, s, bt, lens, 16), bt, lens, count, causal)
+
+
+@pytest.mark.parametrize("dtype,B,T,Hkv,D", [(BF16, 3, 4000, 9, 128), (F16, 2, 4100, 5, 256), (BF16, 1, 9000, 1, 128)])
+def test_append_many_rows(dtype, B, T, Hkv, D):
+    """Enough rows for more heads in flight, and heads that do not divide."""
+    g = torch.Generator().manual_seed(38)
+    per = T // 64 + 1
+    k, v = (torch.randn(B, T, Hkv, D, generator=g).to(dtype) for _ in "kv")
+    bt = torch.randperm(B * per, generator=g).view(B, per).int().numpy()
+    start, count = np.arange(B, dtype=np.int32) * 20, np.array([T, T - 1, 5], np.int32)[:B]
+    codes, scales = _pools(B * per, Hkv, 64, D)
+    got = _append(k, v, start, count, bt, codes, scales)
+    exp = ref.kv4_append_ref(k, v, start, count, bt, codes.numpy(), scales.numpy())
+    assert np.array_equal(got[0], exp[0]) and np.array_equal(got[1], exp[1])

@@ -10,7 +10,7 @@
 //
 // Bound: HBM. A token and head moves 4 D bytes of 16-bit rows and 1.0625 D bytes of cache. 8 heads of 128: 65,536 tokens read
 // back in 53 us (6.2 TB/s; with plain stores 70 us, one 8-dim chunk per thread with its own search and divisions 148 us);
-// 13,500 tokens appended in 17.6 us (3.9 TB/s; one chunk per thread 30 us). A decode step's rows take 3.6 us,
+// 13,500 tokens appended in 16.2 us (4.3 TB/s; one chunk per thread 30 us). A decode step's rows take 3.6 us,
 // which is launch and three dependent loads.
 #include "tlm_kv4.h"
 
@@ -47,7 +47,7 @@ TLM_DEV bool place(const Cache& c, int b, int64_t p, int64_t& pid, int& off) {
 // A workgroup takes K4_T / (D / 8) tokens, 8 dims of a head per thread, and walks through its share of the 2 H_kv
 // heads of K and V, U of them in flight: tokens next to each other make whole lines of codes, a head's D / 8 threads
 // whole lines of rows.
-constexpr int K4_U = 4;
+constexpr int K4_U = 4;  // twice as many for long appends
 struct Lane {
   int d8, tok;  // 8 dims, token of the workgroup
   bool live;
@@ -57,7 +57,7 @@ TLM_DEV Lane lane_of(int D) {
   return Lane{(int)threadIdx.x - tok * per, tok, tok < K4_T / per};
 }
 
-template <bool BF16>
+template <bool BF16, int U>
 __global__ __launch_bounds__(K4_T) void kv4_append_kernel(Cache c, const uint16_t* k, const uint16_t* v,
                                                           int64_t kb, int64_t kr, int64_t vb, int64_t vr,
                                                           const int32_t* start, const int32_t* count, int B,
@@ -75,15 +75,15 @@ __global__ __launch_bounds__(K4_T) void kv4_append_kernel(Cache c, const uint16_
       const uint16_t* const vs = v + b * vb + j * vr + 8 * t.d8;
       uint8_t* const codes = c.codes + pid * c.codes_page + (int64_t)off * (c.D / 2) + 4 * t.d8;
       uint8_t* const scales = c.scales + pid * c.scales_page + (int64_t)(t.d8 / 4) * c.page + off;
-      for (int h = h0; h < h1; h += K4_U) {
-        u32x4 x[K4_U];
+      for (int h = h0; h < h1; h += U) {
+        u32x4 x[U];
 #pragma unroll
-        for (int u = 0; u < K4_U; ++u) {
+        for (int u = 0; u < U; ++u) {
           const int hu = min(h + u, h1 - 1);
           x[u] = ld_nt((const u32x4*)(hu < c.Hkv ? ks + (int64_t)hu * c.D : vs + (int64_t)(hu - c.Hkv) * c.D));
         }
 #pragma unroll
-        for (int u = 0; u < K4_U; ++u) {
+        for (int u = 0; u < U; ++u) {
           if (h + u >= h1) break;
           uint32_t m = 0;
 #pragma unroll
@@ -189,9 +189,9 @@ __global__ __launch_bounds__(K4_T) void kv4_read_kernel(Cache c, const int32_t* 
 }
 
 // Heads (of 2 H_kv) per workgroup: all of them, or fewer where `wgs` workgroups would not fill the CUs.
-inline int heads_per_wg(int64_t wgs, int64_t Hkv) {
+inline int heads_per_wg(int64_t wgs, int64_t Hkv, int U) {
   int64_t heads = 2 * Hkv;
-  while (heads > K4_U && wgs * ((2 * Hkv + heads - 1) / heads) < 16384) heads = (heads + 1) / 2;
+  while (heads > U && wgs * ((2 * Hkv + heads - 1) / heads) < 16384) heads = (heads + 1) / 2;
   return (int)heads;
 }
 
@@ -220,15 +220,19 @@ extern "C" int tlm_kv4_append(const void* k, const void* v, int64_t k_batch_stri
   c.max_pages = (int)max_pages, c.page = (int)page, c.Hkv = (int)H_kv, c.D = (int)D;
   const int64_t per = K4_T / (D / 8), gx = std::min<int64_t>((T + per - 1) / per, K4_GRID);
   const int64_t gz = std::min<int64_t>(B, 65535);
-  const int heads = heads_per_wg(gx * gz, H_kv);
+  // eight heads in flight where that leaves 8 workgroups per CU (40,000 tokens of 8 heads of 128: 28.3 instead of 30.9 us), else
+  // four (32 tokens: 3.7 instead of 4.6 us)
+  const int U = gx * gz * ((2 * H_kv + 7) / 8) >= 2048 ? 2 * K4_U : K4_U;
+  const int heads = heads_per_wg(gx * gz, H_kv, U);
   const dim3 grid((unsigned)gx, (unsigned)((2 * H_kv + heads - 1) / heads), (unsigned)gz);
   auto go = [&](auto kern) {
     kern<<<grid, K4_T, 0, (hipStream_t)stream>>>(c, (const uint16_t*)k, (const uint16_t*)v, k_batch_stride,
                                                  k_row_stride, v_batch_stride, v_row_stride, start, count,
                                                  (int)B, (int)T, heads);
   };
-  if (x_dtype == TLM_BF16) go(kv4_append_kernel<true>);
-  else go(kv4_append_kernel<false>);
+  const bool bf = x_dtype == TLM_BF16;
+  if (U > K4_U) bf ? go(kv4_append_kernel<true, 2 * K4_U>) : go(kv4_append_kernel<false, 2 * K4_U>);
+  else bf ? go(kv4_append_kernel<true, K4_U>) : go(kv4_append_kernel<false, K4_U>);
   TLM_LAUNCH_CHECK("tlm_kv4_append");
   return TLM_OK;
 }
@@ -259,7 +263,7 @@ extern "C" int tlm_kv4_read(const void* codes, int64_t codes_page_stride, const 
   if (B == 0 || total == 0) return TLM_OK;
   c.max_pages = (int)max_pages, c.page = (int)page, c.Hkv = (int)H_kv, c.D = (int)D;
   const int64_t per = K4_T / (D / 8), gx = std::min<int64_t>((total + per - 1) / per, K4_GRID);
-  const int heads = heads_per_wg(gx, H_kv);
+  const int heads = heads_per_wg(gx, H_kv, K4_U);
   const dim3 grid((unsigned)gx, (unsigned)((2 * H_kv + heads - 1) / heads));
   auto go = [&](auto kern) {
     kern<<<grid, K4_T, 0, (hipStream_t)stream>>>(c, start, cu_seqlens, (uint8_t*)k_out, (uint8_t*)v_out,
