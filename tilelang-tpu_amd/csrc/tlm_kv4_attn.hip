@@ -6,9 +6,9 @@
 // workgroup holds 16 or 32 of them (QT).
 //
 // What bounds it: one new token, the stream of codes: 64 sequences of 512 .. 8,192 tokens, 32 / 8 heads of 128 (bf16): 304 MB
-// in 55 us, 5.5 TB/s; the same without the arithmetic 52 us. Few tokens, the chain launch, lengths, table, tile, exchange: 6.4 us
-// for one sequence of 1,000, 2.9 for the join. Prompt chunks, instruction issue: two chunks of 1,024 over 8,192 and 16,384
-// tokens 530 us (690 TFLOP/s); a 32-token tile of 32 rows issues 32 MFMAs (512 cycles), 64 conversions and 32 permutations (420) and
+// in 55 us, 5.6 TB/s; the same without the arithmetic 52 us. Few tokens, the chain launch, lengths, table, tile, exchange: 6.4 us
+// for one sequence of 1,000, 2.8 for the join. Prompt chunks, instruction issue: two chunks of 1,024 over 8,192 and 16,384
+// tokens 502 us (725 TFLOP/s); a 32-token tile of 32 rows issues 32 MFMAs (512 cycles), 64 conversions and 32 permutations (420) and
 // the softmax (340), which hide under each other little (one wave's MFMA and VALU work do not overlap at all).
 //
 //   * Partition: entry (sequence, row tile) costs its 128-token units plus KA_PIECE; the cost line of the batch is cut into
@@ -30,7 +30,8 @@
 //   * The reference of a row moves when a score passes it by 2^KA_SLACK only, so O is rescaled a few times per row.
 //   * Codes that only one row tile reads bypass the caches (74 -> 65 us); those of longer chunks are shared through the L2 of
 //     the XCD that the K/V head's workgroups are on (8 heads).
-//   * 64 rows per wave (one wave per SIMD): 680 instead of 555 us for the chunks.
+//   * 64 rows per wave (one wave per SIMD): 680 instead of 555 us for the chunks. Four waves of 32 rows sharing each tile's
+//     conversions through LDS, a barrier per tile: 550 instead of 528.
 #include "tlm_kv4.h"
 
 #include <algorithm>
