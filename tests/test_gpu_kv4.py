@@ -666,3 +666,23 @@ def test_append_many_rows(dtype, B, T, Hkv, D):
     got = _append(k, v, start, count, bt, codes, scales)
     exp = ref.kv4_append_ref(k, v, start, count, bt, codes.numpy(), scales.numpy())
     assert np.array_equal(got[0], exp[0]) and np.array_equal(got[1], exp[1])
+
+
+def test_read_of_more_than_2_30_sequences():
+    """Where the sum of two sequences' numbers does not fit 32 bits: all empty but the last ones."""
+    B, Hkv, D, page, pages = (1 << 30) + 5, 1, 32, 8, 3
+    codes, scales = _pools(pages, Hkv, page, D, 39)
+    cu = torch.zeros(B + 1, dtype=torch.int32, device=DEV)
+    cu[-3:] = _i32([5, 5, 12])
+    bt = torch.full((B, 1), -1, dtype=torch.int32, device=DEV)
+    bt[-3:, 0] = _i32([2, -1, 0])
+    outs = [torch.full((14, Hkv, D), 7.0, dtype=F16, device=DEV) for _ in "kv"]
+    ops.kv4_read(codes.to(DEV), scales.to(DEV), bt, None, cu, *outs)
+    outs = [x.cpu() for x in outs]
+    del cu, bt
+    torch.cuda.empty_cache()
+    last = np.array([[2], [-1], [0]], np.int32)
+    for w, out in enumerate(outs):
+        exp = np.concatenate([ref.kv4_rows_ref(codes.numpy(), scales.numpy(), last, b, 0, n)[w]
+                              for b, n in ((0, 5), (2, 7))])
+        assert np.array_equal(out[:12].double().numpy(), exp) and (out[12:] == 7).all()

@@ -207,3 +207,12 @@ def test_workspace_of_a_chunk_is_enough_for_steps(H, Hkv, D):
     assert sizes == sorted(sizes) and sizes[0] > 0
     assert size(100, 8, H, Hkv, D) == size(1, 8, H, Hkv, D)
     assert size(0, 1, H, Hkv, D) == 0
+
+
+@pytest.mark.parametrize("call", [_append, _read, _attn])
+def test_more_sequences_than_their_numbers_hold(call):
+    """From 2^31 - 2^16 sequences on, the number of one and the depth of a grid would pass 2^31 together."""
+    small = dict(mp=1, Hkv=1, H=1, page=8, cs=8 * 128, ss=2 * 8 * 4)
+    for B in (2 ** 31 - 2 ** 16, 2 ** 31 - 100):
+        assert call(B=B, **small) == EINVAL
+        assert "sequences" in lib.load().tlm_last_error().decode()

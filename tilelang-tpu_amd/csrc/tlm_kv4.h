@@ -6,6 +6,7 @@
 namespace kv4 {
 
 constexpr int BLOCK = 32;  // dims per scale
+constexpr int MAX_B = INT32_MAX - (1 << 16);  // a sequence's number plus a grid's depth stays in 32 bits
 
 // The cache as the kernels get it. Offsets into the pools are 64-bit: a pool may pass 4 GB.
 struct Cache {
@@ -34,6 +35,10 @@ inline int check(const char* fn, const Cache& c, int64_t max_pages, int64_t page
   if (D % BLOCK != 0 || D > 256 || page % 8 != 0) {
     tlm_set_error("%s: D must be a multiple of 32 up to 256 and page a multiple of 8", fn);
     return TLM_EUNSUPPORTED;
+  }
+  if (B > MAX_B) {
+    tlm_set_error("%s: problem too large (%d sequences)", fn, MAX_B);
+    return TLM_EINVAL;
   }
   if (page > (1 << 20) || Hkv > (1 << 16) || max_pages > (INT32_MAX - 4096) / page || B > INT32_MAX / max_pages) {
     tlm_set_error("%s: problem too large (2^31 positions per table row and entries per table)", fn);

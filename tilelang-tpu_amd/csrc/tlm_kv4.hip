@@ -155,7 +155,7 @@ __global__ __launch_bounds__(K4_T) void kv4_read_kernel(Cache c, const int32_t* 
   for (int64_t r = (int64_t)blockIdx.x * tokens + t.tok; t.live && r < total; r += (int64_t)gridDim.x * tokens) {
     int lo = 0, hi = B + 1;  // cu[lo - 1] <= r < cu[hi]
     while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
+      const int mid = lo + ((hi - lo) >> 1);  // lo + hi passes 2^31 from 2^30 sequences on
       if ((B < K4_CU ? cu_s[mid] : cu[mid]) <= r) lo = mid + 1;
       else hi = mid;
     }
