@@ -440,9 +440,10 @@ int tlm_kv_append_fp8(const void* x, int64_t x_batch_stride, int64_t x_row_strid
  *   codes   uint8 [pages, 2, H_kv, page, D / 2]: index 0 is K, 1 is V; the even dim in the low half of its
  *           byte. 16-byte aligned; codes_page_stride bytes from page to page (a multiple of 16, so the pools
  *           of several layers may alternate), the rest dense.
- *   scales  uint8 [pages, 2, H_kv, D / 32, page]: exponent + 127, 1 .. 252; 255 is NaN (253 and 254, whose
- *           larger values overflow fp32, are never written). 8-byte aligned, scales_page_stride bytes from page to page (a
- *           multiple of 8).
+ *   scales  uint8 [pages, 2, H_kv, D / 32, page]: exponent + 127, 1 .. 252; 255 is NaN. 253 and 254, whose
+ *           larger values overflow fp32, are never written; tlm_kv4_read returns their values, infinite ones beyond
+ *           fp32, and tlm_kv4_attn takes them so in K and as NaN in V. 8-byte aligned, scales_page_stride bytes
+ *           from page to page (a multiple of 8).
  *   D       a multiple of 32, 32 .. 256; page a multiple of 8; pages and H_kv >= 1; B below 2^31 - 2^16.
  * Pools may be of any size (64-bit offsets). Table entries outside [0, pages) are read as zeros and never
  * written through. Calls without rows (B, T or total 0) do nothing; what would hold rows or sequences may be null then. */

@@ -686,3 +686,22 @@ def test_read_of_more_than_2_30_sequences():
         exp = np.concatenate([ref.kv4_rows_ref(codes.numpy(), scales.numpy(), last, b, 0, n)[w]
                               for b, n in ((0, 5), (2, 7))])
         assert np.array_equal(out[:12].double().numpy(), exp) and (out[12:] == 7).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("D,T,H,Hkv,codes", [(64, 3, 4, 2, 0x10), (128, 9, 8, 2, 0x00), (256, 1, 2, 1, 0x21), (32, 2, 8, 1, 0x77)])
+def test_attn_scale_bytes_253_and_254_of_v_are_nan(dtype, D, T, H, Hkv, codes):
+    """In a tile that every query sees whole, in one that only later queries see and in one of the slower form, alone and
+    together: NaN of the queries that see the block, as from byte 255."""
+    lens = [200, 200, 333, 200, 40]
+    q, c, s, bt = _attn_case(dtype, 5, T, H, Hkv, D, 16, lens, D + T + 40)
+    for b, p, byte in ((0, 10, 253), (1, 199, 254), (2, 40, 254), (2, 332, 253), (3, 70, 253)):
+        i, off = int(bt[b, p // 16]), p % 16
+        s[i, 1, Hkv - 1, p % (D // 32), off] = byte
+        c[i, 1, Hkv - 1, off] = codes
+    for w in (0, 1):  # next to nothing and beyond fp16, so that all of sequence 3 is in the slower form
+        s[int(bt[3, 0]), w, :, :, 0] = 60
+    out = _run(q, c, s, bt, lens)
+    s255 = s.clone()
+    s255[:, 1][s255[:, 1] >= 253] = 255
+    _check(q, c, s255, bt, lens, got=out)

@@ -365,6 +365,8 @@ TLM_DEV f32x4 ka_mma(u32x4 a, u32x4 b, f32x4 c) {
 // the matrix cores take. Zero where all bytes of w are such: plus 19 they are 128 .. 159, and a byte's carry comes from
 // one that is out of range itself.
 TLM_DEV uint32_t ka_not_f16(uint32_t w) { return ((w + 0x13131313u) ^ 0x80808080u) & 0xe0e0e0e0u; }
+// Scale bytes 253 .. 255, which V takes as NaN: bit 7 of each such byte of w.
+TLM_DEV uint32_t ka_nan(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x03030303u) & w & 0x80808080u; }
 
 // Two floats -> their bf16 parts and the bf16 parts of what is left: 16 bits of each. An infinity leaves nothing.
 TLM_DEV void ka_split(float x, float y, uint32_t& hi, uint32_t& lo) {
@@ -636,16 +638,16 @@ TLM_DEV void ka_piece(const KaArgs& a, const KaPiece& pc, const KaFetch<D, NP>& 
       for (int i = 0; i < 8; ++i) x.v[i][s] = tk + ka_token(g, i) < e.keys ? x.v[i][s] : 0u;
     });
   };
-  // Whether fp16 holds all V (bf16 queries) or K (fp16 queries) of the tile.
+  // Whether fp16 holds all V (bf16 queries) or K (fp16 queries) of the tile, and no V is NaN.
   auto suits = [&](const KaTile<D>& x) {
     uint32_t no = 0;
     unroll<0, S::N>([&](auto s) {
       no |= BF16 ? ka_not_f16(x.vs[s][0]) | ka_not_f16(x.vs[s][1])
-                 : (ka_not_f16(x.ks[0][s]) | ka_not_f16(x.ks[1][s])) & 255u;
+                 : ((ka_not_f16(x.ks[0][s]) | ka_not_f16(x.ks[1][s])) & 255u) | ka_nan(x.vs[s][0]) | ka_nan(x.vs[s][1]);
     });
     return !__any(no != 0);
   };
-  // A tile. ALL: every row sees all of it. FAST (it suits): V (bf16 queries) or K (fp16) in fp16; else all in bf16, weights
+  // A tile. ALL: every row sees all of it (FAST only). FAST (it suits): V (bf16 queries) or K (fp16) in fp16; else all in bf16, weights
   // and fp16 queries in two terms.
   auto compute = [&](KaTile<D>& x, int tk, auto all, auto form) {
     constexpr bool ALL = decltype(all)::value, FAST = decltype(form)::value, PV16 = BF16 && FAST;
@@ -684,7 +686,7 @@ TLM_DEV void ka_piece(const KaArgs& a, const KaPiece& pc, const KaFetch<D, NP>& 
     }
     read_v(x);
     if constexpr (!ALL) clear_v(x, tk);
-    if constexpr (!ALL && !PV16) {
+    if constexpr (!FAST) {
       // NaN of V that a row does not see must not meet its weight of 0: such blocks become zeros, and the rows that see
       // one become NaN by their count of it
       u32x4 seen[QT];
@@ -701,7 +703,7 @@ TLM_DEV void ka_piece(const KaArgs& a, const KaPiece& pc, const KaFetch<D, NP>& 
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const int at = 8 * (i & 3);
-          const bool nan = ((x.vs[s][i >> 2] >> at) & 255u) > 252u;
+          const bool nan = (ka_nan(x.vs[s][i >> 2]) >> at & 128u) != 0;
           bad[i >> 1] |= !nan ? 0u : (i & 1) ? 0x3f800000u : 0x3f80u;
           x.v[i][s] = nan ? 0u : x.v[i][s];
           x.vs[s][i >> 2] = nan ? (x.vs[s][i >> 2] & ~(255u << at)) | 127u << at : x.vs[s][i >> 2];
