@@ -705,3 +705,30 @@ def test_attn_scale_bytes_253_and_254_of_v_are_nan(dtype, D, T, H, Hkv, codes):
     s255 = s.clone()
     s255[:, 1][s255[:, 1] >= 253] = 255
     _check(q, c, s255, bt, lens, got=out)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("page", [8, 16, 24, 32, 64, 128])
+@pytest.mark.parametrize("D,T,H,Hkv", [(64, 1, 96, 96), (128, 9, 128, 64)])
+def test_attn_missing_pages_after_full_rings(D, T, H, Hkv, page, dtype):
+    """Pages outside the pool between others, in whole tiles and in the last one, where every stage of a wave's ring has
+    held codes before: few ranges of 6 units or more for each of many K/V heads (of which the first and the last are
+    compared)."""
+    lens = [3000, 1700, 905]
+    g = torch.Generator().manual_seed(page + D)
+    per = -(-lens[0] // page)
+    c, s = _pools(3 * per + 2, Hkv, page, D, page)
+    bt = torch.randperm(3 * per + 2, generator=g)[:3 * per].view(3, per).int().numpy()
+    q = torch.randn(3, T, H, D, generator=g).to(dtype)
+    c, s = _stale(c, s, bt, lens, page)
+    none = [-1, c.shape[0], -2147483648, 2147483647]
+    last = [(n - 1) // page for n in lens]
+    for b in range(3):
+        for p in range(640 // page + b, last[b], 5 if page < 128 else 3):
+            bt[b, p] = none[p % 4]
+    bt[1, last[1]] = -1  # the masked tile's own page
+    out, z = _run(q, c, s, bt, lens)
+    for kv in (0, Hkv - 1):
+        own = slice(kv * (H // Hkv), (kv + 1) * (H // Hkv))
+        _check(q[:, :, own], c[:, :, kv:kv + 1], s[:, :, kv:kv + 1], bt, lens, scale=D ** -0.5,
+               got=(out[:, :, own], z[:, :, own]))
