@@ -732,3 +732,81 @@ def test_attn_missing_pages_after_full_rings(D, T, H, Hkv, page, dtype):
         own = slice(kv * (H // Hkv), (kv + 1) * (H // Hkv))
         _check(q[:, :, own], c[:, :, kv:kv + 1], s[:, :, kv:kv + 1], bt, lens, scale=D ** -0.5,
                got=(out[:, :, own], z[:, :, own]))
+
+
+@pytest.mark.parametrize("first", [False, True])
+@pytest.mark.parametrize("B", [1022, 1023, 1024, 2000])
+def test_read_many_sequences(B, first):
+    """As many sequence starts as are searched in LDS, one fewer, one more, and twice as many; empty sequences among them, at
+    both ends too."""
+    Hkv, D, page, per = 1, 32, 8, 2
+    g = torch.Generator().manual_seed(B)
+    codes, scales = _pools(B * per, Hkv, page, D, B)
+    bt = torch.randperm(B * per, generator=g).view(B, per).int().numpy()
+    n = torch.randint(0, 9, (B,), generator=g).numpy()
+    n[:3] = n[-2:] = n[B // 2:B // 2 + 5] = 0
+    start = torch.randint(0, 9, (B,), generator=g).numpy() if first else np.zeros(B, np.int64)
+    cu = np.concatenate([[0], np.cumsum(n)]).astype(np.int32)
+    outs = [torch.full((int(cu[-1]) + 2, Hkv, D), 7.0, dtype=BF16, device=DEV) for _ in "kv"]
+    ops.kv4_read(codes.to(DEV), scales.to(DEV), _i32(bt), _i32(start) if first else None, _i32(cu), *outs)
+    rows = [ref.kv4_rows_ref(codes.numpy(), scales.numpy(), bt, b, int(start[b]), int(n[b])) for b in range(B)]
+    for w, out in enumerate(outs):
+        exp = np.concatenate([r[w] for r in rows])
+        assert np.array_equal(out[:len(exp)].double().cpu().numpy(), exp) and (out[len(exp):] == 7).all()
+
+
+def test_append_more_sequences_than_a_grid_is_deep():
+    B, Hkv, D, page = 65540, 1, 32, 8
+    g = torch.Generator().manual_seed(41)
+    k, v = (torch.randn(B, 1, Hkv, D, generator=g).to(BF16) for _ in "kv")
+    codes, scales = _pools(B, Hkv, page, D)
+    bt = torch.randperm(B, generator=g).view(B, 1).int().numpy()
+    start, count = (torch.randint(0, m, (B,), generator=g).int().numpy() for m in (page, 2))
+    start[-4:], count[-4:] = [0, 7, 3, 8], [1, 1, 0, 1]  # the last sequence is full
+    got = _append(k, v, start, count, bt, codes, scales)
+    exp = ref.kv4_append_ref(k, v, start, count, bt, codes.numpy(), scales.numpy())
+    assert np.array_equal(got[0], exp[0]) and np.array_equal(got[1], exp[1])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_prompt_read_back_and_attended(dtype):
+    """Rows appended, read back and given to tlm_flash_attn_varlen_fwd: within that kernel's roundings of the float64
+    attention over the cache, and tlm_kv4_attn on the same rows within its own.
+
+    tlm_flash_attn_varlen_fwd rounds each weight to dtype (eps / 2 of it) and sums the rounded or the unrounded ones (eps / 2
+    of the quotient at most); its scores are fp32 sums of D exact products, off by (D + 4) 2^-24 of the sum of their
+    magnitudes A, and a weight by that times 2; the sums of n terms are off by (n + 64) 2^-24 of the sum of magnitudes
+    each. Its weights are relative to a maximum that a row has had, so the small ones of fp16 may fall among subnormal
+    numbers: half a step of those is 2^-25, n times, of the largest |v|. The output is rounded once."""
+    g = torch.Generator().manual_seed(42)
+    H, Hkv, D, page, T = 8, 2, 128, 16, 8
+    have = np.array([103, 40, 67, 8])
+    B, per = len(have), 7
+    codes, scales = (x.to(DEV) for x in _pools(B * per, Hkv, page, D, 43, 255, 256))
+    bt = torch.randperm(B * per, generator=g).view(B, per).int().numpy()
+    k, v = (torch.randn(B, int(have.max()), Hkv, D, generator=g).to(dtype) for _ in "kv")
+    ops.kv4_append(k.to(DEV), v.to(DEV), _i32([0] * B), _i32(have), _i32(bt), codes, scales)
+    cu = np.concatenate([[0], np.cumsum(have)]).astype(np.int32)
+    ko, vo = (torch.empty(int(cu[-1]), Hkv, D, dtype=dtype, device=DEV) for _ in "kv")
+    ops.kv4_read(codes, scales, _i32(bt), None, _i32(cu), ko, vo)
+    q = torch.randn(B, T, H, D, generator=g).to(dtype)
+    o = torch.empty(B * T, H, D, dtype=dtype, device=DEV)
+    ops.flash_attn_varlen_fwd(q.flatten(0, 1).to(DEV), ko, vo, _i32([T * b for b in range(B + 1)]), _i32(cu), T, o, True,
+                              D ** -0.5)
+    c, s = codes.cpu(), scales.cpu()
+    _check(q, c, s, bt, have)
+    exp, _ = ref.kv4_attn_ref(q, c.numpy(), s.numpy(), bt, have, None, D ** -0.5)
+    mag = c.clone()
+    mag[:, 1] &= 0x77
+    spread, _ = ref.kv4_attn_ref(q, mag.numpy(), s.numpy(), bt, have, None, D ** -0.5)
+    eps = torch.finfo(dtype).eps
+    n = int(have.max())
+    for b in range(B):
+        kk, vv = ref.kv4_rows_ref(c.numpy(), s.numpy(), bt, b, 0, int(have[b]))
+        kk = np.abs(kk).repeat(H // Hkv, 1).transpose(1, 2, 0)
+        a = (np.abs(q[b].double().numpy()).transpose(1, 0, 2) @ kk * D ** -0.5).max(-1).T[..., None]  # [T, H, 1]
+        rel = eps + 2 * ((D + 4) * 2.0 ** -24 * a + 2.0 ** -23 + (n + 64) * 2.0 ** -24)
+        small = n * 2.0 ** -25 * np.abs(vv).max() if dtype == F16 else 0.0
+        lim = eps / 2 * (1 + 2 ** -7) * np.abs(exp[b]) + rel * spread[b] + small
+        err = np.abs(o.view(B, T, H, D)[b].double().cpu().numpy() - exp[b])
+        assert (err <= lim).all(), (b, (err / lim).max())
