@@ -810,3 +810,30 @@ def test_prompt_read_back_and_attended(dtype):
         lim = eps / 2 * (1 + 2 ** -7) * np.abs(exp[b]) + rel * spread[b] + small
         err = np.abs(o.view(B, T, H, D)[b].double().cpu().numpy() - exp[b])
         assert (err <= lim).all(), (b, (err / lim).max())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("D,T,H,Hkv", [(64, 1, 4, 1), (128, 9, 8, 2), (256, 1, 2, 2)])
+@pytest.mark.parametrize("power", [10, 19, 21, 22, 23, 24, 25, 27, 30, 40, 90, 118])
+def test_attn_scores_whose_steps_are_wide(power, D, T, H, Hkv, dtype):
+    """Scores of +-1.375 D 2^(power - 7) whose neighbours in fp32 are up to 2^96 apart: one key is half or twice as far as the
+    others, so its V is the output, exactly (a weight's rounding is far below half a step of the output), and its score
+    the log2 of the sum. The key comes first, last, between and alone; its scores above 0 and below."""
+    lens = [600, 300, 1, 40, 33, 600]
+    at = [599 - (T - 1), 0, 0, 17, 31 - (T - 1), 350]
+    q, c, s, bt = _attn_case(dtype, 6, T, H, Hkv, D, 16, [600 + T] * 6, 44)
+    lens = [n + T - 1 for n in lens]  # every query sees the key
+    c[:, 1] |= 0x11  # no zeros in V
+    s[:, 1] = 127 + torch.randint(-3, 3, s[:, 1].shape, generator=torch.Generator().manual_seed(45)).to(torch.uint8)
+    q = torch.full_like(q, 1.375)  # no power of two: the product with log2 e is rounded
+    for sign in (1, -1):
+        c[:, 0], s[:, 0] = (0x22 if sign > 0 else 0xAA), 120  # K: +-1 2^-7
+        for b in range(6):
+            s[int(bt[b, at[b] // 16]), 0, :, :, at[b] % 16] = 120 + sign
+        out, z = _run(q, c, s, bt, lens, scale=2.0 ** power)
+        top = sign * 1.375 * D * 2.0 ** (power - 7 + sign)
+        for b in range(6):
+            v = ref.kv4_rows_ref(c.numpy(), s.numpy(), bt, b, at[b], 1)[1][0].repeat(H // Hkv, 0)  # [H, D]
+            x = out[b].double().numpy()
+            assert np.array_equal(x, np.broadcast_to(v, x.shape)), (sign, b)
+            assert (np.abs(z[b].double().numpy() / (top / np.log(2)) - 1) < 2.0 ** -21).all(), (sign, b)

@@ -56,6 +56,10 @@ constexpr int ka_stages() {
 // Weights are 2^(s - reference): 2^BIAS for the score that set the reference, which is kept until another passes
 // that one by SLACK. At most 2^15, an fp16 number, and normal ones down to 2^-25 of the largest.
 constexpr float KA_BIAS = 11.f, KA_SLACK = 4.f;
+// From here on a reference is the score itself and the tile takes the slower form, which rounds products with the scale before
+// it subtracts: the product inside an fma is exact, the reference was rounded, so a row's weights are off by a common factor of
+// up to 2^(a step of fp32): 2^(1/4) below KA_FAR, but past fp16 from 2^25 on, and nothing or infinite farther out.
+constexpr float KA_FAR = 0x1p22f;
 
 struct alignas(16) KaCut {
   int b, rt, n;  // sequence (-1: nothing to join), row tile, new tokens
@@ -368,6 +372,12 @@ TLM_DEV uint32_t ka_not_f16(uint32_t w) { return ((w + 0x13131313u) ^ 0x80808080
 // Scale bytes 253 .. 255, which V takes as NaN: bit 7 of each such byte of w.
 TLM_DEV uint32_t ka_nan(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x03030303u) & w & 0x80808080u; }
 
+// x y, rounded by itself: no part of an fma.
+TLM_DEV float ka_mul(float x, float y) {
+#pragma clang fp contract(off)
+  return x * y;
+}
+
 // Two floats -> their bf16 parts and the bf16 parts of what is left: 16 bits of each. An infinity leaves nothing.
 TLM_DEV void ka_split(float x, float y, uint32_t& hi, uint32_t& lo) {
   hi = h16<true>::pack(x, y);
@@ -586,18 +596,22 @@ TLM_DEV void ka_piece(const KaArgs& a, const KaPiece& pc, const KaFetch<D, NP>& 
       }
     });
   };
-  // the column's reference moves when a score passes it by too much
+  // the column's reference moves when a score passes it by too much; whether one moved to KA_FAR or beyond
   auto weigh = [&](int t, float top) {
+    bool far = false;
     if (__any(top > thr[t])) {
       top = xhalf_max(xrow_max(top));  // over the four lanes of the column
       const bool up = top > thr[t];
-      const float f = !up ? 1.f : thr[t] == -INFINITY ? 0.f : fast_exp2(ref[t] - (top - KA_BIAS));
-      ref[t] = up ? top - KA_BIAS : ref[t];
+      const float next = fabsf(top) < KA_FAR ? top - KA_BIAS : top;
+      far = __any(up && fabsf(top) >= KA_FAR && top < INFINITY);  // (with an infinity the row is NaN in either form)
+      const float f = !up ? 1.f : thr[t] == -INFINITY ? 0.f : fast_exp2(ref[t] - next);
+      ref[t] = up ? next : ref[t];
       thr[t] = up ? top + KA_SLACK : thr[t];
       l[t] *= f;
 #pragma unroll
       for (int i = 0; i < ND; ++i) o[t][i] *= f;
     }
+    return far;
   };
   // V^T operands of each 16 dims: row jl is a dim, the lane's eight tokens lie along
   auto values = [&](auto f16, auto&& word, auto&& scale, auto&& use) {
@@ -648,7 +662,7 @@ TLM_DEV void ka_piece(const KaArgs& a, const KaPiece& pc, const KaFetch<D, NP>& 
     return !__any(no != 0);
   };
   // A tile. ALL: every row sees all of it (FAST only). FAST (it suits): V (bf16 queries) or K (fp16) in fp16; else all in bf16, weights
-  // and fp16 queries in two terms.
+  // and fp16 queries in two terms. False where a score is too far for the fast form: the tile is still to be done.
   auto compute = [&](KaTile<D>& x, int tk, auto all, auto form) {
     constexpr bool ALL = decltype(all)::value, FAST = decltype(form)::value, PV16 = BF16 && FAST;
     f32x4 sc[QT][2];
@@ -668,10 +682,14 @@ TLM_DEV void ka_piece(const KaArgs& a, const KaPiece& pc, const KaFetch<D, NP>& 
       float top = -INFINITY;
 #pragma unroll
       for (int i = 0; i < 8; ++i) top = fmaxf(top, sc[t][i >> 2][i & 3]);
-      weigh(t, top * a.scale2);
+      const bool far = weigh(t, top * a.scale2);
+      if (FAST && far) return false;
       float y[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = fast_exp2(fmaf(sc[t][i >> 2][i & 3], a.scale2, -ref[t]));
+      for (int i = 0; i < 8; ++i) {
+        const float x = sc[t][i >> 2][i & 3];
+        y[i] = fast_exp2(FAST ? fmaf(x, a.scale2, -ref[t]) : ka_mul(x, a.scale2) - ref[t]);
+      }
       l[t] += ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -730,6 +748,7 @@ TLM_DEV void ka_piece(const KaArgs& a, const KaPiece& pc, const KaFetch<D, NP>& 
              }
              if constexpr (!FAST) __builtin_amdgcn_sched_barrier(0);  // fewer registers
            });
+    return true;
   };
 
   if (t0 < tend) {
@@ -768,16 +787,15 @@ TLM_DEV void ka_piece(const KaArgs& a, const KaPiece& pc, const KaFetch<D, NP>& 
       vm_wait<(NST - 1) * St::PER>();
     };
     // Loops of one form each (a choice within a loop costs registers): tiles that every row sees whole, the others, and
-    // from the first tile on that does not suit
+    // from the first tile on that does not suit or has a score too far
     const int whole_end = min(tend, e.keys_min);
     bool fast = true;
     for (; t0 + KA_BN <= whole_end; t0 += KA_UNIT) {
       next();
       KaTile<D> x;
       read_k(x);
-      fast = suits(x);
+      fast = suits(x) && compute(x, t0, std::true_type{}, std::true_type{});
       if (!fast) break;
-      compute(x, t0, std::true_type{}, std::true_type{});
     }
     if (fast)
       for (; t0 < tend; t0 += KA_UNIT) {
@@ -785,9 +803,8 @@ TLM_DEV void ka_piece(const KaArgs& a, const KaPiece& pc, const KaFetch<D, NP>& 
         KaTile<D> x;
         read_k(x);
         clear_scales(x, t0);
-        fast = suits(x);
+        fast = suits(x) && compute(x, t0, std::false_type{}, std::true_type{});
         if (!fast) break;
-        compute(x, t0, std::false_type{}, std::true_type{});
       }
     for (bool here = true; !fast && t0 < tend; t0 += KA_UNIT, here = false) {
       if (!here) next();
