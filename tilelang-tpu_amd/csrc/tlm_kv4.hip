@@ -8,9 +8,9 @@
 // nearest even, saturates and keeps the sign of zero (every 16-bit pattern compared with exact arithmetic); the reverse
 // conversions are exact and pass a NaN scale on.
 //
-// Bound: HBM. A token and head moves 4 D bytes of 16-bit rows and 1.0625 D bytes of cache. 8 heads of 128: 65,536 tokens read
+// Bound: HBM. A token and head moves 4 D bytes of 16-bit rows and 1.0625 D bytes of cache. 8 heads of 128: 63,997 tokens read
 // back in 53 us (6.2 TB/s; with plain stores 70 us, one 8-dim chunk per thread with its own search and divisions 148 us);
-// 13,500 tokens appended in 16.2 us (4.3 TB/s; one chunk per thread 30 us). A decode step's rows take 3.6 us,
+// 13,312 tokens appended in 16.2 us (4.3 TB/s; one chunk per thread 30 us). A decode step's rows take 3.6 us,
 // which is launch and three dependent loads.
 #include "tlm_kv4.h"
 
@@ -220,7 +220,7 @@ extern "C" int tlm_kv4_append(const void* k, const void* v, int64_t k_batch_stri
   c.max_pages = (int)max_pages, c.page = (int)page, c.Hkv = (int)H_kv, c.D = (int)D;
   const int64_t per = K4_T / (D / 8), gx = std::min<int64_t>((T + per - 1) / per, K4_GRID);
   const int64_t gz = std::min<int64_t>(B, 65535);
-  // eight heads in flight where that leaves 8 workgroups per CU (40,000 tokens of 8 heads of 128: 28.3 instead of 30.9 us), else
+  // eight heads in flight where that leaves 8 workgroups per CU (40,000 tokens of 8 heads of 128: 38.6 instead of 41.4 us), else
   // four (32 tokens: 3.7 instead of 4.6 us)
   const int U = gx * gz * ((2 * H_kv + 7) / 8) >= 2048 ? 2 * K4_U : K4_U;
   const int heads = heads_per_wg(gx * gz, H_kv, U);

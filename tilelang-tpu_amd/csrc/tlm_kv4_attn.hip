@@ -7,9 +7,10 @@
 //
 // What bounds it: one new token, the stream of codes: 64 sequences of 512 .. 8,192 tokens, 32 / 8 heads of 128 (bf16): 304 MB
 // in 55 us, 5.6 TB/s; the same without the arithmetic 52 us. Few tokens, the chain launch, lengths, table, tile, exchange: 6.4 us
-// for one sequence of 1,000, 2.8 for the join. Prompt chunks, instruction issue: two chunks of 1,024 over 8,192 and 16,384
-// tokens 502 us (725 TFLOP/s); a 32-token tile of 32 rows issues 32 MFMAs (512 cycles), 64 conversions and 32 permutations (420) and
-// the softmax (340), which hide under each other little (one wave's MFMA and VALU work do not overlap at all).
+// for one sequence of 1,000, 2.8 for the join. Prompt chunks, instruction issue: chunks of 768 and 1,024 over 8,192 and
+// 16,384 tokens 507 us (720 TFLOP/s); a 32-token tile of 32 rows issues 32 MFMAs (512 cycles), 64 conversions and 32
+// permutations (420) and the softmax (340), which hide under each other little (one wave's MFMA and VALU work do not overlap
+// at all).
 //
 //   * Partition: entry (sequence, row tile) costs its 128-token units plus KA_PIECE; the cost line of the batch is cut into
 //     up to G equal ranges, one workgroup each per K/V head, found from the lengths by the workgroups themselves. A
@@ -24,9 +25,10 @@
 //     are what O^T += V^T P^T wants of it: P never moves between lanes. V^T costs one permutation per pair of values.
 //   * Types: bf16 queries meet K in bf16 and their weights, as fp16 numbers, V in fp16 (half a step of a weight is 2^-12 to
 //     2^-11; the output's is 2^-9 to 2^-8). fp16 queries meet K in fp16, their weights V in bf16 in two terms, since one rounding
-//     to fp16 would show in an fp16 output (1.4 times its error). Where a scale does not suit fp16, the rest of the piece runs in
-//     bf16, weights and fp16 queries in two terms. Both forms in one loop would spill: with scratch memory in use the kernel
-//     above takes 68 instead of 55 us.
+//     to fp16 would show in an fp16 output (1.4 times its error). Where a scale does not suit fp16, a V is NaN or a score far
+//     out, the rest of the piece runs in bf16, weights and fp16 queries in two terms (64 sequences with a V of zeros, scale
+//     byte 1, in every token: 80 us). Both forms in one loop would spill: with scratch memory in use the kernel above takes 68
+//     instead of 55 us.
 //   * The reference of a row moves when a score passes it by 2^KA_SLACK only, so O is rescaled a few times per row.
 //   * Codes that only one row tile reads bypass the caches (74 -> 65 us); those of longer chunks are shared through the L2 of
 //     the XCD that the K/V head's workgroups are on (8 heads).
@@ -378,12 +380,12 @@ TLM_DEV float ka_mul(float x, float y) {
   return x * y;
 }
 
-// Two floats -> their bf16 parts and the bf16 parts of what is left: 16 bits of each. An infinity leaves nothing.
+// Two floats -> their bf16 parts and the bf16 parts of what is left: 16 bits of each.
 TLM_DEV void ka_split(float x, float y, uint32_t& hi, uint32_t& lo) {
   hi = h16<true>::pack(x, y);
   lo = h16<true>::pack(x - h16<true>::lo(hi), y - h16<true>::hi(hi));
 }
-TLM_DEV void ka_split_f16(u32x4 x, u32x4& hi, u32x4& lo) {  // fp16 words: exact
+TLM_DEV void ka_split_f16(u32x4 x, u32x4& hi, u32x4& lo) {  // fp16 words: exact; an infinity leaves nothing
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float y0 = h16<false>::lo(x[i]), y1 = h16<false>::hi(x[i]);
