@@ -497,6 +497,41 @@ int tlm_kv4_attn(const void* q, int64_t q_batch_stride, int64_t q_row_stride, co
                  size_t ws_bytes, int64_t B, int64_t T, int64_t H, int64_t H_kv, int64_t D,
                  int causal, float sm_scale, int dtype, void* stream);
 
+/* Dense layers in 8 bits: OCP MX e4m3 operands with one e8m0 scale (2^e, exponent + 127; 255 is NaN) per 32 values of
+ * a row. No reference program has them.
+ *   codes   [rows, K], dense, 16-byte aligned; K a multiple of 32, up to 2^22.
+ *   scales  [ceil(rows / 64), ceil(K / 128), 4, 64] bytes, 4-byte aligned: that of block b of row r at
+ *           [r / 64, b / 4, b % 4, r % 64], as the matrix instructions take them. Places past the last row or block are
+ *           neither written nor used.
+ * Quantising: a block's scale is the least 2^e, e >= -126, of which its largest magnitude is at most 448 times; codes are
+ * x / 2^e rounded to nearest even. A block with an infinity or a NaN gets scale 255 and codes 0, and reads as NaN.
+ * Calls without rows or columns do nothing; what would hold them may be null then. */
+
+/* Quantises rows x [rows, cols] of x_dtype (F16 | BF16 | F32), x_stride elements apart (a multiple of 8; x 16-byte
+ * aligned). */
+int tlm_mx8_quant(const void* x, int64_t x_stride, int x_dtype, void* codes, void* scales, int64_t rows,
+                  int64_t cols, void* stream);
+
+/* The residual's addition and RMS norm: residual_out = x + residual, rounded to residual_dtype (x_dtype, or F32);
+ * of that, as stored, residual_out * rsqrt(mean(residual_out^2) + eps) * w, in fp32, rounded once to x_dtype (y), to 8 bits
+ * (codes and scales), or to both. x, residual, residual_out, y [rows, cols] dense, w [cols] of x_dtype (F16 | BF16), all
+ * 16-byte aligned. residual and residual_out NULL: the norm of x; residual_out may be residual; w NULL: no weight; y NULL or codes
+ * and scales NULL: not wanted. cols a multiple of 8 (of 32 with codes). */
+int tlm_add_rmsnorm(const void* x, const void* residual, const void* w, void* residual_out, void* y, void* codes,
+                    void* scales, int64_t rows, int64_t cols, float eps, int x_dtype, int residual_dtype,
+                    void* stream);
+
+/* C = A B^T of 8-bit operands A [M, K], B [N, K]; C [M, N] of out_dtype (F16 | BF16), dense. The matrix cores' sums of
+ * 8-bit products hold about 17 bits, which 16-bit results do not show (fp32 ones would). */
+int tlm_gemm_mx8(const void* a, const void* a_scales, const void* b, const void* b_scales, void* c, int64_t M,
+                 int64_t N, int64_t K, int out_dtype, void* stream);
+
+/* up * gate / (1 + exp(-gate)) with gate = A gate^T, up = A up^T (weights [N, K]) in 8 bits: codes [M, N] and scales,
+ * quantised from fp32. N a multiple of 32. */
+int tlm_gemm_mx8_swiglu(const void* a, const void* a_scales, const void* gate, const void* gate_scales,
+                        const void* up, const void* up_scales, void* codes, void* scales, int64_t M, int64_t N,
+                        int64_t K, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -636,3 +636,83 @@ def kv4_attn_ref(q: torch.Tensor, codes: np.ndarray, scales: np.ndarray, block_t
                 out[b, i] = np.where((total[:, i] > 0)[:, None] | np.isnan(o), o / total[:, i, None], 0.0)
                 lse[b, i] = (np.where(np.isneginf(top[:, i]), 0.0, top[:, i]) + np.log(total[:, i])) / np.log(2.0)
     return out, lse
+
+
+# ---------------------------------------------------------------------------------------------
+# Dense layers in 8 bits (tlm_mx8_quant / tlm_add_rmsnorm / tlm_gemm_mx8 / tlm_gemm_mx8_swiglu): OCP MX e4m3
+# elements with one e8m0 scale per 32 values. No reference program; the definition is the header's.
+MX8_BLOCK = 32
+MX8_VALUES = np.concatenate([np.arange(8) / 512.0] + [(1 + np.arange(8) / 8.0) * 2.0 ** (e - 7) for e in range(1, 16)])[:127]
+
+
+def mx8_scale_ref(big: np.ndarray) -> np.ndarray:
+    """Scale bytes of blocks whose largest magnitude is big (float64; 255: infinite or NaN)."""
+    bad = ~np.isfinite(big)
+    e = np.full(big.shape, 127, dtype=np.int64)
+    for t in range(126, -127, -1):  # downwards while it still holds
+        e = np.where(big <= 448.0 * 2.0 ** t, t, e)
+    return np.where(bad, 255, e + 127).astype(np.uint8)
+
+
+def mx8_quantise_ref(x) -> tuple:
+    """Rows [rows, K] (torch or float64) -> codes uint8 [rows, K], scale bytes [rows, K / 32]: the nearest e4m3
+    value (a tie takes the even code), the sign of zero kept; a block without a number has codes 0."""
+    v = (x.double().numpy() if isinstance(x, torch.Tensor) else np.asarray(x, np.float64))
+    rows, K = v.shape
+    v = v.reshape(rows, K // MX8_BLOCK, MX8_BLOCK)
+    with np.errstate(invalid="ignore"):
+        byte = mx8_scale_ref(np.abs(v).max(-1)) if v.size else np.zeros(v.shape[:2], np.uint8)
+    bad = byte == 255
+    y = np.where(bad[..., None], 0.0, v) / (2.0 ** (np.where(bad, 127, byte).astype(np.int64) - 127))[..., None]
+    a = np.minimum(np.abs(y), 448.0)
+    hi = np.searchsorted(MX8_VALUES, a).clip(0, 126)
+    lo = np.maximum(hi - 1, 0)
+    below, above = a - MX8_VALUES[lo], MX8_VALUES[hi] - a
+    code = np.where(above < below, hi, np.where(below < above, lo, np.where(lo % 2 == 0, lo, hi)))
+    code = np.where(MX8_VALUES[hi] == a, hi, code)
+    code = np.where(bad[..., None], 0, code | np.where(np.signbit(y), 128, 0))
+    return code.astype(np.uint8).reshape(rows, K), byte
+
+
+def mx8_values_ref(codes: np.ndarray, scales: np.ndarray) -> np.ndarray:
+    """float64 values of codes uint8 [rows, K] and scale bytes [rows, K / 32]."""
+    table = np.concatenate([MX8_VALUES, [np.nan], -MX8_VALUES, [np.nan]])
+    s = np.where(scales == 255, np.nan, 2.0 ** (scales.astype(np.float64) - 127))
+    return table[codes] * np.repeat(s, MX8_BLOCK, -1)
+
+
+def mx8_tile_ref(scales: np.ndarray, old: np.ndarray) -> np.ndarray:
+    """Scale bytes [rows, K / 32] written into a copy of old [ceil(rows / 64), ceil(K / 128), 4, 64]."""
+    out = old.copy()
+    for r in range(scales.shape[0]):
+        for b in range(scales.shape[1]):
+            out[r // 64, b // 4, b % 4, r % 64] = scales[r, b]
+    return out
+
+
+def mx8_untile_ref(tiled: np.ndarray, rows: int, K: int) -> np.ndarray:
+    r, b = np.arange(rows)[:, None], np.arange(K // MX8_BLOCK)[None]
+    return tiled[r // 64, b // 4, b % 4, r % 64]
+
+
+def add_rmsnorm_ref(x: torch.Tensor, residual, w, eps: float):
+    """(residual_out, norm in float64): the sum in fp32, rounded to the residual's dtype; the norm is that of the
+    rounded sum."""
+    out = None if residual is None else (x.float() + residual.float()).to(residual.dtype)
+    h = (x if out is None else out).double().numpy()
+    y = h / np.sqrt((h * h).mean(-1, keepdims=True) + eps)
+    return out, y if w is None else y * w.double().numpy()
+
+
+def gemm_mx8_ref(a, b):
+    """a @ b.T in float64 of (codes, scale bytes), and the sum of the products' magnitudes."""
+    x, y = mx8_values_ref(*a), mx8_values_ref(*b)
+    return x @ y.T, np.abs(x) @ np.abs(y).T
+
+
+def gemm_mx8_swiglu_ref(a, gate, up):
+    """up * silu(gate) in float64, and how far it moves when every product's magnitude is off by one part."""
+    (g, gs), (u, us) = gemm_mx8_ref(a, gate), gemm_mx8_ref(a, up)
+    with np.errstate(over="ignore", invalid="ignore"):
+        silu = g / (1 + np.exp(-g))
+        return u * silu, np.abs(silu) * us + 1.1 * np.abs(u) * gs  # |silu'| < 1.1

@@ -87,6 +87,10 @@ _SIGNATURES = {
     "tlm_kv4_attn": ([c_void_p] + [c_int64] * 2 + [c_void_p, c_int64] * 2 + [c_int64, c_void_p] +
                      [c_int64] * 2 + [c_void_p] * 5 + [c_size_t] + [c_int64] * 5 +
                      [c_int, c_float, c_int, c_void_p], c_int),
+    "tlm_mx8_quant": ([c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int64, c_int64, c_void_p], c_int),
+    "tlm_add_rmsnorm": ([c_void_p] * 7 + [c_int64] * 2 + [c_float, c_int, c_int, c_void_p], c_int),
+    "tlm_gemm_mx8": ([c_void_p] * 5 + [c_int64] * 3 + [c_int, c_void_p], c_int),
+    "tlm_gemm_mx8_swiglu": ([c_void_p] * 8 + [c_int64] * 3 + [c_void_p], c_int),
 }
 
 EXPORTED = tuple(_SIGNATURES)
