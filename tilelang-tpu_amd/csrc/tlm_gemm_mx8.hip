@@ -151,10 +151,310 @@ __global__ __launch_bounds__(64 * D_WAVES) void gemm_mx8_direct(Args a) {
   }
 }
 
+// ---- whole prompts: 256 x 256 tiles
+
+// The ping-pong schedule of gemm8_256x256 (tlm_gemm_fp8.hip): the two waves of a SIMD take turns, one reads its next operands from LDS
+// while the other multiplies, and LDS-DMA is issued only beside the reads. Here W, the weights, is the operand a wave holds
+// (128 rows: 8 operands) and X the one it reads as it multiplies (64 rows: 4).
+//
+// Slot 16 f + i of a 64-row group of an LDS stage holds row 4 i + f, so that operand f, read from 16 neighbouring slots, has the rows
+// whose scales are byte f of the lanes' words: three words a k step, loaded a step ahead, are all the scales a wave needs. Of the
+// sums, a lane then has 16 neighbouring columns of each of its rows: C is stored, or a block of 32 quantised with one exchange
+// between two lanes, without a way through LDS.
+constexpr int P_T = 512, P_M = 256, P_N = 256, P_ST = 256 * 128;  // P_ST: bytes of a stage of one operand
+constexpr int P_W = 2, P_X = 3;                                   // stages of W and X
+constexpr uint32_t OOB = 0x80000000u;                             // past every descriptor's end, also with 3 K more
+
+TLM_DEV void wait_lgkm0() { __builtin_amdgcn_s_waitcnt(0xc07f); }
+template <int N>
+TLM_DEV void wait_lgkm() {
+  __builtin_amdgcn_s_waitcnt(0xc07f | (N << 8));
+}
+template <int N>
+TLM_DEV void wait_vm() {
+  static_assert(N < 64, "vmcnt is 6 bits");
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_waitcnt(0x3f70 | (N & 15) | ((N >> 4) << 14));
+  __builtin_amdgcn_sched_barrier(0);
+}
+TLM_DEV void barrier() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" ::: "memory");
+  wait_lgkm0();
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+TLM_DEV i32x8 cat8(u32x4 lo, u32x4 hi) {
+  return i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+}
+// 16 bytes per lane at base + off to dst and on; zeros from `end` on.
+TLM_DEV void dma16(const uint8_t* base, int end, uint8_t* dst, uint32_t off) {
+  const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, end, 0x00020000);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)dst, 16, off, 0, 0, 0);
+}
+
+// XCD x (workgroup % 8) takes a contiguous range of tiles, row tiles in groups of four, so that its L2 serves both operands.
+TLM_DEV void tile_of(int wg, int tiles_m, int tiles_n, int& tm, int& tn) {
+  const int total = tiles_m * tiles_n, xcd = wg & 7;
+  const int lin = xcd * (total >> 3) + min(xcd, total & 7) + (wg >> 3);
+  const int per = 4 * tiles_n, first = lin / per * 4, gm = min(tiles_m - first, 4), r = lin % per;
+  tm = first + r % gm;
+  tn = r / gm;
+}
+
+// 16 neighbouring columns col .. of a row of C.
+template <int OUT>
+TLM_DEV void store16(uint16_t* c, const float (&v)[16], int64_t left, bool vec) {
+  using H = h16<OUT == TLM_BF16>;
+  if (vec && left >= 16) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      *(u32x4*)(c + 8 * h) = u32x4{H::pack(v[8 * h], v[8 * h + 1]), H::pack(v[8 * h + 2], v[8 * h + 3]),
+                                   H::pack(v[8 * h + 4], v[8 * h + 5]), H::pack(v[8 * h + 6], v[8 * h + 7])};
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 16; ++j)
+    if (j < left) c[j] = (uint16_t)H::from_f32(v[j]);
+}
+
+TLM_DEV uint32_t xrow_max_bits(uint32_t m) {  // of lanes l and l ^ 16
+  const auto r = __builtin_amdgcn_permlane16_swap(m, m, false, false);
+  return max(r[0], r[1]);
+}
+
+template <int OUT>
+__global__ __launch_bounds__(P_T, 1) void gemm_mx8_256(Args a) {
+  constexpr bool DUAL = OUT == TLM_F8E4M3;
+  constexpr int BN = DUAL ? P_N / 2 : P_N;  // columns of the result
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[(P_W + P_X) * P_ST];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int grp = wave >> 2, quarter = wave & 3;  // half of W, 64 rows of X
+  const int M = (int)a.M, N = (int)a.N, K = a.K, KT = a.kt;
+  int tm, tn;
+  tile_of(blockIdx.x, (M + P_M - 1) / P_M, (N + BN - 1) / BN, tm, tn);
+  const int m0 = tm * P_M, n0 = tn * BN;
+
+  // ---- LDS-DMA: wave w of a group fills slots 64 w .. 64 w + 63 of its operand's stage, 8 a instruction
+  const bool is_w = grp == 0;
+  const bool second = DUAL && is_w && (quarter & 1);
+  // rows of the wave's 64 slots start here (gated: gate and up groups of 64 alternate)
+  const int r0 = is_w ? n0 + (DUAL ? 64 * (quarter >> 1) : 64 * quarter) : m0 + 64 * quarter;
+  const int rows = is_w ? N : M;
+  const uint8_t* const base = (is_w ? (second ? a.b2.codes : a.b.codes) : a.a.codes) + (int64_t)min(r0, rows) * K;
+  // instruction j: slots 8 j + lane / 8, rows 32 (j % 2) + 4 (lane / 8) + j / 2; what is past the last row lies past the
+  // descriptor's end
+  const int left = max(0, min(64, rows - r0)) * K;
+  int chunk[2];
+  uint32_t off[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    chunk[h] = 16 * ((lane & 7) ^ (4 * h + (lane >> 4)));
+    off[h] = (uint32_t)((32 * h + 4 * (lane >> 3)) * K + chunk[h]);
+  }
+  auto w_st = [&](int t) { return smem + (t & 1) * P_ST; };
+  auto x_st = [&](int t) { return smem + P_W * P_ST + (t % P_X) * P_ST; };
+  auto fill = [&](int t, uint8_t* st, int j) {
+    const uint32_t o = chunk[j & 1] < K - t * 128 ? off[j & 1] : OOB;
+    dma16(base + (int64_t)t * 128, max(0, left - t * 128), st + quarter * 8192 + j * 1024, o + (j >> 1) * K);
+  };
+
+  // ---- scales: words of the wave's two groups of W and its group of X; past the last row, another's
+  auto words = [&](const uint8_t* s, int r, int n) {
+    return s + (int64_t)(min(r, n - 1) >> 6) * KT * 256 + 4 * lane;
+  };
+  const uint8_t* const s0 = words(a.b.scales, n0 + (DUAL ? 64 : 128) * grp, N);
+  const uint8_t* const s1 = DUAL ? words(a.b2.scales, n0 + 64 * grp, N) : words(a.b.scales, n0 + 128 * grp + 64, N);
+  const uint8_t* const sx = words(a.a.scales, m0 + 64 * quarter, M);
+  struct Scales {
+    uint32_t w[2], x;
+  };
+  auto scales_of = [&](int t) {
+    const int64_t o = (int64_t)t * 256;
+    Scales s{{*(const uint32_t*)(s0 + o), *(const uint32_t*)(s1 + o)}, *(const uint32_t*)(sx + o)};
+    return s;
+  };
+  auto mask_tail = [&](Scales& s, int t) {  // past K: codes 0, scale 1
+    if (t * 128 + 32 * (lane >> 4) >= K) s = Scales{{0x7f7f7f7fu, 0x7f7f7f7fu}, 0x7f7f7f7fu};
+  };
+
+  // ---- operands
+  const int q = lane >> 4;
+  const int xr = ((lane & 15) >> 1) & 7;
+  const uint32_t w_row = ldsop::lds_u32(smem) + (grp * 128 + (lane & 15)) * 128;
+  const uint32_t x_row = ldsop::lds_u32(smem) + P_W * P_ST + (quarter * 64 + (lane & 15)) * 128;
+  uint32_t ch[2];
+#pragma unroll
+  for (int p = 0; p < 2; ++p) ch[p] = 16 * ((4 * p + q) ^ xr);
+  f32x4 acc[8][4];
+#pragma unroll
+  for (int f = 0; f < 8; ++f)
+#pragma unroll
+    for (int t = 0; t < 4; ++t) acc[f][t] = f32x4{};
+  u32x4 wop[8][2], xop0[2];
+  auto read_x = [&](int t, auto nc, u32x4 (&o)[2]) {
+    constexpr int n = decltype(nc)::value;
+    const uint32_t st = x_row + (t % P_X) * P_ST;
+#pragma unroll
+    for (int p = 0; p < 2; ++p) ldsop::ds_b128<n * 2048>(o[p], st + ch[p]);
+  };
+  // the wave's 8 operands of W and its first of X, a pair of DMA instructions after every four reads
+  auto load_phase = [&](int t, int dma_t, uint8_t* dma_st) {
+    const uint32_t st = w_row + (t & 1) * P_ST;
+    unroll<0, 4>([&](auto qc) {
+      constexpr int j = decltype(qc)::value;
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        ldsop::ds_b128<2 * j * 2048>(wop[2 * j][p], st + ch[p]);
+        ldsop::ds_b128<(2 * j + 1) * 2048>(wop[2 * j + 1][p], st + ch[p]);
+      }
+      if (dma_t >= 0) {
+        fill(dma_t, dma_st, 2 * j);
+        fill(dma_t, dma_st, 2 * j + 1);
+      }
+    });
+    read_x(t, std::integral_constant<int, 0>{}, xop0);
+    __builtin_amdgcn_sched_barrier(0);
+    wait_lgkm0();
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int f = 0; f < 8; ++f)
+#pragma unroll
+      for (int p = 0; p < 2; ++p) ldsop::landed(wop[f][p]);
+    ldsop::landed(xop0[0]);
+    ldsop::landed(xop0[1]);
+  };
+  auto compute_phase = [&](int t, const Scales& s) {
+    u32x4 x[3][2];  // ring: operand n in x[n % 3], read two ahead
+    x[0][0] = xop0[0];
+    x[0][1] = xop0[1];
+    read_x(t, std::integral_constant<int, 1>{}, x[1]);
+    unroll<0, 4>([&](auto nc) {
+      constexpr int n = decltype(nc)::value;
+      if constexpr (n + 2 < 4) read_x(t, std::integral_constant<int, n + 2>{}, x[(n + 2) % 3]);
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (n + 2 < 4) wait_lgkm<4>();
+      else if constexpr (n + 1 < 4) wait_lgkm<2>();
+      else wait_lgkm<0>();
+      __builtin_amdgcn_sched_barrier(0);
+      ldsop::landed(x[n % 3][0]);
+      ldsop::landed(x[n % 3][1]);
+      unroll<0, 8>([&](auto fc) {
+        constexpr int f = decltype(fc)::value;
+        acc[f][n] = mma<f % 4, n>(cat8(wop[f][0], wop[f][1]), cat8(x[n % 3][0], x[n % 3][1]), acc[f][n], s.w[f / 4], s.x);
+      });
+    });
+  };
+  Scales cur = scales_of(0);
+  if (KT == 1) mask_tail(cur, 0);
+  // prologue: W of step 0 (group 0), X of steps 0 and 1 (group 1)
+  if (grp == 0) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) fill(0, w_st(0), j);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) fill(0, x_st(0), j);
+    if (1 < KT) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) fill(1, x_st(1), j);
+    }
+  }
+  wait_vm<0>();
+  barrier();
+  if (grp == 0) {
+    for (int t = 0; t < KT; ++t) {
+      Scales nxt = scales_of(min(t + 1, KT - 1));
+      load_phase(t, t + 1 < KT ? t + 1 : -1, w_st(t + 1));
+      barrier();
+      compute_phase(t, cur);
+      wait_vm<0>();  // W of t + 1 and its scales
+      cur = nxt;
+      if (t + 2 == KT) mask_tail(cur, t + 1);
+      barrier();
+    }
+    barrier();  // group 1 multiplies the last step
+  } else {
+    barrier();
+    for (int t = 0; t < KT; ++t) {
+      const bool more = t + 2 < KT;
+      Scales nxt = scales_of(min(t + 1, KT - 1));
+      load_phase(t, more ? t + 2 : -1, x_st(t + 2));
+      // X of t + 1 (issued a load phase ago) and the scales, older than this phase's 8, have landed
+      if (more) wait_vm<8>();
+      else wait_vm<0>();
+      barrier();
+      compute_phase(t, cur);
+      cur = nxt;
+      if (t + 2 == KT) mask_tail(cur, t + 1);
+      barrier();
+    }
+  }
+
+  // ---- the lane's rows are m0 + 64 quarter + 4 i + t, its columns 16 g + 4 e + f of a group
+  const int i = lane & 15, g = lane >> 4;
+  if constexpr (DUAL) {
+    const int col = n0 + 64 * grp + 16 * g;
+    uint32_t byte[4];
+    unroll<0, 4>([&](auto tc) {
+      constexpr int t = decltype(tc)::value;
+      const int row = m0 + 64 * quarter + 4 * i + t;
+      float v[16];
+      uint32_t m = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int f = 0; f < 4; ++f) {
+          v[4 * e + f] = gated(acc[f][t][e], acc[4 + f][t][e]);
+          m = max(m, mx8::abs_bits(v[4 * e + f]));
+        }
+      byte[t] = mx8::scale_byte(xrow_max_bits(m));
+      const float inv = mx8::inverse(byte[t]);
+      u32x4 p;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        p[e] = mx8::codes4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3], inv, byte[t] < 255);
+      if (row < M && col < N) *(u32x4*)((uint8_t*)a.c + (int64_t)row * N + col) = p;
+    });
+    if ((g & 1) == 0 && col < N) {
+      const int row = m0 + 64 * quarter + 4 * i;
+      uint8_t* const s = a.c_scales + mx8::scale_at(row, col / BLOCK, (N + 127) / 128);
+      if (row + 4 <= M) *(uint32_t*)s = byte[0] | byte[1] << 8 | byte[2] << 16 | byte[3] << 24;
+      else
+        for (int t = 0; t < 3; ++t)
+          if (row + t < M) s[t] = (uint8_t)byte[t];
+    }
+  } else {
+    const bool vec = N % 8 == 0 && ((uintptr_t)a.c & 15) == 0;
+    unroll<0, 4>([&](auto tc) {
+      constexpr int t = decltype(tc)::value;
+      const int row = m0 + 64 * quarter + 4 * i + t;
+      if (row >= M) return;
+      unroll<0, 2>([&](auto pc) {
+        constexpr int p = decltype(pc)::value;
+        const int col = n0 + 128 * grp + 64 * p + 16 * g;
+        float v[16];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int f = 0; f < 4; ++f) v[4 * e + f] = acc[4 * p + f][t][e];
+        store16<OUT>((uint16_t*)a.c + (int64_t)row * N + col, v, (int64_t)N - col, vec);
+      });
+    });
+  }
+}
+
 template <int OUT>
 int direct(const Args& a, hipStream_t s) {
   constexpr int NF = OUT == TLM_F8E4M3 ? 2 : 1;
   const int mt = a.M <= 16 ? 1 : a.M <= 32 ? 2 : 4;
+  if (a.M > 256 && a.K > 0) {
+    const int bn = OUT == TLM_F8E4M3 ? P_N / 2 : P_N;
+    const int64_t tiles = ((a.M + P_M - 1) / P_M) * ((a.N + bn - 1) / bn);
+    gemm_mx8_256<OUT><<<(unsigned)tiles, P_T, 0, s>>>(a);
+    return TLM_OK;
+  }
   const dim3 grid((unsigned)((a.N + 16 * NF - 1) / (16 * NF)), (unsigned)((a.M + 16 * mt - 1) / (16 * mt)));
   auto go = [&](auto kern) { kern<<<grid, 64 * D_WAVES, 0, s>>>(a); };
   if (mt == 1) go(gemm_mx8_direct<1, NF, OUT>);
