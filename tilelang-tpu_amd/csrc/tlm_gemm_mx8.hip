@@ -1,8 +1,10 @@
 // Products of 8-bit operands with power-of-two scales: C = A B^T, and SwiGLU of two of them with an 8-bit result.
 //
+// Tiles of 16 to 256 rows, chosen by a model of their time (choose, below).
 // v_mfma_scale_f32_16x16x128_f8f6f4 multiplies each block of 32 k by 2^(ea + eb) as it adds it. Lane l holds row l % 16 of
 // its operand and the 16-byte chunks q and q + 4 of its 128 k (q = l / 16), and the scale of k block q. The weights are the first
 // operand, so that a lane's sums are neighbouring columns of one row of C.
+#include "tlm_gemm_tile.h"
 #include "tlm_mx8.h"
 
 #include <algorithm>
@@ -24,37 +26,6 @@ struct Args {
   int K, kt;  // kt: k steps of 128
 };
 
-// Rows r0 + F i + f, f = 0 .. F - 1, of a matrix as F operands: row i of operand f. Rows behind the last are the last.
-template <int F>
-struct Rows {
-  const uint8_t* p[F];
-  const uint8_t* s;
-  TLM_DEV Rows(const Mat& m, int64_t rows, int64_t r0, int K, int kt, int lane) {
-    const int i = lane & 15, q = lane >> 4;
-#pragma unroll
-    for (int f = 0; f < F; ++f) p[f] = m.codes + min(r0 + F * i + f, rows - 1) * K + 16 * q;
-    s = m.scales + mx8::scale_at(r0, 0, kt) + q * 64 + F * i;
-  }
-  // operands and scales (operand f's in byte f) of k step t; past K: codes 0, scale 1
-  template <bool TAIL>
-  TLM_DEV void load(int t, int K, int lane, i32x8 (&o)[F], uint32_t& sc) const {
-    const int q = lane >> 4;
-    const bool ok0 = !TAIL || t * 128 + 16 * q < K, ok1 = !TAIL || t * 128 + 64 + 16 * q < K;
-#pragma unroll
-    for (int f = 0; f < F; ++f) {
-      u32x4 x = {}, y = {};
-      if (ok0) x = *(const u32x4*)(p[f] + (int64_t)t * 128);
-      if (ok1) y = *(const u32x4*)(p[f] + (int64_t)t * 128 + 64);
-      o[f] = i32x8{(int)x[0], (int)x[1], (int)x[2], (int)x[3], (int)y[0], (int)y[1], (int)y[2], (int)y[3]};
-    }
-    const uint8_t* const at = s + (int64_t)t * 256;
-    if constexpr (F == 1) sc = *at;
-    else if constexpr (F == 2) sc = *(const uint16_t*)at;
-    else sc = *(const uint32_t*)at;
-    if (TAIL && t * 128 + 32 * q >= K) sc = 0x7f7f7f7fu;
-  }
-};
-
 template <int SA, int SB>
 TLM_DEV f32x4 mma(const i32x8& a, const i32x8& b, f32x4 c, uint32_t sa, uint32_t sb) {
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, SA, (int)sa, SB, (int)sb);
@@ -64,92 +35,6 @@ using ldsop::unroll;
 
 // up * silu(gate).
 TLM_DEV float gated(float gate, float up) { return up * (gate * __builtin_amdgcn_rcpf(fast_exp(-gate) + 1.0f)); }
-
-constexpr int D_WAVES = 8;
-
-// OUT: TLM_F16, TLM_BF16: C = A B^T. TLM_F8E4M3: up * silu(gate) with its scales.
-// A workgroup computes 16 MT rows and 16 NF columns (32 of the gated product: NF 2 of each matrix), its waves
-// every 8th k step of them.
-template <int MT, int NF, int OUT>
-__global__ __launch_bounds__(64 * D_WAVES) void gemm_mx8_direct(Args a) {
-  constexpr bool DUAL = OUT == TLM_F8E4M3;
-  constexpr int W = DUAL ? 2 * NF : NF;
-  __shared__ f32x4 red[D_WAVES][W * MT][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t m0 = (int64_t)blockIdx.y * 16 * MT, n0 = (int64_t)blockIdx.x * 16 * NF;
-  const Rows<MT> x(a.a, a.M, m0, a.K, a.kt, lane);
-  const Rows<NF> w(a.b, a.N, n0, a.K, a.kt, lane), w2(DUAL ? a.b2 : a.b, a.N, n0, a.K, a.kt, lane);
-  f32x4 acc[W][MT];
-#pragma unroll
-  for (int f = 0; f < W; ++f)
-#pragma unroll
-    for (int t = 0; t < MT; ++t) acc[f][t] = f32x4{};
-  auto step = [&](int t, auto tail) {
-    constexpr bool TAIL = decltype(tail)::value;
-    i32x8 xo[MT], wo[NF], vo[NF];
-    uint32_t xs, ws, vs = 0;
-    x.template load<TAIL>(t, a.K, lane, xo, xs);
-    w.template load<TAIL>(t, a.K, lane, wo, ws);
-    if constexpr (DUAL) w2.template load<TAIL>(t, a.K, lane, vo, vs);
-    unroll<0, W>([&](auto fc) {
-      constexpr int f = decltype(fc)::value;
-      unroll<0, MT>([&](auto tc) {
-        constexpr int m = decltype(tc)::value;
-        if constexpr (f < NF) acc[f][m] = mma<f, m>(wo[f], xo[m], acc[f][m], ws, xs);
-        else acc[f][m] = mma<f - NF, m>(vo[f - NF], xo[m], acc[f][m], vs, xs);
-      });
-    });
-  };
-  const int full = a.K / 128;
-  for (int t = wave; t < full; t += D_WAVES) step(t, std::false_type{});
-  if (full < a.kt && full % D_WAVES == wave) step(full, std::true_type{});
-
-#pragma unroll
-  for (int f = 0; f < W; ++f)
-#pragma unroll
-    for (int t = 0; t < MT; ++t) red[wave][f * MT + t][lane] = acc[f][t];
-  __syncthreads();
-  // wave t finishes operand t of A: the lane's row is m0 + MT i + t, its columns n0 + NF (4 g + e) + f
-  if (wave >= MT) return;
-  const int i = lane & 15, g = lane >> 4;
-  f32x4 sum[W];
-#pragma unroll
-  for (int f = 0; f < W; ++f) {
-    sum[f] = red[0][f * MT + wave][lane];
-#pragma unroll
-    for (int v = 1; v < D_WAVES; ++v) sum[f] += red[v][f * MT + wave][lane];
-  }
-  const int64_t row = m0 + MT * i + wave, col = n0 + NF * 4 * g;
-  float v[4 * NF];
-#pragma unroll
-  for (int e = 0; e < 4; ++e)
-#pragma unroll
-    for (int f = 0; f < NF; ++f) {
-      if constexpr (DUAL) v[e * NF + f] = gated(sum[f][e], sum[NF + f][e]);
-      else v[e * NF + f] = sum[f][e];
-    }
-  if constexpr (DUAL) {
-    static_assert(NF == 2, "32 columns, a block");
-    uint32_t m = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) m = max(m, mx8::abs_bits(v[j]));
-    m = max(m, (uint32_t)__shfl_xor((int)m, 16));
-    m = max(m, (uint32_t)__shfl_xor((int)m, 32));
-    if (row >= a.M) return;
-    const uint32_t byte = mx8::scale_byte(m);
-    const float inv = mx8::inverse(byte);
-    *(u32x2*)((uint8_t*)a.c + row * a.N + col) = u32x2{mx8::codes4(v[0], v[1], v[2], v[3], inv, byte < 255),
-                                                       mx8::codes4(v[4], v[5], v[6], v[7], inv, byte < 255)};
-    if (g == 0) a.c_scales[mx8::scale_at(row, (int)(n0 / BLOCK), (int)((a.N + 127) / 128))] = (uint8_t)byte;
-  } else {
-    if (row >= a.M) return;
-    using H = h16<OUT == TLM_BF16>;
-    uint16_t* const c = (uint16_t*)a.c + row * a.N + col;
-#pragma unroll
-    for (int j = 0; j < 4 * NF; ++j)
-      if (col + j < a.N) c[j] = (uint16_t)H::from_f32(v[j]);
-  }
-}
 
 // ---- whole prompts: 256 x 256 tiles
 
@@ -221,6 +106,11 @@ TLM_DEV void store16(uint16_t* c, const float (&v)[16], int64_t left, bool vec) 
 
 TLM_DEV uint32_t xrow_max_bits(uint32_t m) {  // of lanes l and l ^ 16
   const auto r = __builtin_amdgcn_permlane16_swap(m, m, false, false);
+  return max(r[0], r[1]);
+}
+
+TLM_DEV uint32_t xhalf_max_bits(uint32_t m) {  // of lanes l and l ^ 32
+  const auto r = __builtin_amdgcn_permlane32_swap(m, m, false, false);
   return max(r[0], r[1]);
 }
 
@@ -445,27 +335,431 @@ __global__ __launch_bounds__(P_T, 1) void gemm_mx8_256(Args a) {
   }
 }
 
-template <int OUT>
-int direct(const Args& a, hipStream_t s) {
-  constexpr int NF = OUT == TLM_F8E4M3 ? 2 : 1;
-  const int mt = a.M <= 16 ? 1 : a.M <= 32 ? 2 : 4;
-  if (a.M > 256 && a.K > 0) {
-    const int bn = OUT == TLM_F8E4M3 ? P_N / 2 : P_N;
-    const int64_t tiles = ((a.M + P_M - 1) / P_M) * ((a.N + bn - 1) / bn);
-    gemm_mx8_256<OUT><<<(unsigned)tiles, P_T, 0, s>>>(a);
-    return TLM_OK;
+// ---- between one decode step and whole prompts: smaller tiles, K split where they are fewer than the CUs
+
+// What bounds it: the stream of B with few rows, with more the rate at which a CU takes operand tiles from L2 (about 55 B/clk).
+// Four waves only fill the ring: an LDS-DMA instruction waits at issue while the CU has enough of them under way, and a wave that
+// multiplies would wait with it. NC others are BM / (16 FX) x BN / 64 wave tiles times KG k-groups. A stage of the NST-stage ring holds
+// KG k steps, one for each k-group, and their scales; the operands of stage t are read from LDS while the products of stage t - 1
+// run. The k-groups' sums meet in LDS, those of the `ns` workgroups that share a tile's K in memory, where the last to arrive adds
+// them in order: the result does not depend on the order of arrival.
+template <int BM_, int BN_, int FX_, int KG_, int NST_, int OUT_>
+struct Tile {
+  static constexpr int BM = BM_, BN = BN_, FX = FX_, KG = KG_, NST = NST_, OUT = OUT_;
+  static constexpr bool DUAL = OUT == TLM_F8E4M3;
+  static constexpr int BNC = DUAL ? BN / 2 : BN;       // columns of the result
+  static constexpr int WM = BM / (16 * FX), WN = BN / 64;
+  static constexpr int NC = WM * WN * KG, NP = 4;      // waves that multiply, waves that load
+  static constexpr int BKB = 128 * KG;                 // bytes of k per stage
+  static constexpr int SX = BM * BKB, SW = BN * BKB;
+  static constexpr int GX = (BM + 63) / 64, GW = DUAL ? 2 * ((BNC + 63) / 64) : BN / 64;  // 64-row groups of scales
+  static constexpr int NX = SX / (NP * 1024), NW = SW / (NP * 1024);  // LDS-DMA instructions per wave: codes
+  static constexpr int NSC = (GX + GW + NP - 1) / NP;                 // and scales, 1 KB per group: KG k steps and nothing
+  static constexpr int PER = NX + NW + NSC;
+  static constexpr int ST = SX + SW + NSC * NP * 1024;
+  static constexpr int TO = FX > KG ? FX / KG : 1, FIN = FX > KG ? KG : FX;  // operands of X that a k-group finishes, k-groups that do
+  static constexpr int RED = KG > 1 ? NC * 4 * FX * 1024 : 0;
+  static constexpr int SMEM = NST * ST > RED ? NST * ST : RED;
+  static constexpr int THREADS = 64 * (NC + NP);
+  static_assert((NC == 4 || NC == 8) && KG <= 4 && NX * NP * 1024 == SX && NW * NP * 1024 == SW && SMEM <= 160 * 1024, "layout");
+};
+
+template <int BKB>
+TLM_DEV int swz(int slot) {  // 16 lanes that read one chunk of 16 neighbouring slots hit all banks
+  return BKB == 128 ? (slot >> 1) & 7 : slot & 15;
+}
+TLM_DEV void ds_b32(uint32_t& r, uint32_t a) { asm volatile("ds_read_b32 %0, %1" : "=v"(r) : "v"(a) : "memory"); }
+TLM_DEV void ds_u16(uint32_t& r, uint32_t a) { asm volatile("ds_read_u16 %0, %1" : "=v"(r) : "v"(a) : "memory"); }
+TLM_DEV void ds_u8(uint32_t& r, uint32_t a) { asm volatile("ds_read_u8 %0, %1" : "=v"(r) : "v"(a) : "memory"); }
+TLM_DEV void landed1(uint32_t& a) { asm volatile("" : "+v"(a)); }
+TLM_DEV void plain_barrier() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+template <typename T>
+__global__ __launch_bounds__(T::THREADS, 1) void gemm_mx8_tile(Args a, int ns, float* __restrict__ part,
+                                                               unsigned* __restrict__ arrivals) {
+  constexpr int BKB = T::BKB, KG = T::KG, FX = T::FX, NST = T::NST;
+  constexpr bool DUAL = T::DUAL;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[T::SMEM];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const bool multiplies = wave < T::NC;
+  const int sp = wave / KG, kg = wave % KG;
+  const int wm = sp / T::WN, wn = sp % T::WN;
+  const int M = (int)a.M, N = (int)a.N, K = a.K;
+
+  // XCD x takes a contiguous range of (split, column tile, row tile), row tiles fastest: they share a strip of B
+  const int tiles_m = (M + T::BM - 1) / T::BM, tiles_n = (N + T::BNC - 1) / T::BNC;
+  const int tiles = tiles_m * tiles_n, total = tiles * ns, xcd = blockIdx.x & 7;
+  const int lin = xcd * (total >> 3) + min(xcd, total & 7) + (blockIdx.x >> 3);
+  const int tile = lin % tiles, split = lin / tiles;
+  const int m0 = tile % tiles_m * T::BM, n0 = tile / tiles_m * T::BNC;
+  const int lo = (int)((int64_t)split * a.kt / ns), hi = (int)((int64_t)(split + 1) * a.kt / ns);  // k steps
+  const int n = (hi - lo + KG - 1) / KG;          // stages
+  const int kend = min(K, hi * 128) - lo * 128;  // bytes of k
+  const int i = lane & 15, q = lane >> 4;
+  f32x4 acc[4][FX];
+
+  // Stage t lives at t % NST. Before barrier t the loading waves wait for stage t; after it stage t - 1, whose operands every wave
+  // has read by then, takes stage t + NST - 1.
+  if (!multiplies) {
+    const int pw = wave - T::NC;
+    uint32_t off[T::NX + T::NW];  // a lane's offset from the stage's first k, and its k within the stage
+    int kch[T::NX + T::NW];
+#pragma unroll
+    for (int j = 0; j < T::NX + T::NW; ++j) {
+      constexpr int CPR = BKB / 16;
+      const int slot = (T::NP * (j < T::NX ? j : j - T::NX) + pw) * (64 / CPR) + lane / CPR;
+      const int c = (lane % CPR) ^ swz<BKB>(slot);
+      int row;
+      if (j < T::NX) row = slot / (16 * FX) * (16 * FX) + FX * (slot & 15) + (slot >> 4) % FX;
+      else if (DUAL) row = (slot >> 6) * 32 + 2 * (slot & 15) + (slot >> 4 & 1);
+      else row = (slot & ~63) + 4 * (slot & 15) + (slot >> 4 & 3);
+      off[j] = (uint32_t)(row * K + 16 * c);
+      kch[j] = 16 * c;
+    }
+    const uint8_t* const x_base = a.a.codes + (int64_t)m0 * K + lo * 128;
+    const uint8_t* const w_base = a.b.codes + (int64_t)n0 * K + lo * 128;
+    const uint8_t* const v_base = (DUAL ? a.b2.codes : a.b.codes) + (int64_t)n0 * K + lo * 128;
+    const int x_end = min(M - m0, T::BM) * K - lo * 128, w_end = min(N - n0, T::BNC) * K - lo * 128;
+    // scales: X's groups, W's (gated: gate's, then up's); past the last row, another's
+    const uint8_t* sc_base[T::NSC];
+#pragma unroll
+    for (int j = 0; j < T::NSC; ++j) {
+      const int g = min(T::NP * j + pw, T::GX + T::GW - 1), h = g - T::GX;
+      const Mat& m = h < 0 ? a.a : DUAL && h >= T::GW / 2 ? a.b2 : a.b;
+      const int r = h < 0 ? min(m0 + 64 * g, M - 1) : min(n0 + 64 * (DUAL && h >= T::GW / 2 ? h - T::GW / 2 : h), N - 1);
+      sc_base[j] = m.scales + (int64_t)(r >> 6) * a.kt * 256;
+    }
+    auto issue = [&](int t, int stage) __attribute__((always_inline)) {
+      uint8_t* const st = smem + stage * T::ST;
+      unroll<0, T::NX + T::NW>([&](auto jc) __attribute__((always_inline)) {
+        constexpr int j = decltype(jc)::value;
+        const uint32_t o = kch[j] < kend - t * BKB ? off[j] : OOB;
+        if constexpr (j < T::NX) {
+          dma16(x_base + t * BKB, max(0, x_end - t * BKB), st + (T::NP * j + pw) * 1024, o);
+        } else {
+          constexpr int u = j - T::NX;
+          const bool second = DUAL && ((T::NP * u + pw) * (1024 / BKB) >> 5 & 1);
+          dma16((second ? v_base : w_base) + t * BKB, max(0, w_end - t * BKB), st + T::SX + (T::NP * u + pw) * 1024, o);
+        }
+      });
+#pragma unroll
+      for (int j = 0; j < T::NSC; ++j)
+        dma16(sc_base[j], a.kt * 256, st + T::SX + T::SW + (T::NP * j + pw) * 1024,
+              lane < 16 * KG ? (uint32_t)((lo + t * KG) * 256 + 16 * lane) : OOB);
+    };
+#pragma unroll
+    for (int t = 0; t < NST - 1; ++t)
+      if (t < n) issue(t, t);
+    int stage = NST - 1;
+    for (int t = 0; t < n; ++t) {
+      const int more = min(NST - 2, n - 1 - t);  // stages after t whose loads may stay in flight
+      unroll<0, NST - 1>([&](auto ic) __attribute__((always_inline)) {
+        constexpr int j = decltype(ic)::value;
+        if (more == j) wait_vm<j * T::PER>();
+      });
+      plain_barrier();
+      if (t + NST - 1 < n) issue(t + NST - 1, stage);
+      stage = stage == NST - 1 ? 0 : stage + 1;
+    }
+  } else {
+  // ---- operand reads (addresses within stage 0)
+  const uint32_t b0 = ldsop::lds_u32(smem);
+  uint32_t x_addr[2], w_addr[2];
+#pragma unroll
+  for (int p = 0; p < 2; ++p) {
+    const int x = 16 * ((8 * kg + 4 * p + q) ^ swz<BKB>(i));
+    x_addr[p] = b0 + (wm * 16 * FX + i) * BKB + x;
+    w_addr[p] = b0 + T::SX + (wn * 64 + i) * BKB + x;
   }
-  const dim3 grid((unsigned)((a.N + 16 * NF - 1) / (16 * NF)), (unsigned)((a.M + 16 * mt - 1) / (16 * mt)));
-  auto go = [&](auto kern) { kern<<<grid, 64 * D_WAVES, 0, s>>>(a); };
-  if (mt == 1) go(gemm_mx8_direct<1, NF, OUT>);
-  else if (mt == 2) go(gemm_mx8_direct<2, NF, OUT>);
-  else go(gemm_mx8_direct<4, NF, OUT>);
+  const uint32_t sc0 = b0 + T::SX + T::SW + kg * 256;
+  const int xrow = (m0 & 63) + wm * 16 * FX;  // the wave's rows within the first group
+  const uint32_t xs_addr = sc0 + (xrow >> 6) * 1024 + q * 64 + (xrow & 63) + FX * i;
+  const int wcol = (n0 & 63) + 32 * wn;  // gated: the wave's columns within the first group
+  const uint32_t ws_addr = DUAL ? sc0 + (T::GX + (wcol >> 6)) * 1024 + q * 64 + (wcol & 63) + 2 * i
+                                : sc0 + (T::GX + wn) * 1024 + 4 * lane;
+  constexpr int VS = T::GW / 2 * 1024;  // from gate's scales to up's
+  struct Ops {
+    u32x4 x[FX][2], w[4][2];
+    uint32_t xs, ws, vs;
+  };
+  constexpr int NR = 2 * FX + 8 + 2;
+  auto read1 = [&](Ops& o, uint32_t so, auto ic) __attribute__((always_inline)) {
+    constexpr int r = decltype(ic)::value;
+    if constexpr (r < 8) ldsop::ds_b128<r / 2 * 16 * BKB>(o.w[r / 2][r % 2], w_addr[r % 2] + so);
+    else if constexpr (r < 8 + 2 * FX) ldsop::ds_b128<(r - 8) / 2 * 16 * BKB>(o.x[(r - 8) / 2][r % 2], x_addr[r % 2] + so);
+    else if constexpr (r == 8 + 2 * FX) {
+      if constexpr (FX == 4) ds_b32(o.xs, xs_addr + so);
+      else if constexpr (FX == 1) ds_u8(o.xs, xs_addr + so);
+      else ds_u16(o.xs, xs_addr + so);
+    } else if constexpr (DUAL) {
+      ds_u16(o.ws, ws_addr + so);
+      ds_u16(o.vs, ws_addr + VS + so);
+    } else {
+      ds_b32(o.ws, ws_addr + so);
+    }
+  };
+  auto ops_landed = [&](Ops& o, int t) __attribute__((always_inline)) {
+    __builtin_amdgcn_sched_barrier(0);
+    wait_lgkm0();
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+#pragma unroll
+      for (int f = 0; f < FX; ++f) ldsop::landed(o.x[f][p]);
+#pragma unroll
+      for (int f = 0; f < 4; ++f) ldsop::landed(o.w[f][p]);
+    }
+    landed1(o.xs);
+    landed1(o.ws);
+    if constexpr (DUAL) landed1(o.vs);
+    // past the end: codes 0, scale 1
+    if ((t * KG + kg) * 128 + 32 * q >= kend) o.xs = o.ws = o.vs = 0x7f7f7f7fu;
+  };
+#pragma unroll
+  for (int f = 0; f < 4; ++f)
+#pragma unroll
+    for (int t = 0; t < FX; ++t) acc[f][t] = f32x4{};
+  constexpr int NM = 4 * FX;
+  auto mul1 = [&](const Ops& o, auto ic) __attribute__((always_inline)) {
+    constexpr int t = decltype(ic)::value / 4, f = decltype(ic)::value % 4;
+    const i32x8 w = cat8(o.w[f][0], o.w[f][1]), x = cat8(o.x[t][0], o.x[t][1]);
+    if constexpr (DUAL) acc[f][t] = mma<f & 1, t>(w, x, acc[f][t], f < 2 ? o.ws : o.vs, o.xs);
+    else acc[f][t] = mma<f, t>(w, x, acc[f][t], o.ws, o.xs);
+  };
+
+  int stage = 0;
+  auto step = [&](int t, Ops& cur, const Ops& prev) __attribute__((always_inline)) {
+    plain_barrier();
+    const uint32_t so = (uint32_t)(stage * T::ST);
+    unroll<0, NM>([&](auto ic) __attribute__((always_inline)) {
+      constexpr int m = decltype(ic)::value;
+      constexpr int RS = NM > 4 ? NM * 3 / 4 : NM;  // the reads go out in the first 3/4
+      unroll<(m < RS ? m * NR / RS : NR), (m + 1 < RS ? (m + 1) * NR / RS : NR)>(
+          [&](auto rc) __attribute__((always_inline)) { read1(cur, so, rc); });
+      mul1(prev, ic);
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    ops_landed(cur, t);
+    stage = stage == NST - 1 ? 0 : stage + 1;
+  };
+  if (n > 0) {
+    Ops x, y;
+    plain_barrier();
+    unroll<0, NR>([&](auto rc) __attribute__((always_inline)) { read1(x, 0, rc); });
+    ops_landed(x, 0);
+    stage = 1;
+    int t = 1;
+    for (; t + 1 < n; t += 2) {
+      step(t, y, x);
+      step(t + 1, x, y);
+    }
+    if (t < n) {
+      step(t, y, x);
+      unroll<0, NM>([&](auto ic) __attribute__((always_inline)) { mul1(y, ic); });
+    } else {
+      unroll<0, NM>([&](auto ic) __attribute__((always_inline)) { mul1(x, ic); });
+    }
+  }
+  }
+
+  // ---- the k-groups' sums: k-group g finishes operands g TO .. g TO + TO - 1 of X
+  const bool fin = multiplies && kg < T::FIN;
+  f32x4 sum[T::TO][4];
+  if constexpr (KG > 1) {
+    f32x4* const red = (f32x4*)smem;
+    __syncthreads();  // every operand has been read
+    unroll<0, FX>([&](auto tc) __attribute__((always_inline)) {
+      constexpr int t = decltype(tc)::value;
+      if (multiplies && kg != t / T::TO)
+#pragma unroll
+        for (int f = 0; f < 4; ++f) red[((wave * FX + t) * 4 + f) * 64 + lane] = acc[f][t];
+    });
+    __syncthreads();
+    unroll<0, FX>([&](auto tc) __attribute__((always_inline)) {
+      constexpr int t = decltype(tc)::value;
+      if (multiplies && kg == t / T::TO) {
+#pragma unroll
+        for (int f = 0; f < 4; ++f) {
+          f32x4 s = {};
+#pragma unroll
+          for (int g = 0; g < KG; ++g)
+            s += g == t / T::TO ? acc[f][t] : red[(((sp * KG + g) * FX + t) * 4 + f) * 64 + lane];
+          sum[t % T::TO][f] = s;
+        }
+      }
+    });
+  } else {
+#pragma unroll
+    for (int t = 0; t < FX; ++t)
+#pragma unroll
+      for (int f = 0; f < 4; ++f) sum[t][f] = acc[f][t];
+  }
+
+  // ---- split K: partial tiles go through memory by write-through stores and loads that miss every cache
+  if (ns > 1) {
+    __shared__ unsigned last;
+    const int at = (((sp * T::FIN + kg) * T::TO * 4) * 64 + lane) * 16;
+    if (fin) {
+      float* const mine = part + ((int64_t)split * tiles + tile) * (T::BM * T::BN);
+#pragma unroll
+      for (int v = 0; v < 4 * T::TO; ++v) st_cp<CP_SC01>(mine, at + v * 1024, __builtin_bit_cast(u32x4, sum[v / 4][v % 4]));
+    }
+    __builtin_amdgcn_s_waitcnt(0x3f70);  // vmcnt(0): the tile has been written
+    __syncthreads();
+    if (tid == 0) last = atomicAdd(&arrivals[tile], 1u) == (unsigned)(ns - 1);
+    __syncthreads();
+    if (!last) return;
+    if (fin) {
+      f32x4 all[T::TO][4];
+#pragma unroll
+      for (int v = 0; v < 4 * T::TO; ++v) all[v / 4][v % 4] = f32x4{};
+      for (int s0 = 0; s0 < ns; s0 += 2) {  // two splits' tiles requested together
+        f32x4 p[2][4 * T::TO];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const float* const src = part + ((int64_t)min(s0 + u, ns - 1) * tiles + tile) * (T::BM * T::BN);
+#pragma unroll
+          for (int v = 0; v < 4 * T::TO; ++v) p[u][v] = __builtin_bit_cast(f32x4, ld_cp<CP_SC01>(src, at + v * 1024));
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          if (s0 + u < ns)
+#pragma unroll
+            for (int v = 0; v < 4 * T::TO; ++v) all[v / 4][v % 4] += p[u][v];
+      }
+#pragma unroll
+      for (int v = 0; v < 4 * T::TO; ++v) sum[v / 4][v % 4] = all[v / 4][v % 4];
+    }
+    if (tid == 0) atomicExch(&arrivals[tile], 0u);
+  }
+  if (!fin) return;
+
+  // ---- the lane's rows are m0 + 16 FX wm + FX i + t; its columns 16 q + 4 e + f (gated: 8 q + 2 e + f) of the wave's
+  const bool vec = N % 8 == 0 && ((uintptr_t)a.c & 15) == 0;
+  unroll<0, T::TO>([&](auto oc) __attribute__((always_inline)) {
+    constexpr int o = decltype(oc)::value;
+    const int row = m0 + 16 * FX * wm + FX * i + kg * T::TO + o;
+    if constexpr (DUAL) {
+      const int col = n0 + 32 * wn;
+      float v[8];
+      uint32_t m = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int f = 0; f < 2; ++f) {
+          v[2 * e + f] = gated(sum[o][f][e], sum[o][2 + f][e]);
+          m = max(m, mx8::abs_bits(v[2 * e + f]));
+        }
+      m = xhalf_max_bits(xrow_max_bits(m));
+      if (row < M && col < N) {
+        const uint32_t byte = mx8::scale_byte(m);
+        const float inv = mx8::inverse(byte);
+        *(u32x2*)((uint8_t*)a.c + (int64_t)row * N + col + 8 * q) =
+            u32x2{mx8::codes4(v[0], v[1], v[2], v[3], inv, byte < 255), mx8::codes4(v[4], v[5], v[6], v[7], inv, byte < 255)};
+        if (q == 0) a.c_scales[mx8::scale_at(row, col / BLOCK, (N + 127) / 128)] = (uint8_t)byte;
+      }
+    } else {
+      const int col = n0 + 64 * wn + 16 * q;
+      if (row < M) {
+        float v[16];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int f = 0; f < 4; ++f) v[4 * e + f] = sum[o][f][e];
+        store16<T::OUT>((uint16_t*)a.c + (int64_t)row * N + col, v, (int64_t)N - col, vec);
+      }
+    }
+  });
+}
+
+// ---- choice of tile and split on the host
+enum { T16 = 0, T32, T16W, T32W, T64, T128, T256, T_COUNT };
+struct Shape {
+  int bm, bn, kg, threads;
+};
+constexpr Shape SHAPES[T_COUNT] = {{16, 64, 4, 512},  {32, 64, 4, 512},   {16, 128, 2, 512}, {32, 128, 2, 512},
+                                   {64, 128, 2, 768}, {128, 128, 1, 512}, {256, 256, 1, 512}};
+struct Plan {
+  int tile, ns;
+};
+// Columns of the result that a tile computes.
+constexpr int cols_of(int t, bool dual) { return dual ? SHAPES[t].bn / 2 : SHAPES[t].bn; }
+inline int64_t tiles_of(int t, bool dual, int64_t M, int64_t N) {
+  return ((M + SHAPES[t].bm - 1) / SHAPES[t].bm) * ((N + cols_of(t, dual) - 1) / cols_of(t, dual));
+}
+
+// The cheapest (tile, split) by a model of the time in us: a launch, its rounds of 256 workgroups times their k steps (dearer the
+// more CUs share L2 and memory) and for a split the exchange. The coefficients are a fit to the times of all tiles and splits at 255
+// products of M 1-4096, N 300-14336, K 512-14336; by it a call takes 1.8% longer than with the best of them on average. max_ns
+// 1: no split.
+inline Plan choose(bool dual, int64_t M, int64_t N, int64_t K, int max_ns) {
+  struct Cost {
+    double a, b0, b1;  // launch; per k step alone; more per k step with every CU at work
+  };
+  static constexpr Cost COST[T_COUNT] = {{3.639, 0.084, 0.120}, {3.920, 0.098, 0.135}, {3.452, 0.164, 0.163},
+                                         {3.839, 0.178, 0.174}, {4.735, 0.214, 0.194}, {4.872, 0.280, 0.252},
+                                         {6.785, 1.247, 0.337}};
+  const int64_t kt = (K + 127) / 128;
+  Plan best{T256, 1};
+  double least = 1e300;
+  for (int t = 0; t < T_COUNT; ++t) {
+    const Shape s = SHAPES[t];
+    const int64_t tiles = tiles_of(t, dual, M, N);
+    for (int ns = 1; ns <= (t == T256 ? 1 : max_ns); ++ns) {
+      const int64_t wg = tiles * ns;
+      if (wg * s.threads > UINT32_MAX) break;  // a launch counts its threads in 32 bits
+      if (ns > 1 && (tiles > TLM_SPLIT_TILES || kt < 2 * ns || (size_t)wg * s.bm * s.bn * 4 > tlm_split_bytes(false)))
+        break;
+      const int64_t steps = ((kt + ns - 1) / ns + s.kg - 1) / s.kg * s.kg;
+      const double rounds = (double)((wg + 255) / 256);
+      double us = COST[t].a + rounds * (double)steps * (COST[t].b0 + COST[t].b1 * (double)wg / rounds / 256.0);
+      if (ns > 1) us += 0.54 + 0.45 * ns + 1.83 * s.bm * s.bn / 4096.0 * std::min(1.0, (double)wg / 256.0);
+      if (us < least) {
+        least = us;
+        best = Plan{t, ns};
+      }
+    }
+  }
+  return best;
+}
+
+template <int OUT>
+int run(const Args& a, hipStream_t s) {
+  constexpr bool DUAL = OUT == TLM_F8E4M3;
+  Plan p = choose(DUAL, a.M, a.N, a.K, 16);
+  float* part = nullptr;
+  unsigned* arrivals = nullptr;
+  if (p.ns > 1 && !gt::split_workspace(false, s, false, &part, &arrivals)) p = choose(DUAL, a.M, a.N, a.K, 1);
+  const unsigned wg = (unsigned)(tiles_of(p.tile, DUAL, a.M, a.N) * p.ns);
+  auto go = [&](auto tile) {
+    using T = decltype(tile);
+    static_assert(T::THREADS == 512 || T::BM == 64, "SHAPES");
+    gemm_mx8_tile<T><<<wg, T::THREADS, 0, s>>>(a, p.ns, part, arrivals);
+  };
+  switch (p.tile) {
+    case T16: go(Tile<16, 64, 1, 4, 3, OUT>{}); break;
+    case T32: go(Tile<32, 64, 2, 4, 3, OUT>{}); break;
+    case T16W: go(Tile<16, 128, 1, 2, 3, OUT>{}); break;
+    case T32W: go(Tile<32, 128, 2, 2, 3, OUT>{}); break;
+    case T64: go(Tile<64, 128, 2, 2, 3, OUT>{}); break;
+    case T128: go(Tile<128, 128, 4, 1, 4, OUT>{}); break;
+    default: gemm_mx8_256<OUT><<<wg, P_T, 0, s>>>(a);
+  }
   return TLM_OK;
 }
 
 int check_sizes(const char* fn, int64_t M, int64_t N, int64_t K) {
-  if (M < 0 || N < 0 || K < 0 || M > INT32_MAX - 255 || N > INT32_MAX - 255 || M > 64 * 65535) {
-    tlm_set_error("%s: bad sizes M=%lld N=%lld K=%lld", fn, (long long)M, (long long)N, (long long)K);
+  if (M < 0 || N < 0 || K < 0 || M > INT32_MAX - 255 || N > INT32_MAX - 255 ||
+      ((M + 255) / 256) * ((N + 127) / 128) > UINT32_MAX / P_T) {
+    tlm_set_error("%s: bad sizes M=%lld N=%lld K=%lld (2^23 tiles of 256 x 128 at most)", fn, (long long)M, (long long)N,
+                  (long long)K);
     return TLM_EINVAL;
   }
   return TLM_OK;
@@ -494,7 +788,7 @@ extern "C" int tlm_gemm_mx8(const void* a, const void* a_scales, const void* b, 
   const Args g{{(const uint8_t*)a, (const uint8_t*)a_scales}, {(const uint8_t*)b, (const uint8_t*)b_scales}, {},
                c, nullptr, M, N, (int)K, (int)((K + 127) / 128)};
   hipStream_t s = (hipStream_t)stream;
-  out_dtype == TLM_BF16 ? direct<TLM_BF16>(g, s) : direct<TLM_F16>(g, s);
+  out_dtype == TLM_BF16 ? run<TLM_BF16>(g, s) : run<TLM_F16>(g, s);
   TLM_LAUNCH_CHECK("tlm_gemm_mx8");
   return TLM_OK;
 }
@@ -512,7 +806,7 @@ extern "C" int tlm_gemm_mx8_swiglu(const void* a, const void* a_scales, const vo
                {(const uint8_t*)gate, (const uint8_t*)gate_scales},
                {(const uint8_t*)up, (const uint8_t*)up_scales},
                codes, (uint8_t*)scales, M, N, (int)K, (int)((K + 127) / 128)};
-  direct<TLM_F8E4M3>(g, (hipStream_t)stream);
+  run<TLM_F8E4M3>(g, (hipStream_t)stream);
   TLM_LAUNCH_CHECK("tlm_gemm_mx8_swiglu");
   return TLM_OK;
 }
