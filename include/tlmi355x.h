@@ -532,6 +532,10 @@ int tlm_gemm_mx8_swiglu(const void* a, const void* a_scales, const void* gate, c
                         const void* up, const void* up_scales, void* codes, void* scales, int64_t M, int64_t N,
                         int64_t K, void* stream);
 
+/* The tile (rows of A, rows of weights) and the number of workgroups that share its K that tlm_gemm_mx8, or with `gated`
+ * tlm_gemm_mx8_swiglu, takes for these sizes; split 0: on a stream without a workspace for partial tiles. Host only. */
+int tlm_gemm_mx8_plan(int64_t M, int64_t N, int64_t K, int gated, int split, int* rows, int* cols, int* ns);
+
 #ifdef __cplusplus
 }
 #endif

@@ -10,6 +10,7 @@ import pytest
 import torch
 
 from oracle import ref
+from test_mx8_oracle import GATED_PLANS, PLANS
 from tilelang.jit.adapter.mi355x import ops
 
 pytestmark = pytest.mark.gpu
@@ -239,6 +240,61 @@ def test_gemm_random(M, N, K):
         tiny = 2.0 ** -25 if dtype is F16 else 0
         fits = np.abs(want) * (1 + 2 * h) + SUM * mag < torch.finfo(dtype).max
         assert (np.abs(got - want) <= h * np.abs(want) + (1 + h) * SUM * mag + tiny)[fits].all()
+
+
+def _device_values(m):
+    """float64 values on the GPU of an 8-bit operand, for sizes that are slow on the host."""
+    codes, scales = m
+    b = scales.view(torch.uint8).permute(0, 3, 1, 2).flatten(2).flatten(0, 1)
+    e = b[:codes.shape[0], :codes.shape[1] // 32].double() - 127
+    return codes.double() * torch.ldexp(torch.ones_like(e), e).repeat_interleave(32, 1)
+
+
+@pytest.mark.parametrize("case", PLANS)
+def test_gemm_every_tile(case):
+    """Each tile, with K whole and split, on whole numbers: equal bits; a graph's replay, which never splits, as well."""
+    M, N, K = case[:3]
+    g = torch.Generator().manual_seed(M + N)
+    a, b = _whole(M, K, g), _whole(N, K, g)
+    if K > 1024:
+        for m in (a, b):
+            m[0][:, 500:-500] = 0
+    a, b = _operand(*a), _operand(*b)
+    c = torch.full((M, N), 7.0, dtype=BF16, device=DEV)
+    for _ in range(3):
+        ops.gemm_mx8(*a, *b, c)
+    want = torch.matmul(_device_values(a), _device_values(b).T.contiguous()).to(BF16)
+    assert torch.equal(c, want)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    d = torch.full_like(c, 7.0)
+    with torch.cuda.graph(graph, stream=s):
+        ops.gemm_mx8(*a, *b, d)
+    for _ in range(3):
+        d.fill_(3.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(d, want)
+
+
+@pytest.mark.parametrize("case", GATED_PLANS)
+def test_gemm_swiglu_every_tile(case):
+    M, N, K = case[:3]
+    g = torch.Generator().manual_seed(M + N)
+    a, gate, up = (_whole(r, K, g) for r in (M, N, N))
+    for m in (a, gate, up):  # exact sums, gates of a few units
+        m[0][:, 500:] = 0
+        m[1][:] -= 2
+    a, gate, up = _operand(*a), _operand(*gate), _operand(*up)
+    codes, scales = _empty(M, N)
+    for _ in range(3):
+        ops.gemm_mx8_swiglu(*a, *gate, *up, codes, scales)
+    x = _device_values(a)
+    v, u = (torch.matmul(x, _device_values(m).T.contiguous()) for m in (gate, up))
+    want = (u * v * torch.sigmoid(v)).cpu().numpy()
+    _check_mx(codes, scales, want, ARITH * np.abs(want) + 2.0 ** -126)
+    _check_unused(scales, M, N)
 
 
 def test_gemm_scales_far_apart():

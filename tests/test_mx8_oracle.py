@@ -10,6 +10,7 @@ from oracle import ref
 from tilelang.jit.adapter.mi355x import lib, ops
 
 E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+EINVAL, EUNSUPPORTED = -1, -2
 
 
 def test_table_is_torch_e4m3():
@@ -62,6 +63,45 @@ def test_norm_ref():
     assert out.dtype is torch.float32 and np.allclose(y, np.array([[4.0, 3.0]]) / np.sqrt(12.5))
 
 
+# ---- the choice of tile
+
+# sizes for every tile, with K whole and split: (M, N, K, rows, columns of weights, workgroups per K is > 1)
+PLANS = [(1, 32, 1056, 16, 64, False), (3, 100, 8192, 16, 64, True), (9, 9000, 96, 16, 128, False),
+         (5, 9000, 14336, 16, 128, True), (257, 1000, 2080, 32, 64, False), (1500, 32, 8192, 32, 64, True),
+         (50, 9000, 160, 32, 128, False), (257, 1000, 14336, 32, 128, True), (400, 9000, 32, 64, 128, False),
+         (33, 9000, 8192, 64, 128, True), (200, 9000, 1056, 128, 128, False), (100, 9000, 8192, 128, 128, True),
+         (2000, 4096, 96, 256, 256, False)]
+GATED_PLANS = [(1, 32, 1056, 16, 64, False), (3, 96, 8192, 16, 64, True), (9, 4096, 96, 16, 128, False),
+               (5, 8992, 14336, 16, 128, True), (2000, 96, 1056, 32, 64, False), (33, 992, 14336, 32, 64, True),
+               (257, 992, 160, 32, 128, False), (130, 992, 14336, 32, 128, True), (130, 8992, 32, 64, 128, False),
+               (257, 992, 8192, 64, 128, True), (100, 8992, 1056, 128, 128, False), (1100, 512, 8192, 128, 128, True),
+               (400, 8992, 96, 256, 256, False)]
+
+
+def plan(M, N, K, gated, split=True):
+    out = [ctypes.c_int() for _ in range(3)]
+    lib.call("tlm_gemm_mx8_plan", M, N, K, gated, split, *(ctypes.byref(o) for o in out))
+    return tuple(o.value for o in out)
+
+
+@pytest.mark.parametrize("gated,case", [(0, c) for c in PLANS] + [(1, c) for c in GATED_PLANS])
+def test_plan(gated, case):
+    M, N, K, rows, cols, split = case
+    got = plan(M, N, K, gated)
+    assert (*got[:2], got[2] > 1) == (rows, cols, split)
+    assert plan(M, N, K, gated, False)[2] == 1
+    tiles = -(-M // rows) * -(-N // (cols // 2 if gated else cols))
+    if split:  # the workspace holds the partial tiles
+        assert tiles <= 512 and tiles * got[2] * rows * cols * 4 <= 16 << 20 and got[2] <= -(-K // 128) // 2
+
+
+def test_plan_refusals():
+    one = ctypes.c_int()
+    assert lib.load().tlm_gemm_mx8_plan(0, 1, 32, 0, 1, *[ctypes.byref(one)] * 3) == EINVAL
+    assert lib.load().tlm_gemm_mx8_plan(1, 1, 32, 0, 1, None, ctypes.byref(one), ctypes.byref(one)) == EINVAL
+    assert lib.load().tlm_gemm_mx8_plan(2 ** 31 - 256, 2 ** 31 - 256, 32, 0, 1, *[ctypes.byref(one)] * 3) == EINVAL
+
+
 # ---- refusals
 
 P = 1 << 20  # an address that is never read: every call here is refused first
@@ -75,7 +115,6 @@ def _refused(fn, *args, code=None):
     return msg
 
 
-EINVAL, EUNSUPPORTED = -1, -2
 
 
 def test_c_codes():
@@ -144,6 +183,7 @@ def test_gemm_refusals():
     call(EUNSUPPORTED, dt=lib.F32)
     call(EINVAL, M=-1)
     call(EINVAL, N=2 ** 31)
+    call(EINVAL, M=2 ** 30, N=2 ** 20)
     call(EINVAL, K=2 ** 22 + 32)
     for kw in (dict(M=0), dict(N=0)):
         assert getattr(lib.load(), f)(*dict(ok, **kw).values(), None) == 0

@@ -38,15 +38,15 @@ TLM_DEV float gated(float gate, float up) { return up * (gate * __builtin_amdgcn
 
 // ---- whole prompts: 256 x 256 tiles
 
-// The ping-pong schedule of gemm8_256x256 (tlm_gemm_fp8.hip): the two waves of a SIMD take turns, one reads its next operands from LDS
-// while the other multiplies, and LDS-DMA is issued only beside the reads. Here W, the weights, is the operand a wave holds
-// (128 rows: 8 operands) and X the one it reads as it multiplies (64 rows: 4).
+// Four waves, one per SIMD, of 128 x 128 each: their sums fill the accumulation registers, and LDS is read 1/4 less than by eight waves of
+// 128 x 64. A wave multiplies without a pause: beside the products of a k step it reads the rest of the step's operands of X (the
+// rows of A; a ring of four registers), all of the next step's of W, and issues the LDS-DMA of the step after that.
 //
 // Slot 16 f + i of a 64-row group of an LDS stage holds row 4 i + f, so that operand f, read from 16 neighbouring slots, has the rows
-// whose scales are byte f of the lanes' words: three words a k step, loaded a step ahead, are all the scales a wave needs. Of the
+// whose scales are byte f of the lanes' words: four words a k step, loaded a step ahead, are all the scales a wave needs. Of the
 // sums, a lane then has 16 neighbouring columns of each of its rows: C is stored, or a block of 32 quantised with one exchange
 // between two lanes, without a way through LDS.
-constexpr int P_T = 512, P_M = 256, P_N = 256, P_ST = 256 * 128;  // P_ST: bytes of a stage of one operand
+constexpr int P_T = 256, P_M = 256, P_N = 256, P_ST = 256 * 128;  // P_ST: bytes of a stage of one operand
 constexpr int P_W = 2, P_X = 3;                                   // stages of W and X
 constexpr uint32_t OOB = 0x80000000u;                             // past every descriptor's end, also with 3 K more
 
@@ -114,6 +114,19 @@ TLM_DEV uint32_t xhalf_max_bits(uint32_t m) {  // of lanes l and l ^ 32
   return max(r[0], r[1]);
 }
 
+// c += the product, in place in the accumulation registers: left to itself, the compiler lets 256 of them change places from step to
+// step and spends an eighth of the loop on moving them. It knows no matrix instruction here, so nothing else reads or writes c until
+// settle(), operands come from waited LDS reads, and 64 of these lie between two on the same c.
+template <int SA, int SB>
+TLM_DEV void mma_in_place(f32x4& c, const i32x8& a, const i32x8& b, uint32_t sa, uint32_t sb) {
+  asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[%5,%6,0] op_sel_hi:[%7,%8,0]"
+               : "+a"(c)
+               : "v"(a), "v"(b), "v"(sa), "v"(sb), "n"(SA & 1), "n"(SB & 1), "n"(SA >> 1), "n"(SB >> 1));
+}
+TLM_DEV void pin(f32x4& c) { asm volatile("" : "+a"(c)); }
+// The last products' results can be read (18 wait states), the first ones' operands have been written.
+TLM_DEV void settle() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
+
 template <int OUT>
 __global__ __launch_bounds__(P_T, 1) void gemm_mx8_256(Args a) {
   constexpr bool DUAL = OUT == TLM_F8E4M3;
@@ -121,22 +134,19 @@ __global__ __launch_bounds__(P_T, 1) void gemm_mx8_256(Args a) {
   __shared__ __attribute__((aligned(1024))) uint8_t smem[(P_W + P_X) * P_ST];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int grp = wave >> 2, quarter = wave & 3;  // half of W, 64 rows of X
+  const int wm = wave >> 1, wn = wave & 1;  // 128 rows of X, of W
   const int M = (int)a.M, N = (int)a.N, K = a.K, KT = a.kt;
   int tm, tn;
   tile_of(blockIdx.x, (M + P_M - 1) / P_M, (N + BN - 1) / BN, tm, tn);
   const int m0 = tm * P_M, n0 = tn * BN;
 
-  // ---- LDS-DMA: wave w of a group fills slots 64 w .. 64 w + 63 of its operand's stage, 8 a instruction
-  const bool is_w = grp == 0;
-  const bool second = DUAL && is_w && (quarter & 1);
-  // rows of the wave's 64 slots start here (gated: gate and up groups of 64 alternate)
-  const int r0 = is_w ? n0 + (DUAL ? 64 * (quarter >> 1) : 64 * quarter) : m0 + 64 * quarter;
-  const int rows = is_w ? N : M;
-  const uint8_t* const base = (is_w ? (second ? a.b2.codes : a.b.codes) : a.a.codes) + (int64_t)min(r0, rows) * K;
-  // instruction j: slots 8 j + lane / 8, rows 32 (j % 2) + 4 (lane / 8) + j / 2; what is past the last row lies past the
-  // descriptor's end
-  const int left = max(0, min(64, rows - r0)) * K;
+  // ---- LDS-DMA: wave w fills the 64 slots of group w of both stages (gated: gate and up groups alternate), 8 an instruction:
+  // instruction j slots 8 j + lane / 8, rows 32 (j % 2) + 4 (lane / 8) + j / 2. What is past the last row or k, and every step from
+  // KT on, lies past the descriptor's end and gives zeros.
+  const int rw = n0 + (DUAL ? 64 * (wave >> 1) : 64 * wave), rx = m0 + 64 * wave;
+  const uint8_t* const w_base = (DUAL && (wave & 1) ? a.b2.codes : a.b.codes) + (int64_t)min(rw, N) * K;
+  const uint8_t* const x_base = a.a.codes + (int64_t)min(rx, M) * K;
+  const int w_end = max(0, min(64, N - rw)) * K, x_end = max(0, min(64, M - rx)) * K;
   int chunk[2];
   uint32_t off[2];
 #pragma unroll
@@ -144,191 +154,189 @@ __global__ __launch_bounds__(P_T, 1) void gemm_mx8_256(Args a) {
     chunk[h] = 16 * ((lane & 7) ^ (4 * h + (lane >> 4)));
     off[h] = (uint32_t)((32 * h + 4 * (lane >> 3)) * K + chunk[h]);
   }
-  auto w_st = [&](int t) { return smem + (t & 1) * P_ST; };
-  auto x_st = [&](int t) { return smem + P_W * P_ST + (t % P_X) * P_ST; };
-  auto fill = [&](int t, uint8_t* st, int j) {
+  auto fill = [&](const uint8_t* base, int end, int t, uint8_t* st, int j) __attribute__((always_inline)) {
     const uint32_t o = chunk[j & 1] < K - t * 128 ? off[j & 1] : OOB;
-    dma16(base + (int64_t)t * 128, max(0, left - t * 128), st + quarter * 8192 + j * 1024, o + (j >> 1) * K);
+    dma16(base + (int64_t)t * 128, t < KT ? max(0, end - t * 128) : 0, st + wave * 8192 + j * 1024, o + (j >> 1) * K);
+  };
+  auto fill_w = [&](int t, int j) __attribute__((always_inline)) { fill(w_base, w_end, t, smem + (t & 1) * P_ST, j); };
+  auto fill_x = [&](int t, int j) __attribute__((always_inline)) {
+    fill(x_base, x_end, t, smem + (P_W + t % P_X) * P_ST, j);
   };
 
-  // ---- scales: words of the wave's two groups of W and its group of X; past the last row, another's
+  // ---- scales: words of the wave's two groups of W and of X; past the last row, another's
   auto words = [&](const uint8_t* s, int r, int n) {
     return s + (int64_t)(min(r, n - 1) >> 6) * KT * 256 + 4 * lane;
   };
-  const uint8_t* const s0 = words(a.b.scales, n0 + (DUAL ? 64 : 128) * grp, N);
-  const uint8_t* const s1 = DUAL ? words(a.b2.scales, n0 + 64 * grp, N) : words(a.b.scales, n0 + 128 * grp + 64, N);
-  const uint8_t* const sx = words(a.a.scales, m0 + 64 * quarter, M);
+  const uint8_t* const sw0 = words(a.b.scales, n0 + (DUAL ? 64 : 128) * wn, N);
+  const uint8_t* const sw1 = DUAL ? words(a.b2.scales, n0 + 64 * wn, N) : words(a.b.scales, n0 + 128 * wn + 64, N);
+  const uint8_t* const sx0 = words(a.a.scales, m0 + 128 * wm, M);
+  const uint8_t* const sx1 = words(a.a.scales, m0 + 128 * wm + 64, M);
   struct Scales {
-    uint32_t w[2], x;
+    uint32_t w[2], x[2];
   };
-  auto scales_of = [&](int t) {
+  auto scales_of = [&](int t) __attribute__((always_inline)) {
     const int64_t o = (int64_t)t * 256;
-    Scales s{{*(const uint32_t*)(s0 + o), *(const uint32_t*)(s1 + o)}, *(const uint32_t*)(sx + o)};
-    return s;
-  };
-  auto mask_tail = [&](Scales& s, int t) {  // past K: codes 0, scale 1
-    if (t * 128 + 32 * (lane >> 4) >= K) s = Scales{{0x7f7f7f7fu, 0x7f7f7f7fu}, 0x7f7f7f7fu};
+    return Scales{{*(const uint32_t*)(sw0 + o), *(const uint32_t*)(sw1 + o)},
+                  {*(const uint32_t*)(sx0 + o), *(const uint32_t*)(sx1 + o)}};
   };
 
   // ---- operands
-  const int q = lane >> 4;
-  const int xr = ((lane & 15) >> 1) & 7;
-  const uint32_t w_row = ldsop::lds_u32(smem) + (grp * 128 + (lane & 15)) * 128;
-  const uint32_t x_row = ldsop::lds_u32(smem) + P_W * P_ST + (quarter * 64 + (lane & 15)) * 128;
+  const uint32_t xr = ((lane & 15) >> 1) & 7;
+  const uint32_t w_row = ldsop::lds_u32(smem) + (wn * 128 + (lane & 15)) * 128;
+  const uint32_t x_row = ldsop::lds_u32(smem) + P_W * P_ST + (wm * 128 + (lane & 15)) * 128;
   uint32_t ch[2];
 #pragma unroll
-  for (int p = 0; p < 2; ++p) ch[p] = 16 * ((4 * p + q) ^ xr);
-  f32x4 acc[8][4];
+  for (int p = 0; p < 2; ++p) ch[p] = 16 * ((4 * p + (lane >> 4)) ^ xr);
+  f32x4 acc[8][8];
 #pragma unroll
   for (int f = 0; f < 8; ++f)
 #pragma unroll
-    for (int t = 0; t < 4; ++t) acc[f][t] = f32x4{};
-  u32x4 wop[8][2], xop0[2];
-  auto read_x = [&](int t, auto nc, u32x4 (&o)[2]) {
-    constexpr int n = decltype(nc)::value;
-    const uint32_t st = x_row + (t % P_X) * P_ST;
-#pragma unroll
-    for (int p = 0; p < 2; ++p) ldsop::ds_b128<n * 2048>(o[p], st + ch[p]);
+    for (int n = 0; n < 8; ++n) {
+      acc[f][n] = f32x4{};
+      pin(acc[f][n]);
+    }
+  u32x4 wa[8][2], wb[8][2], x[4][2];
+  auto read_w = [&](uint32_t st, u32x4 (&o)[8][2], auto rc) __attribute__((always_inline)) {
+    constexpr int r = decltype(rc)::value;
+    ldsop::ds_b128<r / 2 * 2048>(o[r / 2][r % 2], w_row + st + ch[r % 2]);
   };
-  // the wave's 8 operands of W and its first of X, a pair of DMA instructions after every four reads
-  auto load_phase = [&](int t, int dma_t, uint8_t* dma_st) {
-    const uint32_t st = w_row + (t & 1) * P_ST;
-    unroll<0, 4>([&](auto qc) {
-      constexpr int j = decltype(qc)::value;
-#pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        ldsop::ds_b128<2 * j * 2048>(wop[2 * j][p], st + ch[p]);
-        ldsop::ds_b128<(2 * j + 1) * 2048>(wop[2 * j + 1][p], st + ch[p]);
-      }
-      if (dma_t >= 0) {
-        fill(dma_t, dma_st, 2 * j);
-        fill(dma_t, dma_st, 2 * j + 1);
-      }
-    });
-    read_x(t, std::integral_constant<int, 0>{}, xop0);
-    __builtin_amdgcn_sched_barrier(0);
-    wait_lgkm0();
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int f = 0; f < 8; ++f)
-#pragma unroll
-      for (int p = 0; p < 2; ++p) ldsop::landed(wop[f][p]);
-    ldsop::landed(xop0[0]);
-    ldsop::landed(xop0[1]);
+  auto read_x = [&](uint32_t st, auto rc) __attribute__((always_inline)) {  // half r % 2 of operand r / 2
+    constexpr int r = decltype(rc)::value;
+    ldsop::ds_b128<r / 2 * 2048>(x[r / 2 % 4][r % 2], x_row + st + ch[r % 2]);
   };
-  auto compute_phase = [&](int t, const Scales& s) {
-    u32x4 x[3][2];  // ring: operand n in x[n % 3], read two ahead
-    x[0][0] = xop0[0];
-    x[0][1] = xop0[1];
-    read_x(t, std::integral_constant<int, 1>{}, x[1]);
-    unroll<0, 4>([&](auto nc) {
+
+  // ---- k step t, W in `w`: eight products with each operand of X. Operand n + 2 is read beside those of operand n, W of step t + 1
+  // beside the first four. Before operand 6 all waves meet: they have read what is left of step t and all of W of t + 1, and X of
+  // t + 1 and W of t + 2 have landed. From there on the first two operands of X of t + 1 are read and W of t + 3 is fetched;
+  // X of t + 2 is fetched beside operands 2 to 5 of this step, which the next meeting waits for.
+  auto kstep = [&](int t, u32x4 (&w)[8][2], u32x4 (&next)[8][2], Scales& s) __attribute__((always_inline)) {
+    if (t == KT - 1 && t * 128 + 32 * (lane >> 4) >= K)  // past K: codes 0, scale 1
+      s = Scales{{0x7f7f7f7fu, 0x7f7f7f7fu}, {0x7f7f7f7fu, 0x7f7f7f7fu}};
+    const uint32_t xs = (uint32_t)(t % P_X) * P_ST, xn = (uint32_t)((t + 1) % P_X) * P_ST;
+    const uint32_t ws = (uint32_t)((t + 1) & 1) * P_ST;
+    Scales ahead;
+    unroll<0, 8>([&](auto nc) __attribute__((always_inline)) {
       constexpr int n = decltype(nc)::value;
-      if constexpr (n + 2 < 4) read_x(t, std::integral_constant<int, n + 2>{}, x[(n + 2) % 3]);
       __builtin_amdgcn_sched_barrier(0);
-      if constexpr (n + 2 < 4) wait_lgkm<4>();
-      else if constexpr (n + 1 < 4) wait_lgkm<2>();
-      else wait_lgkm<0>();
+      // operand n has landed; younger reads may be under way
+      if constexpr (n == 0) wait_lgkm<2>();
+      else if constexpr (n == 1 || n == 5) wait_lgkm<6>();
+      else if constexpr (n < 5) wait_lgkm<10>();
+      else if constexpr (n == 6) {
+        wait_vm<8>();
+        barrier();
+      }
       __builtin_amdgcn_sched_barrier(0);
-      ldsop::landed(x[n % 3][0]);
-      ldsop::landed(x[n % 3][1]);
-      unroll<0, 8>([&](auto fc) {
+      ldsop::landed(x[n % 4][0]);
+      ldsop::landed(x[n % 4][1]);
+      if constexpr (n == 0) {
+#pragma unroll
+        for (int f = 0; f < 8; ++f)
+#pragma unroll
+          for (int p = 0; p < 2; ++p) ldsop::landed(w[f][p]);
+        ahead = scales_of(min(t + 1, KT - 1));
+        asm volatile("s_nop 1" : "+v"(s.w[0]), "+v"(s.w[1]), "+v"(s.x[0]), "+v"(s.x[1]));
+      }
+      unroll<0, 8>([&](auto fc) __attribute__((always_inline)) {
         constexpr int f = decltype(fc)::value;
-        acc[f][n] = mma<f % 4, n>(cat8(wop[f][0], wop[f][1]), cat8(x[n % 3][0], x[n % 3][1]), acc[f][n], s.w[f / 4], s.x);
+        mma_in_place<f % 4, n % 4>(acc[f][n], cat8(w[f][0], w[f][1]), cat8(x[n % 4][0], x[n % 4][1]), s.w[f / 4], s.x[n / 4]);
+        if constexpr (f < 2) {
+          if constexpr (n < 6) read_x(xs, std::integral_constant<int, 2 * (n + 2) + f>{});
+          else read_x(xn, std::integral_constant<int, 2 * (n - 6) + f>{});
+        } else if constexpr (f < 6) {
+          if constexpr (n < 4) read_w(ws, next, std::integral_constant<int, 4 * n + f - 2>{});
+          if constexpr (n >= 6) fill_w(t + 3, 4 * (n - 6) + f - 2);
+        } else if constexpr (n >= 2 && n < 6) {
+          fill_x(t + 2, 2 * (n - 2) + f - 6);
+        }
+        __builtin_amdgcn_sched_barrier(0);
       });
     });
+    s = ahead;
   };
-  Scales cur = scales_of(0);
-  if (KT == 1) mask_tail(cur, 0);
-  // prologue: W of step 0 (group 0), X of steps 0 and 1 (group 1)
-  if (grp == 0) {
+  Scales s = scales_of(0);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) fill(0, w_st(0), j);
-  } else {
+  for (int j = 0; j < 8; ++j) fill_w(0, j);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) fill(0, x_st(0), j);
-    if (1 < KT) {
+  for (int j = 0; j < 8; ++j) fill_x(0, j);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) fill(1, x_st(1), j);
-    }
-  }
-  wait_vm<0>();
+  for (int j = 0; j < 8; ++j) fill_w(1, j);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) fill_x(1, j);
+  wait_vm<8>();
   barrier();
-  if (grp == 0) {
-    for (int t = 0; t < KT; ++t) {
-      Scales nxt = scales_of(min(t + 1, KT - 1));
-      load_phase(t, t + 1 < KT ? t + 1 : -1, w_st(t + 1));
-      barrier();
-      compute_phase(t, cur);
-      wait_vm<0>();  // W of t + 1 and its scales
-      cur = nxt;
-      if (t + 2 == KT) mask_tail(cur, t + 1);
-      barrier();
-    }
-    barrier();  // group 1 multiplies the last step
-  } else {
-    barrier();
-    for (int t = 0; t < KT; ++t) {
-      const bool more = t + 2 < KT;
-      Scales nxt = scales_of(min(t + 1, KT - 1));
-      load_phase(t, more ? t + 2 : -1, x_st(t + 2));
-      // X of t + 1 (issued a load phase ago) and the scales, older than this phase's 8, have landed
-      if (more) wait_vm<8>();
-      else wait_vm<0>();
-      barrier();
-      compute_phase(t, cur);
-      cur = nxt;
-      if (t + 2 == KT) mask_tail(cur, t + 1);
-      barrier();
-    }
+  unroll<0, 16>([&](auto rc) __attribute__((always_inline)) { read_w(0, wa, rc); });
+  wait_vm<8>();
+  barrier();
+#pragma unroll
+  for (int j = 0; j < 8; ++j) fill_w(2, j);
+  unroll<0, 4>([&](auto rc) __attribute__((always_inline)) { read_x(0, rc); });
+  int t = 0;
+  for (; t + 1 < KT; t += 2) {
+    kstep(t, wa, wb, s);
+    kstep(t + 1, wb, wa, s);
   }
+  if (t < KT) kstep(t, wa, wb, s);
+  wait_vm<0>();  // nothing is written to LDS that is no longer the workgroup's
+  wait_lgkm0();
+  settle();
+#pragma unroll
+  for (int f = 0; f < 8; ++f)
+#pragma unroll
+    for (int n = 0; n < 8; ++n) pin(acc[f][n]);
 
-  // ---- the lane's rows are m0 + 64 quarter + 4 i + t, its columns 16 g + 4 e + f of a group
+  // ---- the lane's rows are m0 + 128 wm + 64 (n / 4) + 4 i + n % 4, its columns 16 g + 4 e + f of a group
   const int i = lane & 15, g = lane >> 4;
   if constexpr (DUAL) {
-    const int col = n0 + 64 * grp + 16 * g;
-    uint32_t byte[4];
-    unroll<0, 4>([&](auto tc) {
-      constexpr int t = decltype(tc)::value;
-      const int row = m0 + 64 * quarter + 4 * i + t;
-      float v[16];
-      uint32_t m = 0;
+    const int col = n0 + 64 * wn + 16 * g;
+    unroll<0, 2>([&](auto hc) __attribute__((always_inline)) {
+      constexpr int h = decltype(hc)::value;
+      const int row0 = m0 + 128 * wm + 64 * h + 4 * i;
+      uint32_t byte[4];
+      unroll<0, 4>([&](auto tc) __attribute__((always_inline)) {
+        constexpr int r = decltype(tc)::value, n = 4 * h + r;
+        float v[16];
+        uint32_t m = 0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
+        for (int e = 0; e < 4; ++e)
 #pragma unroll
-        for (int f = 0; f < 4; ++f) {
-          v[4 * e + f] = gated(acc[f][t][e], acc[4 + f][t][e]);
-          m = max(m, mx8::abs_bits(v[4 * e + f]));
+          for (int f = 0; f < 4; ++f) {
+            v[4 * e + f] = gated(acc[f][n][e], acc[4 + f][n][e]);
+            m = max(m, mx8::abs_bits(v[4 * e + f]));
+          }
+        byte[r] = mx8::scale_byte(xrow_max_bits(m));
+        const float inv = mx8::inverse(byte[r]);
+        u32x4 p;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          p[e] = mx8::codes4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3], inv, byte[r] < 255);
+        if (row0 + r < M && col < N) *(u32x4*)((uint8_t*)a.c + (int64_t)(row0 + r) * N + col) = p;
+      });
+      if ((g & 1) == 0 && col < N) {
+        uint8_t* const sc = a.c_scales + mx8::scale_at(row0, col / BLOCK, (N + 127) / 128);
+        if (row0 + 4 <= M) {
+          *(uint32_t*)sc = byte[0] | byte[1] << 8 | byte[2] << 16 | byte[3] << 24;
+        } else {
+#pragma unroll
+          for (int r = 0; r < 3; ++r)
+            if (row0 + r < M) sc[r] = (uint8_t)byte[r];
         }
-      byte[t] = mx8::scale_byte(xrow_max_bits(m));
-      const float inv = mx8::inverse(byte[t]);
-      u32x4 p;
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        p[e] = mx8::codes4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3], inv, byte[t] < 255);
-      if (row < M && col < N) *(u32x4*)((uint8_t*)a.c + (int64_t)row * N + col) = p;
+      }
     });
-    if ((g & 1) == 0 && col < N) {
-      const int row = m0 + 64 * quarter + 4 * i;
-      uint8_t* const s = a.c_scales + mx8::scale_at(row, col / BLOCK, (N + 127) / 128);
-      if (row + 4 <= M) *(uint32_t*)s = byte[0] | byte[1] << 8 | byte[2] << 16 | byte[3] << 24;
-      else
-        for (int t = 0; t < 3; ++t)
-          if (row + t < M) s[t] = (uint8_t)byte[t];
-    }
   } else {
     const bool vec = N % 8 == 0 && ((uintptr_t)a.c & 15) == 0;
-    unroll<0, 4>([&](auto tc) {
-      constexpr int t = decltype(tc)::value;
-      const int row = m0 + 64 * quarter + 4 * i + t;
+    unroll<0, 8>([&](auto nc) __attribute__((always_inline)) {
+      constexpr int n = decltype(nc)::value;
+      const int row = m0 + 128 * wm + 64 * (n / 4) + 4 * i + n % 4;
       if (row >= M) return;
-      unroll<0, 2>([&](auto pc) {
+      unroll<0, 2>([&](auto pc) __attribute__((always_inline)) {
         constexpr int p = decltype(pc)::value;
-        const int col = n0 + 128 * grp + 64 * p + 16 * g;
+        const int col = n0 + 128 * wn + 64 * p + 16 * g;
         float v[16];
 #pragma unroll
         for (int e = 0; e < 4; ++e)
 #pragma unroll
-          for (int f = 0; f < 4; ++f) v[4 * e + f] = acc[4 * p + f][t][e];
+          for (int f = 0; f < 4; ++f) v[4 * e + f] = acc[4 * p + f][n][e];
         store16<OUT>((uint16_t*)a.c + (int64_t)row * N + col, v, (int64_t)N - col, vec);
       });
     });
@@ -685,7 +693,7 @@ struct Shape {
   int bm, bn, kg, threads;
 };
 constexpr Shape SHAPES[T_COUNT] = {{16, 64, 4, 512},  {32, 64, 4, 512},   {16, 128, 2, 512}, {32, 128, 2, 512},
-                                   {64, 128, 2, 768}, {128, 128, 1, 512}, {256, 256, 1, 512}};
+                                   {64, 128, 2, 768}, {128, 128, 1, 512}, {256, 256, 1, 256}};
 struct Plan {
   int tile, ns;
 };
@@ -695,17 +703,18 @@ inline int64_t tiles_of(int t, bool dual, int64_t M, int64_t N) {
   return ((M + SHAPES[t].bm - 1) / SHAPES[t].bm) * ((N + cols_of(t, dual) - 1) / cols_of(t, dual));
 }
 
-// The cheapest (tile, split) by a model of the time in us: a launch, its rounds of 256 workgroups times their k steps (dearer the
-// more CUs share L2 and memory) and for a split the exchange. The coefficients are a fit to the times of all tiles and splits at 255
-// products of M 1-4096, N 300-14336, K 512-14336; by it a call takes 1.8% longer than with the best of them on average. max_ns
-// 1: no split.
+// The cheapest (tile, split) by a model of the time in us: a launch, the operands from memory, the rounds of 256 workgroups times their
+// k steps (dearer the more CUs share L2) with a ramp for each after the first, and for a split the exchange. The coefficients are a
+// fit to the times of all tiles and splits at 323 products of M 1-4096, N 300-22016, K 512-14336; by it a call takes 0.5% longer
+// than with the best of them on average, 17% at worst. max_ns 1: no split.
 inline Plan choose(bool dual, int64_t M, int64_t N, int64_t K, int max_ns) {
   struct Cost {
-    double a, b0, b1;  // launch; per k step alone; more per k step with every CU at work
+    double a, b0, b1, r;  // launch; per k step alone; more per k step with every CU at work; a further round
   };
-  static constexpr Cost COST[T_COUNT] = {{3.639, 0.084, 0.120}, {3.920, 0.098, 0.135}, {3.452, 0.164, 0.163},
-                                         {3.839, 0.178, 0.174}, {4.735, 0.214, 0.194}, {4.872, 0.280, 0.252},
-                                         {6.785, 1.247, 0.337}};
+  static constexpr Cost COST[T_COUNT] = {{3.685, 0.082, 0.023, 2.64}, {3.984, 0.096, 0.024, 3.09}, {3.510, 0.152, 0.036, 2.65},
+                                         {3.852, 0.166, 0.043, 3.03}, {4.715, 0.187, 0.096, 3.50}, {4.823, 0.252, 0.170, 3.86},
+                                         {8.409, 0.832, 0.449, 8.24}};
+  const double memory = 0.078e-6 * (double)((dual ? 2 * N : N) + M) * (double)K;
   const int64_t kt = (K + 127) / 128;
   Plan best{T256, 1};
   double least = 1e300;
@@ -719,8 +728,9 @@ inline Plan choose(bool dual, int64_t M, int64_t N, int64_t K, int max_ns) {
         break;
       const int64_t steps = ((kt + ns - 1) / ns + s.kg - 1) / s.kg * s.kg;
       const double rounds = (double)((wg + 255) / 256);
-      double us = COST[t].a + rounds * (double)steps * (COST[t].b0 + COST[t].b1 * (double)wg / rounds / 256.0);
-      if (ns > 1) us += 0.54 + 0.45 * ns + 1.83 * s.bm * s.bn / 4096.0 * std::min(1.0, (double)wg / 256.0);
+      double us = COST[t].a + memory + COST[t].r * (rounds - 1) +
+                  rounds * (double)steps * (COST[t].b0 + COST[t].b1 * (double)wg / rounds / 256.0);
+      if (ns > 1) us += 0.78 + 0.36 * ns + 1.29 * s.bm * s.bn / 4096.0 * std::min(1.0, (double)wg / 256.0);
       if (us < least) {
         least = us;
         best = Plan{t, ns};
@@ -757,7 +767,7 @@ int run(const Args& a, hipStream_t s) {
 
 int check_sizes(const char* fn, int64_t M, int64_t N, int64_t K) {
   if (M < 0 || N < 0 || K < 0 || M > INT32_MAX - 255 || N > INT32_MAX - 255 ||
-      ((M + 255) / 256) * ((N + 127) / 128) > UINT32_MAX / P_T) {
+      ((M + 255) / 256) * ((N + 127) / 128) > UINT32_MAX / 512) {
     tlm_set_error("%s: bad sizes M=%lld N=%lld K=%lld (2^23 tiles of 256 x 128 at most)", fn, (long long)M, (long long)N,
                   (long long)K);
     return TLM_EINVAL;
@@ -766,6 +776,17 @@ int check_sizes(const char* fn, int64_t M, int64_t N, int64_t K) {
 }
 
 }  // namespace
+
+extern "C" int tlm_gemm_mx8_plan(int64_t M, int64_t N, int64_t K, int gated, int split, int* rows, int* cols, int* ns) {
+  if (M <= 0 || N <= 0 || K < 0 || !rows || !cols || !ns) {
+    tlm_set_error("tlm_gemm_mx8_plan: bad sizes or null pointer");
+    return TLM_EINVAL;
+  }
+  if (int rc = check_sizes("tlm_gemm_mx8_plan", M, N, K)) return rc;
+  const Plan p = choose(gated != 0, M, N, K, split ? 16 : 1);
+  *rows = SHAPES[p.tile].bm, *cols = SHAPES[p.tile].bn, *ns = p.ns;
+  return TLM_OK;
+}
 
 extern "C" int tlm_gemm_mx8(const void* a, const void* a_scales, const void* b, const void* b_scales, void* c,
                             int64_t M, int64_t N, int64_t K, int out_dtype, void* stream) {
