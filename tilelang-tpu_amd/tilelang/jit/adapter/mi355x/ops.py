@@ -564,9 +564,9 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, start: torch.Tensor, count: tor
     _i32("count", count, (B,))
     max_pages = _kv4_table(block_table, B)
     _call("tlm_kv4_append", (k, v, start, count, block_table, codes, scales), k.data_ptr(),
-              v.data_ptr(), kb, kr, vb, vr, dtype_code(k.dtype), start.data_ptr(), count.data_ptr(),
-              block_table.data_ptr(), max_pages, page, codes.data_ptr(), cs, scales.data_ptr(), ss,
-              pages, B, T, Hkv, D)
+          v.data_ptr(), kb, kr, vb, vr, dtype_code(k.dtype), start.data_ptr(), count.data_ptr(),
+          block_table.data_ptr(), max_pages, page, codes.data_ptr(), cs, scales.data_ptr(), ss,
+          pages, B, T, Hkv, D)
     return codes, scales
 
 
@@ -590,9 +590,9 @@ def kv4_read(codes: torch.Tensor, scales: torch.Tensor, block_table: torch.Tenso
     if start is not None:
         _i32("start", start, (B,))
     _call("tlm_kv4_read", (codes, scales, block_table, start, cu_seqlens, k_out, v_out),
-              codes.data_ptr(), cs, scales.data_ptr(), ss, pages, block_table.data_ptr(), max_pages,
-              page, _ptr(start), cu_seqlens.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), B,
-              shape[0], Hkv, D, dtype_code(k_out.dtype))
+          codes.data_ptr(), cs, scales.data_ptr(), ss, pages, block_table.data_ptr(), max_pages,
+          page, _ptr(start), cu_seqlens.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), B,
+          shape[0], Hkv, D, dtype_code(k_out.dtype))
     return k_out, v_out
 
 
@@ -626,10 +626,10 @@ def kv4_attn(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, block_t
     if not workspace.is_contiguous():
         raise ValueError("workspace must be contiguous")
     _call("tlm_kv4_attn", (q, codes, scales, block_table, seqlens, out, workspace, count, lse),
-              q.data_ptr(), qb, qr, codes.data_ptr(), cs, scales.data_ptr(), ss, pages,
-              block_table.data_ptr(), max_pages, page, seqlens.data_ptr(), _ptr(count),
-              out.data_ptr(), _ptr(lse), workspace.data_ptr(), workspace.nbytes, B, T, H, Hkv, D,
-              1 if causal else 0, sm_scale, dtype_code(q.dtype))
+          q.data_ptr(), qb, qr, codes.data_ptr(), cs, scales.data_ptr(), ss, pages,
+          block_table.data_ptr(), max_pages, page, seqlens.data_ptr(), _ptr(count),
+          out.data_ptr(), _ptr(lse), workspace.data_ptr(), workspace.nbytes, B, T, H, Hkv, D,
+          1 if causal else 0, sm_scale, dtype_code(q.dtype))
     return out
 
 
@@ -648,15 +648,20 @@ def mx8_tile_scales(scales: torch.Tensor) -> torch.Tensor:
     return b.contiguous().view(torch.float8_e8m0fnu)
 
 
+_E4M3, _E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+
+
 def _mx8(name: str, codes: torch.Tensor, scales: torch.Tensor, rows: int, K: int):
     """Checks an 8-bit operand [rows, K] and its scales."""
-    if codes.dtype is not torch.float8_e4m3fn or codes.shape != (rows, K) or not codes.is_contiguous():
+    if codes.dtype is _E4M3 and scales.dtype is _E8M0 and codes.shape == (rows, K) and \
+            scales.shape == (-(-rows // 64), -(-K // 128), 4, 64) and codes.is_contiguous() and \
+            scales.is_contiguous():
+        return
+    if codes.dtype is not _E4M3 or codes.shape != (rows, K) or not codes.is_contiguous():
         raise ValueError(f"{name} must be a contiguous float8_e4m3fn tensor [{rows}, {K}], got "
                          f"{codes.dtype} {list(codes.shape)}")
-    if scales.dtype is not torch.float8_e8m0fnu or not scales.is_contiguous() or \
-            scales.shape != (-(-rows // 64), -(-K // 128), 4, 64):
-        raise ValueError(f"scales of {name} must be a contiguous float8_e8m0fnu tensor "
-                         f"{list(mx8_scales_shape(rows, K))}, got {scales.dtype} {list(scales.shape)}")
+    raise ValueError(f"scales of {name} must be a contiguous float8_e8m0fnu tensor "
+                     f"{list(mx8_scales_shape(rows, K))}, got {scales.dtype} {list(scales.shape)}")
 
 
 def mx8_quant(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor):
@@ -668,7 +673,7 @@ def mx8_quant(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor):
     rows, K = x.shape
     _mx8("the result", codes, scales, rows, K)
     _call("tlm_mx8_quant", (x, codes, scales), x.data_ptr(), x.stride(0) if rows > 1 else K,
-              dtype_code(x.dtype), codes.data_ptr(), scales.data_ptr(), rows, K)
+          dtype_code(x.dtype), codes.data_ptr(), scales.data_ptr(), rows, K)
     return codes, scales
 
 
@@ -678,30 +683,33 @@ def add_rmsnorm(x: torch.Tensor, residual: Optional[torch.Tensor], w: Optional[t
     """residual_out = x + residual (rounded to the residual's dtype: x's or fp32; residual_out may be
     residual itself), and the norm residual_out * rsqrt(mean(residual_out^2) + eps) * w over the last dim
     in x's dtype (y), in 8 bits (codes, scales as mx8_quant's), or both. residual None: the norm of x."""
-    shape = x.shape
-    cols = shape[-1] if len(shape) else 0
+    shape, dtype = x.shape, x.dtype
+    cols = shape[-1] if shape else 0
     rows = x.numel() // cols if cols else 0
-    for n, t in (("x", x), ("residual", residual), ("residual_out", residual_out), ("y", y)):
-        if t is not None and (t.shape != shape or not t.is_contiguous()):
-            raise ValueError(f"{n} must be contiguous and match x in shape")
-    if (residual is None) != (residual_out is None) or (codes is None) != (scales is None):
-        raise ValueError("residual and residual_out, codes and scales are given together")
-    if y is None and codes is None:
-        raise ValueError("y or codes must be given")
-    r_dtype = x.dtype
-    if residual is not None:
+    if not x.is_contiguous():
+        raise ValueError("x must be contiguous")
+    r_dtype = dtype
+    if residual is not None and residual_out is not None:
         r_dtype = residual.dtype
-        if residual_out.dtype is not r_dtype:
-            raise ValueError("residual_out must have the residual's dtype")
-    if y is not None and y.dtype is not x.dtype:
-        raise ValueError("y must have x's dtype")
-    if w is not None and (w.dtype is not x.dtype or w.shape != (cols,) or not w.is_contiguous()):
-        raise ValueError(f"w must be a contiguous {x.dtype} tensor [{cols}]")
-    if codes is not None:
+        if residual.shape != shape or not residual.is_contiguous() or residual_out.dtype is not r_dtype or \
+                residual_out.shape != shape or not residual_out.is_contiguous():
+            raise ValueError("residual and residual_out must be contiguous and match x in shape, residual_out "
+                             "with the residual's dtype")
+    elif residual is not residual_out:
+        raise ValueError("residual and residual_out are given together")
+    if w is not None and (w.dtype is not dtype or w.dim() != 1 or w.numel() != cols or not w.is_contiguous()):
+        raise ValueError(f"w must be a contiguous {dtype} tensor [{cols}]")
+    if y is not None and (y.dtype is not dtype or y.shape != shape or not y.is_contiguous()):
+        raise ValueError("y must be contiguous and match x in shape and dtype")
+    if codes is not None and scales is not None:
         _mx8("the result", codes, scales, rows, cols)
+    elif codes is not scales:
+        raise ValueError("codes and scales are given together")
+    elif y is None:
+        raise ValueError("y or codes must be given")
     _call("tlm_add_rmsnorm", (x, residual, w, residual_out, y, codes, scales), x.data_ptr(),
-              _ptr(residual), _ptr(w), _ptr(residual_out), _ptr(y), _ptr(codes), _ptr(scales), rows, cols,
-              eps, dtype_code(x.dtype), dtype_code(r_dtype))
+          _ptr(residual), _ptr(w), _ptr(residual_out), _ptr(y), _ptr(codes), _ptr(scales), rows, cols,
+          eps, dtype_code(dtype), dtype_code(r_dtype))
     return residual_out, y, codes, scales
 
 
@@ -710,14 +718,13 @@ def gemm_mx8(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scales:
     """c = a @ b.T (fp16/bf16) of 8-bit operands a [M, K], b [N, K] with their scales."""
     if a.dim() != 2 or b.dim() != 2:
         raise ValueError("A must be [M, K] and B [N, K]")
-    M, K = a.shape
-    N = b.shape[0]
+    (M, K), N = a.shape, b.shape[0]
     _mx8("A", a, a_scales, M, K)
     _mx8("B", b, b_scales, N, K)
     if c.shape != (M, N) or not c.is_contiguous():
         raise ValueError(f"C must be contiguous [{M}, {N}]")
     _call("tlm_gemm_mx8", (a, a_scales, b, b_scales, c), a.data_ptr(), a_scales.data_ptr(), b.data_ptr(),
-              b_scales.data_ptr(), c.data_ptr(), M, N, K, dtype_code(c.dtype))
+          b_scales.data_ptr(), c.data_ptr(), M, N, K, dtype_code(c.dtype))
     return c
 
 
@@ -734,8 +741,8 @@ def gemm_mx8_swiglu(a: torch.Tensor, a_scales: torch.Tensor, b_gate: torch.Tenso
     _mx8("B_up", b_up, up_scales, N, K)
     _mx8("the result", codes, scales, M, N)
     _call("tlm_gemm_mx8_swiglu", (a, a_scales, b_gate, gate_scales, b_up, up_scales, codes, scales),
-              a.data_ptr(), a_scales.data_ptr(), b_gate.data_ptr(), gate_scales.data_ptr(), b_up.data_ptr(),
-              up_scales.data_ptr(), codes.data_ptr(), scales.data_ptr(), M, N, K)
+          a.data_ptr(), a_scales.data_ptr(), b_gate.data_ptr(), gate_scales.data_ptr(), b_up.data_ptr(),
+          up_scales.data_ptr(), codes.data_ptr(), scales.data_ptr(), M, N, K)
     return codes, scales
 
 
