@@ -351,6 +351,20 @@ def test_gemm_swiglu(M, N, K):
     _check_unused(scales, M, N)
 
 
+@pytest.mark.parametrize("M,N,K", [(1, 512, 4096), (13, 320, 2080), (32, 2048, 1024), (32, 64, 4096)])
+def test_gemm_swiglu_few_rows(M, N, K):
+    """Up to 32 rows are summed in fp32: K / 32 + 40 roundings of 2^-24 at most, below 2^-16 of the magnitudes."""
+    g = torch.Generator().manual_seed(M * N)
+    a, gate, up = _random(M, K, g, 0.3), _random(N, K, g, 0.3), _random(N, K, g, 0.3)
+    for m in (gate, up):
+        m[1][:] -= int(np.log2(K) / 2)
+    codes, scales = _empty(M, N)
+    ops.gemm_mx8_swiglu(*_operand(*a), *_operand(*gate), *_operand(*up), codes, scales)
+    want, move = ref.gemm_mx8_swiglu_ref(a, gate, up)
+    _check_mx(codes, scales, want, 2.0 ** -16 * move + ARITH * np.abs(want) + 2.0 ** -126)
+    _check_unused(scales, M, N)
+
+
 def test_gemm_swiglu_large_gates():
     """Gates of +-hundreds: exp overflows to infinity or vanishes, the result is up * gate or 0; NaN fills its block."""
     g = torch.Generator().manual_seed(12)

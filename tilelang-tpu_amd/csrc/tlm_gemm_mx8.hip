@@ -351,9 +351,15 @@ __global__ __launch_bounds__(P_T, 1) void gemm_mx8_256(Args a) {
 // KG k steps, one for each k-group, and their scales; the operands of stage t are read from LDS while the products of stage t - 1
 // run. The k-groups' sums meet in LDS, those of the `ns` workgroups that share a tile's K in memory, where the last to arrive adds
 // them in order: the result does not depend on the order of arrival.
-template <int BM_, int BN_, int FX_, int KG_, int NST_, int OUT_>
+//
+// WIDE: the operands are widened to bf16, exactly, and multiplied by v_mfma_f32_16x16x32_bf16, whose sums are those of fp32. (The
+// 8-bit instruction cuts each of 8 neighbouring products below 2^-14 of the largest one's leading bit: 4e-5 of a result, which 16 bits do
+// not show, but which sends 1 in 2,500 of a gated product's values to the other side of an 8-bit step.) Elements of 2^128
+// and more count as infinite there.
+template <int BM_, int BN_, int FX_, int KG_, int NST_, int OUT_, bool WIDE_ = false>
 struct Tile {
   static constexpr int BM = BM_, BN = BN_, FX = FX_, KG = KG_, NST = NST_, OUT = OUT_;
+  static constexpr bool WIDE = WIDE_;
   static constexpr bool DUAL = OUT == TLM_F8E4M3;
   static constexpr int BNC = DUAL ? BN / 2 : BN;       // columns of the result
   static constexpr int WM = BM / (16 * FX), WN = BN / 64;
@@ -376,9 +382,18 @@ template <int BKB>
 TLM_DEV int swz(int slot) {  // 16 lanes that read one chunk of 16 neighbouring slots hit all banks
   return BKB == 128 ? (slot >> 1) & 7 : slot & 15;
 }
-TLM_DEV void ds_b32(uint32_t& r, uint32_t a) { asm volatile("ds_read_b32 %0, %1" : "=v"(r) : "v"(a) : "memory"); }
-TLM_DEV void ds_u16(uint32_t& r, uint32_t a) { asm volatile("ds_read_u16 %0, %1" : "=v"(r) : "v"(a) : "memory"); }
-TLM_DEV void ds_u8(uint32_t& r, uint32_t a) { asm volatile("ds_read_u8 %0, %1" : "=v"(r) : "v"(a) : "memory"); }
+template <int OFF>
+TLM_DEV void ds_b32(uint32_t& r, uint32_t a) {
+  asm volatile("ds_read_b32 %0, %1 offset:%2" : "=v"(r) : "v"(a), "i"(OFF) : "memory");
+}
+template <int OFF>
+TLM_DEV void ds_u16(uint32_t& r, uint32_t a) {
+  asm volatile("ds_read_u16 %0, %1 offset:%2" : "=v"(r) : "v"(a), "i"(OFF) : "memory");
+}
+template <int OFF>
+TLM_DEV void ds_u8(uint32_t& r, uint32_t a) {
+  asm volatile("ds_read_u8 %0, %1 offset:%2" : "=v"(r) : "v"(a), "i"(OFF) : "memory");
+}
 TLM_DEV void landed1(uint32_t& a) { asm volatile("" : "+v"(a)); }
 TLM_DEV void plain_barrier() {
   __builtin_amdgcn_sched_barrier(0);
@@ -386,6 +401,24 @@ TLM_DEV void plain_barrier() {
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
   __builtin_amdgcn_sched_barrier(0);
+}
+
+// A lane's 32 codes as bf16, times the scales in byte B of s (one for each half).
+template <int B>
+TLM_DEV void widen(bf16x8 (&o)[4], const u32x4 (&x)[2], const uint32_t (&s)[2]) {
+  typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const float scale = __uint_as_float((s[h] >> (8 * B) & 255u) << 23);
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+      const b2 lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[h][d], scale, false);
+      const b2 hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[h][d], scale, true);
+      const int j = 4 * (d & 1);
+      o[2 * h + d / 2][j] = lo[0], o[2 * h + d / 2][j + 1] = lo[1];
+      o[2 * h + d / 2][j + 2] = hi[0], o[2 * h + d / 2][j + 3] = hi[1];
+    }
+  }
 }
 
 template <typename T>
@@ -488,30 +521,37 @@ __global__ __launch_bounds__(T::THREADS, 1) void gemm_mx8_tile(Args a, int ns, f
   }
   const uint32_t sc0 = b0 + T::SX + T::SW + kg * 256;
   const int xrow = (m0 & 63) + wm * 16 * FX;  // the wave's rows within the first group
-  const uint32_t xs_addr = sc0 + (xrow >> 6) * 1024 + q * 64 + (xrow & 63) + FX * i;
+  // the lane's block of the k step: q; wide, where each half of an operand has a scale of its own, q / 2 and q / 2 + 2
+  const int blk = T::WIDE ? q >> 1 : q;
+  const uint32_t xs_addr = sc0 + (xrow >> 6) * 1024 + blk * 64 + (xrow & 63) + FX * i;
   const int wcol = (n0 & 63) + 32 * wn;  // gated: the wave's columns within the first group
-  const uint32_t ws_addr = DUAL ? sc0 + (T::GX + (wcol >> 6)) * 1024 + q * 64 + (wcol & 63) + 2 * i
-                                : sc0 + (T::GX + wn) * 1024 + 4 * lane;
+  const uint32_t ws_addr = DUAL ? sc0 + (T::GX + (wcol >> 6)) * 1024 + blk * 64 + (wcol & 63) + 2 * i
+                                : sc0 + (T::GX + wn) * 1024 + blk * 64 + 4 * i;
   constexpr int VS = T::GW / 2 * 1024;  // from gate's scales to up's
+  constexpr int HALVES = T::WIDE ? 2 : 1;
   struct Ops {
     u32x4 x[FX][2], w[4][2];
-    uint32_t xs, ws, vs;
+    uint32_t xs[HALVES], ws[HALVES], vs[HALVES];
   };
   constexpr int NR = 2 * FX + 8 + 2;
   auto read1 = [&](Ops& o, uint32_t so, auto ic) __attribute__((always_inline)) {
     constexpr int r = decltype(ic)::value;
     if constexpr (r < 8) ldsop::ds_b128<r / 2 * 16 * BKB>(o.w[r / 2][r % 2], w_addr[r % 2] + so);
     else if constexpr (r < 8 + 2 * FX) ldsop::ds_b128<(r - 8) / 2 * 16 * BKB>(o.x[(r - 8) / 2][r % 2], x_addr[r % 2] + so);
-    else if constexpr (r == 8 + 2 * FX) {
-      if constexpr (FX == 4) ds_b32(o.xs, xs_addr + so);
-      else if constexpr (FX == 1) ds_u8(o.xs, xs_addr + so);
-      else ds_u16(o.xs, xs_addr + so);
-    } else if constexpr (DUAL) {
-      ds_u16(o.ws, ws_addr + so);
-      ds_u16(o.vs, ws_addr + VS + so);
-    } else {
-      ds_b32(o.ws, ws_addr + so);
-    }
+    else
+      unroll<0, HALVES>([&](auto hc) __attribute__((always_inline)) {
+        constexpr int h = decltype(hc)::value;
+        if constexpr (r == 8 + 2 * FX) {
+          if constexpr (FX == 4) ds_b32<128 * h>(o.xs[h], xs_addr + so);
+          else if constexpr (FX == 1) ds_u8<128 * h>(o.xs[h], xs_addr + so);
+          else ds_u16<128 * h>(o.xs[h], xs_addr + so);
+        } else if constexpr (DUAL) {
+          ds_u16<128 * h>(o.ws[h], ws_addr + so);
+          ds_u16<128 * h>(o.vs[h], ws_addr + VS + so);
+        } else {
+          ds_b32<128 * h>(o.ws[h], ws_addr + so);
+        }
+      });
   };
   auto ops_landed = [&](Ops& o, int t) __attribute__((always_inline)) {
     __builtin_amdgcn_sched_barrier(0);
@@ -524,22 +564,42 @@ __global__ __launch_bounds__(T::THREADS, 1) void gemm_mx8_tile(Args a, int ns, f
 #pragma unroll
       for (int f = 0; f < 4; ++f) ldsop::landed(o.w[f][p]);
     }
-    landed1(o.xs);
-    landed1(o.ws);
-    if constexpr (DUAL) landed1(o.vs);
-    // past the end: codes 0, scale 1
-    if ((t * KG + kg) * 128 + 32 * q >= kend) o.xs = o.ws = o.vs = 0x7f7f7f7fu;
+#pragma unroll
+    for (int h = 0; h < HALVES; ++h) {
+      landed1(o.xs[h]);
+      landed1(o.ws[h]);
+      if constexpr (DUAL) landed1(o.vs[h]);
+      // past the end: codes 0, scale 1
+      if ((t * KG + kg) * 128 + 32 * (blk + 2 * h) >= kend) o.xs[h] = o.ws[h] = o.vs[h] = 0x7f7f7f7fu;
+    }
   };
 #pragma unroll
   for (int f = 0; f < 4; ++f)
 #pragma unroll
     for (int t = 0; t < FX; ++t) acc[f][t] = f32x4{};
   constexpr int NM = 4 * FX;
+  struct Widened {
+    bf16x8 x[T::WIDE ? FX : 1][4], w[4];
+  } wide;
   auto mul1 = [&](const Ops& o, auto ic) __attribute__((always_inline)) {
-    constexpr int t = decltype(ic)::value / 4, f = decltype(ic)::value % 4;
-    const i32x8 w = cat8(o.w[f][0], o.w[f][1]), x = cat8(o.x[t][0], o.x[t][1]);
-    if constexpr (DUAL) acc[f][t] = mma<f & 1, t>(w, x, acc[f][t], f < 2 ? o.ws : o.vs, o.xs);
-    else acc[f][t] = mma<f, t>(w, x, acc[f][t], o.ws, o.xs);
+    constexpr int m = decltype(ic)::value;
+    if constexpr (T::WIDE) {
+      constexpr int f = m / FX, t = m % FX;
+      if constexpr (m == 0)
+        unroll<0, FX>([&](auto uc) __attribute__((always_inline)) {
+          constexpr int u = decltype(uc)::value;
+          widen<u>(wide.x[u], o.x[u], o.xs);
+        });
+      if constexpr (t == 0) widen<DUAL ? f & 1 : f>(wide.w, o.w[f], DUAL && f >= 2 ? o.vs : o.ws);
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        acc[f][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wide.w[g], wide.x[t][g], acc[f][t], 0, 0, 0);
+    } else {
+      constexpr int t = m / 4, f = m % 4;
+      const i32x8 w = cat8(o.w[f][0], o.w[f][1]), x = cat8(o.x[t][0], o.x[t][1]);
+      if constexpr (DUAL) acc[f][t] = mma<f & 1, t>(w, x, acc[f][t], f < 2 ? o.ws[0] : o.vs[0], o.xs[0]);
+      else acc[f][t] = mma<f, t>(w, x, acc[f][t], o.ws[0], o.xs[0]);
+    }
   };
 
   int stage = 0;
@@ -703,6 +763,11 @@ inline int64_t tiles_of(int t, bool dual, int64_t M, int64_t N) {
   return ((M + SHAPES[t].bm - 1) / SHAPES[t].bm) * ((N + cols_of(t, dual) - 1) / cols_of(t, dual));
 }
 
+// Whether a call multiplies widened operands: gated products of few rows, which wait for memory (16 x 4096 x 14336 25.2 instead of
+// 24.7 us, 32 x 14336 x 4096 26.8 instead of 27.8, 32 x 4096 x 4096 9.7 instead of 9.0). From 33 rows on they would wait for the
+// conversions (48 x 11008 x 1280 14.1 instead of 9.3, 64 x 14336 x 4096 37.7 instead of 27.1).
+constexpr bool is_wide(bool dual, int64_t M) { return dual && M <= 32; }
+
 // The cheapest (tile, split) by a model of the time in us: a launch, the operands from memory, the rounds of 256 workgroups times their
 // k steps (dearer the more CUs share L2) with a ramp for each after the first, and for a split the exchange. The coefficients are a
 // fit to the times of all tiles and splits at 323 products of M 1-4096, N 300-22016, K 512-14336; by it a call takes 0.5% longer
@@ -711,14 +776,18 @@ inline Plan choose(bool dual, int64_t M, int64_t N, int64_t K, int max_ns) {
   struct Cost {
     double a, b0, b1, r;  // launch; per k step alone; more per k step with every CU at work; a further round
   };
+  static constexpr Cost WIDE_COST[T64] = {{3.914, 0.097, 0.017, 2.88}, {4.478, 0.109, 0.011, 3.55}, {3.870, 0.189, 0.013, 2.98},
+                                          {4.366, 0.219, 0.000, 3.73}};  // of 91 products, gated, M 1-64
   static constexpr Cost COST[T_COUNT] = {{3.685, 0.082, 0.023, 2.64}, {3.984, 0.096, 0.024, 3.09}, {3.510, 0.152, 0.036, 2.65},
                                          {3.852, 0.166, 0.043, 3.03}, {4.715, 0.187, 0.096, 3.50}, {4.823, 0.252, 0.170, 3.86},
                                          {8.409, 0.832, 0.449, 8.24}};
-  const double memory = 0.078e-6 * (double)((dual ? 2 * N : N) + M) * (double)K;
+  const bool wide = is_wide(dual, M);
+  const Cost* const cost = wide ? WIDE_COST : COST;
+  const double memory = (wide ? 0.103e-6 : 0.078e-6) * (double)((dual ? 2 * N : N) + M) * (double)K;
   const int64_t kt = (K + 127) / 128;
   Plan best{T256, 1};
   double least = 1e300;
-  for (int t = 0; t < T_COUNT; ++t) {
+  for (int t = 0; t < (wide ? T64 : T_COUNT); ++t) {
     const Shape s = SHAPES[t];
     const int64_t tiles = tiles_of(t, dual, M, N);
     for (int ns = 1; ns <= (t == T256 ? 1 : max_ns); ++ns) {
@@ -728,8 +797,8 @@ inline Plan choose(bool dual, int64_t M, int64_t N, int64_t K, int max_ns) {
         break;
       const int64_t steps = ((kt + ns - 1) / ns + s.kg - 1) / s.kg * s.kg;
       const double rounds = (double)((wg + 255) / 256);
-      double us = COST[t].a + memory + COST[t].r * (rounds - 1) +
-                  rounds * (double)steps * (COST[t].b0 + COST[t].b1 * (double)wg / rounds / 256.0);
+      double us = cost[t].a + memory + cost[t].r * (rounds - 1) +
+                  rounds * (double)steps * (cost[t].b0 + cost[t].b1 * (double)wg / rounds / 256.0);
       if (ns > 1) us += 0.78 + 0.36 * ns + 1.29 * s.bm * s.bn / 4096.0 * std::min(1.0, (double)wg / 256.0);
       if (us < least) {
         least = us;
@@ -753,14 +822,26 @@ int run(const Args& a, hipStream_t s) {
     static_assert(T::THREADS == 512 || T::BM == 64, "SHAPES");
     gemm_mx8_tile<T><<<wg, T::THREADS, 0, s>>>(a, p.ns, part, arrivals);
   };
+  auto ring = [&](auto wide) {
+    constexpr bool W = decltype(wide)::value;
+    switch (p.tile) {
+      case T16: return go(Tile<16, 64, 1, 4, 3, OUT, W>{});
+      case T32: return go(Tile<32, 64, 2, 4, 3, OUT, W>{});
+      case T16W: return go(Tile<16, 128, 1, 2, 3, OUT, W>{});
+      default: return go(Tile<32, 128, 2, 2, 3, OUT, W>{});
+    }
+  };
   switch (p.tile) {
-    case T16: go(Tile<16, 64, 1, 4, 3, OUT>{}); break;
-    case T32: go(Tile<32, 64, 2, 4, 3, OUT>{}); break;
-    case T16W: go(Tile<16, 128, 1, 2, 3, OUT>{}); break;
-    case T32W: go(Tile<32, 128, 2, 2, 3, OUT>{}); break;
     case T64: go(Tile<64, 128, 2, 2, 3, OUT>{}); break;
     case T128: go(Tile<128, 128, 4, 1, 4, OUT>{}); break;
-    default: gemm_mx8_256<OUT><<<wg, P_T, 0, s>>>(a);
+    case T256: gemm_mx8_256<OUT><<<wg, P_T, 0, s>>>(a); break;
+    default:
+      if constexpr (DUAL)
+        if (is_wide(DUAL, a.M)) {
+          ring(std::true_type{});
+          break;
+        }
+      ring(std::false_type{});
   }
   return TLM_OK;
 }
