@@ -505,7 +505,8 @@ int tlm_kv4_attn(const void* q, int64_t q_batch_stride, int64_t q_row_stride, co
  *           neither written nor used.
  * Quantising: a block's scale is the least 2^e, e >= -126, of which its largest magnitude is at most 448 times; codes are
  * x / 2^e rounded to nearest even. A block with an infinity or a NaN gets scale 255 and codes 0, and reads as NaN.
- * Calls without rows or columns do nothing; what would hold them may be null then. */
+ * Calls without rows or columns do nothing; what would hold them may be null then (without k, products are 0).
+ * Outputs overlap no other argument, but for residual_out. */
 
 /* Quantises rows x [rows, cols] of x_dtype (F16 | BF16 | F32), x_stride elements apart (a multiple of 8; x 16-byte
  * aligned). */

@@ -328,11 +328,29 @@ def test_gemm_nan_stays_in_its_row_and_column():
     assert torch.equal(nan, want)
 
 
-def test_gemm_no_columns_of_k():
-    a, b = _empty(3, 0), _empty(40, 0)
-    c = torch.full((3, 40), 7.0, dtype=F16, device=DEV)
+@pytest.mark.parametrize("M,N", [(3, 40), (1000, 1024), (4096, 4096)])
+def test_no_columns_of_k(M, N):
+    """Sums of nothing: zeros, from every tile."""
+    a, b = _empty(M, 0), _empty(N, 0)
+    c = torch.full((M, N), 7.0, dtype=F16, device=DEV)
     ops.gemm_mx8(*a, *b, c)
     assert not c.any()
+    if N % 32 == 0:
+        codes, scales = _empty(M, N)
+        ops.gemm_mx8_swiglu(*a, *b, *b, codes, scales)
+        assert not codes.view(torch.uint8).any()
+        assert (ref.mx8_untile_ref(_bytes(scales), M, N) == 1).all()
+
+
+@pytest.mark.parametrize("M", [5, 300])
+def test_gemm_first_and_last_scale(M):
+    """Scales that the quantiser never writes but others may: 2^-127 and 2^127, in products that fit."""
+    g = torch.Generator().manual_seed(M)
+    a, b = _whole(M, 256, g), _whole(64, 256, g)
+    a[1][:], b[1][:] = 0, 254
+    c = torch.empty(M, 64, dtype=BF16, device=DEV)
+    ops.gemm_mx8(*_operand(*a), *_operand(*b), c)
+    assert torch.equal(c.cpu(), torch.from_numpy(ref.gemm_mx8_ref(a, b)[0]).to(BF16))
 
 
 @pytest.mark.parametrize("M,N,K", [(1, 32, 32), (2, 64, 160), (16, 96, 1056), (17, 128, 256), (33, 544, 128), (64, 256, 4096),

@@ -88,15 +88,17 @@ TLM_DEV void tile_of(int wg, int tiles_m, int tiles_n, int& tm, int& tn) {
   tn = r / gm;
 }
 
-// 16 neighbouring columns col .. of a row of C.
+// 16 neighbouring columns of a row of C, the first `left` of them there. Rows of any width start on any element: the 16-byte stores are
+// such as need no alignment beyond an element's (2-byte ones took 16 times as many).
 template <int OUT>
-TLM_DEV void store16(uint16_t* c, const float (&v)[16], int64_t left, bool vec) {
+TLM_DEV void store16(uint16_t* c, const float (&v)[16], int64_t left) {
   using H = h16<OUT == TLM_BF16>;
-  if (vec && left >= 16) {
+  typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+  if (left >= 16) {
 #pragma unroll
     for (int h = 0; h < 2; ++h)
-      *(u32x4*)(c + 8 * h) = u32x4{H::pack(v[8 * h], v[8 * h + 1]), H::pack(v[8 * h + 2], v[8 * h + 3]),
-                                   H::pack(v[8 * h + 4], v[8 * h + 5]), H::pack(v[8 * h + 6], v[8 * h + 7])};
+      *(u32x4_any*)(c + 8 * h) = u32x4{H::pack(v[8 * h], v[8 * h + 1]), H::pack(v[8 * h + 2], v[8 * h + 3]),
+                                       H::pack(v[8 * h + 4], v[8 * h + 5]), H::pack(v[8 * h + 6], v[8 * h + 7])};
     return;
   }
 #pragma unroll
@@ -206,9 +208,11 @@ __global__ __launch_bounds__(P_T, 1) void gemm_mx8_256(Args a) {
   };
 
   // ---- k step t, W in `w`: eight products with each operand of X. Operand n + 2 is read beside those of operand n, W of step t + 1
-  // beside the first four. Before operand 6 all waves meet: they have read what is left of step t and all of W of t + 1, and X of
-  // t + 1 and W of t + 2 have landed. From there on the first two operands of X of t + 1 are read and W of t + 3 is fetched;
-  // X of t + 2 is fetched beside operands 2 to 5 of this step, which the next meeting waits for.
+  // beside the first five. Before operand 6 all waves meet: they have read what is left of step t and all of W of t + 1, and X of
+  // t + 1 and W of t + 2 have landed. From there on the first two operands of X of t + 1 are read. Two LDS-DMA instructions go
+  // with every operand (more at once would wait at issue, and the products with them): W of t + 3 with the last two and the next
+  // step's first two, X of t + 2 with the four between, which the next meeting waits for.
+  constexpr int W_READS[8] = {4, 3, 3, 3, 3, 0, 0, 0}, W_FIRST[8] = {0, 4, 7, 10, 13, 16, 16, 16};
   auto kstep = [&](int t, u32x4 (&w)[8][2], u32x4 (&next)[8][2], Scales& s) __attribute__((always_inline)) {
     if (t == KT - 1 && t * 128 + 32 * (lane >> 4) >= K)  // past K: codes 0, scale 1
       s = Scales{{0x7f7f7f7fu, 0x7f7f7f7fu}, {0x7f7f7f7fu, 0x7f7f7f7fu}};
@@ -219,9 +223,7 @@ __global__ __launch_bounds__(P_T, 1) void gemm_mx8_256(Args a) {
       constexpr int n = decltype(nc)::value;
       __builtin_amdgcn_sched_barrier(0);
       // operand n has landed; younger reads may be under way
-      if constexpr (n == 0) wait_lgkm<2>();
-      else if constexpr (n == 1 || n == 5) wait_lgkm<6>();
-      else if constexpr (n < 5) wait_lgkm<10>();
+      if constexpr (n < 6) wait_lgkm<(n > 1 ? W_READS[n - 2] : 0) + 2 + (n > 0 ? W_READS[n - 1] : 0)>();
       else if constexpr (n == 6) {
         wait_vm<8>();
         barrier();
@@ -244,17 +246,21 @@ __global__ __launch_bounds__(P_T, 1) void gemm_mx8_256(Args a) {
           if constexpr (n < 6) read_x(xs, std::integral_constant<int, 2 * (n + 2) + f>{});
           else read_x(xn, std::integral_constant<int, 2 * (n - 6) + f>{});
         } else if constexpr (f < 6) {
-          if constexpr (n < 4) read_w(ws, next, std::integral_constant<int, 4 * n + f - 2>{});
-          if constexpr (n >= 6) fill_w(t + 3, 4 * (n - 6) + f - 2);
-        } else if constexpr (n >= 2 && n < 6) {
+          if constexpr (f - 2 < W_READS[n]) read_w(ws, next, std::integral_constant<int, W_FIRST[n] + f - 2>{});
+        } else if constexpr (n < 2) {
+          fill_w(t + 2, 4 + 2 * n + f - 6);
+        } else if constexpr (n < 6) {
           fill_x(t + 2, 2 * (n - 2) + f - 6);
+        } else {
+          fill_w(t + 3, 2 * (n - 6) + f - 6);
         }
         __builtin_amdgcn_sched_barrier(0);
       });
     });
     s = ahead;
   };
-  Scales s = scales_of(0);
+  Scales s = {};
+  if (KT > 0) s = scales_of(0);  // without k there are none
 #pragma unroll
   for (int j = 0; j < 8; ++j) fill_w(0, j);
 #pragma unroll
@@ -269,7 +275,7 @@ __global__ __launch_bounds__(P_T, 1) void gemm_mx8_256(Args a) {
   wait_vm<8>();
   barrier();
 #pragma unroll
-  for (int j = 0; j < 8; ++j) fill_w(2, j);
+  for (int j = 0; j < 4; ++j) fill_w(2, j);
   unroll<0, 4>([&](auto rc) __attribute__((always_inline)) { read_x(0, rc); });
   int t = 0;
   for (; t + 1 < KT; t += 2) {
@@ -324,7 +330,6 @@ __global__ __launch_bounds__(P_T, 1) void gemm_mx8_256(Args a) {
       }
     });
   } else {
-    const bool vec = N % 8 == 0 && ((uintptr_t)a.c & 15) == 0;
     unroll<0, 8>([&](auto nc) __attribute__((always_inline)) {
       constexpr int n = decltype(nc)::value;
       const int row = m0 + 128 * wm + 64 * (n / 4) + 4 * i + n % 4;
@@ -337,7 +342,7 @@ __global__ __launch_bounds__(P_T, 1) void gemm_mx8_256(Args a) {
         for (int e = 0; e < 4; ++e)
 #pragma unroll
           for (int f = 0; f < 4; ++f) v[4 * e + f] = acc[4 * p + f][n][e];
-        store16<OUT>((uint16_t*)a.c + (int64_t)row * N + col, v, (int64_t)N - col, vec);
+        store16<OUT>((uint16_t*)a.c + (int64_t)row * N + col, v, (int64_t)N - col);
       });
     });
   }
@@ -710,7 +715,6 @@ __global__ __launch_bounds__(T::THREADS, 1) void gemm_mx8_tile(Args a, int ns, f
   if (!fin) return;
 
   // ---- the lane's rows are m0 + 16 FX wm + FX i + t; its columns 16 q + 4 e + f (gated: 8 q + 2 e + f) of the wave's
-  const bool vec = N % 8 == 0 && ((uintptr_t)a.c & 15) == 0;
   unroll<0, T::TO>([&](auto oc) __attribute__((always_inline)) {
     constexpr int o = decltype(oc)::value;
     const int row = m0 + 16 * FX * wm + FX * i + kg * T::TO + o;
@@ -741,7 +745,7 @@ __global__ __launch_bounds__(T::THREADS, 1) void gemm_mx8_tile(Args a, int ns, f
         for (int e = 0; e < 4; ++e)
 #pragma unroll
           for (int f = 0; f < 4; ++f) v[4 * e + f] = sum[o][f][e];
-        store16<T::OUT>((uint16_t*)a.c + (int64_t)row * N + col, v, (int64_t)N - col, vec);
+        store16<T::OUT>((uint16_t*)a.c + (int64_t)row * N + col, v, (int64_t)N - col);
       }
     }
   });
