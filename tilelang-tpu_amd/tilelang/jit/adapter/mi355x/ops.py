@@ -17,9 +17,10 @@ _FP8 = (torch.float8_e4m3fn, torch.float8_e5m2)
 
 
 def dtype_code(dt: torch.dtype) -> int:
-    if dt not in _DT:
-        raise ValueError(f"dtype {dt} is not supported by the mi355x kernels")
-    return _DT[dt]
+    try:
+        return _DT[dt]
+    except KeyError:
+        raise ValueError(f"dtype {dt} is not supported by the mi355x kernels") from None
 
 
 def _dev(*tensors):
@@ -39,6 +40,11 @@ def _dev(*tensors):
         dev = d
     lib.ensure_device(dev.index if dev.index is not None else torch.cuda.current_device())
     return dev
+
+
+# (absent from a build of torch without devices, whose tensors no call gets past its checks with)
+_get_device = getattr(torch._C, "_cuda_getDevice", None)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _stream(dev) -> int:
@@ -541,13 +547,13 @@ def _call(fn: str, tensors, *args):
     if index < 0:
         _dev(*tensors)  # says what is wrong
         raise ValueError("the mi355x kernels take HIP device tensors")
-    if torch._C._cuda_getDevice() != index:
+    if _get_device() != index:
         with torch.cuda.device(index):
             lib.ensure_device(index)
-            return lib.call(fn, *args, torch._C._cuda_getCurrentRawStream(index))
+            return lib.call(fn, *args, _raw_stream(index))
     if index not in lib._inited:
         lib.ensure_device(index)
-    return lib.call(fn, *args, torch._C._cuda_getCurrentRawStream(index))
+    return lib.call(fn, *args, _raw_stream(index))
 
 
 def kv4_append(k: torch.Tensor, v: torch.Tensor, start: torch.Tensor, count: torch.Tensor,
@@ -707,9 +713,12 @@ def add_rmsnorm(x: torch.Tensor, residual: Optional[torch.Tensor], w: Optional[t
         raise ValueError("codes and scales are given together")
     elif y is None:
         raise ValueError("y or codes must be given")
+    x_code = dtype_code(dtype)
     _call("tlm_add_rmsnorm", (x, residual, w, residual_out, y, codes, scales), x.data_ptr(),
-          _ptr(residual), _ptr(w), _ptr(residual_out), _ptr(y), _ptr(codes), _ptr(scales), rows, cols,
-          eps, dtype_code(dtype), dtype_code(r_dtype))
+          None if residual is None else residual.data_ptr(), None if w is None else w.data_ptr(),
+          None if residual is None else residual_out.data_ptr(), None if y is None else y.data_ptr(),
+          None if codes is None else codes.data_ptr(), None if codes is None else scales.data_ptr(), rows, cols,
+          eps, x_code, x_code if r_dtype is dtype else dtype_code(r_dtype))
     return residual_out, y, codes, scales
 
 
