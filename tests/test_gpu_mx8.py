@@ -203,6 +203,36 @@ def test_norm_zero_and_nan_rows():
     assert (byte[1] == 1).all() and (byte[2] == 255).all() and not _bytes(codes)[1:3].any()
 
 
+def test_norm_more_rows_than_a_launch_has_threads():
+    """2^26 rows and some of 64 threads each: a launch counts 2^32 threads along a side."""
+    rows = (1 << 26) + 70
+    x = torch.randn(rows, 32, dtype=BF16, device=DEV)
+    y = torch.zeros_like(x)
+    ops.add_rmsnorm(x, None, None, None, 1e-6, y)
+    at = torch.tensor([0, 1, (1 << 20) - 1, 1 << 20, (1 << 26) - 1, 1 << 26, rows - 1], device=DEV)
+    _, want = ref.add_rmsnorm_ref(x[at].cpu(), None, None, 1e-6)
+    got = y[at].double().cpu().numpy()
+    assert (np.abs(got - want) <= (2.0 ** -8 * (1 + ARITH) + ARITH) * np.abs(want)).all()
+    assert bool((y[-100000:] != 0).any(1).all())
+
+
+def test_quant_past_32_bits():
+    """Codes past 2^31 and 2^32 bytes."""
+    rows, K = 140000, 32768
+    x = torch.zeros(rows, K, dtype=F16, device=DEV)
+    at = [0, 65535, 65536, 70001, 131072, rows - 1]
+    g = torch.Generator().manual_seed(8)
+    some = torch.randn(len(at), K, generator=g).half()
+    x[at] = some.to(DEV)
+    codes, scales = _empty(rows, K)
+    ops.mx8_quant(x, codes, scales)
+    want, byte = ref.mx8_quantise_ref(some)
+    r = torch.tensor(at, device=DEV)
+    assert np.array_equal(codes.view(torch.uint8)[r].cpu().numpy(), want)
+    got = scales.view(torch.uint8)[r // 64, :, :, r % 64].cpu().numpy().reshape(len(at), -1)
+    assert np.array_equal(got, byte)
+
+
 # ---- products
 
 SIZES = [(1, 1, 32), (1, 5, 64), (2, 32, 96), (3, 100, 128), (7, 64, 160), (15, 250, 1056), (16, 256, 416), (17, 33, 256),
@@ -340,6 +370,28 @@ def test_no_columns_of_k(M, N):
         ops.gemm_mx8_swiglu(*a, *b, *b, codes, scales)
         assert not codes.view(torch.uint8).any()
         assert (ref.mx8_untile_ref(_bytes(scales), M, N) == 1).all()
+
+
+def test_gemm_past_32_bits():
+    """Operands and a result past 2^31 bytes: the rows about the borders and the last ones."""
+    g = torch.Generator().manual_seed(21)
+    M, N, K = 600000, 2048, 4128
+    a, b = _whole(64, K, g), _whole(N, K, g)
+    for m in (a, b):
+        m[0][:, 500:-500] = 0
+    big = torch.zeros(M, K, dtype=torch.uint8, device=DEV)
+    s = torch.full(ops.mx8_scales_shape(M, K), 127, dtype=torch.uint8, device=DEV)
+    codes = torch.from_numpy(a[0]).to(DEV)
+    at = [0, 64 * 8127, 64 * 8191, 64 * (M // 64 - 1)]  # whole groups of 64 rows
+    for r in at:
+        big[r:r + 64] = codes
+        s[r // 64] = _operand(*a)[1].view(torch.uint8)[0]
+    c = torch.full((M, N), 7.0, dtype=BF16, device=DEV)
+    ops.gemm_mx8(big.view(E4M3), s.view(E8M0), *_operand(*b), c)
+    want = torch.from_numpy(ref.gemm_mx8_ref(a, b)[0]).to(BF16).to(DEV)
+    for r in at:
+        assert torch.equal(c[r:r + 64], want)
+    assert not c[64:64 * 8127].any() and not c[-64 - M % 64 - 1:-64 - M % 64].any()
 
 
 @pytest.mark.parametrize("M", [5, 300])

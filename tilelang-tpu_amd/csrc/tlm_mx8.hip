@@ -76,12 +76,15 @@ struct Norm {
   float inv_cols, eps;
 };
 
+constexpr int N_GRID = 1 << 20;  // rows along x: a launch counts its threads along a side in 32 bits
+
 // A workgroup of T threads per row, V pieces of 8 columns per thread in registers.
 template <bool BF16, bool R32, int T, int V>
 __global__ __launch_bounds__(T) void add_rmsnorm_kernel(Norm a) {
   __shared__ float part[T / 64];
   constexpr int X = BF16, R = R32 ? 2 : X;
-  const int64_t row = blockIdx.x, at = row * a.cols;
+  const int64_t row = (int64_t)blockIdx.y * N_GRID + blockIdx.x, at = row * a.cols;
+  if (row >= a.rows) return;
   float h[V][8];
   float ss = 0.f;
 #pragma unroll
@@ -115,7 +118,7 @@ __global__ __launch_bounds__(T) void add_rmsnorm_kernel(Norm a) {
   }
   // one Newton step makes r exact to its last place; of 16-bit streams h w is exact, so that the result is rounded once
   const float m = ss * a.inv_cols + a.eps, r0 = __frsqrt_rn(m);
-  const float r = m > 0.f && m < INFINITY ? fmaf(0.5f * r0, fmaf(-m * r0, r0, 1.f), r0) : r0;
+  const float r = m < INFINITY && r0 < INFINITY ? fmaf(0.5f * r0, fmaf(-m * r0, r0, 1.f), r0) : r0;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int c = 8 * (i * T + (int)threadIdx.x);
@@ -133,7 +136,8 @@ template <bool BF16, bool R32>
 void norm_go(const Norm& a, hipStream_t s) {
   auto go = [&](auto t, auto v) {
     constexpr int T = decltype(t)::value, V = decltype(v)::value;
-    add_rmsnorm_kernel<BF16, R32, T, V><<<(unsigned)a.rows, T, 0, s>>>(a);
+    const dim3 grid((unsigned)std::min<int64_t>(a.rows, N_GRID), (unsigned)((a.rows + N_GRID - 1) / N_GRID));
+    add_rmsnorm_kernel<BF16, R32, T, V><<<grid, T, 0, s>>>(a);
   };
   using std::integral_constant;
   const int per = a.cols / 8;
