@@ -1,9 +1,17 @@
 // Products of 8-bit operands with power-of-two scales: C = A B^T, and SwiGLU of two of them with an 8-bit result.
 //
-// Tiles of 16 to 256 rows, chosen by a model of their time (choose, below).
-// v_mfma_scale_f32_16x16x128_f8f6f4 multiplies each block of 32 k by 2^(ea + eb) as it adds it. Lane l holds row l % 16 of
-// its operand and the 16-byte chunks q and q + 4 of its 128 k (q = l / 16), and the scale of k block q. The weights are the first
-// operand, so that a lane's sums are neighbouring columns of one row of C.
+//   c[m][n] = sum over blocks b of 32 k:  2^(ea[m][b] + eb[n][b]) sum over the block of a[m][k] b[n][k]
+//
+// v_mfma_scale_f32_16x16x128_f8f6f4 multiplies each block of 32 k by 2^(ea + eb) as it adds it, at 35 cycles instead of the
+// plain form's 32. Lane l holds row l % 16 of its operand and the 16-byte chunks q and q + 4 of its 128 k (q = l / 16), and the
+// scale of k block q. The weights are the first operand, so that a lane's sums are neighbouring columns of one row of C. The
+// sums are fp32; of 8 neighbouring products each is cut below 2^-14 of the largest one's leading bit before they are added
+// (4e-5 of a result of K 4096), which is why no 32-bit C is offered.
+//
+// Tiles of 16 to 256 rows, chosen by a model of their time (choose, below). Few rows wait for the stream of B, some hundreds for
+// the operands' way from L2 to a CU, whole prompts for the matrix cores' power. Measured in us: 16 x 4096 x 14336 13.5 (4.5
+// TB/s), 500 x 4096 x 4096 13.7, 4096^3 52 to 55 (2.5 to 2.6 PFLOP/s; the library's product without scales 51 to 52), gated
+// 64 x 2048 x 7168 10.3, gated 4096 x 11008 x 4096 290.
 #include "tlm_gemm_tile.h"
 #include "tlm_mx8.h"
 
@@ -38,14 +46,16 @@ TLM_DEV float gated(float gate, float up) { return up * (gate * __builtin_amdgcn
 
 // ---- whole prompts: 256 x 256 tiles
 
-// Four waves, one per SIMD, of 128 x 128 each: their sums fill the accumulation registers, and LDS is read 1/4 less than by eight waves of
-// 128 x 64. A wave multiplies without a pause: beside the products of a k step it reads the rest of the step's operands of X (the
-// rows of A; a ring of four registers), all of the next step's of W, and issues the LDS-DMA of the step after that.
+// Four waves, one per SIMD, of 128 x 128 each: their sums fill the accumulation registers, and LDS is read a third less than by
+// eight waves of 128 x 64 that take turns (57.9 us at 4096^3, now 52 to 55). A wave multiplies without a pause: beside the
+// products of a k step it reads the rest of the step's operands of X (the rows of A; a ring of four registers), all of the next
+// step's of W, and issues the LDS-DMA of steps to come. A step takes 2,420 cycles, its 64 products alone 2,240; the clock is
+// what power leaves, 1.5 to 1.7 GHz with data and 2.2 with zeros.
 //
-// Slot 16 f + i of a 64-row group of an LDS stage holds row 4 i + f, so that operand f, read from 16 neighbouring slots, has the rows
-// whose scales are byte f of the lanes' words: four words a k step, loaded a step ahead, are all the scales a wave needs. Of the
-// sums, a lane then has 16 neighbouring columns of each of its rows: C is stored, or a block of 32 quantised with one exchange
-// between two lanes, without a way through LDS.
+// Slot 16 f + i of a 64-row group of an LDS stage holds row 4 i + f, so that operand f, read from 16 neighbouring slots, has the
+// rows whose scales are byte f of the lanes' words: four words a k step, loaded a step ahead, are all the scales a wave needs. Of
+// the sums, a lane then has 16 neighbouring columns of each of its rows: C is stored, or a block of 32 quantised with one
+// exchange between two lanes, without a way through LDS.
 constexpr int P_T = 256, P_M = 256, P_N = 256, P_ST = 256 * 128;  // P_ST: bytes of a stage of one operand
 constexpr int P_W = 2, P_X = 3;                                   // stages of W and X
 constexpr uint32_t OOB = 0x80000000u;                             // past every descriptor's end, also with 3 K more
@@ -88,8 +98,8 @@ TLM_DEV void tile_of(int wg, int tiles_m, int tiles_n, int& tm, int& tn) {
   tn = r / gm;
 }
 
-// 16 neighbouring columns of a row of C, the first `left` of them there. Rows of any width start on any element: the 16-byte stores are
-// such as need no alignment beyond an element's (2-byte ones took 16 times as many).
+// 16 neighbouring columns of a row of C, the first `left` of them there. Rows of any width start on any element: the 16-byte
+// stores are such as need no alignment beyond an element's (4096 x 4091 x 4096 65 us, with 2-byte stores 95).
 template <int OUT>
 TLM_DEV void store16(uint16_t* c, const float (&v)[16], int64_t left) {
   using H = h16<OUT == TLM_BF16>;
@@ -116,9 +126,9 @@ TLM_DEV uint32_t xhalf_max_bits(uint32_t m) {  // of lanes l and l ^ 32
   return max(r[0], r[1]);
 }
 
-// c += the product, in place in the accumulation registers: left to itself, the compiler lets 256 of them change places from step to
-// step and spends an eighth of the loop on moving them. It knows no matrix instruction here, so nothing else reads or writes c until
-// settle(), operands come from waited LDS reads, and 64 of these lie between two on the same c.
+// c += the product, in place in the accumulation registers: left to itself, the compiler lets 256 of them change places from step
+// to step and spends 168 moves on that in two of them. It knows no matrix instruction here, so nothing else reads or writes c
+// until settle(), operands come from waited LDS reads, and 64 of these lie between two on the same c.
 template <int SA, int SB>
 TLM_DEV void mma_in_place(f32x4& c, const i32x8& a, const i32x8& b, uint32_t sa, uint32_t sb) {
   asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[%5,%6,0] op_sel_hi:[%7,%8,0]"
@@ -350,17 +360,17 @@ __global__ __launch_bounds__(P_T, 1) void gemm_mx8_256(Args a) {
 
 // ---- between one decode step and whole prompts: smaller tiles, K split where they are fewer than the CUs
 
-// What bounds it: the stream of B with few rows, with more the rate at which a CU takes operand tiles from L2 (about 55 B/clk).
-// Four waves only fill the ring: an LDS-DMA instruction waits at issue while the CU has enough of them under way, and a wave that
-// multiplies would wait with it. NC others are BM / (16 FX) x BN / 64 wave tiles times KG k-groups. A stage of the NST-stage ring holds
-// KG k steps, one for each k-group, and their scales; the operands of stage t are read from LDS while the products of stage t - 1
-// run. The k-groups' sums meet in LDS, those of the `ns` workgroups that share a tile's K in memory, where the last to arrive adds
-// them in order: the result does not depend on the order of arrival.
+// What bounds it: the stream of B with few rows, with more the rate at which a CU takes operand tiles from L2 (40 to 48 B/clk).
+// Four waves only fill the ring: an LDS-DMA instruction waits at issue while the CU has enough of them under way, and a wave
+// that multiplies would wait with it (500 x 4096 x 4096 16.8 us, with waves of their own 13.7). NC others are BM / (16 FX) x
+// BN / 64 wave tiles times KG k-groups. A stage of the NST-stage ring holds KG k steps, one for each k-group, and their scales;
+// the operands of stage t are read from LDS while the products of stage t - 1 run. The k-groups' sums meet in LDS, those of the
+// `ns` workgroups that share a tile's K in memory, where the last to arrive adds them in order: the result does not depend on
+// the order of arrival.
 //
-// WIDE: the operands are widened to bf16, exactly, and multiplied by v_mfma_f32_16x16x32_bf16, whose sums are those of fp32. (The
-// 8-bit instruction cuts each of 8 neighbouring products below 2^-14 of the largest one's leading bit: 4e-5 of a result, which 16 bits do
-// not show, but which sends 1 in 2,500 of a gated product's values to the other side of an 8-bit step.) Elements of 2^128
-// and more count as infinite there.
+// WIDE: the operands are widened to bf16, exactly, and multiplied by v_mfma_f32_16x16x32_bf16, whose sums are those of fp32. What
+// the 8-bit instruction cuts off does not show in 16 bits, but sends 1 in 2,500 of a gated product's values to the other side
+// of an 8-bit step. Elements of 2^128 and more count as infinite there.
 template <int BM_, int BN_, int FX_, int KG_, int NST_, int OUT_, bool WIDE_ = false>
 struct Tile {
   static constexpr int BM = BM_, BN = BN_, FX = FX_, KG = KG_, NST = NST_, OUT = OUT_;
