@@ -534,8 +534,10 @@ int tlm_gemm_mx8_swiglu(const void* a, const void* a_scales, const void* gate, c
                         int64_t K, void* stream);
 
 /* The tile (rows of A, rows of weights) and the number of workgroups that share its K that tlm_gemm_mx8, or with `gated`
- * tlm_gemm_mx8_swiglu, takes for these sizes; split 0: on a stream without a workspace for partial tiles. Host only. */
-int tlm_gemm_mx8_plan(int64_t M, int64_t N, int64_t K, int gated, int split, int* rows, int* cols, int* ns);
+ * tlm_gemm_mx8_swiglu, takes for these sizes, and how many rows and columns of the result they are for: all, or whole rounds of
+ * the CUs, and another launch computes the rest. split 0: on a stream without a workspace for partial tiles. Host only. */
+int tlm_gemm_mx8_plan(int64_t M, int64_t N, int64_t K, int gated, int split, int* rows, int* cols, int* ns,
+                      int64_t* first_rows, int64_t* first_cols);
 
 #ifdef __cplusplus
 }

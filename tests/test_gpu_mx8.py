@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from oracle import ref
-from test_mx8_oracle import GATED_PLANS, PLANS
+from test_mx8_oracle import CUTS, GATED_CUTS, GATED_PLANS, PLANS
 from tilelang.jit.adapter.mi355x import ops
 
 pytestmark = pytest.mark.gpu
@@ -280,7 +280,7 @@ def _device_values(m):
     return codes.double() * torch.ldexp(torch.ones_like(e), e).repeat_interleave(32, 1)
 
 
-@pytest.mark.parametrize("case", PLANS)
+@pytest.mark.parametrize("case", PLANS + CUTS)
 def test_gemm_every_tile(case):
     """Each tile, with K whole and split, on whole numbers: equal bits; a graph's replay, which never splits, as well."""
     M, N, K = case[:3]
@@ -308,7 +308,7 @@ def test_gemm_every_tile(case):
         assert torch.equal(d, want)
 
 
-@pytest.mark.parametrize("case", GATED_PLANS)
+@pytest.mark.parametrize("case", GATED_PLANS + GATED_CUTS)
 def test_gemm_swiglu_every_tile(case):
     M, N, K = case[:3]
     g = torch.Generator().manual_seed(M + N)

@@ -79,7 +79,7 @@ GATED_PLANS = [(1, 32, 1056, 16, 64, False), (3, 96, 8192, 16, 64, True), (9, 40
 
 
 def plan(M, N, K, gated, split=True):
-    out = [ctypes.c_int() for _ in range(3)]
+    out = [ctypes.c_int() for _ in range(3)] + [ctypes.c_int64() for _ in range(2)]
     lib.call("tlm_gemm_mx8_plan", M, N, K, gated, split, *(ctypes.byref(o) for o in out))
     return tuple(o.value for o in out)
 
@@ -88,18 +88,30 @@ def plan(M, N, K, gated, split=True):
 def test_plan(gated, case):
     M, N, K, rows, cols, split = case
     got = plan(M, N, K, gated)
-    assert (*got[:2], got[2] > 1) == (rows, cols, split)
+    assert (*got[:2], got[2] > 1, *got[3:]) == (rows, cols, split, M, N)
     assert plan(M, N, K, gated, False)[2] == 1
     tiles = -(-M // rows) * -(-N // (cols // 2 if gated else cols))
     if split:  # the workspace holds the partial tiles
         assert tiles <= 512 and tiles * got[2] * rows * cols * 4 <= 16 << 20 and got[2] <= -(-K // 128) // 2
 
 
+# more than whole rounds of 256 x 256 tiles: (M, N, K, rows and columns of the part that is whole rounds)
+CUTS = [(4400, 4096, 2080, 4096, 4096), (2000, 9000, 4096, 2000, 8192), (4100, 4100, 1056, 3840, 4100)]
+GATED_CUTS = [(4400, 2048, 2080, 4096, 2048), (2000, 4512, 4096, 2000, 4096), (2100, 4352, 1056, 2100, 3584)]
+
+
+@pytest.mark.parametrize("gated,case", [(0, c) for c in CUTS] + [(1, c) for c in GATED_CUTS])
+def test_plan_cuts(gated, case):
+    M, N, K, rows, cols = case
+    assert plan(M, N, K, gated) == (256, 256, 1, rows, cols)
+
+
 def test_plan_refusals():
-    one = ctypes.c_int()
-    assert lib.load().tlm_gemm_mx8_plan(0, 1, 32, 0, 1, *[ctypes.byref(one)] * 3) == EINVAL
-    assert lib.load().tlm_gemm_mx8_plan(1, 1, 32, 0, 1, None, ctypes.byref(one), ctypes.byref(one)) == EINVAL
-    assert lib.load().tlm_gemm_mx8_plan(2 ** 31 - 256, 2 ** 31 - 256, 32, 0, 1, *[ctypes.byref(one)] * 3) == EINVAL
+    one, two = ctypes.c_int(), ctypes.c_int64()
+    f, out = lib.load().tlm_gemm_mx8_plan, [ctypes.byref(one)] * 3 + [ctypes.byref(two)] * 2
+    assert f(0, 1, 32, 0, 1, *out) == EINVAL
+    assert f(1, 1, 32, 0, 1, None, *out[1:]) == EINVAL and f(1, 1, 32, 0, 1, *out[:4], None) == EINVAL
+    assert f(2 ** 31 - 256, 2 ** 31 - 256, 32, 0, 1, *out) == EINVAL
 
 
 # ---- refusals
