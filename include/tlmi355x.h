@@ -517,7 +517,8 @@ int tlm_mx8_quant(const void* x, int64_t x_stride, int x_dtype, void* codes, voi
  * of that, as stored, residual_out * rsqrt(mean(residual_out^2) + eps) * w, in fp32, rounded once to x_dtype (y), to 8 bits
  * (codes and scales), or to both. x, residual, residual_out, y [rows, cols] dense, w [cols] of x_dtype (F16 | BF16), all
  * 16-byte aligned. residual and residual_out NULL: the norm of x; residual_out may be residual; w NULL: no weight; y NULL or codes
- * and scales NULL: not wanted. cols a multiple of 8 (of 32 with codes), up to 32768. */
+ * and scales NULL: not wanted. cols a multiple of 8 (of 32 with codes), up to 32768. The sum of squares and
+ * residual_out * w are held in fp32: beyond 2^128 they are infinite. */
 int tlm_add_rmsnorm(const void* x, const void* residual, const void* w, void* residual_out, void* y, void* codes,
                     void* scales, int64_t rows, int64_t cols, float eps, int x_dtype, int residual_dtype,
                     void* stream);
@@ -528,7 +529,8 @@ int tlm_gemm_mx8(const void* a, const void* a_scales, const void* b, const void*
                  int64_t N, int64_t K, int out_dtype, void* stream);
 
 /* up * gate / (1 + exp(-gate)) with gate = A gate^T, up = A up^T (weights [N, K]) in 8 bits: codes [M, N] and scales,
- * quantised from fp32. N a multiple of 32. */
+ * quantised from fp32. N a multiple of 32. Elements of the operands that bf16 does not hold, 2^128 and more or below 2^-126,
+ * may count as infinite or as 0. */
 int tlm_gemm_mx8_swiglu(const void* a, const void* a_scales, const void* gate, const void* gate_scales,
                         const void* up, const void* up_scales, void* codes, void* scales, int64_t M, int64_t N,
                         int64_t K, void* stream);
