@@ -65,12 +65,13 @@ def test_norm_ref():
 
 # ---- the choice of tile
 
-# sizes for every tile, with K whole and split: (M, N, K, rows, columns of weights, workgroups per K is > 1)
-PLANS = [(1, 32, 1056, 16, 64, False), (3, 100, 8192, 16, 64, True), (9, 9000, 96, 16, 128, False),
-         (5, 9000, 14336, 16, 128, True), (257, 1000, 2080, 32, 64, False), (1500, 32, 8192, 32, 64, True),
-         (50, 9000, 160, 32, 128, False), (257, 1000, 14336, 32, 128, True), (400, 9000, 32, 64, 128, False),
-         (33, 9000, 8192, 64, 128, True), (200, 9000, 1056, 128, 128, False), (100, 9000, 8192, 128, 128, True),
-         (2000, 4096, 96, 256, 256, False)]
+# sizes for every tile, with K whole and, where calls take it so, split: (M, N, K, rows, columns of weights, workgroups per K is > 1)
+PLANS = [(1, 32, 1056, 16, 16, False), (3, 100, 14336, 16, 16, True), (3, 9001, 1056, 16, 64, False),
+         (5, 5003, 14336, 16, 64, True), (9, 9000, 96, 16, 128, False), (5, 9000, 14336, 16, 128, True),
+         (20, 2563, 1056, 32, 16, False), (20, 1057, 14336, 32, 16, True), (30, 5003, 2080, 32, 32, False),
+         (17, 2563, 14336, 32, 32, True), (257, 1000, 2080, 32, 64, False), (50, 9000, 160, 32, 128, False),
+         (257, 1000, 14336, 32, 128, True), (400, 9000, 32, 64, 128, False), (33, 9000, 8192, 64, 128, True),
+         (200, 9000, 1056, 128, 128, False), (100, 9000, 8192, 128, 128, True), (2000, 4096, 96, 256, 256, False)]
 GATED_PLANS = [(1, 32, 1056, 16, 64, False), (3, 96, 8192, 16, 64, True), (9, 4096, 96, 16, 128, False),
                (5, 8992, 14336, 16, 128, True), (2000, 96, 1056, 32, 64, False), (33, 992, 14336, 32, 64, True),
                (257, 992, 160, 32, 128, False), (130, 992, 14336, 32, 128, True), (130, 8992, 32, 64, 128, False),

@@ -9,7 +9,7 @@
 // (4e-5 of a result of K 4096), which is why no 32-bit C is offered.
 //
 // Tiles of 16 to 256 rows, chosen by a model of their time (choose, below). Few rows wait for the stream of B, some hundreds for
-// the operands' way from L2 to a CU, whole prompts for the matrix cores' power. Measured in us: 16 x 4096 x 14336 13.5 (4.5
+// the operands' way from L2 to a CU, whole prompts for the matrix cores' power. Measured in us: 16 x 4096 x 14336 11.6 (5.2
 // TB/s), 500 x 4096 x 4096 13.7, 4096^3 52 to 55 (2.5 to 2.6 PFLOP/s; the library's product without scales 51 to 52), gated
 // 64 x 2048 x 7168 10.3, gated 4096 x 11008 x 4096 290.
 #include "tlm_gemm_tile.h"
@@ -99,21 +99,25 @@ TLM_DEV void tile_of(int wg, int tiles_m, int tiles_n, int& tm, int& tn) {
   tn = r / gm;
 }
 
-// 16 neighbouring columns of a row of C, the first `left` of them there. Rows of any width start on any element: the 16-byte
-// stores are such as need no alignment beyond an element's (4096 x 4091 x 4096 65 us, with 2-byte stores 95).
-template <int OUT>
-TLM_DEV void store16(uint16_t* c, const float (&v)[16], int64_t left) {
+// W neighbouring columns of a row of C (16; 4 or 8 of narrow tiles), the first `left` of them there. Rows of any width start on
+// any element: the wide stores are such as need no alignment beyond an element's (4096 x 4091 x 4096 65 us, with 2-byte stores 95).
+template <int OUT, int W>
+TLM_DEV void store_cols(uint16_t* c, const float (&v)[W], int64_t left) {
   using H = h16<OUT == TLM_BF16>;
-  typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
-  if (left >= 16) {
+  constexpr int P = W < 8 ? W : 8;
+  typedef uint32_t any __attribute__((ext_vector_type(P / 2), aligned(2)));
+  if (left >= W) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-      *(u32x4_any*)(c + 8 * h) = u32x4{H::pack(v[8 * h], v[8 * h + 1]), H::pack(v[8 * h + 2], v[8 * h + 3]),
-                                       H::pack(v[8 * h + 4], v[8 * h + 5]), H::pack(v[8 * h + 6], v[8 * h + 7])};
+    for (int h = 0; h < W / P; ++h) {
+      any x;
+#pragma unroll
+      for (int j = 0; j < P / 2; ++j) x[j] = H::pack(v[P * h + 2 * j], v[P * h + 2 * j + 1]);
+      *(any*)(c + P * h) = x;
+    }
     return;
   }
 #pragma unroll
-  for (int j = 0; j < 16; ++j)
+  for (int j = 0; j < W; ++j)
     if (j < left) c[j] = (uint16_t)H::from_f32(v[j]);
 }
 
@@ -353,7 +357,7 @@ __global__ __launch_bounds__(P_T, 1) void gemm_mx8_256(Args a) {
         for (int e = 0; e < 4; ++e)
 #pragma unroll
           for (int f = 0; f < 4; ++f) v[4 * e + f] = acc[4 * p + f][n][e];
-        store16<OUT>((uint16_t*)a.c + row * a.ld + col, v, (int64_t)N - col);
+        store_cols<OUT>((uint16_t*)a.c + row * a.ld + col, v, (int64_t)N - col);
       });
     });
   }
@@ -369,6 +373,11 @@ __global__ __launch_bounds__(P_T, 1) void gemm_mx8_256(Args a) {
 // `ns` workgroups that share a tile's K in memory, where the last to arrive adds them in order: the result does not depend on
 // the order of arrival.
 //
+// Narrow tiles, of 16 or 32 columns, give few rows' products a workgroup per CU without a split, with 512 neighbouring bytes
+// of a row in a load: 16 x 4096 x 14336 11.6 instead of 13.1 (64 columns, two workgroups on a tile's K), 1 x 4096 x 11008 10.3
+// instead of 12.2, 16 x 8192 x 14336 22.9 instead of 24.5. There a wave has NF = 1 or 2 operands of W, row NF i + f in slot
+// 16 f + i.
+//
 // WIDE: the operands are widened to bf16, exactly, and multiplied by v_mfma_f32_16x16x32_bf16, whose sums are those of fp32. What
 // the 8-bit instruction cuts off does not show in 16 bits, but sends 1 in 2,500 of a gated product's values to the other side
 // of an 8-bit step. Elements of 2^128 and more count as infinite there.
@@ -378,17 +387,18 @@ struct Tile {
   static constexpr bool WIDE = WIDE_;
   static constexpr bool DUAL = OUT == TLM_F8E4M3;
   static constexpr int BNC = DUAL ? BN / 2 : BN;       // columns of the result
-  static constexpr int WM = BM / (16 * FX), WN = BN / 64;
+  static constexpr int NF = BN < 64 ? BN / 16 : 4;      // operands of W per wave
+  static constexpr int WM = BM / (16 * FX), WN = BN / (16 * NF);
   static constexpr int NC = WM * WN * KG, NP = 4;      // waves that multiply, waves that load
   static constexpr int BKB = 128 * KG;                 // bytes of k per stage
   static constexpr int SX = BM * BKB, SW = BN * BKB;
-  static constexpr int GX = (BM + 63) / 64, GW = DUAL ? 2 * ((BNC + 63) / 64) : BN / 64;  // 64-row groups of scales
+  static constexpr int GX = (BM + 63) / 64, GW = DUAL ? 2 * ((BNC + 63) / 64) : (BN + 63) / 64;  // 64-row groups of scales
   static constexpr int NX = SX / (NP * 1024), NW = SW / (NP * 1024);  // LDS-DMA instructions per wave: codes
   static constexpr int NSC = (GX + GW + NP - 1) / NP;                 // and scales, 1 KB per group: KG k steps and nothing
   static constexpr int PER = NX + NW + NSC;
   static constexpr int ST = SX + SW + NSC * NP * 1024;
   static constexpr int TO = FX > KG ? FX / KG : 1, FIN = FX > KG ? KG : FX;  // operands of X that a k-group finishes, k-groups that do
-  static constexpr int RED = KG > 1 ? NC * 4 * FX * 1024 : 0;
+  static constexpr int RED = KG > 1 ? NC * NF * FX * 1024 : 0;
   static constexpr int SMEM = NST * ST > RED ? NST * ST : RED;
   static constexpr int THREADS = 64 * (NC + NP);
   static_assert((NC == 4 || NC == 8) && KG <= 4 && NX * NP * 1024 == SX && NW * NP * 1024 == SW && SMEM <= 160 * 1024, "layout");
@@ -442,6 +452,7 @@ __global__ __launch_bounds__(T::THREADS, 1) void gemm_mx8_tile(Args a, int ns, f
                                                                unsigned* __restrict__ arrivals) {
   constexpr int BKB = T::BKB, KG = T::KG, FX = T::FX, NST = T::NST;
   constexpr bool DUAL = T::DUAL;
+  constexpr int NF = T::NF;
   __shared__ __attribute__((aligned(1024))) uint8_t smem[T::SMEM];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -460,7 +471,7 @@ __global__ __launch_bounds__(T::THREADS, 1) void gemm_mx8_tile(Args a, int ns, f
   const int n = (hi - lo + KG - 1) / KG;          // stages
   const int kend = min(K, hi * 128) - lo * 128;  // bytes of k
   const int i = lane & 15, q = lane >> 4;
-  f32x4 acc[4][FX];
+  f32x4 acc[NF][FX];
 
   // Stage t lives at t % NST. Before barrier t the loading waves wait for stage t; after it stage t - 1, whose operands every wave
   // has read by then, takes stage t + NST - 1.
@@ -476,7 +487,7 @@ __global__ __launch_bounds__(T::THREADS, 1) void gemm_mx8_tile(Args a, int ns, f
       int row;
       if (j < T::NX) row = slot / (16 * FX) * (16 * FX) + FX * (slot & 15) + (slot >> 4) % FX;
       else if (DUAL) row = (slot >> 6) * 32 + 2 * (slot & 15) + (slot >> 4 & 1);
-      else row = (slot & ~63) + 4 * (slot & 15) + (slot >> 4 & 3);
+      else row = (slot & ~63) + NF * (slot & 15) + (slot >> 4 & 3);
       off[j] = (uint32_t)(row * K + 16 * c);
       kch[j] = 16 * c;
     }
@@ -533,7 +544,7 @@ __global__ __launch_bounds__(T::THREADS, 1) void gemm_mx8_tile(Args a, int ns, f
   for (int p = 0; p < 2; ++p) {
     const int x = 16 * ((8 * kg + 4 * p + q) ^ swz<BKB>(i));
     x_addr[p] = b0 + (wm * 16 * FX + i) * BKB + x;
-    w_addr[p] = b0 + T::SX + (wn * 64 + i) * BKB + x;
+    w_addr[p] = b0 + T::SX + (wn * 16 * NF + i) * BKB + x;
   }
   const uint32_t sc0 = b0 + T::SX + T::SW + kg * 256;
   const int xrow = (m0 & 63) + wm * 16 * FX;  // the wave's rows within the first group
@@ -542,28 +553,34 @@ __global__ __launch_bounds__(T::THREADS, 1) void gemm_mx8_tile(Args a, int ns, f
   const uint32_t xs_addr = sc0 + (xrow >> 6) * 1024 + blk * 64 + (xrow & 63) + FX * i;
   const int wcol = (n0 & 63) + 32 * wn;  // gated: the wave's columns within the first group
   const uint32_t ws_addr = DUAL ? sc0 + (T::GX + (wcol >> 6)) * 1024 + blk * 64 + (wcol & 63) + 2 * i
-                                : sc0 + (T::GX + wn) * 1024 + blk * 64 + 4 * i;
+                       : NF < 4 ? sc0 + T::GX * 1024 + blk * 64 + (n0 & 63) + NF * i
+                                 : sc0 + (T::GX + wn) * 1024 + blk * 64 + 4 * i;
   constexpr int VS = T::GW / 2 * 1024;  // from gate's scales to up's
   constexpr int HALVES = T::WIDE ? 2 : 1;
   struct Ops {
-    u32x4 x[FX][2], w[4][2];
+    u32x4 x[FX][2], w[NF][2];
     uint32_t xs[HALVES], ws[HALVES], vs[HALVES];
   };
-  constexpr int NR = 2 * FX + 8 + 2;
+  constexpr int NR = 2 * FX + 2 * NF + 2;
   auto read1 = [&](Ops& o, uint32_t so, auto ic) __attribute__((always_inline)) {
     constexpr int r = decltype(ic)::value;
-    if constexpr (r < 8) ldsop::ds_b128<r / 2 * 16 * BKB>(o.w[r / 2][r % 2], w_addr[r % 2] + so);
-    else if constexpr (r < 8 + 2 * FX) ldsop::ds_b128<(r - 8) / 2 * 16 * BKB>(o.x[(r - 8) / 2][r % 2], x_addr[r % 2] + so);
+    if constexpr (r < 2 * NF) ldsop::ds_b128<r / 2 * 16 * BKB>(o.w[r / 2][r % 2], w_addr[r % 2] + so);
+    else if constexpr (r < 2 * NF + 2 * FX)
+      ldsop::ds_b128<(r - 2 * NF) / 2 * 16 * BKB>(o.x[(r - 2 * NF) / 2][r % 2], x_addr[r % 2] + so);
     else
       unroll<0, HALVES>([&](auto hc) __attribute__((always_inline)) {
         constexpr int h = decltype(hc)::value;
-        if constexpr (r == 8 + 2 * FX) {
+        if constexpr (r == 2 * NF + 2 * FX) {
           if constexpr (FX == 4) ds_b32<128 * h>(o.xs[h], xs_addr + so);
           else if constexpr (FX == 1) ds_u8<128 * h>(o.xs[h], xs_addr + so);
           else ds_u16<128 * h>(o.xs[h], xs_addr + so);
         } else if constexpr (DUAL) {
           ds_u16<128 * h>(o.ws[h], ws_addr + so);
           ds_u16<128 * h>(o.vs[h], ws_addr + VS + so);
+        } else if constexpr (NF == 2) {
+          ds_u16<128 * h>(o.ws[h], ws_addr + so);
+        } else if constexpr (NF == 1) {
+          ds_u8<128 * h>(o.ws[h], ws_addr + so);
         } else {
           ds_b32<128 * h>(o.ws[h], ws_addr + so);
         }
@@ -578,7 +595,7 @@ __global__ __launch_bounds__(T::THREADS, 1) void gemm_mx8_tile(Args a, int ns, f
 #pragma unroll
       for (int f = 0; f < FX; ++f) ldsop::landed(o.x[f][p]);
 #pragma unroll
-      for (int f = 0; f < 4; ++f) ldsop::landed(o.w[f][p]);
+      for (int f = 0; f < NF; ++f) ldsop::landed(o.w[f][p]);
     }
 #pragma unroll
     for (int h = 0; h < HALVES; ++h) {
@@ -590,10 +607,10 @@ __global__ __launch_bounds__(T::THREADS, 1) void gemm_mx8_tile(Args a, int ns, f
     }
   };
 #pragma unroll
-  for (int f = 0; f < 4; ++f)
+  for (int f = 0; f < NF; ++f)
 #pragma unroll
     for (int t = 0; t < FX; ++t) acc[f][t] = f32x4{};
-  constexpr int NM = 4 * FX;
+  constexpr int NM = NF * FX;
   struct Widened {
     bf16x8 x[T::WIDE ? FX : 1][4], w[4];
   } wide;
@@ -611,7 +628,7 @@ __global__ __launch_bounds__(T::THREADS, 1) void gemm_mx8_tile(Args a, int ns, f
       for (int g = 0; g < 4; ++g)
         acc[f][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wide.w[g], wide.x[t][g], acc[f][t], 0, 0, 0);
     } else {
-      constexpr int t = m / 4, f = m % 4;
+      constexpr int t = m / NF, f = m % NF;
       const i32x8 w = cat8(o.w[f][0], o.w[f][1]), x = cat8(o.x[t][0], o.x[t][1]);
       if constexpr (DUAL) acc[f][t] = mma<f & 1, t>(w, x, acc[f][t], f < 2 ? o.ws[0] : o.vs[0], o.xs[0]);
       else acc[f][t] = mma<f, t>(w, x, acc[f][t], o.ws[0], o.xs[0]);
@@ -655,7 +672,7 @@ __global__ __launch_bounds__(T::THREADS, 1) void gemm_mx8_tile(Args a, int ns, f
 
   // ---- the k-groups' sums: k-group g finishes operands g TO .. g TO + TO - 1 of X
   const bool fin = multiplies && kg < T::FIN;
-  f32x4 sum[T::TO][4];
+  f32x4 sum[T::TO][NF];
   if constexpr (KG > 1) {
     f32x4* const red = (f32x4*)smem;
     __syncthreads();  // every operand has been read
@@ -663,18 +680,18 @@ __global__ __launch_bounds__(T::THREADS, 1) void gemm_mx8_tile(Args a, int ns, f
       constexpr int t = decltype(tc)::value;
       if (multiplies && kg != t / T::TO)
 #pragma unroll
-        for (int f = 0; f < 4; ++f) red[((wave * FX + t) * 4 + f) * 64 + lane] = acc[f][t];
+        for (int f = 0; f < NF; ++f) red[((wave * FX + t) * NF + f) * 64 + lane] = acc[f][t];
     });
     __syncthreads();
     unroll<0, FX>([&](auto tc) __attribute__((always_inline)) {
       constexpr int t = decltype(tc)::value;
       if (multiplies && kg == t / T::TO) {
 #pragma unroll
-        for (int f = 0; f < 4; ++f) {
+        for (int f = 0; f < NF; ++f) {
           f32x4 s = {};
 #pragma unroll
           for (int g = 0; g < KG; ++g)
-            s += g == t / T::TO ? acc[f][t] : red[(((sp * KG + g) * FX + t) * 4 + f) * 64 + lane];
+            s += g == t / T::TO ? acc[f][t] : red[(((sp * KG + g) * FX + t) * NF + f) * 64 + lane];
           sum[t % T::TO][f] = s;
         }
       }
@@ -683,17 +700,17 @@ __global__ __launch_bounds__(T::THREADS, 1) void gemm_mx8_tile(Args a, int ns, f
 #pragma unroll
     for (int t = 0; t < FX; ++t)
 #pragma unroll
-      for (int f = 0; f < 4; ++f) sum[t][f] = acc[f][t];
+      for (int f = 0; f < NF; ++f) sum[t][f] = acc[f][t];
   }
 
   // ---- split K: partial tiles go through memory by write-through stores and loads that miss every cache
   if (ns > 1) {
     __shared__ unsigned last;
-    const int at = (((sp * T::FIN + kg) * T::TO * 4) * 64 + lane) * 16;
+    const int at = (((sp * T::FIN + kg) * T::TO * NF) * 64 + lane) * 16;
     if (fin) {
       float* const mine = part + ((int64_t)split * tiles + tile) * (T::BM * T::BN);
 #pragma unroll
-      for (int v = 0; v < 4 * T::TO; ++v) st_cp<CP_SC01>(mine, at + v * 1024, __builtin_bit_cast(u32x4, sum[v / 4][v % 4]));
+      for (int v = 0; v < NF * T::TO; ++v) st_cp<CP_SC01>(mine, at + v * 1024, __builtin_bit_cast(u32x4, sum[v / NF][v % NF]));
     }
     __builtin_amdgcn_s_waitcnt(0x3f70);  // vmcnt(0): the tile has been written
     __syncthreads();
@@ -701,25 +718,25 @@ __global__ __launch_bounds__(T::THREADS, 1) void gemm_mx8_tile(Args a, int ns, f
     __syncthreads();
     if (!last) return;
     if (fin) {
-      f32x4 all[T::TO][4];
+      f32x4 all[T::TO][NF];
 #pragma unroll
-      for (int v = 0; v < 4 * T::TO; ++v) all[v / 4][v % 4] = f32x4{};
+      for (int v = 0; v < NF * T::TO; ++v) all[v / NF][v % NF] = f32x4{};
       for (int s0 = 0; s0 < ns; s0 += 2) {  // two splits' tiles requested together
-        f32x4 p[2][4 * T::TO];
+        f32x4 p[2][NF * T::TO];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const float* const src = part + ((int64_t)min(s0 + u, ns - 1) * tiles + tile) * (T::BM * T::BN);
 #pragma unroll
-          for (int v = 0; v < 4 * T::TO; ++v) p[u][v] = __builtin_bit_cast(f32x4, ld_cp<CP_SC01>(src, at + v * 1024));
+          for (int v = 0; v < NF * T::TO; ++v) p[u][v] = __builtin_bit_cast(f32x4, ld_cp<CP_SC01>(src, at + v * 1024));
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u)
           if (s0 + u < ns)
 #pragma unroll
-            for (int v = 0; v < 4 * T::TO; ++v) all[v / 4][v % 4] += p[u][v];
+            for (int v = 0; v < NF * T::TO; ++v) all[v / NF][v % NF] += p[u][v];
       }
 #pragma unroll
-      for (int v = 0; v < 4 * T::TO; ++v) sum[v / 4][v % 4] = all[v / 4][v % 4];
+      for (int v = 0; v < NF * T::TO; ++v) sum[v / NF][v % NF] = all[v / NF][v % NF];
     }
     if (tid == 0) atomicExch(&arrivals[tile], 0u);
   }
@@ -749,26 +766,27 @@ __global__ __launch_bounds__(T::THREADS, 1) void gemm_mx8_tile(Args a, int ns, f
         if (q == 0) a.c_scales[mx8::scale_at(row, col / BLOCK, (int)((a.ld + 127) / 128))] = (uint8_t)byte;
       }
     } else {
-      const int col = n0 + 64 * wn + 16 * q;
+      const int col = n0 + 16 * NF * wn + 4 * NF * q;
       if (row < M) {
-        float v[16];
+        float v[4 * NF];
 #pragma unroll
         for (int e = 0; e < 4; ++e)
 #pragma unroll
-          for (int f = 0; f < 4; ++f) v[4 * e + f] = sum[o][f][e];
-        store16<T::OUT>((uint16_t*)a.c + row * a.ld + col, v, (int64_t)N - col);
+          for (int f = 0; f < NF; ++f) v[NF * e + f] = sum[o][f][e];
+        store_cols<T::OUT>((uint16_t*)a.c + row * a.ld + col, v, (int64_t)N - col);
       }
     }
   });
 }
 
 // ---- choice of tile and split on the host
-enum { T16 = 0, T32, T16W, T32W, T64, T128, T256, T_COUNT };
+enum { T16 = 0, T32, T16W, T32W, T64, T128, T256, T16N, T32N, T32H, T_COUNT };  // the last three: not gated
 struct Shape {
   int bm, bn, kg, threads;
 };
 constexpr Shape SHAPES[T_COUNT] = {{16, 64, 4, 512},  {32, 64, 4, 512},   {16, 128, 2, 512}, {32, 128, 2, 512},
-                                   {64, 128, 2, 768}, {128, 128, 1, 512}, {256, 256, 1, 256}};
+                                   {64, 128, 2, 768}, {128, 128, 1, 512}, {256, 256, 1, 256}, {16, 16, 4, 512},
+                                   {32, 16, 4, 512},  {32, 32, 4, 512}};
 struct Plan {
   int tile, ns;
   double us;
@@ -784,10 +802,11 @@ inline int64_t tiles_of(int t, bool dual, int64_t M, int64_t N) {
 // conversions (48 x 11008 x 1280 14.1 instead of 9.3, 64 x 14336 x 4096 37.7 instead of 27.1).
 constexpr bool is_wide(bool dual, int64_t M) { return dual && M <= 32; }
 
-// The cheapest (tile, split) by a model of the time in us: a launch, the operands from memory, the rounds of 256 workgroups times their
-// k steps (dearer the more CUs share L2) with a ramp for each after the first, and for a split the exchange. The coefficients are a
-// fit to the times of all tiles and splits at 323 products of M 1-4096, N 300-22016, K 512-14336; by it a call takes 0.5% longer
-// than with the best of them on average, 17% at worst. max_ns 1: no split.
+// The cheapest (tile, split) by a model of the time in us: a launch, the operands from memory, the rounds of 256 workgroups
+// times their k steps (dearer the more CUs share L2) with a ramp for each after the first, and for a split the exchange. The coefficients are a
+// fit to the times of all tiles and splits at 459 products of M 1-4096, N 100-22016, K 512-14336; by it, 1,231 other products of
+// M 1-2048, N 32-20000, K 128-16352 take 0.7% longer than with the best of them on average, 36% at worst (without narrow tiles 17%
+// longer). max_ns 1: no split.
 inline double price(bool dual, int t, int ns, int64_t M, int64_t N, int64_t K) {
   struct Cost {
     double a, b0, b1, r;  // launch; per k step alone; more per k step with every CU at work; a further round
@@ -796,7 +815,8 @@ inline double price(bool dual, int t, int ns, int64_t M, int64_t N, int64_t K) {
                                           {4.366, 0.219, 0.000, 3.73}};  // of 91 products, gated, M 1-64
   static constexpr Cost COST[T_COUNT] = {{3.685, 0.082, 0.023, 2.64}, {3.984, 0.096, 0.024, 3.09}, {3.510, 0.152, 0.036, 2.65},
                                          {3.852, 0.166, 0.043, 3.03}, {4.715, 0.187, 0.096, 3.50}, {4.823, 0.252, 0.170, 3.86},
-                                         {8.409, 0.832, 0.449, 8.24}};
+                                         {8.409, 0.832, 0.449, 8.24}, {3.049, 0.043, 0.000, 1.59}, {3.308, 0.052, 0.000, 1.93},
+                                         {3.434, 0.066, 0.000, 2.47}};
   const bool wide = is_wide(dual, M);
   const Cost& c = wide ? WIDE_COST[t] : COST[t];
   const Shape s = SHAPES[t];
@@ -811,7 +831,7 @@ inline double price(bool dual, int t, int ns, int64_t M, int64_t N, int64_t K) {
 inline Plan choose(bool dual, int64_t M, int64_t N, int64_t K, int max_ns) {
   const int64_t kt = (K + 127) / 128;
   Plan best{T256, 1, 1e300};
-  for (int t = 0; t < (is_wide(dual, M) ? T64 : T_COUNT); ++t) {
+  for (int t = 0; t < (is_wide(dual, M) ? T64 : dual ? T16N : T_COUNT); ++t) {
     const Shape s = SHAPES[t];
     const int64_t tiles = tiles_of(t, dual, M, N);
     for (int ns = 1; ns <= (t == T256 ? 1 : max_ns); ++ns) {
@@ -874,12 +894,16 @@ void run_part(const Args& a, Plan p, hipStream_t s) {
     case T128: go(Tile<128, 128, 4, 1, 4, OUT>{}); break;
     case T256: gemm_mx8_256<OUT><<<wg, P_T, 0, s>>>(a); break;
     default:
-      if constexpr (DUAL)
-        if (is_wide(DUAL, a.M)) {
-          ring(std::true_type{});
-          break;
+      if constexpr (DUAL) {
+        is_wide(DUAL, a.M) ? ring(std::true_type{}) : ring(std::false_type{});
+      } else {
+        switch (p.tile) {
+          case T16N: go(Tile<16, 16, 1, 4, 4, OUT>{}); break;
+          case T32N: go(Tile<32, 16, 2, 4, 4, OUT>{}); break;
+          case T32H: go(Tile<32, 32, 2, 4, 4, OUT>{}); break;
+          default: ring(std::false_type{});
         }
-      ring(std::false_type{});
+      }
   }
 }
 
