@@ -375,8 +375,9 @@ __global__ __launch_bounds__(P_T, 1) void gemm_mx8_256(Args a) {
 //
 // Narrow tiles, of 16 or 32 columns, give few rows' products a workgroup per CU without a split, with 512 neighbouring bytes
 // of a row in a load: 16 x 4096 x 14336 11.6 instead of 13.1 (64 columns, two workgroups on a tile's K), 1 x 4096 x 11008 10.3
-// instead of 12.2, 16 x 8192 x 14336 22.9 instead of 24.5. There a wave has NF = 1 or 2 operands of W, row NF i + f in slot
-// 16 f + i.
+// instead of 12.2, 16 x 8192 x 14336 22.9 instead of 24.5; weights that the 256 MB cache no longer holds, 1 x 4096 x 4096 6.1
+// instead of 8.2, 1 x 4096 x 11008 14.2 instead of 14.4, 16 x 4096 x 14336 17.2 where the best split takes 16.6. Up to 7 stages are
+// no faster there. A wave has NF = 1 or 2 operands of W, row NF i + f in slot 16 f + i.
 //
 // WIDE: the operands are widened to bf16, exactly, and multiplied by v_mfma_f32_16x16x32_bf16, whose sums are those of fp32. What
 // the 8-bit instruction cuts off does not show in 16 bits, but sends 1 in 2,500 of a gated product's values to the other side
