@@ -818,7 +818,7 @@ inline double price(bool dual, int t, int ns, int64_t M, int64_t N, int64_t K) {
                                          {3.852, 0.166, 0.043, 3.03}, {4.715, 0.187, 0.096, 3.50}, {4.823, 0.252, 0.170, 3.86},
                                          {8.409, 0.832, 0.449, 8.24}, {3.049, 0.043, 0.000, 1.59}, {3.308, 0.052, 0.000, 1.93},
                                          {3.434, 0.066, 0.000, 2.47}};
-  const bool wide = is_wide(dual, M);
+  const bool wide = t < T64 && is_wide(dual, M);  // larger tiles have no such form
   const Cost& c = wide ? WIDE_COST[t] : COST[t];
   const Shape s = SHAPES[t];
   const int64_t wg = tiles_of(t, dual, M, N) * ns, kt = (K + 127) / 128;
@@ -849,12 +849,14 @@ inline Plan choose(bool dual, int64_t M, int64_t N, int64_t K, int max_ns) {
 
 // 256 x 256 tiles in whole rounds of the CUs, the rest of the rows or columns by what is cheapest for it, where the model says that
 // this saves 3%: a last round of a few tiles takes as long as a full one. (4096 x 4352 x 4096
-// 79 instead of 91 us, 4400 x 4096 x 4096 68 instead of 90, 2000 x 9000 x 4096 71 instead of 96.)
+// 79 instead of 91 us, 4400 x 4096 x 4096 68 instead of 90, 2000 x 9000 x 4096 71 instead of 96.) Not of products that widen
+// their operands, which 256 x 256 tiles do not.
 struct Cut {
   int64_t rows, cols;  // of the first part; 0: no cut
 };
 inline Cut cut_of(bool dual, int64_t M, int64_t N, int64_t K, const Plan& whole) {
   Cut best{0, 0};
+  if (is_wide(dual, M)) return best;
   const int64_t tm = (M + 255) / 256, bn = cols_of(T256, dual), tn = (N + bn - 1) / bn, full = tm * tn / 256 * 256;
   if (full == 0 || full == tm * tn) return best;
   double least = 0.97 * whole.us;
