@@ -800,7 +800,8 @@ inline int64_t tiles_of(int t, bool dual, int64_t M, int64_t N) {
 
 // Whether a call multiplies widened operands: gated products of few rows, which wait for memory (16 x 4096 x 14336 25.2 instead of
 // 24.7 us, 32 x 14336 x 4096 26.8 instead of 27.8, 32 x 4096 x 4096 9.7 instead of 9.0). From 33 rows on they would wait for the
-// conversions (48 x 11008 x 1280 14.1 instead of 9.3, 64 x 14336 x 4096 37.7 instead of 27.1).
+// conversions (48 x 11008 x 1280 14.1 instead of 9.3, 64 x 14336 x 4096 37.7 instead of 27.1). It is the call's rows that count, so
+// that its parts (Cut, below) are summed alike.
 constexpr bool is_wide(bool dual, int64_t M) { return dual && M <= 32; }
 
 // The cheapest (tile, split) by a model of the time in us: a launch, the operands from memory, the rounds of 256 workgroups
@@ -808,7 +809,7 @@ constexpr bool is_wide(bool dual, int64_t M) { return dual && M <= 32; }
 // fit to the times of all tiles and splits at 459 products of M 1-4096, N 100-22016, K 512-14336; by it, 1,231 other products of
 // M 1-2048, N 32-20000, K 128-16352 take 0.7% longer than with the best of them on average, 36% at worst (without narrow tiles 17%
 // longer). max_ns 1: no split.
-inline double price(bool dual, int t, int ns, int64_t M, int64_t N, int64_t K) {
+inline double price(bool dual, bool wide, int t, int ns, int64_t M, int64_t N, int64_t K) {
   struct Cost {
     double a, b0, b1, r;  // launch; per k step alone; more per k step with every CU at work; a further round
   };
@@ -818,8 +819,7 @@ inline double price(bool dual, int t, int ns, int64_t M, int64_t N, int64_t K) {
                                          {3.852, 0.166, 0.043, 3.03}, {4.715, 0.187, 0.096, 3.50}, {4.823, 0.252, 0.170, 3.86},
                                          {8.409, 0.832, 0.449, 8.24}, {3.049, 0.043, 0.000, 1.59}, {3.308, 0.052, 0.000, 1.93},
                                          {3.434, 0.066, 0.000, 2.47}};
-  const bool wide = t < T64 && is_wide(dual, M);  // larger tiles have no such form
-  const Cost& c = wide ? WIDE_COST[t] : COST[t];
+  const Cost& c = wide && t < T64 ? WIDE_COST[t] : COST[t];  // larger tiles have no such form
   const Shape s = SHAPES[t];
   const int64_t wg = tiles_of(t, dual, M, N) * ns, kt = (K + 127) / 128;
   const int64_t steps = ((kt + ns - 1) / ns + s.kg - 1) / s.kg * s.kg;
@@ -829,10 +829,10 @@ inline double price(bool dual, int t, int ns, int64_t M, int64_t N, int64_t K) {
   if (ns > 1) us += 0.78 + 0.36 * ns + 1.29 * s.bm * s.bn / 4096.0 * std::min(1.0, (double)wg / 256.0);
   return us;
 }
-inline Plan choose(bool dual, int64_t M, int64_t N, int64_t K, int max_ns) {
+inline Plan choose(bool dual, bool wide, int64_t M, int64_t N, int64_t K, int max_ns) {
   const int64_t kt = (K + 127) / 128;
   Plan best{T256, 1, 1e300};
-  for (int t = 0; t < (is_wide(dual, M) ? T64 : dual ? T16N : T_COUNT); ++t) {
+  for (int t = 0; t < (wide ? T64 : dual ? T16N : T_COUNT); ++t) {
     const Shape s = SHAPES[t];
     const int64_t tiles = tiles_of(t, dual, M, N);
     for (int ns = 1; ns <= (t == T256 ? 1 : max_ns); ++ns) {
@@ -840,7 +840,7 @@ inline Plan choose(bool dual, int64_t M, int64_t N, int64_t K, int max_ns) {
       if (wg * s.threads > UINT32_MAX) break;  // a launch counts its threads in 32 bits
       if (ns > 1 && (tiles > TLM_SPLIT_TILES || kt < 2 * ns || (size_t)wg * s.bm * s.bn * 4 > tlm_split_bytes(false)))
         break;
-      const double us = price(dual, t, ns, M, N, K);
+      const double us = price(dual, wide, t, ns, M, N, K);
       if (us < best.us) best = Plan{t, ns, us};
     }
   }
@@ -854,16 +854,16 @@ inline Plan choose(bool dual, int64_t M, int64_t N, int64_t K, int max_ns) {
 struct Cut {
   int64_t rows, cols;  // of the first part; 0: no cut
 };
-inline Cut cut_of(bool dual, int64_t M, int64_t N, int64_t K, const Plan& whole) {
+inline Cut cut_of(bool dual, bool wide, int64_t M, int64_t N, int64_t K, const Plan& whole) {
   Cut best{0, 0};
-  if (is_wide(dual, M)) return best;
+  if (wide) return best;
   const int64_t tm = (M + 255) / 256, bn = cols_of(T256, dual), tn = (N + bn - 1) / bn, full = tm * tn / 256 * 256;
   if (full == 0 || full == tm * tn) return best;
   double least = 0.97 * whole.us;
   auto consider = [&](int64_t rows, int64_t cols) {
     if (rows <= 0 || cols <= 0 || rows > M || cols > N) return;
-    const double us = price(dual, T256, 1, rows, cols, K) +
-                      (rows < M ? choose(dual, M - rows, N, K, 16) : choose(dual, M, N - cols, K, 16)).us;
+    const double us = price(dual, false, T256, 1, rows, cols, K) +
+                      (rows < M ? choose(dual, false, M - rows, N, K, 16) : choose(dual, false, M, N - cols, K, 16)).us;
     if (us < least) least = us, best = Cut{rows, cols};
   };
   consider(M, full / tm * bn);
@@ -872,19 +872,19 @@ inline Cut cut_of(bool dual, int64_t M, int64_t N, int64_t K, const Plan& whole)
 }
 
 template <int OUT>
-void run_part(const Args& a, Plan p, hipStream_t s) {
+void run_part(const Args& a, bool wide, Plan p, hipStream_t s) {
   constexpr bool DUAL = OUT == TLM_F8E4M3;
   float* part = nullptr;
   unsigned* arrivals = nullptr;
-  if (p.ns > 1 && !gt::split_workspace(false, s, false, &part, &arrivals)) p = choose(DUAL, a.M, a.N, a.K, 1);
+  if (p.ns > 1 && !gt::split_workspace(false, s, false, &part, &arrivals)) p = choose(DUAL, wide, a.M, a.N, a.K, 1);
   const unsigned wg = (unsigned)(tiles_of(p.tile, DUAL, a.M, a.N) * p.ns);
   auto go = [&](auto tile) {
     using T = decltype(tile);
     static_assert(T::THREADS == 512 || T::BM == 64, "SHAPES");
     gemm_mx8_tile<T><<<wg, T::THREADS, 0, s>>>(a, p.ns, part, arrivals);
   };
-  auto ring = [&](auto wide) {
-    constexpr bool W = decltype(wide)::value;
+  auto ring = [&](auto w) {
+    constexpr bool W = decltype(w)::value;
     switch (p.tile) {
       case T16: return go(Tile<16, 64, 1, 4, 3, OUT, W>{});
       case T32: return go(Tile<32, 64, 2, 4, 3, OUT, W>{});
@@ -898,7 +898,7 @@ void run_part(const Args& a, Plan p, hipStream_t s) {
     case T256: gemm_mx8_256<OUT><<<wg, P_T, 0, s>>>(a); break;
     default:
       if constexpr (DUAL) {
-        is_wide(DUAL, a.M) ? ring(std::true_type{}) : ring(std::false_type{});
+        wide ? ring(std::true_type{}) : ring(std::false_type{});
       } else {
         switch (p.tile) {
           case T16N: go(Tile<16, 16, 1, 4, 4, OUT>{}); break;
@@ -913,10 +913,11 @@ void run_part(const Args& a, Plan p, hipStream_t s) {
 template <int OUT>
 int run(const Args& a, hipStream_t s) {
   constexpr bool DUAL = OUT == TLM_F8E4M3;
-  const Plan p = choose(DUAL, a.M, a.N, a.K, 16);
-  const Cut cut = cut_of(DUAL, a.M, a.N, a.K, p);
+  const bool wide = is_wide(DUAL, a.M);
+  const Plan p = choose(DUAL, wide, a.M, a.N, a.K, 16);
+  const Cut cut = cut_of(DUAL, wide, a.M, a.N, a.K, p);
   if (cut.rows == 0) {
-    run_part<OUT>(a, p, s);
+    run_part<OUT>(a, wide, p, s);
     return TLM_OK;
   }
   Args first = a, rest = a;
@@ -938,8 +939,8 @@ int run(const Args& a, hipStream_t s) {
     rest.c = (uint8_t*)a.c + cut.cols * (DUAL ? 1 : 2);
     if (DUAL) rest.c_scales += cut.cols / 128 * 256;
   }
-  run_part<OUT>(first, Plan{T256, 1, 0}, s);
-  run_part<OUT>(rest, choose(DUAL, rest.M, rest.N, a.K, 16), s);
+  run_part<OUT>(first, false, Plan{T256, 1, 0}, s);
+  run_part<OUT>(rest, false, choose(DUAL, false, rest.M, rest.N, a.K, 16), s);
   return TLM_OK;
 }
 
@@ -962,8 +963,9 @@ extern "C" int tlm_gemm_mx8_plan(int64_t M, int64_t N, int64_t K, int gated, int
     return TLM_EINVAL;
   }
   if (int rc = check_sizes("tlm_gemm_mx8_plan", M, N, K)) return rc;
-  const Plan p = choose(gated != 0, M, N, K, split ? 16 : 1);
-  const Cut cut = cut_of(gated != 0, M, N, K, p);
+  const bool dual = gated != 0, wide = is_wide(dual, M);
+  const Plan p = choose(dual, wide, M, N, K, split ? 16 : 1);
+  const Cut cut = cut_of(dual, wide, M, N, K, p);
   const Shape t = SHAPES[cut.rows ? T256 : p.tile];
   *rows = t.bm, *cols = t.bn, *ns = cut.rows ? 1 : p.ns;
   *first_rows = cut.rows ? cut.rows : M, *first_cols = cut.rows ? cut.cols : N;
