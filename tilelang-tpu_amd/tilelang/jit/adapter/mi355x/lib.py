@@ -90,9 +90,11 @@ _SIGNATURES = {
     "tlm_mx8_quant": ([c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int64, c_int64, c_void_p], c_int),
     "tlm_add_rmsnorm": ([c_void_p] * 7 + [c_int64] * 2 + [c_float, c_int, c_int, c_void_p], c_int),
     "tlm_gemm_mx8": ([c_void_p] * 5 + [c_int64] * 3 + [c_int, c_void_p], c_int),
+    "tlm_gemm_mx8_ex": ([c_void_p] * 5 + [c_int64] * 3 + [c_int] * 2 + [c_void_p], c_int),
     "tlm_gemm_mx8_plan": ([c_int64] * 3 + [c_int] * 2 + [ctypes.POINTER(c_int)] * 3 +
                           [ctypes.POINTER(c_int64)] * 2, c_int),
     "tlm_gemm_mx8_swiglu": ([c_void_p] * 8 + [c_int64] * 3 + [c_void_p], c_int),
+    "tlm_gemm_mx8_swiglu_ex": ([c_void_p] * 8 + [c_int64] * 3 + [c_int, c_void_p], c_int),
 }
 
 EXPORTED = tuple(_SIGNATURES)
