@@ -1,4 +1,6 @@
 """The tiles that 8-bit products take, without a GPU: what tlm_gemm_mx8_plan answers."""
+import ctypes
+
 import pytest
 
 from test_mx8_oracle import EINVAL, EUNSUPPORTED, _refused, plan
@@ -67,3 +69,13 @@ def test_fp32_sums_refusals():
     _refused("tlm_gemm_mx8_ex", P, P, P, P, P, 4, 8, 64, lib.F32, 1, None, code=EUNSUPPORTED)
     _refused("tlm_gemm_mx8_swiglu_ex", P, P, P, P, P, P, P, P, 4, 48, 64, 1, None, code=EUNSUPPORTED)
     _refused("tlm_gemm_mx8_swiglu_ex", P, None, P, P, P, P, P, P, 4, 64, 64, 1, None, code=EINVAL)
+
+
+def test_plan_refuses_k_that_products_refuse():
+    one, two = ctypes.c_int(), ctypes.c_int64()
+    out = [ctypes.byref(one)] * 3 + [ctypes.byref(two)] * 2
+    f = lib.load().tlm_gemm_mx8_plan
+    for K in (2 ** 22 + 32, 2 ** 62, 2 ** 63 - 1):
+        for flags in range(4):
+            assert f(16, 4096, K, flags, 1, *out) == EINVAL
+    assert f(16, 4096, 2 ** 22, 0, 1, *out) == 0

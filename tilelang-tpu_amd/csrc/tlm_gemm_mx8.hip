@@ -1005,8 +1005,8 @@ int gated_product(const char* fn, const void* a, const void* a_scales, const voi
 
 extern "C" int tlm_gemm_mx8_plan(int64_t M, int64_t N, int64_t K, int gated, int split, int* rows, int* cols, int* ns,
                                  int64_t* first_rows, int64_t* first_cols) {
-  if (M <= 0 || N <= 0 || K < 0 || !rows || !cols || !ns || !first_rows || !first_cols) {
-    tlm_set_error("tlm_gemm_mx8_plan: bad sizes or null pointer");
+  if (M <= 0 || N <= 0 || K < 0 || K > mx8::MAX_K || !rows || !cols || !ns || !first_rows || !first_cols) {
+    tlm_set_error("tlm_gemm_mx8_plan: bad sizes (K up to 2^22) or null pointer");
     return TLM_EINVAL;
   }
   const bool dual = gated & 1, fp32_sums = gated & 2;

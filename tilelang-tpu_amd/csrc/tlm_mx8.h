@@ -9,7 +9,8 @@
 
 namespace mx8 {
 
-constexpr int BLOCK = 32;  // values per scale
+constexpr int BLOCK = 32;       // values per scale
+constexpr int MAX_K = 1 << 22;  // values per row
 
 // Byte offset of the scale of row r, block b. kt: k steps of 128, ceil(K / 128).
 TLM_DEV int64_t scale_at(int64_t r, int b, int kt) {
@@ -43,7 +44,7 @@ TLM_DEV uint32_t quad_max(uint32_t m) {
 
 // Checks codes [rows, K] and their scales; 0 or a status with the message set.
 inline int check(const char* fn, const char* name, const void* codes, const void* scales, int64_t rows, int64_t K) {
-  if (rows < 0 || K < 0 || rows > INT32_MAX - 255 || K > (1 << 22)) {
+  if (rows < 0 || K < 0 || rows > INT32_MAX - 255 || K > MAX_K) {
     tlm_set_error("%s: bad sizes of %s (rows below 2^31 - 255, up to 2^22 columns)", fn, name);
     return TLM_EINVAL;
   }
