@@ -517,8 +517,8 @@ int tlm_mx8_quant(const void* x, int64_t x_stride, int x_dtype, void* codes, voi
  * of that, as stored, residual_out * rsqrt(mean(residual_out^2) + eps) * w, in fp32, rounded once to x_dtype (y), to 8 bits
  * (codes and scales), or to both. x, residual, residual_out, y [rows, cols] dense, w [cols] of x_dtype (F16 | BF16), all
  * 16-byte aligned. residual and residual_out NULL: the norm of x; residual_out may be residual; w NULL: no weight; y NULL or codes
- * and scales NULL: not wanted. cols a multiple of 8 (of 32 with codes), up to 32768. The sum of squares and
- * residual_out * w are held in fp32: beyond 2^128 they are infinite. */
+ * and scales NULL: not wanted. cols a multiple of 8 (of 32 with codes), up to 32768. residual_out * w is
+ * held in fp32: beyond 2^128 it is infinite, but for rows whose mean square is, which are scaled first. A row of zeros with eps 0 is NaN. */
 int tlm_add_rmsnorm(const void* x, const void* residual, const void* w, void* residual_out, void* y, void* codes,
                     void* scales, int64_t rows, int64_t cols, float eps, int x_dtype, int residual_dtype,
                     void* stream);

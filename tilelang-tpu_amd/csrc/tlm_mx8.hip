@@ -94,7 +94,6 @@ __global__ __launch_bounds__(T) void add_rmsnorm_kernel(Norm a) {
   if (row >= a.rows) return;
   float h[V][8];
   u32x4 w[V];  // asked for with the row, not after its sum
-  float ss = 0.f;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int c = 8 * (i * T + (int)threadIdx.x);
@@ -114,19 +113,37 @@ __global__ __launch_bounds__(T) void add_rmsnorm_kernel(Norm a) {
       }
       store8<R, true>(a.residual_out, at + c, h[i]);
     }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) ss = fmaf(h[i][j], h[i][j], ss);
   }
-  ss = wave_sum(ss);
-  if constexpr (T > 64) {
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = ss;
-    __syncthreads();
-    ss = 0.f;
+  auto squares = [&]() __attribute__((always_inline)) {  // the row's sum of them, the same bits in all its threads
+    float ss = 0.f;
 #pragma unroll
-    for (int i = 0; i < T / 64; ++i) ss += part[i];
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) ss = fmaf(h[i][j], h[i][j], ss);
+    ss = wave_sum(ss);
+    if constexpr (T > 64) {
+      if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = ss;
+      __syncthreads();
+      ss = 0.f;
+#pragma unroll
+      for (int i = 0; i < T / 64; ++i) ss += part[i];
+    }
+    return ss;
+  };
+  float m = squares() * a.inv_cols + a.eps;
+  // Rows whose mean square is no normal number of fp32 are scaled by a power of two, eps with them: up from below 2^-126, all of which
+  // the root would take for 0, or down from 2^128 on, where what falls below 2^-118 of the root loses bits.
+  if (m < 0x1p-126f || m == INFINITY) {
+    const float f = m < 1.f ? 0x1p96f : 0x1p-72f;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) h[i][j] *= f;
+    __syncthreads();  // `part` has been read
+    m = squares() * a.inv_cols + a.eps * f * f;
   }
   // one Newton step makes r exact to its last place; of 16-bit streams h w is exact, so that the result is rounded once
-  const float m = ss * a.inv_cols + a.eps, r0 = __frsqrt_rn(m);
+  const float r0 = __frsqrt_rn(m);
   const float r = m < INFINITY && r0 < INFINITY ? fmaf(0.5f * r0, fmaf(-m * r0, r0, 1.f), r0) : r0;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
