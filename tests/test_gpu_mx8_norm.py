@@ -1,12 +1,11 @@
-"""tlm_add_rmsnorm on the GPU at the ends of fp32's range. Tolerances are those of test_gpu_mx8.py."""
+"""tlm_add_rmsnorm and tlm_mx8_quant on the GPU at the ends of what they take. Tolerances are those of test_gpu_mx8.py."""
 import numpy as np
 import pytest
 import torch
 
-from test_gpu_mx8 import BF16, DEV, F32, _empty, _norm_case
 from oracle import ref
-from test_gpu_mx8 import _bytes
-from tilelang.jit.adapter.mi355x import ops
+from test_gpu_mx8 import BF16, DEV, F32, _bytes, _empty, _norm_case
+from tilelang.jit.adapter.mi355x import lib, ops
 
 pytestmark = pytest.mark.gpu
 
@@ -48,3 +47,21 @@ def test_rows_without_a_mean():
     byte = ref.mx8_untile_ref(_bytes(scales), *x.shape)
     assert byte[0, 0] == 255 and (byte[0, 1:] == 1).all() and (byte[1:3] == 255).all() and (byte[3] < 255).all()
     assert np.array_equal(np.unique(_bytes(codes)[:3] & 127), [0])
+
+
+@pytest.mark.parametrize("dtype", [BF16, torch.float16, F32])
+def test_quant_strides(dtype):
+    """Rows a multiple of 8 elements apart, 0 among them, in any 16 bytes of a buffer; what its docstring excludes is refused."""
+    x = torch.randn(6, 96 + 1001, generator=torch.Generator().manual_seed(2)).to(dtype).to(DEV)
+    flat = x.flatten()
+    for stride, at in ((0, 0), (8, 8), (96, 16), (104, 8), (1000, 24)):
+        rows = flat.as_strided((5, 96), (stride, 1), at)
+        codes, scales = ops.mx8_quant(rows, *_empty(5, 96))
+        want, byte = ref.mx8_quantise_ref(rows.cpu())
+        assert np.array_equal(_bytes(codes), want)
+        assert np.array_equal(ref.mx8_untile_ref(_bytes(scales), 5, 96), byte)
+    for stride, at in ((97, 0), (100, 0), (96, 1)):
+        with pytest.raises(lib.TLMError, match="multiple of 8"):
+            ops.mx8_quant(flat.as_strided((5, 96), (stride, 1), at), *_empty(5, 96))
+    # a single row has no stride
+    ops.mx8_quant(flat.as_strided((1, 96), (97, 1), 0), *_empty(1, 96))

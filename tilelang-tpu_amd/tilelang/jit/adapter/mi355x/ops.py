@@ -671,9 +671,9 @@ def _mx8(name: str, codes: torch.Tensor, scales: torch.Tensor, rows: int, K: int
 
 
 def mx8_quant(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor):
-    """Quantise rows x [rows, K] (fp16/bf16/fp32, any row stride) to 8 bits: codes float8_e4m3fn
-    [rows, K] and one power-of-two scale per 32 values, scales float8_e8m0fnu of mx8_scales_shape(rows, K).
-    Returns codes, scales."""
+    """Quantise rows x [rows, K] (fp16/bf16/fp32, 16-byte aligned, a multiple of 8 elements apart) to 8 bits:
+    codes float8_e4m3fn [rows, K] and one power-of-two scale per 32 values, scales float8_e8m0fnu of
+    mx8_scales_shape(rows, K). Returns codes, scales."""
     if x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1):
         raise ValueError("x must be [rows, K] with contiguous rows")
     rows, K = x.shape
