@@ -79,3 +79,16 @@ def test_plan_refuses_k_that_products_refuse():
         for flags in range(4):
             assert f(16, 4096, K, flags, 1, *out) == EINVAL
     assert f(16, 4096, 2 ** 22, 0, 1, *out) == 0
+
+
+# products whose workgroups share K: (M, N, K, tlm_gemm_mx8_plan's `gated`)
+SPLITS = [(3, 100, 14336, 0), (17, 2563, 14336, 0), (257, 1000, 14336, 0), (100, 9000, 8192, 0), (33, 992, 14336, 1),
+          (257, 992, 8192, 1), (1100, 512, 8192, 1), (17, 1600, 8192, 1), (30, 5024, 14336, 1), (50, 1601, 8192, 2),
+          (130, 992, 14336, 3)]
+
+
+def test_splits_are_split():
+    """What the tests of shared workspaces run uses them."""
+    for case in SPLITS:
+        assert plan(*case)[2] > 1 and plan(*case)[3:] == case[:2], case
+        assert plan(*case, False)[2] == 1
