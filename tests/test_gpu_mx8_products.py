@@ -8,9 +8,9 @@ import numpy as np
 import pytest
 import torch
 
-from test_mx8_oracle import PLANS, plan
-from test_mx8_plans import FP32_PLANS, FP32_SUMS, SPLITS
-from test_gpu_mx8 import ARITH, BF16, DEV, E4M3, E8M0, F16, _check_mx, _check_unused, _device_values, _empty
+from test_mx8_oracle import CUTS, GATED_CUTS, GATED_PLANS, PLANS, plan
+from test_mx8_plans import FP32_PLANS, FP32_SUMS, MORE_GATED_PLANS, MORE_PLANS, SPLITS
+from test_gpu_mx8 import ARITH, BF16, DEV, E4M3, E8M0, F16, SUM, _check_mx, _check_unused, _device_values, _empty
 from tilelang.jit.adapter.mi355x import ops
 
 pytestmark = pytest.mark.gpu
@@ -157,7 +157,7 @@ def _powers(m):
     return torch.exp2(field - 7) * scale
 
 
-@pytest.mark.parametrize("case", PLANS)
+@pytest.mark.parametrize("case", PLANS + MORE_PLANS)
 def test_bound_of_the_core(case):
     """The 8-bit instruction's sums: each product is cut below 2^-13 of the largest power of its eight neighbours, towards
     zero, and fp32 rounds once for every eight k and 40 times behind them."""
@@ -265,3 +265,69 @@ def test_splits_on_six_streams():
     # The others ran unsplit: sums of fp32 in another order round otherwise somewhere. (Of the 8-bit instruction's sums few do: what it
     # leaves of eight products is a multiple of 2^-13 of the largest, 2^11 of fp32's steps and more, so most sums are exact.)
     assert SPLITS[-2] == (50, 1601, 8192, 2) and said["WHOLE"].count("False]") == 2, r.stdout
+
+
+# every tile, whole and split, and every cut: (M, N, K, tlm_gemm_mx8_plan's `gated`)
+EVERY = [(*c[:3], 0) for c in PLANS + MORE_PLANS + CUTS] + [(*c[:3], 1) for c in GATED_PLANS + MORE_GATED_PLANS + GATED_CUTS]
+
+
+def _products(a, b, up):
+    """want = a @ b.T, the sum of its magnitudes, and the same of up, in float64."""
+    x, v, u = (_device_values(m) for m in (a, b, up))
+    v, u = v.T.contiguous(), u.T.contiguous()
+    return x @ v, x.abs() @ v.abs(), x @ u, x.abs() @ u.abs()
+
+
+@pytest.mark.parametrize("case", EVERY)
+def test_every_tile_random(case):
+    """Operands of any value over the whole of K."""
+    M, N, K, gated = case
+    g = torch.Generator(device=DEV).manual_seed(M * 3 + N + K)
+    a, b, up = _rows(M, K, g), _rows(N, K, g, K ** -0.5), _rows(N, K, g, K ** -0.5)
+    if gated:
+        codes, scales = _empty(M, N)
+        ops.gemm_mx8_swiglu(*a, *b, *up, codes, scales)
+        want, move = _gated(a, b, up)
+        _check_mx(codes, scales, want, SUM * 2 * move + ARITH * np.abs(want) + 2.0 ** -126)
+        _check_unused(scales, M, N)
+        return
+    x, y = _device_values(a), _device_values(b).T.contiguous()
+    want, mag = x @ y, x.abs() @ y.abs()
+    for dtype in (BF16, F16):
+        c = torch.full((M, N), 7.0, dtype=dtype, device=DEV)
+        ops.gemm_mx8(*a, *b, c)
+        h, tiny = torch.finfo(dtype).eps / 2, 2.0 ** -25 if dtype is F16 else 0
+        assert bool(((c.double() - want).abs() <= h * want.abs() + (1 + h) * SUM * mag + tiny).all())
+
+
+def _sparse(rows, K, at, g):
+    """Whole numbers -4 .. 4 at the places `at` of every row, zeros elsewhere; scales 1/2, 1 and 2."""
+    v = torch.zeros(rows, K, device=DEV)
+    v[:, at] = torch.randint(-4, 5, (rows, len(at)), generator=g, device=DEV).float()
+    s = torch.randint(126, 129, ops.mx8_scales_shape(rows, K), generator=g, device=DEV, dtype=torch.int32)
+    return v.to(E4M3), s.to(torch.uint8).view(E8M0)
+
+
+@pytest.mark.parametrize("case", EVERY)
+def test_every_tile_exact_over_k(case):
+    """Sums of whole numbers that lie all over K, in every stage and split: exact, whatever their order."""
+    M, N, K, gated = case
+    g = torch.Generator(device=DEV).manual_seed(M + N * 3 + K)
+    at = torch.randperm(K, generator=g, device=DEV)[:500]
+    at[0] = K - 1
+    a, b, up = (_sparse(r, K, at, g) for r in (M, N, N))
+    if gated:
+        for m in (b, up):  # gates of a few units
+            m[1].view(torch.uint8).sub_(4)
+    x, v, u = (_device_values(m) for m in (a, b, up))
+    v, u = x @ v.T.contiguous(), x @ u.T.contiguous()
+    for _ in range(2):
+        if gated:
+            codes, scales = _empty(M, N)
+            ops.gemm_mx8_swiglu(*a, *b, *up, codes, scales)
+            want = (u * v * torch.sigmoid(v)).cpu().numpy()
+            _check_mx(codes, scales, want, ARITH * np.abs(want) + 2.0 ** -126)
+        else:
+            c = torch.full((M, N), 7.0, dtype=BF16, device=DEV)
+            ops.gemm_mx8(*a, *b, c)
+            assert torch.equal(c, v.to(BF16))

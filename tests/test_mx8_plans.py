@@ -1,9 +1,11 @@
 """The tiles that 8-bit products take, without a GPU: what tlm_gemm_mx8_plan answers."""
 import ctypes
+import math
+import random
 
 import pytest
 
-from test_mx8_oracle import EINVAL, EUNSUPPORTED, _refused, plan
+from test_mx8_oracle import EINVAL, EUNSUPPORTED, GATED_PLANS, PLANS, _refused, plan
 from tilelang.jit.adapter.mi355x import lib
 
 # gated products of few rows and more than 32768 columns, some whole rounds of 256 x 256 tiles and a rest: (M, N, K)
@@ -92,3 +94,35 @@ def test_splits_are_split():
     for case in SPLITS:
         assert plan(*case)[2] > 1 and plan(*case)[3:] == case[:2], case
         assert plan(*case, False)[2] == 1
+
+
+# what PLANS and GATED_PLANS, whose gated products of 16-row tiles have up to 32 rows, leave out: (M, N, K, rows, columns of weights,
+# whether workgroups share K), and gated
+MORE_PLANS = [(2274, 61, 15552, 32, 64, True)]
+MORE_GATED_PLANS = [(134, 64, 3712, 16, 64, False), (76, 64, 8224, 16, 64, True), (55, 2944, 352, 16, 128, False)]
+
+
+@pytest.mark.parametrize("gated,case", [(0, c) for c in MORE_PLANS] + [(1, c) for c in MORE_GATED_PLANS])
+def test_more_plans(gated, case):
+    M, N, K, rows, cols, split = case
+    got = plan(M, N, K, gated)
+    assert (*got[:2], got[2] > 1, *got[3:]) == (rows, cols, split, M, N)
+
+
+def _kernel(M, N, K, flags):
+    """What tells kernels apart: gated, widened operands, tile, split."""
+    rows, cols, ns, *_ = plan(M, N, K, flags)
+    return flags & 1, bool(flags & FP32_SUMS or (flags & GATED and M <= 32)), rows, cols, ns > 1
+
+
+def test_every_kernel_has_a_case():
+    """No size takes a kernel that no GPU test of tiles takes."""
+    tested = {_kernel(*c[:3], 0) for c in PLANS + MORE_PLANS} | {_kernel(*c[:3], 1) for c in GATED_PLANS + MORE_GATED_PLANS}
+    tested |= {_kernel(*c[:4]) for c in FP32_PLANS}
+    rng, taken = random.Random(0), {}
+    for i in range(40000):
+        M, N, K = (int(math.exp(rng.uniform(math.log(lo), math.log(hi)))) for lo, hi in ((1, 8192), (1, 2000), (1, 512)))
+        flags = i % 4
+        N = 32 * N if flags & GATED else N * 32 - rng.randrange(32)
+        taken.setdefault(_kernel(M, N, 32 * K, flags), (M, N, 32 * K, flags))
+    assert not {k: v for k, v in taken.items() if k not in tested}
