@@ -8,9 +8,10 @@ import numpy as np
 import pytest
 import torch
 
+from oracle import ref
 from test_mx8_oracle import CUTS, GATED_CUTS, GATED_PLANS, PLANS, plan
 from test_mx8_plans import FP32_PLANS, FP32_SUMS, MORE_GATED_PLANS, MORE_PLANS, SPLITS
-from test_gpu_mx8 import ARITH, BF16, DEV, E4M3, E8M0, F16, SUM, _check_mx, _check_unused, _device_values, _empty
+from test_gpu_mx8 import ARITH, BF16, DEV, E4M3, E8M0, F16, SUM, _bytes, _check_mx, _check_unused, _device_values, _empty
 from tilelang.jit.adapter.mi355x import ops
 
 pytestmark = pytest.mark.gpu
@@ -331,3 +332,52 @@ def test_every_tile_exact_over_k(case):
             c = torch.full((M, N), 7.0, dtype=BF16, device=DEV)
             ops.gemm_mx8(*a, *b, c)
             assert torch.equal(c, v.to(BF16))
+
+
+def _call(case, a, b, up):
+    """The bytes of a call's result on the host: codes and scales [M, N / 32] of a gated one."""
+    M, N, K, flags = case
+    fp32_sums = bool(flags & FP32_SUMS)
+    if not flags & 1:
+        c = torch.full((M, N), 7.0, dtype=F16, device=DEV)
+        return ops.gemm_mx8(*a, *b, c, fp32_sums=fp32_sums).cpu(), None
+    codes, scales = ops.gemm_mx8_swiglu(*a, *b, *up, *_empty(M, N), fp32_sums=fp32_sums)
+    return codes.view(torch.uint8).cpu(), torch.from_numpy(ref.mx8_untile_ref(_bytes(scales), M, N))
+
+
+@pytest.mark.parametrize("case", EVERY + [c[:4] for c in FP32_PLANS])
+def test_blocks_without_a_number(case):
+    """Rows and weights with a NaN or an infinity, as the quantiser writes their blocks (scale 255, codes 0): NaN in every result
+    they take part in, and the same bits as without them everywhere else."""
+    M, N, K, flags = case
+    g = torch.Generator(device=DEV).manual_seed(M + N + K + flags)
+
+    def rows(n, scale, bad):
+        x = scale * torch.randn(n, K, generator=g, device=DEV)
+        good = ops.mx8_quant(x, *_empty(n, K, 255))
+        for r, k, v in bad:
+            x[r, k] = v
+        return good, ops.mx8_quant(x, *_empty(n, K, 255))
+    inf, nan = float("inf"), float("nan")
+    a, a_bad = rows(M, 1.0, [(M - 1, K - 1, nan), (M // 2, K // 3, -inf)])
+    b, b_bad = rows(N, K ** -0.5, [(N - 1, 0, inf), (N // 3, K - 32, nan)])
+    up, up_bad = rows(N, K ** -0.5, [(N // 2, K // 2, nan)])
+    row, col = torch.zeros(M, 1, dtype=torch.bool), torch.zeros(1, N, dtype=torch.bool)
+    row[[M - 1, M // 2]] = True
+    col[0, [N - 1, N // 3]] = True
+    plain, scales = _call(case, a, b, up)
+    for ops_in, want in (((a_bad, b, up), row.expand(M, N)), ((a, b_bad, up), col.expand(M, N))):
+        got, byte = _call(case, *ops_in)
+        if flags & 1:  # a block of 32 columns has one scale
+            want = want.unflatten(1, (-1, 32)).any(-1)
+            assert torch.equal(byte == 255, want) and not got.unflatten(1, (-1, 32))[want].any()
+            assert torch.equal(byte[~want], scales[~want])
+            want = want.repeat_interleave(32, 1)
+        else:
+            assert torch.equal(torch.isnan(got), want)
+        assert torch.equal(got[~want], plain[~want])
+    if flags & 1:
+        got, byte = _call(case, a, b, up_bad)
+        want = torch.zeros(M, N // 32, dtype=torch.bool)
+        want[:, N // 2 // 32] = True
+        assert torch.equal(byte == 255, want) and torch.equal(byte[~want], scales[~want])
