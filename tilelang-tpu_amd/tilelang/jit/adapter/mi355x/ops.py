@@ -648,6 +648,8 @@ def mx8_scales_shape(rows: int, K: int):
 def mx8_tile_scales(scales: torch.Tensor) -> torch.Tensor:
     """Scales [rows, K / 32] (one per block, e8m0, as checkpoints hold them) in the layout of
     mx8_scales_shape; for weights, once when they are loaded."""
+    if scales.dim() != 2 or scales.element_size() != 1:
+        raise ValueError(f"scales must be bytes [rows, K / 32], got {scales.dtype} {list(scales.shape)}")
     b = scales.view(torch.uint8)
     b = torch.nn.functional.pad(b, (0, -b.shape[1] % 4, 0, -b.shape[0] % 64))
     b = b.unflatten(0, (-1, 64)).unflatten(2, (-1, 4)).permute(0, 2, 3, 1)
