@@ -525,21 +525,22 @@ int tlm_add_rmsnorm(const void* x, const void* residual, const void* w, void* re
 
 /* C = A B^T of 8-bit operands A [M, K], B [N, K]; C [M, N] of out_dtype (F16 | BF16), dense.
  *
- * How products are summed. fp32_sums 0, which is tlm_gemm_mx8: by the 8-bit matrix instructions. These cut the products of
+ * How products are summed. fp32_sums 0, as tlm_gemm_mx8 does: by the 8-bit matrix instructions. These cut the products of
  * each eight k 8 g .. 8 g + 7, towards zero, below 2^-13 of P, the largest power of two 2^(exponent of a + exponent of b) among the eight
  * (codes below the least normal one, 2^-6 of their scale, have its exponent); the rest is fp32. A sum is off by at most
  * 7 2^-13 of the sum of all P plus K / 8 roundings of fp32, and by about 4e-5 of itself where the operands are as good as random. Where
  * large products cancel, what is left may be cut off whole.
- * fp32_sums 1: in fp32 throughout (the operands are multiplied as bf16, exactly; elements that bf16 does not hold, 2^128 and more
- * or below 2^-126, may count as infinite or as 0). Slower from some dozens of rows on, by tiles of 16 and 32 rows: M N up to
- * 2^23 tiles of 32 x 128 (gated: 32 x 64). */
+ * fp32_sums 1, as tlm_gemm_mx8_swiglu does: in fp32 throughout (the operands are multiplied as bf16, exactly; elements that bf16
+ * does not hold, 2^128 and more or below 2^-126, may count as infinite or as 0). Up to two and a half times the time from some dozens of
+ * rows on; M N up to 2^23 tiles of 128 x 128 (gated: 128 x 64). */
 int tlm_gemm_mx8(const void* a, const void* a_scales, const void* b, const void* b_scales, void* c, int64_t M,
                  int64_t N, int64_t K, int out_dtype, void* stream);
 int tlm_gemm_mx8_ex(const void* a, const void* a_scales, const void* b, const void* b_scales, void* c, int64_t M,
                     int64_t N, int64_t K, int out_dtype, int fp32_sums, void* stream);
 
 /* up * gate / (1 + exp(-gate)) with gate = A gate^T, up = A up^T (weights [N, K]) in 8 bits: codes [M, N] and scales,
- * quantised from fp32. N a multiple of 32. fp32_sums as above; calls of up to 32 rows are summed in fp32 without it, too. */
+ * quantised from fp32. N a multiple of 32. Sums are those of fp32; with fp32_sums 0 (see above) calls of more than 32 rows are
+ * summed by the 8-bit instructions, which sends about 1 in 2,500 of the 8-bit results to the other neighbour. */
 int tlm_gemm_mx8_swiglu(const void* a, const void* a_scales, const void* gate, const void* gate_scales,
                         const void* up, const void* up_scales, void* codes, void* scales, int64_t M, int64_t N,
                         int64_t K, void* stream);
@@ -547,8 +548,8 @@ int tlm_gemm_mx8_swiglu_ex(const void* a, const void* a_scales, const void* gate
                            const void* up, const void* up_scales, void* codes, void* scales, int64_t M, int64_t N,
                            int64_t K, int fp32_sums, void* stream);
 
-/* The tile (rows of A, rows of weights) and the number of workgroups that share its K that tlm_gemm_mx8, or with `gated` 1
- * tlm_gemm_mx8_swiglu, takes for these sizes (`gated` 2 and 3: the same with fp32_sums), and how many rows and columns of the result they are for: all, or whole rounds of
+/* The tile (rows of A, rows of weights) and the number of workgroups that share its K that tlm_gemm_mx8_ex, or with `gated` 1
+ * tlm_gemm_mx8_swiglu_ex, takes for these sizes (with fp32_sums 0; `gated` 2 and 3: with fp32_sums 1), and how many rows and columns of the result they are for: all, or whole rounds of
  * the CUs, and another launch computes the rest. split 0: on a stream without a workspace for partial tiles. Host only. */
 int tlm_gemm_mx8_plan(int64_t M, int64_t N, int64_t K, int gated, int split, int* rows, int* cols, int* ns,
                       int64_t* first_rows, int64_t* first_cols);

@@ -30,11 +30,13 @@ FP32_PLANS = [(1, 32, 4128, 1, 16, 64, True), (5, 1600, 544, 1, 16, 64, False), 
               (5, 5024, 8192, 1, 16, 128, True), (17, 5024, 2080, 1, 32, 64, False), (17, 1600, 8192, 1, 32, 64, True),
               (30, 12000, 160, 1, 32, 128, False), (30, 5024, 14336, 1, 32, 128, True),
               (33, 32, 544, 3, 16, 64, False), (50, 96, 8192, 3, 16, 64, True), (50, 480, 96, 3, 16, 128, False),
-              (50, 2560, 2080, 3, 32, 64, False), (100, 480, 8192, 3, 32, 64, True), (33, 12000, 544, 3, 32, 128, False),
-              (130, 992, 14336, 3, 32, 128, True),
-              (1, 33, 544, 2, 16, 64, False), (1, 5003, 4128, 2, 16, 64, True), (400, 2559, 8192, 2, 16, 128, False),
-              (1, 9001, 8192, 2, 16, 128, True), (257, 993, 4128, 2, 32, 64, False), (50, 1601, 8192, 2, 32, 64, True),
-              (50, 8999, 32, 2, 32, 128, False), (32, 8999, 14336, 2, 32, 128, True)]
+              (130, 992, 4128, 3, 32, 64, False), (100, 480, 8192, 3, 32, 64, True), (100, 4096, 160, 3, 32, 128, False),
+              (130, 992, 14336, 3, 32, 128, True), (130, 4096, 544, 3, 64, 128, False), (50, 5024, 8192, 3, 64, 128, True),
+              (257, 12000, 96, 3, 128, 128, False), (100, 5024, 8192, 3, 128, 128, True),
+              (1, 33, 544, 2, 16, 64, False), (1, 5003, 4128, 2, 16, 64, True), (400, 991, 1056, 2, 16, 128, False),
+              (1, 9001, 8192, 2, 16, 128, True), (257, 1599, 2080, 2, 32, 64, False), (50, 1601, 8192, 2, 32, 64, True),
+              (50, 8999, 32, 2, 32, 128, False), (20, 8999, 14336, 2, 32, 128, True), (257, 4095, 544, 2, 64, 128, False),
+              (50, 8991, 8192, 2, 64, 128, True), (257, 8991, 160, 2, 128, 128, False), (400, 2559, 8192, 2, 128, 128, True)]
 
 
 @pytest.mark.parametrize("case", FP32_PLANS)
@@ -47,25 +49,27 @@ def test_fp32_sums_plan(case):
 
 @pytest.mark.parametrize("M", [1, 16, 17, 32, 33, 256, 4096])
 def test_fp32_sums_take_no_8_bit_tile(M):
-    """No tile of more than 32 rows, none of 16 or 32 columns, no 256 x 256 part."""
+    """No tile of 16 or 32 columns, none of 256 x 256 and no part of them."""
     for N in (32, 480, 4096, 33024):
         for K in (0, 32, 4096, 14336):
             for flags in (FP32_SUMS, FP32_SUMS | GATED):
                 rows, cols, _, *first = plan(M, N, K, flags)
-                assert rows in (16, 32) and cols in (64, 128) and first == [M, N]
+                assert rows <= 128 and cols in (64, 128) and first == [M, N]
             # gated calls of few rows take the same without being asked
             assert M > 32 or plan(M, N, K, GATED) == plan(M, N, K, GATED | FP32_SUMS)
 
 
 def test_fp32_sums_refusals():
-    """More tiles of 32 x 128 (gated 32 x 64) than a launch has."""
+    """More tiles of 128 x 128 (gated 128 x 64) than a launch has."""
     P = 1 << 20  # an address that is never read: these calls are refused first
-    big = dict(M=1 << 20, N=1 << 16, K=32)
+    big = dict(M=1 << 20, N=(1 << 17) + 32, K=32)
     _refused("tlm_gemm_mx8_ex", P, P, P, P, P, *big.values(), lib.BF16, 1, None, code=EINVAL)
     _refused("tlm_gemm_mx8_swiglu_ex", P, P, P, P, P, P, P, P, *big.values(), 1, None, code=EINVAL)
+    _refused("tlm_gemm_mx8_swiglu", P, P, P, P, P, P, P, P, *big.values(), None, code=EINVAL)
     with pytest.raises(lib.TLMError):
         plan(*big.values(), GATED | FP32_SUMS)
-    assert plan(1 << 19, 1 << 14, 32, GATED | FP32_SUMS)[0] == 32
+    assert plan(*big.values(), GATED)[0] == 256  # as 8-bit sums there is such a call
+    assert plan(1 << 20, 1 << 15, 32, GATED | FP32_SUMS)[0] == 128
     # what the plain entry points refuse, these refuse as well
     _refused("tlm_gemm_mx8_ex", P, P, P, P, P, 4, 8, 48, lib.BF16, 1, None, code=EUNSUPPORTED)
     _refused("tlm_gemm_mx8_ex", P, P, P, P, P, 4, 8, 64, lib.F32, 1, None, code=EUNSUPPORTED)

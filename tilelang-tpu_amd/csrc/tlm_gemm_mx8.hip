@@ -382,8 +382,12 @@ __global__ __launch_bounds__(P_T, 1) void gemm_mx8_256(Args a) {
 // no faster there. A wave has NF = 1 or 2 operands of W, row NF i + f in slot 16 f + i.
 //
 // WIDE: the operands are widened to bf16, exactly, and multiplied by v_mfma_f32_16x16x32_bf16, whose sums are those of fp32. What
-// the 8-bit instruction cuts off sends 1 in 2,500 of a random gated product's values to the other side of an 8-bit step, and
-// is all there is where large products cancel. Elements of 2^128 and more count as infinite there.
+// the 8-bit instruction cuts off sends 1 in 2,500 of a random gated product's values to the other side of an 8-bit step (an fp16
+// MLP ends 2e-3 from the formula instead of 2e-4), and is all there is where large products cancel. So gated products are summed
+// this way unless their caller chooses otherwise. It costs half the matrix rate and a conversion of each operand in each wave:
+// gated 64 x 2048 x 7168 12.0 us instead of 10.8, 500 x 11008 x 4096 100 instead of 51, 4096 x 11008 x 4096 720 instead of 290; conversions
+// that take turns with the matrix instructions, and those all at the start of a step, take the same time. Elements of 2^128 and
+// more count as infinite there.
 template <int BM_, int BN_, int FX_, int KG_, int NST_, int OUT_, bool WIDE_ = false>
 struct Tile {
   static constexpr int BM = BM_, BN = BN_, FX = FX_, KG = KG_, NST = NST_, OUT = OUT_;
@@ -800,11 +804,9 @@ inline int64_t tiles_of(int t, bool dual, int64_t M, int64_t N) {
   return ((M + SHAPES[t].bm - 1) / SHAPES[t].bm) * ((N + cols_of(t, dual) - 1) / cols_of(t, dual));
 }
 
-// Whether a call multiplies widened operands: where its caller asks for sums of fp32, and gated products of few rows, which wait for memory (16 x 4096 x 14336 25.2 instead of
-// 24.7 us, 32 x 14336 x 4096 26.8 instead of 27.8, 32 x 4096 x 4096 9.7 instead of 9.0). From 33 rows on they would wait for the
-// conversions (48 x 11008 x 1280 14.1 instead of 9.3, 64 x 14336 x 4096 37.7 instead of 27.1; asked for all the same: gated 64 x 2048 x 7168
-// 11.7 instead of 10.8, 500 x 4096 x 4096 26 instead of 14, 4096^3 196 instead of 53, gated 4096 x 11008 x 4096 1,090 instead of 292).
-// It is the call's rows that count, so that its parts (Cut, below) are summed alike.
+// Whether a call multiplies widened operands: where sums of fp32 are asked for, and gated products of few rows, which wait for memory
+// (16 x 4096 x 14336 25.2 instead of 24.7 us, 32 x 14336 x 4096 26.8 instead of 27.8, 32 x 4096 x 4096 9.7 instead of 9.0). It is the
+// call's rows that count, so that its parts (Cut, below) are summed alike.
 constexpr bool is_wide(bool dual, bool fp32_sums, int64_t M) { return fp32_sums || (dual && M <= 32); }
 
 // The cheapest (tile, split) by a model of the time in us: a launch, the operands from memory, the rounds of 256 workgroups
@@ -816,13 +818,14 @@ inline double price(bool dual, bool wide, int t, int ns, int64_t M, int64_t N, i
   struct Cost {
     double a, b0, b1, r;  // launch; per k step alone; more per k step with every CU at work; a further round
   };
-  static constexpr Cost WIDE_COST[T64] = {{3.914, 0.097, 0.017, 2.88}, {4.478, 0.109, 0.011, 3.55}, {3.870, 0.189, 0.013, 2.98},
-                                          {4.366, 0.219, 0.000, 3.73}};  // of 91 products, gated, M 1-64
+  // of 543 gated products of M 1-2600: 0.4% longer than with the best on average, 15% at worst
+  static constexpr Cost WIDE_COST[T256] = {{3.810, 0.110, 0.011, 2.90}, {4.248, 0.131, 0.007, 3.45}, {3.813, 0.192, 0.019, 2.99},
+                                           {4.182, 0.241, 0.023, 3.25}, {5.034, 0.391, 0.029, 4.13}, {5.583, 0.762, 0.007, 4.51}};
   static constexpr Cost COST[T_COUNT] = {{3.685, 0.082, 0.023, 2.64}, {3.984, 0.096, 0.024, 3.09}, {3.510, 0.152, 0.036, 2.65},
                                          {3.852, 0.166, 0.043, 3.03}, {4.715, 0.187, 0.096, 3.50}, {4.823, 0.252, 0.170, 3.86},
                                          {8.409, 0.832, 0.449, 8.24}, {3.049, 0.043, 0.000, 1.59}, {3.308, 0.052, 0.000, 1.93},
                                          {3.434, 0.066, 0.000, 2.47}};
-  const Cost& c = wide && t < T64 ? WIDE_COST[t] : COST[t];  // larger tiles have no such form
+  const Cost& c = wide && t < T256 ? WIDE_COST[t] : COST[t];  // 256 x 256 has no such form
   const Shape s = SHAPES[t];
   const int64_t wg = tiles_of(t, dual, M, N) * ns, kt = (K + 127) / 128;
   const int64_t steps = ((kt + ns - 1) / ns + s.kg - 1) / s.kg * s.kg;
@@ -835,7 +838,7 @@ inline double price(bool dual, bool wide, int t, int ns, int64_t M, int64_t N, i
 inline Plan choose(bool dual, bool wide, int64_t M, int64_t N, int64_t K, int max_ns) {
   const int64_t kt = (K + 127) / 128;
   Plan best{T256, 1, 1e300};
-  for (int t = 0; t < (wide ? T64 : dual ? T16N : T_COUNT); ++t) {
+  for (int t = 0; t < (wide ? T256 : dual ? T16N : T_COUNT); ++t) {
     const Shape s = SHAPES[t];
     const int64_t tiles = tiles_of(t, dual, M, N);
     for (int ns = 1; ns <= (t == T256 ? 1 : max_ns); ++ns) {
@@ -892,21 +895,19 @@ void run_part(const Args& a, bool wide, Plan p, hipStream_t s) {
       case T16: return go(Tile<16, 64, 1, 4, 3, OUT, W>{});
       case T32: return go(Tile<32, 64, 2, 4, 3, OUT, W>{});
       case T16W: return go(Tile<16, 128, 1, 2, 3, OUT, W>{});
-      default: return go(Tile<32, 128, 2, 2, 3, OUT, W>{});
+      case T32W: return go(Tile<32, 128, 2, 2, 3, OUT, W>{});
+      case T64: return go(Tile<64, 128, 2, 2, 3, OUT, W>{});
+      default: return go(Tile<128, 128, 4, 1, 4, OUT, W>{});
     }
   };
-  switch (p.tile) {
-    case T64: go(Tile<64, 128, 2, 2, 3, OUT>{}); break;
-    case T128: go(Tile<128, 128, 4, 1, 4, OUT>{}); break;
-    case T256: gemm_mx8_256<OUT><<<wg, P_T, 0, s>>>(a); break;
-    default:
-      if constexpr (!DUAL) {
-        if (p.tile == T16N) return go(Tile<16, 16, 1, 4, 4, OUT>{});
-        if (p.tile == T32N) return go(Tile<32, 16, 2, 4, 4, OUT>{});
-        if (p.tile == T32H) return go(Tile<32, 32, 2, 4, 4, OUT>{});
-      }
-      wide ? ring(std::true_type{}) : ring(std::false_type{});
+  if (wide) return ring(std::true_type{});
+  if constexpr (!DUAL) {
+    if (p.tile == T16N) return go(Tile<16, 16, 1, 4, 4, OUT>{});
+    if (p.tile == T32N) return go(Tile<32, 16, 2, 4, 4, OUT>{});
+    if (p.tile == T32H) return go(Tile<32, 32, 2, 4, 4, OUT>{});
   }
+  if (p.tile == T256) return (void)(gemm_mx8_256<OUT><<<wg, P_T, 0, s>>>(a));
+  ring(std::false_type{});
 }
 
 template <int OUT>
@@ -949,9 +950,9 @@ int check_sizes(const char* fn, int64_t M, int64_t N, int64_t K, bool dual, bool
                   (long long)K);
     return TLM_EINVAL;
   }
-  if (fp32_sums && tiles_of(T32W, dual, M, N) > UINT32_MAX / SHAPES[T32W].threads) {
-    tlm_set_error("%s: M=%lld N=%lld has more than 2^23 tiles of 32 rows and %d columns, fp32 sums' largest", fn, (long long)M,
-                  (long long)N, cols_of(T32W, dual));
+  if (fp32_sums && tiles_of(T128, dual, M, N) > UINT32_MAX / SHAPES[T128].threads) {
+    tlm_set_error("%s: M=%lld N=%lld has more than 2^23 tiles of 128 x %d, the largest that sum in fp32", fn, (long long)M,
+                  (long long)N, cols_of(T128, dual));
     return TLM_EINVAL;
   }
   return TLM_OK;
@@ -1033,7 +1034,7 @@ extern "C" int tlm_gemm_mx8_ex(const void* a, const void* a_scales, const void* 
 extern "C" int tlm_gemm_mx8_swiglu(const void* a, const void* a_scales, const void* gate, const void* gate_scales,
                                    const void* up, const void* up_scales, void* codes, void* scales, int64_t M,
                                    int64_t N, int64_t K, void* stream) {
-  return gated_product("tlm_gemm_mx8_swiglu", a, a_scales, gate, gate_scales, up, up_scales, codes, scales, M, N, K, false,
+  return gated_product("tlm_gemm_mx8_swiglu", a, a_scales, gate, gate_scales, up, up_scales, codes, scales, M, N, K, true,
                        stream);
 }
 
