@@ -670,10 +670,9 @@ __global__ __launch_bounds__(T::THREADS, 1) void gemm_mx8_tile(Args a, int ns, f
     }
     if (t < n) {
       step(t, y, x);
-      unroll<0, NM>([&](auto ic) __attribute__((always_inline)) { mul1(y, ic); });
-    } else {
-      unroll<0, NM>([&](auto ic) __attribute__((always_inline)) { mul1(x, ic); });
+      x = y;  // a second copy of the last products would take registers from the loop, up to 15 of them to scratch memory
     }
+    unroll<0, NM>([&](auto ic) __attribute__((always_inline)) { mul1(x, ic); });
   }
   }
 
