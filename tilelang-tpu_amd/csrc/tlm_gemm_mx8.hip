@@ -11,9 +11,10 @@
 // below).
 //
 // Tiles of 16 to 256 rows, chosen by a model of their time (choose, below). Few rows wait for the stream of B, some hundreds for
-// the operands' way from L2 to a CU, whole prompts for the matrix cores' power. Measured in us: 16 x 4096 x 14336 11.6 (5.2
-// TB/s), 500 x 4096 x 4096 13.7, 4096^3 52 to 55 (2.5 to 2.6 PFLOP/s; the library's product without scales 51 to 52), gated
-// 64 x 2048 x 7168 10.3, gated 4096 x 11008 x 4096 290.
+// the operands' way from L2 to a CU, whole prompts for the matrix cores' power, where sums are of fp32 for the conversions of the
+// operands as well. Measured in us, several cards: 16 x 4096 x 14336 11.3 with weights in the 256 MB cache, 15 to 17 from HBM; 500 x 4096
+// x 4096 13.4 to 15; 4096^3 50 to 55 (2.5 to 2.7 PFLOP/s; the library's product without scales 51 to 52); gated 64 x 2048 x 7168 12
+// (by the 8-bit instruction 11), gated 4096 x 11008 x 4096 700 to 790 (290).
 #include "tlm_gemm_tile.h"
 #include "tlm_mx8.h"
 
@@ -369,7 +370,7 @@ __global__ __launch_bounds__(P_T, 1) void gemm_mx8_256(Args a) {
 
 // What bounds it: the stream of B with few rows, with more the rate at which a CU takes operand tiles from L2 (40 to 48 B/clk).
 // Four waves only fill the ring: an LDS-DMA instruction waits at issue while the CU has enough of them under way, and a wave
-// that multiplies would wait with it (500 x 4096 x 4096 16.8 us, with waves of their own 13.7). NC others are BM / (16 FX) x
+// that multiplies would wait with it (500 x 4096 x 4096 16.8 us, with waves of their own on the same card 13.7). NC others are BM / (16 FX) x
 // BN / 64 wave tiles times KG k-groups. A stage of the NST-stage ring holds KG k steps, one for each k-group, and their scales;
 // the operands of stage t are read from LDS while the products of stage t - 1 run. The k-groups' sums meet in LDS, those of the
 // `ns` workgroups that share a tile's K in memory, where the last to arrive adds them in order: the result does not depend on
@@ -378,14 +379,15 @@ __global__ __launch_bounds__(P_T, 1) void gemm_mx8_256(Args a) {
 // Narrow tiles, of 16 or 32 columns, give few rows' products a workgroup per CU without a split, with 512 neighbouring bytes
 // of a row in a load: 16 x 4096 x 14336 11.6 instead of 13.1 (64 columns, two workgroups on a tile's K), 1 x 4096 x 11008 10.3
 // instead of 12.2, 16 x 8192 x 14336 22.9 instead of 24.5; weights that the 256 MB cache no longer holds, 1 x 4096 x 4096 6.1
-// instead of 8.2, 1 x 4096 x 11008 14.2 instead of 14.4, 16 x 4096 x 14336 17.2 where the best split takes 16.6. Up to 7 stages are
+// instead of 8.2, 1 x 4096 x 11008 14.2 instead of 14.4, 16 x 4096 x 14336 17.2 where the best split takes 16.6 (another card: 6.1, 13.6,
+// 15.0). Up to 7 stages are
 // no faster there. A wave has NF = 1 or 2 operands of W, row NF i + f in slot 16 f + i.
 //
 // WIDE: the operands are widened to bf16, exactly, and multiplied by v_mfma_f32_16x16x32_bf16, whose sums are those of fp32. What
 // the 8-bit instruction cuts off sends 1 in 2,500 of a random gated product's values to the other side of an 8-bit step (an fp16
 // MLP ends 2e-3 from the formula instead of 2e-4), and is all there is where large products cancel. So gated products are summed
 // this way unless their caller chooses otherwise. It costs half the matrix rate and a conversion of each operand in each wave:
-// gated 64 x 2048 x 7168 12.0 us instead of 10.8, 500 x 11008 x 4096 100 instead of 51, 4096 x 11008 x 4096 720 instead of 290; conversions
+// gated 64 x 2048 x 7168 12.0 us instead of 11.2, 500 x 11008 x 4096 94 instead of 49, 4096 x 11008 x 4096 703 instead of 290; conversions
 // that take turns with the matrix instructions, and those all at the start of a step, take the same time. Elements of 2^128 and
 // more count as infinite there.
 template <int BM_, int BN_, int FX_, int KG_, int NST_, int OUT_, bool WIDE_ = false>
