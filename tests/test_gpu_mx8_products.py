@@ -397,3 +397,59 @@ def test_block_is_as_exact_as_16_bits(M, hidden, inter, dtype):
     exact = torch.from_numpy(ref.mx8_values_ref(*ref.mx8_quantise_ref(want))).to(DEV) @ _device_values(down).T.contiguous()
     h = torch.finfo(dtype).eps / 2
     assert ((c.double() - exact).norm() / exact.norm()).item() <= 1.1 * h / 3 ** 0.5
+
+
+@pytest.mark.parametrize("fp32_sums", [True, False])
+def test_gated_past_32_bits(fp32_sums):
+    """Codes of the result past 2^31 bytes, more rows than tiles of one height count in 16 bits: rows about the border and the last."""
+    M, N, K = 531000, 4128, 96
+    g = torch.Generator(device=DEV).manual_seed(13)
+    at = torch.arange(K, device=DEV)
+    some, gate, up = (_sparse(r, K, at, g) for r in (64, N, N))
+    a = torch.zeros(M, K, dtype=torch.uint8, device=DEV)
+    s = torch.full(ops.mx8_scales_shape(M, K), 127, dtype=torch.uint8, device=DEV)
+    groups = [0, 2 ** 31 // N // 64 - 1, 2 ** 31 // N // 64, 2 ** 31 // N // 64 + 1, M // 64 - 1]
+    for n in groups:
+        a[64 * n:64 * n + 64] = some[0].view(torch.uint8)
+        s[n] = some[1].view(torch.uint8)[0]
+    codes, scales = ops.gemm_mx8_swiglu(a.view(E4M3), s.view(E8M0), *gate, *up, *_empty(M, N), fp32_sums=fp32_sums)
+    want, _ = _gated(some, gate, up)
+    for n in groups:
+        _check_mx(codes[64 * n:64 * n + 64], scales[n:n + 1], want, ARITH * np.abs(want) + 2.0 ** -126)
+    assert not codes.view(torch.uint8)[64:64 * groups[1]].any() and not codes.view(torch.uint8)[64 * (M // 64):].any()
+
+
+@pytest.mark.parametrize("M,N", [(1, 64), (40, 96), (300, 512)])
+def test_longest_k(M, N):
+    """K of 2^22, the longest, in both kinds of sums."""
+    K = 2 ** 22
+    g = torch.Generator(device=DEV).manual_seed(M)
+    at = torch.randperm(K, generator=g, device=DEV)[:500]
+    at[0] = K - 1
+    a, b = _sparse(M, K, at, g), _sparse(N, K, at, g)
+    keep = at // 32  # the blocks that hold a value
+
+    def values(m):
+        byte = m[1].view(torch.uint8).permute(0, 3, 1, 2).flatten(2).flatten(0, 1)[:m[0].shape[0]][:, keep]
+        return m[0].view(torch.uint8)[:, at].view(E4M3).double() * torch.exp2(byte.double() - 127)
+    want = values(a) @ values(b).T.contiguous()
+    for fp32_sums in (False, True):
+        c = torch.full((M, N), 7.0, dtype=BF16, device=DEV)
+        ops.gemm_mx8(*a, *b, c, fp32_sums=fp32_sums)
+        assert torch.equal(c, want.to(BF16))
+
+
+@pytest.mark.parametrize("fp32_sums", [True, False])
+def test_empty_calls(fp32_sums):
+    """No rows, no columns: nothing is done; no k: zeros."""
+    for M, N, K in ((0, 64, 96), (33, 0, 96), (0, 0, 0), (33, 64, 0), (1, 32, 0)):
+        a, b = _empty(M, K, 0), _empty(N, K, 0)
+        c = torch.full((M, N), 7.0, dtype=BF16, device=DEV)
+        ops.gemm_mx8(*a, *b, c, fp32_sums=fp32_sums)
+        assert not c.any()
+        codes, scales = ops.gemm_mx8_swiglu(*a, *b, *b, *_empty(M, N), fp32_sums=fp32_sums)
+        assert not codes.view(torch.uint8).any()
+        assert (ref.mx8_untile_ref(_bytes(scales), M, N) == 1).all()
+        ops.mx8_quant(torch.zeros(M, K, device=DEV), *a)
+    x = torch.zeros(0, 64, dtype=BF16, device=DEV)
+    ops.add_rmsnorm(x, x, None, x, 0.0, x, *_empty(0, 64))

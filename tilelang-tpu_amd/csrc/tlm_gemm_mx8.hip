@@ -5,10 +5,10 @@
 // v_mfma_scale_f32_16x16x128_f8f6f4 multiplies each block of 32 k by 2^(ea + eb) as it adds it, at 35 cycles instead of the
 // plain form's 32. Lane l holds row l % 16 of its operand and the 16-byte chunks q and q + 4 of its 128 k (q = l / 16), and the
 // scale of k block q. The weights are the first operand, so that a lane's sums are neighbouring columns of one row of C. The
-// sums are fp32, but the products of 8 neighbouring k are cut, towards zero, below 2^-13 of the 2^(exponent of a + exponent of b) that
-// is largest among them (of codes below 2^-6, the least normal one, -6) before they are added: 4e-5 of a random result of K 4096,
-// and at worst 7 2^-13 of the sum of the groups' largest. So no 32-bit C is offered, and a caller may ask for sums of fp32 (WIDE,
-// below).
+// sums are fp32, but before they are added the products of 8 neighbouring k are cut, towards zero, below 2^-13 of the largest
+// 2^(exponent of a + exponent of b) among them (codes below the least normal one have its exponent): 4e-5 of a random result of
+// K 4096, and at worst 7 2^-13 of the sum of the groups' largest. So no 32-bit C is offered, and gated products, whose 8-bit results
+// would show it, are summed in fp32 by a form of the tiles that widens its operands (WIDE, below), as a caller may ask of both.
 //
 // Tiles of 16 to 256 rows, chosen by a model of their time (choose, below). Few rows wait for the stream of B, some hundreds for
 // the operands' way from L2 to a CU, whole prompts for the matrix cores' power, where sums are of fp32 for the conversions of the
@@ -370,8 +370,8 @@ __global__ __launch_bounds__(P_T, 1) void gemm_mx8_256(Args a) {
 
 // What bounds it: the stream of B with few rows, with more the rate at which a CU takes operand tiles from L2 (40 to 48 B/clk).
 // Four waves only fill the ring: an LDS-DMA instruction waits at issue while the CU has enough of them under way, and a wave
-// that multiplies would wait with it (500 x 4096 x 4096 16.8 us, with waves of their own on the same card 13.7). NC others are BM / (16 FX) x
-// BN / 64 wave tiles times KG k-groups. A stage of the NST-stage ring holds KG k steps, one for each k-group, and their scales;
+// that multiplies would wait with it (500 x 4096 x 4096 16.8 us, with waves of their own on the same card 13.7). NC others are
+// BM / (16 FX) x BN / 64 wave tiles times KG k-groups. A stage of the NST-stage ring holds KG k steps, one for each k-group, and their scales;
 // the operands of stage t are read from LDS while the products of stage t - 1 run. The k-groups' sums meet in LDS, those of the
 // `ns` workgroups that share a tile's K in memory, where the last to arrive adds them in order: the result does not depend on
 // the order of arrival.
@@ -379,17 +379,16 @@ __global__ __launch_bounds__(P_T, 1) void gemm_mx8_256(Args a) {
 // Narrow tiles, of 16 or 32 columns, give few rows' products a workgroup per CU without a split, with 512 neighbouring bytes
 // of a row in a load: 16 x 4096 x 14336 11.6 instead of 13.1 (64 columns, two workgroups on a tile's K), 1 x 4096 x 11008 10.3
 // instead of 12.2, 16 x 8192 x 14336 22.9 instead of 24.5; weights that the 256 MB cache no longer holds, 1 x 4096 x 4096 6.1
-// instead of 8.2, 1 x 4096 x 11008 14.2 instead of 14.4, 16 x 4096 x 14336 17.2 where the best split takes 16.6 (another card: 6.1, 13.6,
-// 15.0). Up to 7 stages are
-// no faster there. A wave has NF = 1 or 2 operands of W, row NF i + f in slot 16 f + i.
+// instead of 8.2, 1 x 4096 x 11008 14.2 instead of 14.4, 16 x 4096 x 14336 17.2 where the best split takes 16.6 (another card: 6.1,
+// 13.6, 15.0). Up to 7 stages are no faster there. A wave has NF = 1 or 2 operands of W, row NF i + f in slot 16 f + i.
 //
 // WIDE: the operands are widened to bf16, exactly, and multiplied by v_mfma_f32_16x16x32_bf16, whose sums are those of fp32. What
 // the 8-bit instruction cuts off sends 1 in 2,500 of a random gated product's values to the other side of an 8-bit step (an fp16
 // MLP ends 2e-3 from the formula instead of 2e-4), and is all there is where large products cancel. So gated products are summed
 // this way unless their caller chooses otherwise. It costs half the matrix rate and a conversion of each operand in each wave:
-// gated 64 x 2048 x 7168 12.0 us instead of 11.2, 500 x 11008 x 4096 94 instead of 49, 4096 x 11008 x 4096 703 instead of 290; conversions
-// that take turns with the matrix instructions, and those all at the start of a step, take the same time. Elements of 2^128 and
-// more count as infinite there.
+// gated 64 x 2048 x 7168 12.0 us instead of 11.2, 500 x 11008 x 4096 94 instead of 49, 4096 x 11008 x 4096 703 instead of 290;
+// conversions that take turns with the matrix instructions, and those all at the start of a step, take the same time. Elements of
+// 2^128 and more count as infinite there.
 template <int BM_, int BN_, int FX_, int KG_, int NST_, int OUT_, bool WIDE_ = false>
 struct Tile {
   static constexpr int BM = BM_, BN = BN_, FX = FX_, KG = KG_, NST = NST_, OUT = OUT_;
