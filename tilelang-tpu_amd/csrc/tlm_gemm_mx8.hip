@@ -818,7 +818,8 @@ inline double price(bool dual, bool wide, int t, int ns, int64_t M, int64_t N, i
   struct Cost {
     double a, b0, b1, r;  // launch; per k step alone; more per k step with every CU at work; a further round
   };
-  // of 543 gated products of M 1-2600: 0.4% longer than with the best on average, 15% at worst
+  // of 543 gated products of M 1-2600, which take 0.4% longer than with the best on average, 15% at worst; by it 1,082 products
+  // that are not gated take 0.4% longer, 19% at worst
   static constexpr Cost WIDE_COST[T256] = {{3.810, 0.110, 0.011, 2.90}, {4.248, 0.131, 0.007, 3.45}, {3.813, 0.192, 0.019, 2.99},
                                            {4.182, 0.241, 0.023, 3.25}, {5.034, 0.391, 0.029, 4.13}, {5.583, 0.762, 0.007, 4.51}};
   static constexpr Cost COST[T_COUNT] = {{3.685, 0.082, 0.023, 2.64}, {3.984, 0.096, 0.024, 3.09}, {3.510, 0.152, 0.036, 2.65},
